@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MO_ABI_VERSION 23
+#define MO_ABI_VERSION 24
 #define MO_MAX_DIMS 8
 
 /* Error codes outside the hipError_t range. */
@@ -534,6 +534,106 @@ uint64_t mo_int8_strip_workspace_bytes(uint32_t rows, uint32_t cols, uint32_t re
  * per split. For tests and tools. */
 int mo_int8_strip_plan(uint32_t rows, uint32_t cols, uint32_t reduction, uint32_t cus, uint32_t may_split,
                        uint32_t* plan);
+
+/* ---- 8-bit floating point with a scale for each 128 values ---------------------------------- */
+
+/* A matrix as e4m3 bytes (OCP: 4 exponent and 3 mantissa bits, largest 448) with a scale for each group
+ * of 128: along a row, along a column, or 128 x 128 blocks of a weight. The quantizers make scales that
+ * are powers of two, one E8M0 byte b for 2^(b - 127): the smallest, from 2^-126 on, that brings the
+ * group's largest magnitude within 448; the values are rounded to nearest, ties to even. A group with
+ * an infinity or a NaN gets the byte 255 and reads back as NaN. No counterpart in the reference, whose
+ * quantized bases are int8.
+ *
+ * Features (row lengths of a matrix, in and out of a weight) are multiples of 16, at most 2^20; rows
+ * are any number below 2^31. Values and matrix rows are 16-byte aligned. Everything is enqueued on
+ * `stream` on the current device: no allocation, no host synchronisation. Element types: MO_DTYPE_*
+ * (below). */
+enum { MO_FP8_SCALE_E8M0 = 0, MO_FP8_SCALE_F32 = 1 };
+enum { MO_FP8_FORWARD = 0, MO_FP8_BACKWARD = 1, MO_FP8_WEIGHT = 2 };
+
+/* x[rows][cols] (rows `row_stride` elements apart) in groups along its rows and / or its columns (0 for
+ * the pair that is not wanted), in one reading:
+ *   row_values [rows][cols], row_scales [rows][ceil(ceil(cols / 128) / 4) * 4];
+ *   col_values [cols][ceil(rows / 128) * 128], the values past `rows` zero,
+ *   col_scales [cols][ceil(ceil(rows / 128) / 4) * 4].
+ * Scale bytes past a row's groups are not written. */
+int mo_fp8_quantize(uint64_t x, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t row_stride,
+                    uint64_t row_values, uint64_t row_scales, uint64_t col_values, uint64_t col_scales,
+                    uint64_t stream);
+
+/* w[rows][cols] in blocks of 128 x 128: values [rows][cols], scales [ceil(rows / 128)][ceil(cols / 128)]. */
+int mo_fp8_quantize_weight(uint64_t w, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t row_stride,
+                           uint64_t values, uint64_t scales, uint64_t stream);
+
+/* out[rows][cols] = value * scale, rounded to `dtype`: values `pitch` bytes a row (a multiple of 16, at
+ * least cols; cols is any number here), the scale of (r, c) at scales[r / block_rows * scale_stride +
+ * c / 128] (block_rows 1 or 128), E8M0 bytes or fp32. */
+int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t scale_kind, uint64_t scale_stride,
+                  uint32_t block_rows, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t stream);
+
+/* y[rows][out] = x . w^T (+ bias), fp32 sums, on the scaled f8f6f4 matrix instructions. x: a matrix of
+ * `dtype` that the call quantizes along its rows, or (x_scales not 0) row_values and row_scales of
+ * mo_fp8_quantize. w: e4m3 [out][in], w_scale [ceil(out / 128)][ceil(in / 128)], E8M0 or any fp32. bias:
+ * [out] in y's type, or 0. `workspace`: 256-byte aligned, at least mo_fp8_workspace_bytes(MO_FP8_FORWARD,
+ * rows, in, out, x_scales != 0) bytes. */
+int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_t rows, uint32_t in_features,
+                          uint64_t row_stride, uint64_t w, uint64_t w_scale, uint32_t scale_kind,
+                          uint32_t out_features, uint64_t bias, uint64_t y, uint32_t y_dtype, uint64_t workspace,
+                          uint64_t workspace_bytes, uint64_t stream);
+
+/* dx[rows][in] = dy . w: the input gradient, dy quantized along its rows (out) or given so. */
+int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint64_t rows, uint32_t in_features,
+                           uint32_t out_features, uint64_t row_stride, uint64_t w, uint64_t w_scale,
+                           uint32_t scale_kind, uint64_t dx, uint32_t dx_dtype, uint64_t workspace,
+                           uint64_t workspace_bytes, uint64_t stream);
+
+/* dw[out][in] = dy^T . x: the weight gradient, both matrices quantized along their columns (the tokens),
+ * or both given as col_values and col_scales of mo_fp8_quantize. */
+int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, uint64_t dy_stride, uint64_t x,
+                           uint64_t x_scales, uint32_t x_dtype, uint64_t x_stride, uint64_t rows,
+                           uint32_t in_features, uint32_t out_features, uint64_t dw, uint32_t dw_dtype,
+                           uint64_t workspace, uint64_t workspace_bytes, uint64_t stream);
+
+uint64_t mo_fp8_workspace_bytes(uint32_t op, uint64_t rows, uint32_t in_features, uint32_t out_features,
+                                uint32_t quantized);
+
+/* ---- rotary positions (training/model.py:41-56, 136-151), with the heads' RMS norm (:154-172) -- */
+
+/* One side (queries or keys): [batch][tokens][heads][head_dim], the last dimension dense; strides in
+ * elements. Outputs are contiguous. heads 0: no such side. */
+typedef struct mo_rotary_side {
+  uint64_t x;           /* input; backward: wanted where weight is not 0 */
+  uint64_t grad;        /* backward: the output's gradient */
+  uint64_t out;         /* forward: the output; backward: the input's gradient */
+  uint64_t weight;      /* [head_dim] scale of the RMS norm before the turn, or 0: no norm */
+  uint64_t weight_grad; /* backward with a norm: [head_dim], in the weight's type */
+  int64_t x_batch, x_token, x_head;
+  int64_t grad_batch, grad_token, grad_head;
+  uint32_t heads, reserved;
+} mo_rotary_side;
+
+typedef struct mo_rotary_call {
+  mo_rotary_side side[2];
+  uint64_t table;       /* [batch or 1][tokens][rotary_dim]: rotary_dim / 2 sines, then as many cosines */
+  uint64_t table_batch; /* elements between batch entries' tables; 0: one for all */
+  uint32_t dtype, table_dtype, weight_dtype; /* MO_DTYPE_* of the heads, the table, the weights */
+  uint32_t batch, tokens, head_dim, rotary_dim; /* both dims even, rotary_dim <= head_dim <= 512 */
+  uint32_t interleaved; /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+  float eps;
+  uint32_t reserved;
+} mo_rotary_call;
+
+/* Each pair (f, s) of the first rotary_dim values becomes (f cos - s sin, s cos + f sin); the others are
+ * passed on. With a weight, every head is first scaled by weight / rms. fp32 inside, rounded once. */
+int mo_rotary_forward(const mo_rotary_call* call, uint64_t stream);
+/* The gradients of that. `workspace`: 256-byte aligned, mo_rotary_workspace_bytes(call) bytes (the norm
+ * weights' partial sums, added in a fixed order). */
+int mo_rotary_backward(const mo_rotary_call* call, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream);
+uint64_t mo_rotary_workspace_bytes(const mo_rotary_call* call);
+/* out[rows][2 * axes * bands]: sines, then cosines, of fp32(coordinate x band), axis by axis, each times
+ * `amplitude`; coordinates fp32 [rows][axes], bands fp32. */
+int mo_rotary_table(uint64_t coordinates, uint64_t bands, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t axes,
+                    uint32_t n_bands, float amplitude, uint64_t stream);
 
 /* ---- host gradient accumulation (training/fused_adafactor.py:327-369) -------------------- */
 

@@ -1,0 +1,25 @@
+// Shared by the device and host sides of the 8-bit floating-point products (mo_fp8.hip, mo_fp8.cpp).
+#pragma once
+#include <stdint.h>
+
+namespace mo_fp8 {
+
+constexpr uint32_t kGroup = 128;                   // values that share a scale
+constexpr uint32_t kF16 = 0, kBF16 = 1, kF32 = 2;  // MO_DTYPE_*
+
+// C[m][n] = sum_k A[m][k] B[n][k] under their scales (+ bias[n]); pitches in bytes, scale strides in
+// elements. B's scale of (n, group) is at (n >> b_shift) * b_scale_row + group * b_scale_col.
+struct ProductArgs {
+  const uint8_t* a;
+  const uint8_t* b;
+  const uint8_t* a_scales;  // one byte a row and group
+  const void* b_scales;     // bytes, or fp32 for the f32 kernels (then b_shift is 7)
+  const void* bias;         // in out's type, or null
+  void* out;                // [m][n]
+  uint64_t m, a_pitch, b_pitch;
+  uint32_t n, r;
+  uint32_t a_scale_pitch, b_scale_row, b_scale_col, b_shift;
+  uint32_t out_kind;
+};
+
+}  // namespace mo_fp8

@@ -15,7 +15,7 @@ import torch  # noqa: F401  (must be imported before the library, see module doc
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmoss_offload.so"
 
-MO_ABI_VERSION = 23
+MO_ABI_VERSION = 24
 MO_MAX_DIMS = 8
 
 MO_E_INVALID = 1001
@@ -37,6 +37,13 @@ MO_FLAG_WIRE_AUTO = 0x400
 MO_TENSOR_BF16_HIGH = 0x1
 MO_INT8_KERNEL_REGISTERS = 0
 MO_INT8_KERNEL_LDS = 1
+MO_FP8_SCALE_E8M0 = 0
+MO_FP8_SCALE_F32 = 1
+MO_FP8_FORWARD = 0
+MO_FP8_BACKWARD = 1
+MO_FP8_WEIGHT = 2
+
+DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # MO_DTYPE_*
 
 NO_GROUP = (1 << 64) - 1
 
@@ -174,6 +181,21 @@ class MoGradaccStats(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class MoRotarySide(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_uint64) for name in ("x", "grad", "out", "weight", "weight_grad")] + [
+        (name, ctypes.c_int64)
+        for name in ("x_batch", "x_token", "x_head", "grad_batch", "grad_token", "grad_head")
+    ] + [("heads", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
+class MoRotaryCall(ctypes.Structure):
+    _fields_ = [("side", MoRotarySide * 2), ("table", ctypes.c_uint64), ("table_batch", ctypes.c_uint64)] + [
+        (name, ctypes.c_uint32)
+        for name in ("dtype", "table_dtype", "weight_dtype", "batch", "tokens", "head_dim", "rotary_dim",
+                     "interleaved")
+    ] + [("eps", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
 class EngineError(RuntimeError):
     """A non-zero status from the engine library, with its message."""
 
@@ -184,6 +206,7 @@ class EngineError(RuntimeError):
 
 _P = ctypes.POINTER
 _u64 = ctypes.c_uint64
+_u32 = ctypes.c_uint32
 
 # name -> (restype, argtypes); mirrors include/moss_offload.h
 SIGNATURES: dict[str, tuple] = {
@@ -270,6 +293,20 @@ SIGNATURES: dict[str, tuple] = {
     "mo_int8_set_kernel": (ctypes.c_int, [ctypes.c_uint32]),
     "mo_int8_launch_plan": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
                                            ctypes.c_uint32, _P(ctypes.c_uint32), _P(ctypes.c_uint32)]),
+    "mo_fp8_quantize": (ctypes.c_int, [_u64, _u32, _u64, _u32, _u64, _u64, _u64, _u64, _u64, _u64]),
+    "mo_fp8_quantize_weight": (ctypes.c_int, [_u64, _u32, _u64, _u32, _u64, _u64, _u64, _u64]),
+    "mo_fp8_decode": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u32, _u64, _u32, _u64, _u32, _u64]),
+    "mo_fp8_linear_forward": (ctypes.c_int, [_u64, _u64, _u32, _u64, _u32, _u64, _u64, _u64, _u32, _u32, _u64, _u64,
+                                             _u32, _u64, _u64, _u64]),
+    "mo_fp8_linear_backward": (ctypes.c_int, [_u64, _u64, _u32, _u64, _u32, _u32, _u64, _u64, _u64, _u32, _u64, _u32,
+                                              _u64, _u64, _u64]),
+    "mo_fp8_weight_gradient": (ctypes.c_int, [_u64, _u64, _u32, _u64, _u64, _u64, _u32, _u64, _u64, _u32, _u32, _u64,
+                                              _u32, _u64, _u64, _u64]),
+    "mo_fp8_workspace_bytes": (_u64, [_u32, _u64, _u32, _u32, _u32]),
+    "mo_rotary_forward": (ctypes.c_int, [_P(MoRotaryCall), _u64]),
+    "mo_rotary_backward": (ctypes.c_int, [_P(MoRotaryCall), _u64, _u64, _u64]),
+    "mo_rotary_workspace_bytes": (_u64, [_P(MoRotaryCall)]),
+    "mo_rotary_table": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u32, _u32, ctypes.c_float, _u64]),
 }
 
 _lock = threading.Lock()

@@ -3,10 +3,11 @@
 Two steps, no torch extension machinery:
 
 1. ``hipcc --genco --offload-arch=gfx950`` compiles each device source (``csrc/mo_device.hip``:
-   pack/unpack/copy kernels; ``csrc/mo_gemm.hip``: int8 weight-only GEMMs) into a standalone
-   code object, embedded as a byte array.
+   pack/unpack/copy kernels; ``csrc/mo_gemm.hip``: int8 weight-only GEMMs; ``csrc/mo_fp8.hip``:
+   8-bit floating-point quantizers and products; ``csrc/mo_rotary.hip``: rotary positions) into a
+   standalone code object, embedded as a byte array.
 2. ``g++`` compiles the host engine and launchers (``csrc/mo_engine.cpp``,
-   ``csrc/mo_launch.cpp``) with the embedded code object into one shared library linked
+   ``csrc/mo_launch.cpp``, ...) with the embedded code objects into one shared library linked
    against the HIP runtime. The library loads its kernels with ``hipModuleLoadData`` on first
    use, so it registers no fat binary with the runtime.
 
@@ -30,8 +31,10 @@ LIB_DIR = PACKAGE_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libmoss_offload.so"
 
 # device source -> symbol of its embedded code object
-DEVICE_SOURCES = {"mo_device.hip": "mo_device_code", "mo_gemm.hip": "mo_gemm_code"}
-HOST_SOURCES = ("mo_engine.cpp", "mo_launch.cpp", "mo_link.cpp", "mo_streamer.cpp", "mo_gemm.cpp", "mo_gradacc.cpp")
+DEVICE_SOURCES = {"mo_device.hip": "mo_device_code", "mo_gemm.hip": "mo_gemm_code", "mo_fp8.hip": "mo_fp8_code",
+                  "mo_rotary.hip": "mo_rotary_code"}
+HOST_SOURCES = ("mo_engine.cpp", "mo_launch.cpp", "mo_link.cpp", "mo_streamer.cpp", "mo_gemm.cpp", "mo_gradacc.cpp",
+                "mo_fp8.cpp", "mo_rotary.cpp")
 
 ARCH = "gfx950"
 

@@ -1,0 +1,104 @@
+"""What the 8-bit floating-point calls refuse, on the CPU: no call here reaches a GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from moss_offload import _native, fp8_kernels as fp8
+
+import fp8_model as model
+
+
+def _weight(out_features=32, in_features=144):
+    scale = torch.full((-(-out_features // 128), -(-in_features // 128)), 127, dtype=torch.uint8)
+    return torch.zeros(out_features, in_features).to(torch.float8_e4m3fn), scale.view(torch.float8_e8m0fnu)
+
+
+def test_model_rounds_as_the_format_does() -> None:
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    every = every[torch.isfinite(every)]
+    assert torch.equal(model.round_e4m3(every), every)
+    between = torch.linspace(-448, 448, 100_001).double()  # float32 numbers: one rounding on either side
+    assert torch.equal(model.round_e4m3(between), between.float().to(torch.float8_e4m3fn).double())
+    assert model.power_for(torch.tensor([448.0, 448.001, 0.0, 224.0, 2.0**-140], dtype=torch.float64)).tolist() == \
+        [0, 1, -126, -1, -126]
+
+
+def test_matrices_the_quantizers_refuse() -> None:
+    for call in (fp8.fp8_quantize_rows, fp8.fp8_quantize_columns, fp8.fp8_quantize_both, fp8.fp8_quantize_weight):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            call(torch.zeros(32, 64))
+        with pytest.raises(TypeError, match="bfloat16, float16 or float32"):
+            call(torch.zeros(32, 64, dtype=torch.float64))
+        with pytest.raises(ValueError, match="multiple"):
+            call(torch.zeros(32, 24))
+        with pytest.raises(ValueError, match="multiple"):
+            call(torch.zeros(32, 0))
+        with pytest.raises(RuntimeError, match="graph"):
+            call(torch.zeros(32, 64, requires_grad=True))
+    with pytest.raises(ValueError, match="multiples of 16"):
+        fp8.fp8_quantize_weight(torch.zeros(24, 64))
+    with pytest.raises(ValueError, match="multiples of 16"):
+        fp8.fp8_quantize_weight(torch.zeros(2, 32, 64))
+
+
+def test_operands_the_products_refuse() -> None:
+    weight, scale = _weight()
+    tokens = torch.zeros(4, 144, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="float8_e4m3fn matrix"):
+        fp8.fp8_linear_forward(tokens, weight.float(), scale)
+    with pytest.raises(RuntimeError, match="float8_e4m3fn matrix"):
+        fp8.fp8_linear_forward(tokens, weight.t(), scale)
+    for bad in (scale[:, :1], scale.view(torch.uint8), scale.float().half(), scale.float().t()):
+        with pytest.raises(RuntimeError, match="weight scale"):
+            fp8.fp8_linear_forward(tokens, weight, bad)
+    with pytest.raises(ValueError, match="144 features"):
+        fp8.fp8_linear_forward(tokens[:, :128], weight, scale)
+    with pytest.raises(ValueError, match="32 features"):
+        fp8.fp8_linear_backward(tokens, weight, scale)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        fp8.fp8_linear_forward(tokens, weight, scale)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        fp8.fp8_linear_backward(tokens[:, :32], weight, scale)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        fp8.fp8_weight_gradient(tokens[:, :32], tokens)
+    with pytest.raises(ValueError, match="same rows"):
+        fp8.fp8_weight_gradient(tokens[:3, :32], tokens)
+    values, scales = weight[:, :144], torch.zeros(32, 2).to(torch.float8_e8m0fnu)
+    with pytest.raises(RuntimeError, match="one scale"):
+        fp8.fp8_linear_forward((values, scales[:, :1]), weight, scale)
+    with pytest.raises(RuntimeError, match="float8_e4m3fn of 144"):
+        fp8.fp8_linear_forward((values.float(), scales), weight, scale)
+    with pytest.raises(TypeError, match="two matrices or two quantized pairs"):
+        fp8.fp8_weight_gradient((values, scales), tokens)
+    with pytest.raises(ValueError, match="number of tokens"):
+        fp8.fp8_weight_gradient((values, scales), (values, scales))
+    with pytest.raises(TypeError):
+        fp8.fp8_decode(values.float(), scales)
+    with pytest.raises(ValueError, match="cols"):
+        fp8.fp8_decode(values, scales, cols=145)
+    with pytest.raises(ValueError, match="do not fit"):
+        fp8.fp8_decode(values, scales[:5])
+
+
+def test_the_library_refuses_before_it_looks_for_a_device() -> None:
+    lib = _native.load()
+    quantize = [4096, 1, 4, 64, 64, 4096, 4096, 0, 0, 0]
+    for index, value, message in [(0, 0, b"null"), (1, 3, b"type"), (2, 0, b"empty"), (3, 24, b"multiples"),
+                                  (4, 32, b"stride"), (4, 68, b"aligned"), (0, 4100, b"aligned"), (6, 0, b"pairs"),
+                                  (2, 1 << 31, b"rows")]:
+        call = list(quantize)
+        call[index] = value
+        assert lib.mo_fp8_quantize(*call) == _native.MO_E_INVALID
+        assert message in lib.mo_last_error(), (index, value, lib.mo_last_error())
+    forward = [4096, 0, 1, 4, 64, 64, 4096, 4096, 0, 32, 0, 4096, 1, 4096, 1 << 20, 0]
+    for index, value, message in [(6, 0, b"null"), (8, 2, b"scale type"), (4, 40, b"multiples"), (9, 0, b"empty"),
+                                  (11, 0, b"null"), (12, 5, b"type"), (11, 4104, b"misaligned"), (13, 0, b"workspace"),
+                                  (14, 16, b"workspace"), (13, 4100, b"workspace"), (3, 0, b"empty")]:
+        call = list(forward)
+        call[index] = value
+        assert lib.mo_fp8_linear_forward(*call) == _native.MO_E_INVALID
+        assert message in lib.mo_last_error(), (index, value, lib.mo_last_error())
+    assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, 0, 64, 64, 0) == 0
+    assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, 5, 64, 64, 1) == 0
