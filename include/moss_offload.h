@@ -553,10 +553,10 @@ enum { MO_FP8_FORWARD = 0, MO_FP8_BACKWARD = 1, MO_FP8_WEIGHT = 2 };
 
 /* x[rows][cols] (rows `row_stride` elements apart) in groups along its rows and / or its columns (0 for
  * the pair that is not wanted), in one reading:
- *   row_values [rows][cols], row_scales [rows][ceil(ceil(cols / 128) / 4) * 4];
+ *   row_values [rows][cols], row_scales [ceil(cols / 128)][rows rounded up to 16];
  *   col_values [cols][ceil(rows / 128) * 128], the values past `rows` zero,
- *   col_scales [cols][ceil(ceil(rows / 128) / 4) * 4].
- * Scale bytes past a row's groups are not written. */
+ *   col_scales [ceil(rows / 128)][cols].
+ * Scales lie group by group, which is how the products read them; bytes past `rows` are not written. */
 int mo_fp8_quantize(uint64_t x, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t row_stride,
                     uint64_t row_values, uint64_t row_scales, uint64_t col_values, uint64_t col_scales,
                     uint64_t stream);
@@ -566,10 +566,10 @@ int mo_fp8_quantize_weight(uint64_t w, uint32_t dtype, uint64_t rows, uint32_t c
                            uint64_t values, uint64_t scales, uint64_t stream);
 
 /* out[rows][cols] = value * scale, rounded to `dtype`: values `pitch` bytes a row (a multiple of 16, at
- * least cols; cols is any number here), the scale of (r, c) at scales[r / block_rows * scale_stride +
- * c / 128] (block_rows 1 or 128), E8M0 bytes or fp32. */
-int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t scale_kind, uint64_t scale_stride,
-                  uint32_t block_rows, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t stream);
+ * least cols; cols is any number here), the scale of (r, c) at scales[r / block_rows * scale_row + c / 128 *
+ * scale_col] (block_rows 1 or 128), E8M0 bytes or fp32. */
+int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t scale_kind, uint64_t scale_row,
+                  uint64_t scale_col, uint32_t block_rows, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t stream);
 
 /* y[rows][out] = x . w^T (+ bias), fp32 sums, on the scaled f8f6f4 matrix instructions. x: a matrix of
  * `dtype` that the call quantizes along its rows, or (x_scales not 0) row_values and row_scales of

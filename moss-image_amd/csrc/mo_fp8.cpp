@@ -32,6 +32,7 @@ struct Module {
   int cus = 0;
   hipFunction_t quantize[kForms][3] = {};
   hipFunction_t decode = nullptr, transpose = nullptr;
+  hipFunction_t large[2] = {};  // [scales a row]
   hipFunction_t plain[2][2] = {};  // [fp32 output][fp32 scales]
 };
 
@@ -54,6 +55,7 @@ int load_module(Module* out) {
       return (e = hipModuleGetFunction(fn, m.module, name.c_str())) == hipSuccess;
     };
     bool ok = get(&m.decode, "mo_fp8_decode_kernel") && get(&m.transpose, "mo_fp8_transpose_kernel") &&
+              get(&m.large[0], "mo_fp8_product_256x256") && get(&m.large[1], "mo_fp8_product_rows_256x256") &&
               get(&m.plain[0][0], "mo_fp8_product_plain") && get(&m.plain[0][1], "mo_fp8_product_plain_f32") &&
               get(&m.plain[1][0], "mo_fp8_product_plain_wide") && get(&m.plain[1][1], "mo_fp8_product_plain_wide_f32");
     for (int f = 0; f < kForms; ++f)
@@ -78,7 +80,7 @@ int guarded(F&& body) {
 
 uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 uint64_t align(uint64_t bytes) { return (bytes + 255) & ~uint64_t(255); }
-uint64_t scale_pitch(uint64_t values) { return (div_up(values, kGroup) + 3) & ~uint64_t(3); }
+uint64_t scale_pitch(uint64_t rows) { return (rows + 15) & ~uint64_t(15); }  // bytes of a group's scales
 
 int launch(hipFunction_t fn, uint64_t blocks, uint32_t threads, void** params, uint64_t stream, const char* what) {
   if (blocks == 0 || blocks >= (1ull << 31)) return mo::set_error(MO_E_INVALID, std::string(what) + ": grid too large");
@@ -111,6 +113,8 @@ int quantize(const Module& m, Form form, uint64_t x, uint32_t dtype, uint64_t ro
 int product(const Module& m, const ProductArgs& p, bool f32_scales, uint64_t stream) {
   ProductArgs args = p;
   void* params[] = {&args};
+  if (p.out_kind != MO_DTYPE_F32 && !f32_scales && p.m > 256)
+    return launch(m.large[p.b_shift == 0], div_up(p.m, 256) * div_up(p.n, 256), 512, params, stream, "fp8 product launch");
   return launch(m.plain[p.out_kind == MO_DTYPE_F32][f32_scales], div_up(p.m, 64) * div_up(p.n, 64), 256, params, stream, "fp8 product launch");
 }
 
@@ -149,9 +153,9 @@ int check_workspace(uint64_t workspace, uint64_t bytes, uint64_t needed) {
 }
 
 // Bytes of a quantized operand in a workspace: values, then scales.
-uint64_t row_bytes(uint64_t rows, uint64_t cols) { return align(rows * cols) + align(rows * scale_pitch(cols)); }
+uint64_t row_bytes(uint64_t rows, uint64_t cols) { return align(rows * cols) + align(div_up(cols, kGroup) * scale_pitch(rows)); }
 uint64_t col_bytes(uint64_t rows, uint64_t cols) {
-  return align(cols * div_up(rows, kGroup) * kGroup) + align(cols * scale_pitch(rows));
+  return align(cols * div_up(rows, kGroup) * kGroup) + align(div_up(rows, kGroup) * cols);
 }
 
 uint64_t workspace_of(uint32_t op, uint64_t rows, uint64_t in_f, uint64_t out_f, bool quantized) {
@@ -195,8 +199,8 @@ int mo_fp8_quantize_weight(uint64_t w, uint32_t dtype, uint64_t rows, uint32_t c
   });
 }
 
-int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t scale_kind, uint64_t scale_stride,
-                  uint32_t block_rows, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t stream) {
+int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t scale_kind, uint64_t scale_row,
+                  uint64_t scale_col, uint32_t block_rows, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t stream) {
   return guarded([&]() -> int {
     if (!values || !scales || !out) return mo::set_error(MO_E_INVALID, "null pointer");
     if (rows == 0 || cols == 0) return mo::set_error(MO_E_INVALID, "empty matrix");
@@ -212,7 +216,7 @@ int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t sca
     const void *V = (const void*)values, *S = (const void*)scales;
     void* O = (void*)out;
     uint32_t shift = block_rows == 1 ? 0 : 7;
-    void* params[] = {&V, &pitch, &S, &scale_kind, &scale_stride, &shift, &O, &dtype, &rows, &cols};
+    void* params[] = {&V, &pitch, &S, &scale_kind, &scale_row, &scale_col, &shift, &O, &dtype, &rows, &cols};
     return launch(m.decode, div_up(rows * div_up(cols, 16), 256), 256, params, stream, "fp8 decode launch");
   });
 }
@@ -237,7 +241,7 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
     }
     ProductArgs p = {};
     p.a = (const uint8_t*)x, p.a_scales = (const uint8_t*)x_scales, p.a_pitch = in_features;
-    p.a_scale_pitch = (uint32_t)scale_pitch(in_features);
+    p.a_scale_pitch = (uint32_t)scale_pitch(rows);
     p.b = (const uint8_t*)w, p.b_scales = (const void*)w_scale, p.b_pitch = in_features;
     p.b_scale_row = (uint32_t)div_up(in_features, kGroup), p.b_scale_col = 1, p.b_shift = 7;
     p.bias = (const void*)bias, p.out = (void*)y, p.out_kind = y_dtype;
@@ -276,7 +280,7 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
     }
     ProductArgs p = {};
     p.a = (const uint8_t*)dy, p.a_scales = (const uint8_t*)dy_scales, p.a_pitch = out_features;
-    p.a_scale_pitch = (uint32_t)scale_pitch(out_features);
+    p.a_scale_pitch = (uint32_t)scale_pitch(rows);
     p.b = (const uint8_t*)workspace, p.b_scales = (const void*)w_scale, p.b_pitch = out_features;
     p.b_scale_row = 1, p.b_scale_col = (uint32_t)div_up(in_features, kGroup), p.b_shift = 7;
     p.out = (void*)dx, p.out_kind = dx_dtype;
@@ -313,9 +317,9 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     }
     ProductArgs p = {};
     p.a = (const uint8_t*)dy, p.a_scales = (const uint8_t*)dy_scales, p.a_pitch = padded;
-    p.a_scale_pitch = (uint32_t)scale_pitch(rows);
+    p.a_scale_pitch = out_features;
     p.b = (const uint8_t*)x, p.b_scales = (const void*)x_scales, p.b_pitch = padded;
-    p.b_scale_row = (uint32_t)scale_pitch(rows), p.b_scale_col = 1, p.b_shift = 0;
+    p.b_scale_row = 1, p.b_scale_col = in_features, p.b_shift = 0;
     p.out = (void*)dw, p.out_kind = dw_dtype;
     p.m = out_features, p.n = in_features, p.r = (uint32_t)padded;
     return product(m, p, false, stream);

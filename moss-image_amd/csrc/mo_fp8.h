@@ -12,7 +12,7 @@ constexpr uint32_t kF16 = 0, kBF16 = 1, kF32 = 2;  // MO_DTYPE_*
 struct ProductArgs {
   const uint8_t* a;
   const uint8_t* b;
-  const uint8_t* a_scales;  // one byte a row and group
+  const uint8_t* a_scales;  // one byte a row and group: group * a_scale_pitch + row
   const void* b_scales;     // bytes, or fp32 for the f32 kernels (then b_shift is 7)
   const void* bias;         // in out's type, or null
   void* out;                // [m][n]

@@ -32,6 +32,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "mo_fp8.h"
 
 namespace {
@@ -160,7 +162,7 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
   }
 
   if (kForm & kRows) {
-    const uint32_t pitch = (tiles_c + 3) & ~3u;
+    const uint64_t pitch = (rows + 15) & ~(uint64_t)15;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t m = 0;
@@ -175,7 +177,7 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
           w[1] = pack4(v[i].get(4) * inv, v[i].get(5) * inv, v[i].get(6) * inv, v[i].get(7) * inv);
           *(u32x2*)(row_values + (row0 + i) * cols + col0) = w;
         }
-        if (c == 0) row_scales[(row0 + i) * pitch + tile_c] = (uint8_t)byte;
+        if (c == 0) row_scales[tile_c * pitch + row0 + i] = (uint8_t)byte;
       }
     }
   }
@@ -214,8 +216,7 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
       }
       if (tid == 0) row_scales[tile_r * tiles_c + tile_c] = (uint8_t)byte;
     } else {
-      const uint64_t groups = (rows + kGroup - 1) / kGroup, pitch = groups * kGroup;
-      const uint64_t scale_pitch = (groups + 3) & ~(uint64_t)3;
+      const uint64_t pitch = (rows + kGroup - 1) / kGroup * kGroup;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t byte = scale_byte(m[j]);
@@ -224,7 +225,7 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
         w[0] = pack4(v[0].get(j) * inv, v[1].get(j) * inv, v[2].get(j) * inv, v[3].get(j) * inv);
         w[1] = pack4(v[4].get(j) * inv, v[5].get(j) * inv, v[6].get(j) * inv, v[7].get(j) * inv);
         *(u32x2*)(turned + (8 * c + j) * kLine + 8 * g) = w;
-        if (g == 0 && in_cols) col_scales[(uint64_t)(col0 + j) * scale_pitch + tile_r] = (uint8_t)byte;
+        if (g == 0 && in_cols) col_scales[tile_r * cols + col0 + j] = (uint8_t)byte;
       }
       __syncthreads();
 #pragma unroll
@@ -282,14 +283,15 @@ __device__ __forceinline__ float load1(const void* base, uint64_t at, uint32_t k
 // One lane reads 16 values and their scale and writes 16 products: bound by memory.
 extern "C" __global__ __launch_bounds__(256) void mo_fp8_decode_kernel(
     const uint8_t* __restrict__ values, uint64_t pitch, const void* __restrict__ scales, uint32_t f32_scales,
-    uint64_t scale_pitch, uint32_t shift, void* __restrict__ out, uint32_t kind, uint64_t rows, uint32_t cols) {
+    uint64_t scale_row, uint64_t scale_col, uint32_t shift, void* __restrict__ out, uint32_t kind, uint64_t rows,
+    uint32_t cols) {
   const uint32_t chunks = (cols + 15) / 16;
   const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint64_t row = at / chunks;
   const uint32_t col = (uint32_t)(at % chunks) * 16;
   if (row >= rows) return;
   const u32x4 w = *(const u32x4*)(values + row * pitch + col);
-  const uint64_t s = (row >> shift) * scale_pitch + col / kGroup;
+  const uint64_t s = (row >> shift) * scale_row + col / kGroup * scale_col;
   const float scale = f32_scales ? ((const float*)scales)[s] : scale_value(((const uint8_t*)scales)[s]);
   const bool whole = col + 16 <= cols && cols % 4 == 0;
 #pragma unroll
@@ -366,6 +368,273 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x16 acc, uin
   }
 }
 
+// ---- tiles in LDS ----
+//
+// A workgroup owns a tile of kBM tokens x kBN features, shared out over WM x WN waves of TM x TN MFMA tiles
+// of 32 x 32 (the weights are the first MFMA operand). The reduction advances a group of 128 a step: kBM +
+// kBN rows of 128 bytes, one cache line each (half lines come at half the rate), go straight from memory
+// into LDS by the buffer-load DMA path, with no register on the way, into one of two buffers; the rows'
+// scale bytes go with them. A step is two halves of 64. While a half's MFMAs run, the other half's
+// fragments are read into the registers as those come free. After the first half every wave has read all it
+// wants of this step's buffer and the next step's DMA has landed (it had a whole step to): the one barrier
+// of a step sits there, and the second half refills the buffer with the step after next.
+//   LDS rows of 128 bytes keep 16-byte piece c of row r at c ^ (r / 2 % 8): 16 lanes of a read then fall on
+//   the 64 banks without a conflict (rows of one parity share a half of the banks), and a DMA instruction
+//   still fills eight whole rows.
+// The scales lie group by group, a byte a row, so that a step's are one dense piece. What lies past the rows
+// or the reduction reads as zero.
+// Tiles are numbered in groups of kGroupM row tiles and then by XCD, so that the workgroups of one XCD
+// (blockIdx % 8) share rows and columns in its L2.
+
+#define MO_LDS __attribute__((address_space(3)))
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+
+// Raw buffer descriptors (gfx9 word 3 = 0x00020000): a read whose vector and scalar offsets add up to
+// num_records or more returns zero and moves no data (into LDS, the zero is written), a write there is
+// dropped. The scalar offset must not pass num_records itself: the check subtracts it.
+constexpr uint32_t kOob = 0x80000000u;
+__device__ __forceinline__ rsrc_t make_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, 0x00020000);
+}
+// s_waitcnt immediate (gfx9): at most n vector-memory operations outstanding, and all LDS operations done.
+constexpr int wait_vm(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4); }
+
+constexpr int kGroupM = 8, kXcds = 8;
+
+template <int WM, int WN, int TM, int TN>
+struct Tile {
+  static constexpr int kWM = WM, kTM = TM, kTN = TN, kWaves = WM * WN;
+  static constexpr int kBM = 32 * WM * TM, kBN = 32 * WN * TN;
+  static constexpr int kDmaA = kBM / 8 / kWaves, kDmaB = kBN / 8 / kWaves;  // 1 KiB pieces a wave and step
+  static_assert(kBM % (16 * kWaves) == 0 && kBN % (16 * kWaves) == 0, "pairs of DMA pieces divide over the waves");
+  static_assert(kBM <= 256 && kBN <= 256 && kWaves >= 2, "one DMA instruction brings an operand's scales");
+};
+
+// How B's scales come: a byte a block of 128 x 128 (a wave's features lie in one block), or a byte a row.
+enum { kBlockBytes = 0, kRowBytes = 1 };
+
+template <class G, int kScales>
+__device__ __forceinline__ void product_tile(const ProductArgs& p) {
+  constexpr int kBM = G::kBM, kBN = G::kBN, kTM = G::kTM, kTN = G::kTN, kDmaA = G::kDmaA, kDmaB = G::kDmaB;
+  // distinct objects, chosen at compile time: the compiler then knows which reads a DMA in flight can reach
+  __shared__ __attribute__((aligned(1024))) uint8_t a_0[kBM * kGroup], a_1[kBM * kGroup];
+  __shared__ __attribute__((aligned(1024))) uint8_t b_0[kBN * kGroup], b_1[kBN * kGroup];
+  __shared__ __attribute__((aligned(256))) uint8_t sa_0[256], sa_1[256], sb_0[256], sb_1[256], nowhere[256];
+  typedef MO_LDS uint8_t* lp;
+  struct Buffer {
+    lp a, b, sa, sb;
+  };
+  const Buffer buf0 = {(lp)a_0, (lp)b_0, (lp)sa_0, (lp)sb_0}, buf1 = {(lp)a_1, (lp)b_1, (lp)sa_1, (lp)sb_1};
+
+  const int lane = threadIdx.x & 63, lr = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % G::kWM, wn = wave / G::kWM;
+
+  const int tiles = gridDim.x, tiles_m = (int)((p.m + kBM - 1) / kBM), tiles_n = tiles / tiles_m;
+  int t;
+  {
+    const int b = blockIdx.x, xcd = b % kXcds, idx = b / kXcds;
+    const int per = tiles / kXcds, rem = tiles % kXcds;
+    t = xcd < rem ? xcd * (per + 1) + idx : rem * (per + 1) + (xcd - rem) * per + idx;
+  }
+  const int group_tiles = kGroupM * tiles_n, first_m = t / group_tiles * kGroupM;
+  const int gm = min(tiles_m - first_m, kGroupM), in_group = t % group_tiles;
+  const uint64_t m0 = (uint64_t)(first_m + in_group % gm) * kBM;
+  const uint32_t n0 = (uint32_t)(in_group / gm) * kBN;
+
+  const uint32_t rows_m = (uint32_t)min((uint64_t)kBM, p.m - m0), rows_n = min((uint32_t)kBN, p.n - n0);
+  const rsrc_t ra = make_rsrc(p.a + m0 * p.a_pitch, (uint32_t)(rows_m * p.a_pitch));
+  const rsrc_t rb = make_rsrc(p.b + (uint64_t)n0 * p.b_pitch, (uint32_t)(rows_n * p.b_pitch));
+  const uint8_t* b_scales = (const uint8_t*)p.b_scales;
+
+  // DMA: piece j of wave w is rows 8 (w kDma + j) .. + 7; lane i fills position i % 8 of row i / 8. The
+  // swizzle goes by row / 2 % 8, of which bit 2 is the piece's parity. The pieces' offsets are sums made
+  // when they are wanted.
+  const uint32_t dma_row = lane >> 3;
+  uint32_t dma_k[2], a_off[2], b_off[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    dma_k[e] = 16 * ((lane & 7) ^ (4 * e + dma_row / 2));
+    a_off[e] = (uint32_t)((wave * kDmaA * 8 + dma_row) * p.a_pitch + dma_k[e]);
+    b_off[e] = (uint32_t)((wave * kDmaB * 8 + dma_row) * p.b_pitch + dma_k[e]);
+  }
+  const uint32_t last_group = (p.r - 1) / kGroup;
+  const bool scales_of_a = wave == 0, scales_of_b = kScales == kRowBytes && wave == 1;
+  auto dma = [&](const Buffer& to, uint32_t k) {
+    const uint32_t group = min(k / kGroup, last_group);
+    // a group's scales of the tile's rows (a word that begins within the rows is within the pitch)
+    const rsrc_t rsa = make_rsrc(p.a_scales + (uint64_t)group * p.a_scale_pitch + m0, (rows_m + 3) & ~3u);
+    const rsrc_t rsb = make_rsrc(b_scales + (uint64_t)group * p.b_scale_col + n0, (rows_n + 3) & ~3u);
+    const int at_k = k < p.r ? (int)k : 0;
+    // steps come in turn: from the one that the reduction ends in on, the pieces past its end read as zero
+    // (an offset from kOob on stays past every descriptor: a tile's rows take less than 2^31 bytes)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool in = k + dma_k[e] < p.r;
+      a_off[e] = in ? a_off[e] : kOob;
+      b_off[e] = in ? b_off[e] : kOob;
+    }
+    // every wave issues the scales' pieces (a branch would cut the loop up), all but one of them zeros to nowhere
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (MO_LDS void*)(scales_of_a ? to.sa : (lp)nowhere), 4, scales_of_a ? 4 * lane : kOob, 0,
+                                             0, 0);
+    if (kScales == kRowBytes)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, (MO_LDS void*)(scales_of_b ? to.sb : (lp)nowhere), 4, scales_of_b ? 4 * lane : kOob, 0,
+                                               0, 0);
+#pragma unroll
+    for (int j = 0; j < kDmaA; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (MO_LDS void*)(to.a + (wave * kDmaA + j) * 1024), 16,
+                                               a_off[j & 1] + 8 * j * (uint32_t)p.a_pitch, at_k, 0, 0);
+#pragma unroll
+    for (int j = 0; j < kDmaB; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (MO_LDS void*)(to.b + (wave * kDmaB + j) * 1024), 16,
+                                               b_off[j & 1] + 8 * j * (uint32_t)p.b_pitch, at_k, 0, 0);
+  };
+
+  f32x16 acc[kTN][kTM];
+#pragma unroll
+  for (int j = 0; j < kTN; ++j)
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) acc[j][i] = f32x16{};
+
+  // A block's scale byte is the same for all lanes, one a step: loaded two steps ahead.
+  const uint32_t n_wave = n0 + 32 * wn * kTN;
+  const uint32_t block_at = n_wave < p.n ? (n_wave >> 7) * p.b_scale_row : 0;
+  auto load_block = [&](uint32_t k) {
+    return (int)b_scales[block_at + (uint64_t)min(k / kGroup, last_group) * p.b_scale_col];
+  };
+
+  // a lane's 32 bytes of a half h are pieces 4 h + 2 half and the next of its row
+  i32x8 fa[kTM], fb[2][kTN];
+  int sa[2][kTM], sb[2][kTN];
+  int at[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) at[h][e] = lr * (int)kGroup + 16 * ((4 * h + 2 * half + e) ^ (lr / 2 & 7));
+  auto fragment = [&](const MO_LDS uint8_t* base, int h) {
+    const u32x4 lo = *(const MO_LDS u32x4*)(base + at[h][0]), hi = *(const MO_LDS u32x4*)(base + at[h][1]);
+    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
+  auto read_a = [&](const Buffer& from, int i, int h) { fa[i] = fragment(from.a + (wm * kTM + i) * 32 * kGroup, h); };
+  auto read_b = [&](const Buffer& from, int h) {
+#pragma unroll
+    for (int j = 0; j < kTN; ++j) fb[h][j] = fragment(from.b + (wn * kTN + j) * 32 * kGroup, h);
+  };
+  auto read_scales = [&](const Buffer& from, int parity) {
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) sa[parity][i] = from.sa[32 * (wm * kTM + i) + lr];
+    if (kScales == kRowBytes) {
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) sb[parity][j] = from.sb[32 * (wn * kTN + j) + lr];
+    }
+  };
+  // the MFMAs of half h, and behind each row of them the fragments of the half after
+  auto multiply = [&](int h, int parity, const Buffer& then) {
+    constexpr int kMfma = 0x008, kDsRead = 0x100;
+    read_b(then, h ^ 1);
+    if (h == 1) read_scales(then, parity ^ 1);
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) {
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+            fb[h][j], fa[i], acc[j][i], 0, 0, 0, kScales == kRowBytes ? sb[parity][j] : sb[parity][0], 0, sa[parity][i]);
+      read_a(then, i, h ^ 1);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kTN, 0);
+    __builtin_amdgcn_sched_group_barrier(kMfma, kTN - 1, 0);
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, kTN, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](int parity, const Buffer& now, const Buffer& next, uint32_t k) {
+    multiply(0, parity, now);
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    int after = 0;
+    if (kScales == kBlockBytes) after = load_block(k + 2 * kGroup);
+    dma(now, k + 2 * kGroup);
+    multiply(1, parity, next);
+    if (kScales == kBlockBytes) sb[parity][0] = after;
+  };
+
+  if (kScales == kBlockBytes) sb[0][0] = load_block(0), sb[1][0] = load_block(kGroup);
+  dma(buf0, 0);
+  dma(buf1, kGroup);
+  __builtin_amdgcn_s_waitcnt(wait_vm(kDmaA + kDmaB + 1 + (kScales == kRowBytes ? 1 : 0)));
+  __syncthreads();
+  read_scales(buf0, 0);
+  read_b(buf0, 0);
+#pragma unroll
+  for (int i = 0; i < kTM; ++i) read_a(buf0, i, 0);
+  // steps in pairs, one a buffer; an odd count gets one more over zeros
+  for (uint32_t k = 0; k < p.r; k += 2 * kGroup) {
+    step(0, buf0, buf1, k);
+    step(1, buf1, buf0, k + kGroup);
+  }
+
+  // Epilogue: 32 tokens at a time through a part of LDS of the wave's own, so that a store writes whole
+  // rows of the wave's features instead of pieces of 32 rows. 16-byte piece c of row r at c ^ (r %
+  // kPieces): writes and reads spread over the banks.
+  constexpr int kLine = 32 * kTN * 2, kPieces = kLine / 16, kRowsAStore = 64 / kPieces;
+  static_assert(32 * kLine * G::kWaves <= kBM * (int)kGroup, "a wave's part of the first buffer");
+  __builtin_amdgcn_s_waitcnt(wait_vm(0));
+  __syncthreads();  // every wave has read its last fragments, every DMA has landed
+  lp own = (lp)a_0 + wave * 32 * kLine;
+  const int out_row = lane / kPieces, piece = lane % kPieces;
+  const bool f16 = p.out_kind != kBF16;
+  const rsrc_t ro = make_rsrc((uint16_t*)p.out + m0 * p.n, (uint32_t)(rows_m * p.n * 2));
+#pragma unroll
+  for (int i = 0; i < kTM; ++i) {
+#pragma unroll
+    for (int j = 0; j < kTN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& w16 = acc[j][i];
+        float o[4] = {w16[4 * q], w16[4 * q + 1], w16[4 * q + 2], w16[4 * q + 3]};
+        if (p.bias) {
+          const uint32_t n = n_wave + 32 * j + 8 * q + 4 * half;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] += n < p.n ? load1(p.bias, n + e, p.out_kind) : 0.0f;
+        }
+        u32x2 w;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+          typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+          w[e] = f16 ? __builtin_bit_cast(uint32_t, f16x2{(_Float16)o[2 * e], (_Float16)o[2 * e + 1]})
+                     : __builtin_bit_cast(uint32_t, bf16x2{(__bf16)o[2 * e], (__bf16)o[2 * e + 1]});
+        }
+        *(MO_LDS u32x2*)(own + lr * kLine + 16 * ((4 * j + q) ^ (lr % kPieces)) + 8 * half) = w;
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 32; r += kRowsAStore) {
+      const int row = r + out_row;
+      const u32x4 w = *(const MO_LDS u32x4*)(own + row * kLine + 16 * (piece ^ (row % kPieces)));
+      const uint32_t to = ((uint32_t)(32 * (wm * kTM + i) + row) * p.n + n_wave + 8 * piece) * 2;
+      __builtin_amdgcn_raw_buffer_store_b128(w, ro, (int)(n_wave + 8 * piece < p.n ? to : kOob), 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+#define MO_TILE(name, WM, WN, TM, TN)                                                                              \
+  extern "C" __global__ __launch_bounds__(64 * WM * WN, 1) void mo_fp8_product_##name(ProductArgs p) {             \
+    product_tile<Tile<WM, WN, TM, TN>, kBlockBytes>(p);                                                            \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(64 * WM * WN, 1) void mo_fp8_product_rows_##name(ProductArgs p) {        \
+    product_tile<Tile<WM, WN, TM, TN>, kRowBytes>(p);                                                              \
+  }
+MO_TILE(256x256, 2, 4, 4, 2)
+
 // Eight e4m3 bytes times a power of two as bf16: exact (four significant bits).
 __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float scale) {
   bf16x8 o;
@@ -394,7 +663,7 @@ __device__ __forceinline__ void product_plain(const ProductArgs& p) {
   f32x16 acc = {};
   for (uint32_t k0 = 0; k0 < p.r; k0 += kGroup) {
     const uint32_t group = k0 / kGroup;
-    const int sa = in_m ? p.a_scales[m * p.a_scale_pitch + group] : 127;
+    const int sa = in_m ? p.a_scales[group * (uint64_t)p.a_scale_pitch + m] : 127;
     const uint64_t at = (uint64_t)((in_n ? n : 0) >> p.b_shift) * p.b_scale_row + (uint64_t)group * p.b_scale_col;
     const int sb = kF32Scales ? 127 : ((const uint8_t*)p.b_scales)[at];
     f32x16 sum = kF32Scales ? f32x16{} : acc;

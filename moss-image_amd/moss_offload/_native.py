@@ -295,7 +295,7 @@ SIGNATURES: dict[str, tuple] = {
                                            ctypes.c_uint32, _P(ctypes.c_uint32), _P(ctypes.c_uint32)]),
     "mo_fp8_quantize": (ctypes.c_int, [_u64, _u32, _u64, _u32, _u64, _u64, _u64, _u64, _u64, _u64]),
     "mo_fp8_quantize_weight": (ctypes.c_int, [_u64, _u32, _u64, _u32, _u64, _u64, _u64, _u64]),
-    "mo_fp8_decode": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u32, _u64, _u32, _u64, _u32, _u64]),
+    "mo_fp8_decode": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u64, _u32, _u64, _u32, _u64, _u32, _u64]),
     "mo_fp8_linear_forward": (ctypes.c_int, [_u64, _u64, _u32, _u64, _u32, _u64, _u64, _u64, _u32, _u32, _u64, _u64,
                                              _u32, _u64, _u64, _u64]),
     "mo_fp8_linear_backward": (ctypes.c_int, [_u64, _u64, _u32, _u64, _u32, _u32, _u64, _u64, _u64, _u32, _u64, _u32,

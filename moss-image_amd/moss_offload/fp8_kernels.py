@@ -51,8 +51,11 @@ def _groups(size: int) -> int:
     return -(-size // GROUP)
 
 
-def _scale_pitch(size: int) -> int:
-    return (_groups(size) + 3) // 4 * 4
+def _scales(rows: int, size: int, device) -> torch.Tensor:
+    """Room for one scale for each 128 of ``size`` values of ``rows`` rows: ``[rows, groups]``, laid group by
+    group (what the products read at a time is then dense)."""
+
+    return torch.empty((_groups(size), -(-rows // 16) * 16), dtype=E8M0, device=device)[:, :rows].t()
 
 
 def _plain(*operands: torch.Tensor | None) -> None:
@@ -94,7 +97,7 @@ def _weight(weight: torch.Tensor, scale: torch.Tensor) -> int:
 
 
 def _pair(pair: tuple[torch.Tensor, torch.Tensor], features: int, what: str) -> tuple[torch.Tensor, torch.Tensor]:
-    """A quantized operand as the kernels read it: dense rows, scale rows of whole 4-byte words."""
+    """A quantized operand as the kernels read it: dense rows, scales group by group."""
 
     values, scales = pair
     if values.dtype != E4M3 or scales.dtype != E8M0 or values.ndim < 2 or values.shape[-1] != features:
@@ -105,11 +108,11 @@ def _pair(pair: tuple[torch.Tensor, torch.Tensor], features: int, what: str) -> 
     rows, groups = values.shape[0], _groups(features)
     if scales.shape != (rows, groups) or scales.get_device() != values.get_device():
         raise RuntimeError(f"quantized fp8 {what} must have one scale for each 128 values of a row, on its device.")
-    pitch = _scale_pitch(features)
-    if rows and (scales.stride(1) != 1 or scales.stride(0) != pitch or scales.data_ptr() % 4):
-        laid = torch.empty((rows, pitch), dtype=torch.uint8, device=scales.device)
-        laid[:, :groups] = scales.view(torch.uint8)
-        scales = laid.view(E8M0)[:, :groups]
+    if rows and (scales.stride(0) != 1 or groups > 1 and scales.stride(1) != -(-rows // 16) * 16
+                 or scales.data_ptr() % 4):
+        laid = _scales(rows, features, scales.device)
+        laid.view(torch.uint8).copy_(scales.view(torch.uint8))
+        scales = laid
     return values, scales
 
 
@@ -147,10 +150,10 @@ def _quantize(x: torch.Tensor, rows: bool, columns: bool):
     with _device(x):
         if rows:
             row = (torch.empty((m, n), dtype=E4M3, device=device),
-                   torch.empty((m, _scale_pitch(n)), dtype=E8M0, device=device)[:, : _groups(n)])
+                   _scales(m, n, device))
         if columns:
             column = (torch.empty((n, _groups(m) * GROUP), dtype=E4M3, device=device),
-                      torch.empty((n, _scale_pitch(m)), dtype=E8M0, device=device)[:, : _groups(m)])
+                      _scales(n, m, device))
         if m:
             pointers = [t.data_ptr() if t is not None else 0 for pair in (row, column) for t in (pair or (None, None))]
             _native.check("mo_fp8_quantize", lib.mo_fp8_quantize(
@@ -222,13 +225,12 @@ def fp8_decode(values: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype
     if scales.shape[0] not in (rows, _groups(rows)) or scales.shape[1] < _groups(cols) \
             or scales.get_device() != values.get_device():
         raise ValueError("fp8 scales do not fit the values.")
-    scales = scales if scales.stride(1) == 1 else scales.contiguous()
     out = torch.empty((*values.shape[:-1], cols), dtype=dtype, device=values.device)
     if out.numel():
         kind = _native.MO_FP8_SCALE_F32 if scales.dtype == torch.float32 else _native.MO_FP8_SCALE_E8M0
         with _device(values):
             _native.check("mo_fp8_decode", lib.mo_fp8_decode(
-                matrix.data_ptr(), _stride(matrix), scales.data_ptr(), kind, scales.stride(0),
+                matrix.data_ptr(), _stride(matrix), scales.data_ptr(), kind, *scales.stride(),
                 1 if scales.shape[0] == rows else GROUP, out.data_ptr(), _CODES[dtype], rows, cols, _stream(values)))
     return out
 
