@@ -27,12 +27,16 @@ const char* const kFormNames[kForms] = {"rows", "columns", "both", "weight"};
 const char* const kTypeNames[3] = {"f16", "bf16", "f32"};  // by MO_DTYPE_*
 constexpr uint32_t kTypeBytes[3] = {2, 2, 4};
 
+// How the second operand's scales come: a byte or an fp32 number a block of 128 x 128, or a byte a row.
+enum { kScaleBytes = MO_FP8_SCALE_E8M0, kScaleFloats = MO_FP8_SCALE_F32, kScaleRows = 2 };
+const char* const kScaleNames[3] = {"bytes", "floats", "rows"};
+
 struct Module {
   hipModule_t module = nullptr;
   int cus = 0;
   hipFunction_t quantize[kForms][3] = {};
   hipFunction_t decode = nullptr, transpose = nullptr;
-  hipFunction_t large[2] = {};  // [scales a row]
+  hipFunction_t large[3][2][2] = {};  // [scales][fp32 output][transposed]
   hipFunction_t plain[2][2] = {};  // [fp32 output][fp32 scales]
 };
 
@@ -55,12 +59,18 @@ int load_module(Module* out) {
       return (e = hipModuleGetFunction(fn, m.module, name.c_str())) == hipSuccess;
     };
     bool ok = get(&m.decode, "mo_fp8_decode_kernel") && get(&m.transpose, "mo_fp8_transpose_kernel") &&
-              get(&m.large[0], "mo_fp8_product_256x256") && get(&m.large[1], "mo_fp8_product_rows_256x256") &&
               get(&m.plain[0][0], "mo_fp8_product_plain") && get(&m.plain[0][1], "mo_fp8_product_plain_f32") &&
               get(&m.plain[1][0], "mo_fp8_product_plain_wide") && get(&m.plain[1][1], "mo_fp8_product_plain_wide_f32");
     for (int f = 0; f < kForms; ++f)
       for (int t = 0; t < 3; ++t)
         ok = ok && get(&m.quantize[f][t], std::string("mo_fp8_quantize_") + kFormNames[f] + "_" + kTypeNames[t]);
+    for (int k = 0; k < 3; ++k)
+      for (int wide = 0; wide < 2; ++wide)
+        for (int trans = 0; trans < (k == kScaleRows ? 1 : 2); ++trans) {
+          std::string name = std::string("mo_fp8_product_large_") + kScaleNames[k];
+          if (trans || wide) name += std::string("_") + (trans ? "t" : "") + (wide ? "w" : "");
+          ok = ok && get(&m.large[k][wide][trans], name);
+        }
     if (!ok) return mo::set_hip_error((int)e, "hipModuleGetFunction (fp8)");
     it = g_modules.emplace(device, m).first;
   }
@@ -110,12 +120,19 @@ int quantize(const Module& m, Form form, uint64_t x, uint32_t dtype, uint64_t ro
                 "fp8 quantize launch");
 }
 
-int product(const Module& m, const ProductArgs& p, bool f32_scales, uint64_t stream) {
+// Whether a call of `rows` runs on the tiles (below, on the plain kernel, whose second operand lies along the
+// reduction).
+bool tiles(uint64_t rows) { return rows > 256; }
+
+int product(const Module& m, const ProductArgs& p, int scales, bool trans, uint64_t stream) {
   ProductArgs args = p;
   void* params[] = {&args};
-  if (p.out_kind != MO_DTYPE_F32 && !f32_scales && p.m > 256)
-    return launch(m.large[p.b_shift == 0], div_up(p.m, 256) * div_up(p.n, 256), 512, params, stream, "fp8 product launch");
-  return launch(m.plain[p.out_kind == MO_DTYPE_F32][f32_scales], div_up(p.m, 64) * div_up(p.n, 64), 256, params, stream, "fp8 product launch");
+  const bool wide = p.out_kind == MO_DTYPE_F32;
+  if (tiles(p.m))
+    return launch(m.large[scales][wide][trans], div_up(p.m, 256) * div_up(p.n, 256), 512, params, stream,
+                  "fp8 product launch");
+  return launch(m.plain[wide][scales == kScaleFloats], div_up(p.m, 64) * div_up(p.n, 64), 256, params, stream,
+                "fp8 product launch");
 }
 
 int check_weight(uint64_t w, uint64_t scale, uint32_t kind, uint32_t in_f, uint32_t out_f) {
@@ -125,6 +142,8 @@ int check_weight(uint64_t w, uint64_t scale, uint32_t kind, uint32_t in_f, uint3
   if (in_f % 16 || out_f % 16 || in_f > (1u << 20) || out_f > (1u << 20))
     return mo::set_error(MO_E_INVALID, "features must be multiples of 16, at most 2^20 (got " + std::to_string(in_f) +
                                            ", " + std::to_string(out_f) + ")");
+  // 32-bit buffer offsets
+  if ((uint64_t)in_f * out_f >= (1ull << 31)) return mo::set_error(MO_E_INVALID, "weight too large (2^31 values or more)");
   if (w % 16 || (kind == MO_FP8_SCALE_F32 && scale % 4))
     return mo::set_error(MO_E_INVALID, "misaligned weight or scale pointer");
   return 0;
@@ -246,7 +265,7 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
     p.b_scale_row = (uint32_t)div_up(in_features, kGroup), p.b_scale_col = 1, p.b_shift = 7;
     p.bias = (const void*)bias, p.out = (void*)y, p.out_kind = y_dtype;
     p.m = rows, p.n = out_features, p.r = in_features;
-    return product(m, p, scale_kind == MO_FP8_SCALE_F32, stream);
+    return product(m, p, (int)scale_kind, false, stream);
   });
 }
 
@@ -262,8 +281,8 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
     if (int rc = check_workspace(workspace, workspace_bytes, needed)) return rc;
     Module m;
     if (int rc = load_module(&m)) return rc;
-    // the weight with the reduction (out_features) contiguous
-    {
+    const bool trans = tiles(rows);
+    if (!trans) {  // the weight with the reduction (out_features) contiguous
       const void* in = (const void*)w;
       void* out = (void*)workspace;
       uint32_t r = out_features, c = in_features;
@@ -281,11 +300,12 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
     ProductArgs p = {};
     p.a = (const uint8_t*)dy, p.a_scales = (const uint8_t*)dy_scales, p.a_pitch = out_features;
     p.a_scale_pitch = (uint32_t)scale_pitch(rows);
-    p.b = (const uint8_t*)workspace, p.b_scales = (const void*)w_scale, p.b_pitch = out_features;
+    p.b = trans ? (const uint8_t*)w : (const uint8_t*)workspace;
+    p.b_scales = (const void*)w_scale, p.b_pitch = trans ? in_features : out_features;
     p.b_scale_row = 1, p.b_scale_col = (uint32_t)div_up(in_features, kGroup), p.b_shift = 7;
     p.out = (void*)dx, p.out_kind = dx_dtype;
     p.m = rows, p.n = in_features, p.r = out_features;
-    return product(m, p, scale_kind == MO_FP8_SCALE_F32, stream);
+    return product(m, p, (int)scale_kind, trans, stream);
   });
 }
 
@@ -306,7 +326,8 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     Module m;
     if (int rc = load_module(&m)) return rc;
     const uint64_t padded = div_up(rows, kGroup) * kGroup;
-    if (padded >= (1ull << 32)) return mo::set_error(MO_E_INVALID, "too many rows");
+    if (padded * 256 >= (1ull << 31))  // 32-bit buffer offsets over a tile's rows
+      return mo::set_error(MO_E_INVALID, "too many rows for one weight gradient (2^23 - 128 at most)");
     if (!dy_scales) {
       const uint64_t dv = workspace, ds = dv + align(out_features * padded);
       const uint64_t xv = workspace + col_bytes(rows, out_features), xs = xv + align(in_features * padded);
@@ -322,7 +343,7 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     p.b_scale_row = 1, p.b_scale_col = in_features, p.b_shift = 0;
     p.out = (void*)dw, p.out_kind = dw_dtype;
     p.m = out_features, p.n = in_features, p.r = (uint32_t)padded;
-    return product(m, p, false, stream);
+    return product(m, p, kScaleRows, false, stream);
   });
 }
 

@@ -44,6 +44,7 @@ using mo_fp8::kF32;
 using mo_fp8::kGroup;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -383,6 +384,19 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x16 acc, uin
 //   still fills eight whole rows.
 // The scales lie group by group, a byte a row, so that a step's are one dense piece. What lies past the rows
 // or the reduction reads as zero.
+//
+// An input gradient reads the weight as it is stored, [reduction][features]: kTrans keeps 128 rows of kBN
+// features in LDS and reads fragments with ds_read_b64_tr_b8, which hands each lane of 16 eight bytes of one
+// column (16 lanes transpose 8 rows x 16 bytes). The rows' 32-byte units are XOR-swizzled by row, so that the
+// 8 rows of a read lie on distinct banks.
+//
+// fp32 block scales (kBlockFloats): a wave's features lie in one block, so a step has one scale s = f 2^e, f
+// in [1, 2). The instructions take 2^e; the accumulators are held in units of f, multiplied by f(before) /
+// f(now) before a step's first products and by f once at the end. That keeps every factor between 1/2 and 2,
+// needs no second set of accumulators, and its multiplications run in the shadow of the MFMAs. Scales under
+// 2^-126 count as zero, an infinite one as NaN.
+//
+// kWide (fp32 outputs): operands decoded to bf16 in registers, the power-of-two scales with them.
 // Tiles are numbered in groups of kGroupM row tiles and then by XCD, so that the workgroups of one XCD
 // (blockIdx % 8) share rows and columns in its L2.
 
@@ -403,17 +417,40 @@ constexpr int kGroupM = 8, kXcds = 8;
 
 template <int WM, int WN, int TM, int TN>
 struct Tile {
-  static constexpr int kWM = WM, kTM = TM, kTN = TN, kWaves = WM * WN;
+  static constexpr int kWM = WM, kTM = TM, kTN = TN, kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int kBM = 32 * WM * TM, kBN = 32 * WN * TN;
   static constexpr int kDmaA = kBM / 8 / kWaves, kDmaB = kBN / 8 / kWaves;  // 1 KiB pieces a wave and step
   static_assert(kBM % (16 * kWaves) == 0 && kBN % (16 * kWaves) == 0, "pairs of DMA pieces divide over the waves");
   static_assert(kBM <= 256 && kBN <= 256 && kWaves >= 2, "one DMA instruction brings an operand's scales");
 };
 
-// How B's scales come: a byte a block of 128 x 128 (a wave's features lie in one block), or a byte a row.
-enum { kBlockBytes = 0, kRowBytes = 1 };
+// How B's scales come: a byte or an fp32 number a block of 128 x 128, or a byte a row.
+enum { kBlockBytes = 0, kRowBytes = 1, kBlockFloats = 2 };
 
-template <class G, int kScales>
+// Eight e4m3 bytes times a power of two as bf16: exact (four significant bits), or rounded towards zero
+// under 2^-126.
+__device__ __forceinline__ bf16x8 widen(int lo, int hi, float power) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// acc (+)= the products of one fragment pair (64 of the reduction), under the scale bytes sb and sa.
+template <bool kWide>
+__device__ __forceinline__ f32x16 products(i32x8 fb, i32x8 fa, f32x16 acc, int sb, int sa) {
+  if (!kWide) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb, fa, acc, 0, 0, 0, sb, 0, sa);
+  const float pb = __builtin_bit_cast(float, sb << 23), pa = __builtin_bit_cast(float, sa << 23);
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(fb[2 * q], fb[2 * q + 1], pb), widen(fa[2 * q], fa[2 * q + 1], pa),
+                                                  acc, 0, 0, 0);
+  return acc;
+}
+
+template <class G, int kScales, bool kWide, bool kTrans>
 __device__ __forceinline__ void product_tile(const ProductArgs& p) {
   constexpr int kBM = G::kBM, kBN = G::kBN, kTM = G::kTM, kTN = G::kTN, kDmaA = G::kDmaA, kDmaB = G::kDmaB;
   // distinct objects, chosen at compile time: the compiler then knows which reads a DMA in flight can reach
@@ -444,7 +481,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
 
   const uint32_t rows_m = (uint32_t)min((uint64_t)kBM, p.m - m0), rows_n = min((uint32_t)kBN, p.n - n0);
   const rsrc_t ra = make_rsrc(p.a + m0 * p.a_pitch, (uint32_t)(rows_m * p.a_pitch));
-  const rsrc_t rb = make_rsrc(p.b + (uint64_t)n0 * p.b_pitch, (uint32_t)(rows_n * p.b_pitch));
+  const rsrc_t rb = kTrans ? make_rsrc(p.b + n0, (uint32_t)(p.r * p.b_pitch - n0))
+                           : make_rsrc(p.b + (uint64_t)n0 * p.b_pitch, (uint32_t)(rows_n * p.b_pitch));
   const uint8_t* b_scales = (const uint8_t*)p.b_scales;
 
   // DMA: piece j of wave w is rows 8 (w kDma + j) .. + 7; lane i fills position i % 8 of row i / 8. The
@@ -457,6 +495,17 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
     dma_k[e] = 16 * ((lane & 7) ^ (4 * e + dma_row / 2));
     a_off[e] = (uint32_t)((wave * kDmaA * 8 + dma_row) * p.a_pitch + dma_k[e]);
     b_off[e] = (uint32_t)((wave * kDmaB * 8 + dma_row) * p.b_pitch + dma_k[e]);
+  }
+  // kTrans: piece j of wave w is 1024 / kBN rows of the reduction; unit(row): the row's swizzle. Four pieces on,
+  // the swizzle is the same (the rows are a multiple of 8 further).
+  auto unit = [](int row) { return kBN >= 256 ? row & 7 : kBN == 128 ? (row >> 1) & 3 : (row >> 2) & 1; };
+  constexpr int kPieceRows = 1024 / kBN, kTransOffs = kDmaB < 4 ? kDmaB : 4;
+  uint32_t t_off[kTransOffs];
+#pragma unroll
+  for (int j = 0; j < kTransOffs; ++j) {
+    const int place = (wave * kDmaB + j) * 64 + lane, row = place / (kBN / 16);
+    const int chunk = (place % (kBN / 16)) ^ (unit(row) << 1);
+    t_off[j] = n0 + 16 * chunk < p.n ? (uint32_t)(row * p.b_pitch + 16 * chunk) : kOob;
   }
   const uint32_t last_group = (p.r - 1) / kGroup;
   const bool scales_of_a = wave == 0, scales_of_b = kScales == kRowBytes && wave == 1;
@@ -486,8 +535,11 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
                                                a_off[j & 1] + 8 * j * (uint32_t)p.a_pitch, at_k, 0, 0);
 #pragma unroll
     for (int j = 0; j < kDmaB; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (MO_LDS void*)(to.b + (wave * kDmaB + j) * 1024), 16,
-                                               b_off[j & 1] + 8 * j * (uint32_t)p.b_pitch, at_k, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rb, (MO_LDS void*)(to.b + (wave * kDmaB + j) * 1024), 16,
+          kTrans ? (k < p.r ? t_off[j % kTransOffs] + j / kTransOffs * kTransOffs * kPieceRows * (uint32_t)p.b_pitch : kOob)
+                 : b_off[j & 1] + 8 * j * (uint32_t)p.b_pitch,
+          kTrans ? at_k * (int)p.b_pitch : at_k, 0, 0);
   };
 
   f32x16 acc[kTN][kTM];
@@ -500,7 +552,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
   const uint32_t n_wave = n0 + 32 * wn * kTN;
   const uint32_t block_at = n_wave < p.n ? (n_wave >> 7) * p.b_scale_row : 0;
   auto load_block = [&](uint32_t k) {
-    return (int)b_scales[block_at + (uint64_t)min(k / kGroup, last_group) * p.b_scale_col];
+    const uint64_t at = block_at + (uint64_t)min(k / kGroup, last_group) * p.b_scale_col;
+    return kScales == kBlockFloats ? ((const int*)p.b_scales)[at] : (int)b_scales[at];
   };
 
   // a lane's 32 bytes of a half h are pieces 4 h + 2 half and the next of its row
@@ -516,9 +569,22 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
     return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
   };
   auto read_a = [&](const Buffer& from, int i, int h) { fa[i] = fragment(from.a + (wm * kTM + i) * 32 * kGroup, h); };
+  const int t_row = 32 * half + ((lane & 15) >> 1);
   auto read_b = [&](const Buffer& from, int h) {
 #pragma unroll
-    for (int j = 0; j < kTN; ++j) fb[h][j] = fragment(from.b + (wn * kTN + j) * 32 * kGroup, h);
+    for (int j = 0; j < kTN; ++j) {
+      if (kTrans) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int row = t_row + 8 * q, byte = 32 * (wn * kTN + j) + 16 * ((lane >> 4) & 1) + 8 * (lane & 1);
+          const i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (MO_LDS i32x2*)(from.b + 64 * h * kBN + row * kBN + (byte ^ (unit(row) << 5))));
+          fb[h][j][2 * q] = v[0], fb[h][j][2 * q + 1] = v[1];
+        }
+      } else {
+        fb[h][j] = fragment(from.b + (wn * kTN + j) * 32 * kGroup, h);
+      }
+    }
   };
   auto read_scales = [&](const Buffer& from, int parity) {
 #pragma unroll
@@ -528,26 +594,51 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
       for (int j = 0; j < kTN; ++j) sb[parity][j] = from.sb[32 * (wn * kTN + j) + lr];
     }
   };
+  // kBlockFloats: the byte of the step's scale, and the accumulators' unit and its change
+  int block_byte = 0, a_keep = 0xff;
+  float in_units = 1.0f, change = 1.0f, poison = 0.0f;
+  auto begin = [&](int parity) {
+    if (kScales == kRowBytes) return;
+    block_byte = sb[parity][0];
+    if (kScales == kBlockFloats) {
+      const int bits = sb[parity][0];
+      block_byte = bits >> 23 & 0xff;
+      a_keep = block_byte ? 0xff : 0;  // nothing: 2^-254 of the products
+      const float f = block_byte ? __builtin_bit_cast(float, (bits & 0x807fffff) | 0x3f800000) : in_units;
+      change = in_units / f;
+      in_units = f;
+    }
+    if (kWide) poison = block_byte == 255 ? __builtin_nanf("") : poison;
+  };
   // the MFMAs of half h, and behind each row of them the fragments of the half after
   auto multiply = [&](int h, int parity, const Buffer& then) {
     constexpr int kMfma = 0x008, kDsRead = 0x100;
+    if (h == 0) begin(parity);
     read_b(then, h ^ 1);
     if (h == 1) read_scales(then, parity ^ 1);
 #pragma unroll
     for (int i = 0; i < kTM; ++i) {
 #pragma unroll
       for (int j = 0; j < kTN; ++j)
-        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-            fb[h][j], fa[i], acc[j][i], 0, 0, 0, kScales == kRowBytes ? sb[parity][j] : sb[parity][0], 0, sa[parity][i]);
+      {
+        if (kScales == kBlockFloats && h == 0) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[j][i][e] *= change;
+        }
+        acc[j][i] = products<kWide>(fb[h][j], fa[i], acc[j][i], kScales == kRowBytes ? sb[parity][j] : block_byte,
+                                    kScales == kBlockFloats ? sa[parity][i] & a_keep : sa[parity][i]);
+      }
       read_a(then, i, h ^ 1);
     }
-    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kTN, 0);
-    __builtin_amdgcn_sched_group_barrier(kMfma, kTN - 1, 0);
+    if (!kWide && kScales != kBlockFloats) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, (kTrans ? 4 : 2) * kTN, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, kTN - 1, 0);
 #pragma unroll
-    for (int i = 0; i < kTM; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(kMfma, kTN, 0);
+      for (int i = 0; i < kTM; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, kTN, 0);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -557,13 +648,13 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
     int after = 0;
-    if (kScales == kBlockBytes) after = load_block(k + 2 * kGroup);
+    if (kScales != kRowBytes) after = load_block(k + 2 * kGroup);
     dma(now, k + 2 * kGroup);
     multiply(1, parity, next);
-    if (kScales == kBlockBytes) sb[parity][0] = after;
+    if (kScales != kRowBytes) sb[parity][0] = after;
   };
 
-  if (kScales == kBlockBytes) sb[0][0] = load_block(0), sb[1][0] = load_block(kGroup);
+  if (kScales != kRowBytes) sb[0][0] = load_block(0), sb[1][0] = load_block(kGroup);
   dma(buf0, 0);
   dma(buf1, kGroup);
   __builtin_amdgcn_s_waitcnt(wait_vm(kDmaA + kDmaB + 1 + (kScales == kRowBytes ? 1 : 0)));
@@ -578,65 +669,88 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
     step(1, buf1, buf0, k + kGroup);
   }
 
-  // Epilogue: 32 tokens at a time through a part of LDS of the wave's own, so that a store writes whole
-  // rows of the wave's features instead of pieces of 32 rows. 16-byte piece c of row r at c ^ (r %
-  // kPieces): writes and reads spread over the banks.
-  constexpr int kLine = 32 * kTN * 2, kPieces = kLine / 16, kRowsAStore = 64 / kPieces;
+  // Epilogue: 32 tokens by 128 bytes of features at a time through a part of LDS of the wave's own, so that a
+  // store writes whole lines instead of pieces of 32 rows. 16-byte piece c of row r at c ^ (r % 8): writes
+  // and reads spread over the banks.
+  constexpr int kAcross = kWide ? 1 : kTN;  // MFMA tiles of a line
+  constexpr int kLine = 32 * kAcross * (kWide ? 4 : 2), kPieces = kLine / 16, kRowsAStore = 64 / kPieces;
   static_assert(32 * kLine * G::kWaves <= kBM * (int)kGroup, "a wave's part of the first buffer");
   __builtin_amdgcn_s_waitcnt(wait_vm(0));
   __syncthreads();  // every wave has read its last fragments, every DMA has landed
   lp own = (lp)a_0 + wave * 32 * kLine;
   const int out_row = lane / kPieces, piece = lane % kPieces;
   const bool f16 = p.out_kind != kBF16;
-  const rsrc_t ro = make_rsrc((uint16_t*)p.out + m0 * p.n, (uint32_t)(rows_m * p.n * 2));
+  constexpr int kBytes = kWide ? 4 : 2, kValues = 16 / kBytes;
+  const rsrc_t ro = make_rsrc((uint8_t*)p.out + m0 * p.n * kBytes, (uint32_t)(rows_m * p.n * kBytes));
 #pragma unroll
-  for (int i = 0; i < kTM; ++i) {
+  for (int i = 0; i < kTM; ++i)
 #pragma unroll
-    for (int j = 0; j < kTN; ++j)
+    for (int j0 = 0; j0 < kTN; j0 += kAcross) {
+      const uint32_t n_line = n_wave + 32 * j0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x16& w16 = acc[j][i];
-        float o[4] = {w16[4 * q], w16[4 * q + 1], w16[4 * q + 2], w16[4 * q + 3]};
-        if (p.bias) {
-          const uint32_t n = n_wave + 32 * j + 8 * q + 4 * half;
+      for (int j = 0; j < kAcross; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] += n < p.n ? load1(p.bias, n + e, p.out_kind) : 0.0f;
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& w16 = acc[j0 + j][i];
+          f32x4 o = {w16[4 * q], w16[4 * q + 1], w16[4 * q + 2], w16[4 * q + 3]};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (kScales == kBlockFloats) o[e] *= in_units;
+            if (kWide && kScales != kRowBytes) o[e] += poison;
+          }
+          if (p.bias) {
+            const uint32_t n = n_line + 32 * j + 8 * q + 4 * half;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += n < p.n ? load1(p.bias, n + e, p.out_kind) : 0.0f;
+          }
+          if (kWide) {
+            *(MO_LDS f32x4*)(own + lr * kLine + 16 * ((2 * q + half) ^ (lr % kPieces))) = o;
+          } else {
+            u32x2 w;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+              typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+              w[e] = f16 ? __builtin_bit_cast(uint32_t, f16x2{(_Float16)o[2 * e], (_Float16)o[2 * e + 1]})
+                         : __builtin_bit_cast(uint32_t, bf16x2{(__bf16)o[2 * e], (__bf16)o[2 * e + 1]});
+            }
+            *(MO_LDS u32x2*)(own + lr * kLine + 16 * ((4 * j + q) ^ (lr % kPieces)) + 8 * half) = w;
+          }
         }
-        u32x2 w;
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-          typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-          w[e] = f16 ? __builtin_bit_cast(uint32_t, f16x2{(_Float16)o[2 * e], (_Float16)o[2 * e + 1]})
-                     : __builtin_bit_cast(uint32_t, bf16x2{(__bf16)o[2 * e], (__bf16)o[2 * e + 1]});
-        }
-        *(MO_LDS u32x2*)(own + lr * kLine + 16 * ((4 * j + q) ^ (lr % kPieces)) + 8 * half) = w;
+      for (int r = 0; r < 32; r += kRowsAStore) {
+        const int row = r + out_row;
+        const u32x4 w = *(const MO_LDS u32x4*)(own + row * kLine + 16 * (piece ^ (row % kPieces)));
+        const uint32_t n = n_line + kValues * piece;
+        const uint32_t to = ((uint32_t)(32 * (wm * kTM + i) + row) * p.n + n) * kBytes;
+        __builtin_amdgcn_raw_buffer_store_b128(w, ro, (int)(n < p.n ? to : kOob), 0, 0);
       }
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int r = 0; r < 32; r += kRowsAStore) {
-      const int row = r + out_row;
-      const u32x4 w = *(const MO_LDS u32x4*)(own + row * kLine + 16 * (piece ^ (row % kPieces)));
-      const uint32_t to = ((uint32_t)(32 * (wm * kTM + i) + row) * p.n + n_wave + 8 * piece) * 2;
-      __builtin_amdgcn_raw_buffer_store_b128(w, ro, (int)(n_wave + 8 * piece < p.n ? to : kOob), 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_wave_barrier();
-  }
 }
 
-#define MO_TILE(name, WM, WN, TM, TN)                                                                              \
-  extern "C" __global__ __launch_bounds__(64 * WM * WN, 1) void mo_fp8_product_##name(ProductArgs p) {             \
-    product_tile<Tile<WM, WN, TM, TN>, kBlockBytes>(p);                                                            \
-  }                                                                                                                \
-  extern "C" __global__ __launch_bounds__(64 * WM * WN, 1) void mo_fp8_product_rows_##name(ProductArgs p) {        \
-    product_tile<Tile<WM, WN, TM, TN>, kRowBytes>(p);                                                              \
+#define MO_TILE_KERNEL(name, G, scales, wide, trans)                                                        \
+  extern "C" __global__ __launch_bounds__(G::kThreads) void mo_fp8_product_##name(ProductArgs p) {          \
+    product_tile<G, scales, wide, trans>(p);                                                                \
   }
-MO_TILE(256x256, 2, 4, 4, 2)
+#define MO_TILE(name, G)                                            \
+  MO_TILE_KERNEL(name##_bytes, G, kBlockBytes, false, false)        \
+  MO_TILE_KERNEL(name##_floats, G, kBlockFloats, false, false)      \
+  MO_TILE_KERNEL(name##_rows, G, kRowBytes, false, false)           \
+  MO_TILE_KERNEL(name##_bytes_t, G, kBlockBytes, false, true)       \
+  MO_TILE_KERNEL(name##_floats_t, G, kBlockFloats, false, true)     \
+  MO_TILE_KERNEL(name##_bytes_w, G, kBlockBytes, true, false)       \
+  MO_TILE_KERNEL(name##_floats_w, G, kBlockFloats, true, false)     \
+  MO_TILE_KERNEL(name##_rows_w, G, kRowBytes, true, false)          \
+  MO_TILE_KERNEL(name##_bytes_tw, G, kBlockBytes, true, true)       \
+  MO_TILE_KERNEL(name##_floats_tw, G, kBlockFloats, true, true)
+typedef Tile<2, 4, 4, 2> Large;
+MO_TILE(large, Large)
 
-// Eight e4m3 bytes times a power of two as bf16: exact (four significant bits).
-__device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float scale) {
+__device__ __forceinline__ bf16x8 widen_plain(uint32_t lo, uint32_t hi, float scale) {
   bf16x8 o;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -683,8 +797,8 @@ __device__ __forceinline__ void product_plain(const ProductArgs& p) {
         const float xa = scale_value((uint32_t)sa), xb = scale_value((uint32_t)sb);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(fb[2 * q], fb[2 * q + 1], xb),
-                                                        widen(fa[2 * q], fa[2 * q + 1], xa), sum, 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen_plain(fb[2 * q], fb[2 * q + 1], xb),
+                                                        widen_plain(fa[2 * q], fa[2 * q + 1], xa), sum, 0, 0, 0);
       } else {
         sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb, fa, sum, 0, 0, 0, sb, 0, sa);
       }
