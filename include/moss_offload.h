@@ -575,7 +575,7 @@ int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t sca
  * `dtype` that the call quantizes along its rows, or (x_scales not 0) row_values and row_scales of
  * mo_fp8_quantize. w: e4m3 [out][in], w_scale [ceil(out / 128)][ceil(in / 128)], E8M0 or any fp32. bias:
  * [out] in y's type, or 0. `workspace`: 256-byte aligned, at least mo_fp8_workspace_bytes(MO_FP8_FORWARD,
- * rows, in, out, x_scales != 0) bytes. */
+ * rows, in, out, x_scales != 0, scale_kind, y_dtype) bytes. */
 int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_t rows, uint32_t in_features,
                           uint64_t row_stride, uint64_t w, uint64_t w_scale, uint32_t scale_kind,
                           uint32_t out_features, uint64_t bias, uint64_t y, uint32_t y_dtype, uint64_t workspace,
@@ -594,8 +594,17 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
                            uint32_t in_features, uint32_t out_features, uint64_t dw, uint32_t dw_dtype,
                            uint64_t workspace, uint64_t workspace_bytes, uint64_t stream);
 
+/* Bytes of a call's workspace on the current device: the operands it quantizes, and the fp32 planes of a
+ * reduction that its plan shares out over workgroups. `quantized`: the operands are given so; out_dtype: the
+ * result's. */
 uint64_t mo_fp8_workspace_bytes(uint32_t op, uint64_t rows, uint32_t in_features, uint32_t out_features,
-                                uint32_t quantized);
+                                uint32_t quantized, uint32_t scale_kind, uint32_t out_dtype);
+
+/* The plan of a product [rows][cols] from a `reduction` on a device of `cus` CUs, host only: plan[0..2] = the
+ * tile's edge, splits (workgroups a tile), groups of 128 of the reduction a split. The same call gives the
+ * same bits every time. For tests and tools. */
+int mo_fp8_plan(uint64_t rows, uint32_t cols, uint32_t reduction, uint32_t scale_kind, uint32_t out_dtype, uint32_t cus,
+                uint32_t* plan);
 
 /* ---- rotary positions (training/model.py:41-56, 136-151), with the heads' RMS norm (:154-172) -- */
 

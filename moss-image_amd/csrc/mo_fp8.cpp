@@ -31,13 +31,39 @@ constexpr uint32_t kTypeBytes[3] = {2, 2, 4};
 enum { kScaleBytes = MO_FP8_SCALE_E8M0, kScaleFloats = MO_FP8_SCALE_F32, kScaleRows = 2 };
 const char* const kScaleNames[3] = {"bytes", "floats", "rows"};
 
+// The tiles (mo_fp8.hip): edge, workgroups that fit a CU, and what the cost model knows of them on an MI355X,
+// in us, for 16-bit outputs, 16-bit outputs with fp32 block scales, and fp32 outputs: a call's fixed part, what
+// a further round of workgroups adds of it, and a step of 128 of the reduction with one workgroup on a CU and
+// with all that fit. Fitted to 12 400 timed calls (110 shapes of 1 to 17 792 rows, every tile, 1 to 32
+// splits, eight kinds of operands, replayed back to back): the model's choice takes 1 % longer than the
+// fastest one on average, 4 % at the ninetieth percentile, 31 % at worst (199 rows of 3072 from 24576).
+struct Cost {
+  double fixed, again, alone, together;
+};
+struct TileShape {
+  const char* name;
+  uint32_t edge, threads;
+  int resident;
+  Cost cost[3];  // [kCostNarrow ..]
+};
+enum { kCostNarrow, kCostFloats, kCostWide };
+constexpr int kTiles = 3;
+constexpr TileShape kTileShapes[kTiles] = {
+    {"large", 256, 512, 1, {{6.2, 0.86, 1.10, 1.10}, {7.0, 0.79, 1.48, 1.48}, {6.4, 0.79, 2.27, 2.27}}},
+    {"middle", 128, 256, 2, {{4.1, 0.63, 0.54, 0.91}, {4.5, 0.46, 0.78, 1.19}, {4.5, 0.19, 0.91, 1.64}}},
+    {"small", 64, 256, 4, {{3.1, 0.31, 0.32, 0.92}, {3.2, 0.32, 0.37, 1.00}, {3.2, 0.19, 0.44, 1.21}}},
+};
+// The sum of a split call's planes: fixed, a plane, a MB of planes.
+constexpr double kSumFixed = 1.1, kSumPlane = 0.26, kSumMb = 0.32;
+constexpr uint32_t kMaxSplits = 32, kMinSplitSteps = 2;
+constexpr uint64_t kMaxPlanes = 1ull << 31;  // bytes
+
 struct Module {
   hipModule_t module = nullptr;
   int cus = 0;
   hipFunction_t quantize[kForms][3] = {};
-  hipFunction_t decode = nullptr, transpose = nullptr;
-  hipFunction_t large[3][2][2] = {};  // [scales][fp32 output][transposed]
-  hipFunction_t plain[2][2] = {};  // [fp32 output][fp32 scales]
+  hipFunction_t decode = nullptr, sum = nullptr;
+  hipFunction_t product[kTiles][3][2][2] = {};  // [tile][scales][fp32 output][weight as stored]
 };
 
 std::mutex g_mu;
@@ -58,19 +84,18 @@ int load_module(Module* out) {
     auto get = [&](hipFunction_t* fn, const std::string& name) {
       return (e = hipModuleGetFunction(fn, m.module, name.c_str())) == hipSuccess;
     };
-    bool ok = get(&m.decode, "mo_fp8_decode_kernel") && get(&m.transpose, "mo_fp8_transpose_kernel") &&
-              get(&m.plain[0][0], "mo_fp8_product_plain") && get(&m.plain[0][1], "mo_fp8_product_plain_f32") &&
-              get(&m.plain[1][0], "mo_fp8_product_plain_wide") && get(&m.plain[1][1], "mo_fp8_product_plain_wide_f32");
+    bool ok = get(&m.decode, "mo_fp8_decode_kernel") && get(&m.sum, "mo_fp8_plane_sum");
     for (int f = 0; f < kForms; ++f)
       for (int t = 0; t < 3; ++t)
         ok = ok && get(&m.quantize[f][t], std::string("mo_fp8_quantize_") + kFormNames[f] + "_" + kTypeNames[t]);
-    for (int k = 0; k < 3; ++k)
-      for (int wide = 0; wide < 2; ++wide)
-        for (int trans = 0; trans < (k == kScaleRows ? 1 : 2); ++trans) {
-          std::string name = std::string("mo_fp8_product_large_") + kScaleNames[k];
-          if (trans || wide) name += std::string("_") + (trans ? "t" : "") + (wide ? "w" : "");
-          ok = ok && get(&m.large[k][wide][trans], name);
-        }
+    for (int tile = 0; tile < kTiles; ++tile)
+      for (int k = 0; k < 3; ++k)
+        for (int wide = 0; wide < 2; ++wide)
+          for (int trans = 0; trans < (k == kScaleRows ? 1 : 2); ++trans) {
+            std::string name = std::string("mo_fp8_product_") + kTileShapes[tile].name + "_" + kScaleNames[k];
+            if (trans || wide) name += std::string("_") + (trans ? "t" : "") + (wide ? "w" : "");
+            ok = ok && get(&m.product[tile][k][wide][trans], name);
+          }
     if (!ok) return mo::set_hip_error((int)e, "hipModuleGetFunction (fp8)");
     it = g_modules.emplace(device, m).first;
   }
@@ -120,19 +145,61 @@ int quantize(const Module& m, Form form, uint64_t x, uint32_t dtype, uint64_t ro
                 "fp8 quantize launch");
 }
 
-// Whether a call of `rows` runs on the tiles (below, on the plain kernel, whose second operand lies along the
-// reduction).
-bool tiles(uint64_t rows) { return rows > 256; }
+struct Plan {
+  int tile;
+  uint32_t splits, split_steps;
+};
 
-int product(const Module& m, const ProductArgs& p, int scales, bool trans, uint64_t stream) {
-  ProductArgs args = p;
-  void* params[] = {&args};
-  const bool wide = p.out_kind == MO_DTYPE_F32;
-  if (tiles(p.m))
-    return launch(m.large[scales][wide][trans], div_up(p.m, 256) * div_up(p.n, 256), 512, params, stream,
-                  "fp8 product launch");
-  return launch(m.plain[wide][scales == kScaleFloats], div_up(p.m, 64) * div_up(p.n, 64), 256, params, stream,
-                "fp8 product launch");
+// Modelled time (us) of a call whose reduction is shared out over `splits` workgroups a tile, `per` steps each.
+double cost_of(const TileShape& t, const Cost& c, uint64_t rows, uint64_t cols, uint32_t splits, uint32_t per, int cus) {
+  const uint64_t each = div_up(div_up(rows, t.edge) * div_up(cols, t.edge) * splits, (uint64_t)cus);
+  const uint64_t full = each / t.resident, left = each % t.resident;
+  const uint32_t steps = (per + 1) & ~1u;  // the loop runs steps in pairs
+  double step = (double)full * c.together;
+  if (left) step += c.alone + (t.resident > 1 ? (c.together - c.alone) * (double)(left - 1) / (t.resident - 1) : 0.0);
+  double us = c.fixed * (1 + c.again * (double)(full + (left > 0) - 1)) + steps * step;
+  if (splits > 1) us += kSumFixed + kSumPlane * splits + kSumMb * (double)splits * (double)rows * (double)cols * 4e-6;
+  return us;
+}
+
+Plan plan_of(uint64_t rows, uint64_t cols, uint32_t steps, int kind, int cus) {
+  Plan best{0, 1, steps};
+  double best_us = 0;
+  for (int i = 0; i < kTiles; ++i) {
+    const TileShape& t = kTileShapes[i];
+    uint32_t tried = 0;
+    for (uint32_t want = 1; want <= kMaxSplits; ++want) {
+      if (want > 1 && (steps / want < kMinSplitSteps || want * rows * cols * 4 > kMaxPlanes)) break;
+      const uint32_t per = (uint32_t)div_up(steps, want), splits = (uint32_t)div_up(steps, per);
+      if (splits == tried) continue;
+      tried = splits;
+      const double us = cost_of(t, t.cost[kind], rows, cols, splits, per, cus);
+      if (best_us == 0 || us < best_us) best = Plan{i, splits, per}, best_us = us;
+    }
+  }
+  return best;
+}
+
+int cost_kind(int scales, uint32_t out_kind) {
+  return out_kind == MO_DTYPE_F32 ? kCostWide : scales == kScaleFloats ? kCostFloats : kCostNarrow;
+}
+
+uint64_t plane_bytes(const Plan& p, uint64_t rows, uint64_t cols) {
+  return p.splits > 1 ? align(p.splits * rows * cols * 4) : 0;
+}
+
+// `planes`: room for plane_bytes of the plan of this call.
+int product(const Module& m, ProductArgs p, int scales, bool trans, uint64_t planes, uint64_t stream) {
+  const Plan plan = plan_of(p.m, p.n, (uint32_t)div_up(p.r, kGroup), cost_kind(scales, p.out_kind), m.cus);
+  const TileShape& t = kTileShapes[plan.tile];
+  p.splits = plan.splits, p.split_steps = plan.split_steps, p.planes = plan.splits > 1 ? (float*)planes : nullptr;
+  void* params[] = {&p};
+  if (int rc = launch(m.product[plan.tile][scales][p.out_kind == MO_DTYPE_F32][trans],
+                      div_up(p.m, t.edge) * div_up(p.n, t.edge) * plan.splits, t.threads, params, stream,
+                      "fp8 product launch"))
+    return rc;
+  if (plan.splits == 1) return 0;
+  return launch(m.sum, div_up(p.m * p.n / 4, 256), 256, params, stream, "fp8 plane sum launch");
 }
 
 int check_weight(uint64_t w, uint64_t scale, uint32_t kind, uint32_t in_f, uint32_t out_f) {
@@ -177,11 +244,25 @@ uint64_t col_bytes(uint64_t rows, uint64_t cols) {
   return align(cols * div_up(rows, kGroup) * kGroup) + align(div_up(rows, kGroup) * cols);
 }
 
-uint64_t workspace_of(uint32_t op, uint64_t rows, uint64_t in_f, uint64_t out_f, bool quantized) {
-  if (op == MO_FP8_FORWARD) return quantized ? 0 : row_bytes(rows, in_f);
-  if (op == MO_FP8_BACKWARD) return (quantized ? 0 : row_bytes(rows, out_f)) + align(in_f * out_f);
-  if (op == MO_FP8_WEIGHT) return quantized ? 0 : col_bytes(rows, out_f) + col_bytes(rows, in_f);
-  return 0;
+// A call's workspace: the operands it quantizes, then its planes.
+struct Room {
+  uint64_t operands, planes;
+  uint64_t bytes() const { return operands + planes; }
+};
+
+Room room_of(uint32_t op, uint64_t rows, uint64_t in_f, uint64_t out_f, bool quantized, uint32_t scale_kind,
+             uint32_t out_kind, int cus) {
+  Room r = {};
+  const uint64_t m = op == MO_FP8_WEIGHT ? out_f : rows, n = op == MO_FP8_FORWARD ? out_f : in_f;
+  const uint64_t reduction = op == MO_FP8_FORWARD ? in_f : op == MO_FP8_BACKWARD ? out_f : rows;
+  if (!quantized) {
+    if (op == MO_FP8_FORWARD) r.operands = row_bytes(rows, in_f);
+    if (op == MO_FP8_BACKWARD) r.operands = row_bytes(rows, out_f);
+    if (op == MO_FP8_WEIGHT) r.operands = col_bytes(rows, out_f) + col_bytes(rows, in_f);
+  }
+  const int scales = op == MO_FP8_WEIGHT ? kScaleRows : (int)scale_kind;
+  r.planes = plane_bytes(plan_of(m, n, (uint32_t)div_up(reduction, kGroup), cost_kind(scales, out_kind), cus), m, n);
+  return r;
 }
 
 }  // namespace
@@ -189,8 +270,29 @@ uint64_t workspace_of(uint32_t op, uint64_t rows, uint64_t in_f, uint64_t out_f,
 extern "C" {
 
 uint64_t mo_fp8_workspace_bytes(uint32_t op, uint64_t rows, uint32_t in_features, uint32_t out_features,
-                                uint32_t quantized) {
-  return rows ? workspace_of(op, rows, in_features, out_features, quantized != 0) : 0;
+                                uint32_t quantized, uint32_t scale_kind, uint32_t out_dtype) {
+  if (op > MO_FP8_WEIGHT || rows == 0 || rows >= (1ull << 31) || in_features == 0 || out_features == 0 ||
+      scale_kind > MO_FP8_SCALE_F32 || out_dtype > MO_DTYPE_F32)
+    return 0;
+  uint64_t bytes = 0;
+  const int rc = guarded([&]() -> int {
+    Module m;
+    if (int bad = load_module(&m)) return bad;
+    bytes = room_of(op, rows, in_features, out_features, quantized != 0, scale_kind, out_dtype, m.cus).bytes();
+    return 0;
+  });
+  return rc ? 0 : bytes;
+}
+
+int mo_fp8_plan(uint64_t rows, uint32_t cols, uint32_t reduction, uint32_t scale_kind, uint32_t out_dtype, uint32_t cus,
+                uint32_t* plan) {
+  if (!plan) return mo::set_error(MO_E_INVALID, "null output pointer");
+  if (rows == 0 || rows >= (1ull << 31) || cols == 0 || reduction == 0 || cus == 0)
+    return mo::set_error(MO_E_INVALID, "empty shape, or too many rows");
+  if (scale_kind > MO_FP8_SCALE_F32 || out_dtype > MO_DTYPE_F32) return mo::set_error(MO_E_INVALID, "unknown type");
+  const Plan p = plan_of(rows, cols, (uint32_t)div_up(reduction, kGroup), cost_kind((int)scale_kind, out_dtype), (int)cus);
+  plan[0] = kTileShapes[p.tile].edge, plan[1] = p.splits, plan[2] = p.split_steps;
+  return 0;
 }
 
 int mo_fp8_quantize(uint64_t x, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t row_stride, uint64_t row_values,
@@ -248,10 +350,11 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
     if (int rc = check_weight(w, w_scale, scale_kind, in_features, out_features)) return rc;
     if (int rc = check_operand(x, x_scales, dtype, rows, in_features, row_stride)) return rc;
     if (int rc = check_output(y, y_dtype, bias)) return rc;
-    const uint64_t needed = workspace_of(MO_FP8_FORWARD, rows, in_features, out_features, x_scales != 0);
-    if (int rc = check_workspace(workspace, workspace_bytes, needed)) return rc;
     Module m;
     if (int rc = load_module(&m)) return rc;
+    const Room room =
+        room_of(MO_FP8_FORWARD, rows, in_features, out_features, x_scales != 0, scale_kind, y_dtype, m.cus);
+    if (int rc = check_workspace(workspace, workspace_bytes, room.bytes())) return rc;
     if (!x_scales) {
       const uint64_t scales = workspace + align(rows * in_features);
       if (int rc = quantize(m, kFormRows, x, dtype, rows, in_features, row_stride, workspace, scales, 0, 0, stream))
@@ -265,7 +368,7 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
     p.b_scale_row = (uint32_t)div_up(in_features, kGroup), p.b_scale_col = 1, p.b_shift = 7;
     p.bias = (const void*)bias, p.out = (void*)y, p.out_kind = y_dtype;
     p.m = rows, p.n = out_features, p.r = in_features;
-    return product(m, p, (int)scale_kind, false, stream);
+    return product(m, p, (int)scale_kind, false, workspace + room.operands, stream);
   });
 }
 
@@ -277,22 +380,13 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
     if (int rc = check_weight(w, w_scale, scale_kind, in_features, out_features)) return rc;
     if (int rc = check_operand(dy, dy_scales, dtype, rows, out_features, row_stride)) return rc;
     if (int rc = check_output(dx, dx_dtype, 0)) return rc;
-    const uint64_t needed = workspace_of(MO_FP8_BACKWARD, rows, in_features, out_features, dy_scales != 0);
-    if (int rc = check_workspace(workspace, workspace_bytes, needed)) return rc;
     Module m;
     if (int rc = load_module(&m)) return rc;
-    const bool trans = tiles(rows);
-    if (!trans) {  // the weight with the reduction (out_features) contiguous
-      const void* in = (const void*)w;
-      void* out = (void*)workspace;
-      uint32_t r = out_features, c = in_features;
-      void* params[] = {&in, &out, &r, &c};
-      if (int rc = launch(m.transpose, div_up(r, 128) * div_up(c, 128), 256, params, stream, "fp8 transpose launch"))
-        return rc;
-    }
+    const Room room =
+        room_of(MO_FP8_BACKWARD, rows, in_features, out_features, dy_scales != 0, scale_kind, dx_dtype, m.cus);
+    if (int rc = check_workspace(workspace, workspace_bytes, room.bytes())) return rc;
     if (!dy_scales) {
-      const uint64_t values = workspace + align((uint64_t)in_features * out_features);
-      const uint64_t scales = values + align(rows * out_features);
+      const uint64_t values = workspace, scales = workspace + align(rows * out_features);
       if (int rc = quantize(m, kFormRows, dy, dtype, rows, out_features, row_stride, values, scales, 0, 0, stream))
         return rc;
       dy = values, dy_scales = scales;
@@ -300,12 +394,11 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
     ProductArgs p = {};
     p.a = (const uint8_t*)dy, p.a_scales = (const uint8_t*)dy_scales, p.a_pitch = out_features;
     p.a_scale_pitch = (uint32_t)scale_pitch(rows);
-    p.b = trans ? (const uint8_t*)w : (const uint8_t*)workspace;
-    p.b_scales = (const void*)w_scale, p.b_pitch = trans ? in_features : out_features;
+    p.b = (const uint8_t*)w, p.b_scales = (const void*)w_scale, p.b_pitch = in_features;  // as stored
     p.b_scale_row = 1, p.b_scale_col = (uint32_t)div_up(in_features, kGroup), p.b_shift = 7;
     p.out = (void*)dx, p.out_kind = dx_dtype;
     p.m = rows, p.n = in_features, p.r = out_features;
-    return product(m, p, (int)scale_kind, trans, stream);
+    return product(m, p, (int)scale_kind, true, workspace + room.operands, stream);
   });
 }
 
@@ -321,13 +414,14 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     if (int rc = check_operand(dy, dy_scales, dy_dtype, rows, out_features, dy_stride)) return rc;
     if (int rc = check_operand(x, x_scales, x_dtype, rows, in_features, x_stride)) return rc;
     if (int rc = check_output(dw, dw_dtype, 0)) return rc;
-    const uint64_t needed = workspace_of(MO_FP8_WEIGHT, rows, in_features, out_features, dy_scales != 0);
-    if (int rc = check_workspace(workspace, workspace_bytes, needed)) return rc;
-    Module m;
-    if (int rc = load_module(&m)) return rc;
     const uint64_t padded = div_up(rows, kGroup) * kGroup;
     if (padded * 256 >= (1ull << 31))  // 32-bit buffer offsets over a tile's rows
       return mo::set_error(MO_E_INVALID, "too many rows for one weight gradient (2^23 - 128 at most)");
+    Module m;
+    if (int rc = load_module(&m)) return rc;
+    const Room room = room_of(MO_FP8_WEIGHT, rows, in_features, out_features, dy_scales != 0, MO_FP8_SCALE_E8M0,
+                              dw_dtype, m.cus);
+    if (int rc = check_workspace(workspace, workspace_bytes, room.bytes())) return rc;
     if (!dy_scales) {
       const uint64_t dv = workspace, ds = dv + align(out_features * padded);
       const uint64_t xv = workspace + col_bytes(rows, out_features), xs = xv + align(in_features * padded);
@@ -343,7 +437,7 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     p.b_scale_row = 1, p.b_scale_col = in_features, p.b_shift = 0;
     p.out = (void*)dw, p.out_kind = dw_dtype;
     p.m = out_features, p.n = in_features, p.r = (uint32_t)padded;
-    return product(m, p, kScaleRows, false, stream);
+    return product(m, p, kScaleRows, false, workspace + room.operands, stream);
   });
 }
 

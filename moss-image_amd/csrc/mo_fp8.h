@@ -20,6 +20,10 @@ struct ProductArgs {
   uint32_t n, r;
   uint32_t a_scale_pitch, b_scale_row, b_scale_col, b_shift;
   uint32_t out_kind;
+  // the reduction shared out over workgroups: each takes split_steps groups of it and leaves fp32 sums in its
+  // plane, [splits][m][n]; out and bias are then the sum kernel's. splits 1: planes is null
+  uint32_t splits, split_steps;
+  float* planes;
 };
 
 }  // namespace mo_fp8

@@ -317,57 +317,7 @@ extern "C" __global__ __launch_bounds__(256) void mo_fp8_decode_kernel(
   }
 }
 
-// out[c][r] = in[r][c], bytes; rows and cols multiples of 16. A tile of 128 x 128 through LDS.
-extern "C" __global__ __launch_bounds__(256) void mo_fp8_transpose_kernel(const uint8_t* __restrict__ in,
-                                                                          uint8_t* __restrict__ out, uint32_t rows,
-                                                                          uint32_t cols) {
-  constexpr int kLine = 128 + 4;
-  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * kLine];
-  const uint32_t tiles_c = (cols + 127) / 128;
-  const uint32_t r0 = blockIdx.x / tiles_c * 128, c0 = blockIdx.x % tiles_c * 128;
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t r = (tid >> 3) + 32 * i, c = (tid & 7) * 16;
-    u32x4 v = {};
-    if (r0 + r < rows && c0 + c < cols) v = *(const u32x4*)(in + (uint64_t)(r0 + r) * cols + c0 + c);
-    uint32_t* to = (uint32_t*)(tile + r * kLine + c);
-    to[0] = v[0], to[1] = v[1], to[2] = v[2], to[3] = v[3];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t c = (tid & 31) + 32 * i, r = (tid >> 5) * 16;
-    if (c0 + c >= cols || r0 + r >= rows) continue;
-    u32x4 v;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      uint32_t x = 0;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) x |= (uint32_t)tile[(r + 4 * w + b) * kLine + c] << (8 * b);
-      v[w] = x;
-    }
-    *(u32x4*)(out + (uint64_t)(c0 + c) * rows + r0 + r) = v;
-  }
-}
-
 // ---- products -------------------------------------------------------------------------------------
-
-// Output of one 32 x 32 tile: a lane holds token m and features n0 + 8 (r / 4) + 4 (l / 32) + r % 4.
-__device__ __forceinline__ void store_tile(const ProductArgs& p, f32x16 acc, uint64_t m, uint32_t n0, int half) {
-  if (m >= p.m) return;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint32_t n = n0 + 8 * q + 4 * half;
-    if (n >= p.n) continue;  // p.n is a multiple of 16
-    f32x4 v = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-    if (p.bias) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += load1(p.bias, n + i, p.out_kind);
-    }
-    store4(p.out, m * p.n + n, v, p.out_kind);
-  }
-}
 
 // ---- tiles in LDS ----
 //
@@ -467,13 +417,17 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % G::kWM, wn = wave / G::kWM;
 
-  const int tiles = gridDim.x, tiles_m = (int)((p.m + kBM - 1) / kBM), tiles_n = tiles / tiles_m;
+  const int items = gridDim.x, tiles = items / p.splits;
+  const int tiles_m = (int)((p.m + kBM - 1) / kBM), tiles_n = tiles / tiles_m;
   int t;
   {
     const int b = blockIdx.x, xcd = b % kXcds, idx = b / kXcds;
-    const int per = tiles / kXcds, rem = tiles % kXcds;
+    const int per = items / kXcds, rem = items % kXcds;
     t = xcd < rem ? xcd * (per + 1) + idx : rem * (per + 1) + (xcd - rem) * per + idx;
   }
+  const int split = t / tiles;
+  t -= split * tiles;
+  const uint32_t k_begin = split * p.split_steps * kGroup, k_end = min(p.r, k_begin + p.split_steps * kGroup);
   const int group_tiles = kGroupM * tiles_n, first_m = t / group_tiles * kGroupM;
   const int gm = min(tiles_m - first_m, kGroupM), in_group = t % group_tiles;
   const uint64_t m0 = (uint64_t)(first_m + in_group % gm) * kBM;
@@ -496,30 +450,28 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
     a_off[e] = (uint32_t)((wave * kDmaA * 8 + dma_row) * p.a_pitch + dma_k[e]);
     b_off[e] = (uint32_t)((wave * kDmaB * 8 + dma_row) * p.b_pitch + dma_k[e]);
   }
-  // kTrans: piece j of wave w is 1024 / kBN rows of the reduction; unit(row): the row's swizzle. Four pieces on,
-  // the swizzle is the same (the rows are a multiple of 8 further).
+  // kTrans: piece j of wave w is 1024 / kBN rows of the reduction; unit(row): the row's swizzle
   auto unit = [](int row) { return kBN >= 256 ? row & 7 : kBN == 128 ? (row >> 1) & 3 : (row >> 2) & 1; };
-  constexpr int kPieceRows = 1024 / kBN, kTransOffs = kDmaB < 4 ? kDmaB : 4;
-  uint32_t t_off[kTransOffs];
+  uint32_t t_off[kDmaB];
 #pragma unroll
-  for (int j = 0; j < kTransOffs; ++j) {
+  for (int j = 0; j < kDmaB; ++j) {
     const int place = (wave * kDmaB + j) * 64 + lane, row = place / (kBN / 16);
     const int chunk = (place % (kBN / 16)) ^ (unit(row) << 1);
     t_off[j] = n0 + 16 * chunk < p.n ? (uint32_t)(row * p.b_pitch + 16 * chunk) : kOob;
   }
-  const uint32_t last_group = (p.r - 1) / kGroup;
+  const uint32_t last_group = (k_end - 1) / kGroup;
   const bool scales_of_a = wave == 0, scales_of_b = kScales == kRowBytes && wave == 1;
   auto dma = [&](const Buffer& to, uint32_t k) {
     const uint32_t group = min(k / kGroup, last_group);
     // a group's scales of the tile's rows (a word that begins within the rows is within the pitch)
     const rsrc_t rsa = make_rsrc(p.a_scales + (uint64_t)group * p.a_scale_pitch + m0, (rows_m + 3) & ~3u);
     const rsrc_t rsb = make_rsrc(b_scales + (uint64_t)group * p.b_scale_col + n0, (rows_n + 3) & ~3u);
-    const int at_k = k < p.r ? (int)k : 0;
+    const int at_k = k < k_end ? (int)k : 0;
     // steps come in turn: from the one that the reduction ends in on, the pieces past its end read as zero
     // (an offset from kOob on stays past every descriptor: a tile's rows take less than 2^31 bytes)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const bool in = k + dma_k[e] < p.r;
+      const bool in = k + dma_k[e] < k_end;
       a_off[e] = in ? a_off[e] : kOob;
       b_off[e] = in ? b_off[e] : kOob;
     }
@@ -537,7 +489,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
     for (int j = 0; j < kDmaB; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rb, (MO_LDS void*)(to.b + (wave * kDmaB + j) * 1024), 16,
-          kTrans ? (k < p.r ? t_off[j % kTransOffs] + j / kTransOffs * kTransOffs * kPieceRows * (uint32_t)p.b_pitch : kOob)
+          kTrans ? (k < k_end ? t_off[j] : kOob)
                  : b_off[j & 1] + 8 * j * (uint32_t)p.b_pitch,
           kTrans ? at_k * (int)p.b_pitch : at_k, 0, 0);
   };
@@ -654,9 +606,9 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
     if (kScales != kRowBytes) sb[parity][0] = after;
   };
 
-  if (kScales != kRowBytes) sb[0][0] = load_block(0), sb[1][0] = load_block(kGroup);
-  dma(buf0, 0);
-  dma(buf1, kGroup);
+  if (kScales != kRowBytes) sb[0][0] = load_block(k_begin), sb[1][0] = load_block(k_begin + kGroup);
+  dma(buf0, k_begin);
+  dma(buf1, k_begin + kGroup);
   __builtin_amdgcn_s_waitcnt(wait_vm(kDmaA + kDmaB + 1 + (kScales == kRowBytes ? 1 : 0)));
   __syncthreads();
   read_scales(buf0, 0);
@@ -664,72 +616,94 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
 #pragma unroll
   for (int i = 0; i < kTM; ++i) read_a(buf0, i, 0);
   // steps in pairs, one a buffer; an odd count gets one more over zeros
-  for (uint32_t k = 0; k < p.r; k += 2 * kGroup) {
+  for (uint32_t k = k_begin; k < k_end; k += 2 * kGroup) {
     step(0, buf0, buf1, k);
     step(1, buf1, buf0, k + kGroup);
   }
 
-  // Epilogue: 32 tokens by 128 bytes of features at a time through a part of LDS of the wave's own, so that a
-  // store writes whole lines instead of pieces of 32 rows. 16-byte piece c of row r at c ^ (r % 8): writes
-  // and reads spread over the banks.
-  constexpr int kAcross = kWide ? 1 : kTN;  // MFMA tiles of a line
-  constexpr int kLine = 32 * kAcross * (kWide ? 4 : 2), kPieces = kLine / 16, kRowsAStore = 64 / kPieces;
-  static_assert(32 * kLine * G::kWaves <= kBM * (int)kGroup, "a wave's part of the first buffer");
+  // Epilogue: 32 tokens by up to 128 bytes of features at a time through a part of LDS of the wave's own, so
+  // that a store writes whole lines instead of pieces of 32 rows. 16-byte piece c of row r at c ^ (r % kPieces):
+  // writes and reads spread over the banks.
   __builtin_amdgcn_s_waitcnt(wait_vm(0));
   __syncthreads();  // every wave has read its last fragments, every DMA has landed
-  lp own = (lp)a_0 + wave * 32 * kLine;
-  const int out_row = lane / kPieces, piece = lane % kPieces;
-  const bool f16 = p.out_kind != kBF16;
-  constexpr int kBytes = kWide ? 4 : 2, kValues = 16 / kBytes;
-  const rsrc_t ro = make_rsrc((uint8_t*)p.out + m0 * p.n * kBytes, (uint32_t)(rows_m * p.n * kBytes));
+  auto emit = [&](auto value_bytes, void* out, bool last) {
+    constexpr int kBytes = decltype(value_bytes)::value;
+    constexpr int kAcross = kBytes == 4 ? 1 : kTN < 2 ? kTN : 2;  // MFMA tiles of a line
+    constexpr int kLine = 32 * kAcross * kBytes, kPieces = kLine / 16, kRowsAStore = 64 / kPieces;
+    constexpr int kOwn = 32 * kLine, kValues = 16 / kBytes;
+    static_assert(kOwn * G::kWaves <= (kBM + kBN) * (int)kGroup && kBM * kGroup % kOwn == 0, "a wave's part of a buffer");
+    const int in_a = kBM * kGroup / kOwn;
+    lp own = wave < in_a ? (lp)a_0 + wave * kOwn : (lp)b_0 + (wave - in_a) * kOwn;
+    const int out_row = lane / kPieces, piece = lane % kPieces;
+    const bool f16 = p.out_kind != kBF16;
+    const rsrc_t ro = make_rsrc((uint8_t*)out + m0 * p.n * kBytes, (uint32_t)(rows_m * p.n * kBytes));
 #pragma unroll
-  for (int i = 0; i < kTM; ++i)
+    for (int i = 0; i < kTM; ++i)
 #pragma unroll
-    for (int j0 = 0; j0 < kTN; j0 += kAcross) {
-      const uint32_t n_line = n_wave + 32 * j0;
+      for (int j0 = 0; j0 < kTN; j0 += kAcross) {
+        const uint32_t n_line = n_wave + 32 * j0;
 #pragma unroll
-      for (int j = 0; j < kAcross; ++j)
+        for (int j = 0; j < kAcross; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x16& w16 = acc[j0 + j][i];
-          f32x4 o = {w16[4 * q], w16[4 * q + 1], w16[4 * q + 2], w16[4 * q + 3]};
+          for (int q = 0; q < 4; ++q) {
+            const f32x16& w16 = acc[j0 + j][i];
+            f32x4 o = {w16[4 * q], w16[4 * q + 1], w16[4 * q + 2], w16[4 * q + 3]};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (kScales == kBlockFloats) o[e] *= in_units;
-            if (kWide && kScales != kRowBytes) o[e] += poison;
-          }
-          if (p.bias) {
-            const uint32_t n = n_line + 32 * j + 8 * q + 4 * half;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] += n < p.n ? load1(p.bias, n + e, p.out_kind) : 0.0f;
-          }
-          if (kWide) {
-            *(MO_LDS f32x4*)(own + lr * kLine + 16 * ((2 * q + half) ^ (lr % kPieces))) = o;
-          } else {
-            u32x2 w;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-              typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-              w[e] = f16 ? __builtin_bit_cast(uint32_t, f16x2{(_Float16)o[2 * e], (_Float16)o[2 * e + 1]})
-                         : __builtin_bit_cast(uint32_t, bf16x2{(__bf16)o[2 * e], (__bf16)o[2 * e + 1]});
+            for (int e = 0; e < 4; ++e) {
+              if (kScales == kBlockFloats) o[e] *= in_units;
+              if (kWide && kScales != kRowBytes) o[e] += poison;
             }
-            *(MO_LDS u32x2*)(own + lr * kLine + 16 * ((4 * j + q) ^ (lr % kPieces)) + 8 * half) = w;
-          }
-        }
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_wave_barrier();
+            if (last && p.bias) {
+              const uint32_t n = n_line + 32 * j + 8 * q + 4 * half;
 #pragma unroll
-      for (int r = 0; r < 32; r += kRowsAStore) {
-        const int row = r + out_row;
-        const u32x4 w = *(const MO_LDS u32x4*)(own + row * kLine + 16 * (piece ^ (row % kPieces)));
-        const uint32_t n = n_line + kValues * piece;
-        const uint32_t to = ((uint32_t)(32 * (wm * kTM + i) + row) * p.n + n) * kBytes;
-        __builtin_amdgcn_raw_buffer_store_b128(w, ro, (int)(n < p.n ? to : kOob), 0, 0);
+              for (int e = 0; e < 4; ++e) o[e] += n < p.n ? load1(p.bias, n + e, p.out_kind) : 0.0f;
+            }
+            if (kBytes == 4) {
+              *(MO_LDS f32x4*)(own + lr * kLine + 16 * ((2 * q + half) ^ (lr % kPieces))) = o;
+            } else {
+              u32x2 w;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+                typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+                w[e] = f16 ? __builtin_bit_cast(uint32_t, f16x2{(_Float16)o[2 * e], (_Float16)o[2 * e + 1]})
+                           : __builtin_bit_cast(uint32_t, bf16x2{(__bf16)o[2 * e], (__bf16)o[2 * e + 1]});
+              }
+              *(MO_LDS u32x2*)(own + lr * kLine + 16 * ((4 * j + q) ^ (lr % kPieces)) + 8 * half) = w;
+            }
+          }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 32; r += kRowsAStore) {
+          const int row = r + out_row;
+          const u32x4 w = *(const MO_LDS u32x4*)(own + row * kLine + 16 * (piece ^ (row % kPieces)));
+          const uint32_t n = n_line + kValues * piece;
+          const uint32_t to = ((uint32_t)(32 * (wm * kTM + i) + row) * p.n + n) * kBytes;
+          __builtin_amdgcn_raw_buffer_store_b128(w, ro, (int)(n < p.n ? to : kOob), 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_wave_barrier();
-    }
+  };
+  if (p.splits > 1)
+    emit(std::integral_constant<int, 4>{}, p.planes + (uint64_t)split * p.m * p.n, false);
+  else
+    emit(std::integral_constant<int, kWide ? 4 : 2>{}, p.out, true);
+}
+
+// The sum of a call's planes, in the order of the reduction, + bias: four outputs a lane.
+extern "C" __global__ __launch_bounds__(256) void mo_fp8_plane_sum(ProductArgs p) {
+  const uint64_t count = p.m * p.n, at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= count) return;  // a multiple of 16
+  f32x4 v = *(const f32x4*)(p.planes + at);
+  for (uint32_t s = 1; s < p.splits; ++s) v += *(const f32x4*)(p.planes + s * count + at);
+  if (p.bias) {
+    const uint32_t n = (uint32_t)(at % p.n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += load1(p.bias, n + e, p.out_kind);
+  }
+  store4(p.out, at, v, p.out_kind);
 }
 
 #define MO_TILE_KERNEL(name, G, scales, wide, trans)                                                        \
@@ -747,81 +721,11 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
   MO_TILE_KERNEL(name##_rows_w, G, kRowBytes, true, false)          \
   MO_TILE_KERNEL(name##_bytes_tw, G, kBlockBytes, true, true)       \
   MO_TILE_KERNEL(name##_floats_tw, G, kBlockFloats, true, true)
-typedef Tile<2, 4, 4, 2> Large;
+typedef Tile<2, 4, 4, 2> Large;  // 256 x 256
+typedef Tile<2, 2, 2, 2> Middle;  // 128 x 128
+typedef Tile<2, 2, 1, 1> Small;  // 64 x 64
 MO_TILE(large, Large)
-
-__device__ __forceinline__ bf16x8 widen_plain(uint32_t lo, uint32_t hi, float scale) {
-  bf16x8 o;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i ? hi : lo), false);
-    const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i ? hi : lo), true);
-    o[4 * i] = (__bf16)(a[0] * scale), o[4 * i + 1] = (__bf16)(a[1] * scale);
-    o[4 * i + 2] = (__bf16)(b[0] * scale), o[4 * i + 3] = (__bf16)(b[1] * scale);
-  }
-  return o;
-}
-
-// The plain kernel: four waves of one 32 x 32 tile each, operands straight from memory.
-template <bool kF32Scales, bool kWide>
-__device__ __forceinline__ void product_plain(const ProductArgs& p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 31, half = lane >> 5;
-  const uint32_t tiles_n = (p.n + 63) / 64;
-  const uint64_t m0 = (uint64_t)(blockIdx.x / tiles_n) * 64 + 32 * (wave & 1);
-  const uint32_t n0 = blockIdx.x % tiles_n * 64 + 32 * (wave >> 1);
-  const uint64_t m = m0 + lr;
-  const uint32_t n = n0 + lr;
-  const bool in_m = m < p.m, in_n = n < p.n;
-  const uint8_t* a = p.a + (in_m ? m : 0) * p.a_pitch;
-  const uint8_t* b = p.b + (uint64_t)(in_n ? n : 0) * p.b_pitch;
-  f32x16 acc = {};
-  for (uint32_t k0 = 0; k0 < p.r; k0 += kGroup) {
-    const uint32_t group = k0 / kGroup;
-    const int sa = in_m ? p.a_scales[group * (uint64_t)p.a_scale_pitch + m] : 127;
-    const uint64_t at = (uint64_t)((in_n ? n : 0) >> p.b_shift) * p.b_scale_row + (uint64_t)group * p.b_scale_col;
-    const int sb = kF32Scales ? 127 : ((const uint8_t*)p.b_scales)[at];
-    f32x16 sum = kF32Scales ? f32x16{} : acc;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i32x8 fa = {}, fb = {};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t k = k0 + 64 * h + 32 * half + 16 * c;
-        u32x4 va = {}, vb = {};
-        if (in_m && k < p.r) va = *(const u32x4*)(a + k);
-        if (in_n && k < p.r) vb = *(const u32x4*)(b + k);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) fa[4 * c + i] = (int)va[i], fb[4 * c + i] = (int)vb[i];
-      }
-      if (kWide) {
-        const float xa = scale_value((uint32_t)sa), xb = scale_value((uint32_t)sb);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen_plain(fb[2 * q], fb[2 * q + 1], xb),
-                                                        widen_plain(fa[2 * q], fa[2 * q + 1], xa), sum, 0, 0, 0);
-      } else {
-        sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb, fa, sum, 0, 0, 0, sb, 0, sa);
-      }
-    }
-    if (kF32Scales) {
-      const float s = ((const float*)p.b_scales)[(uint64_t)((n0 < p.n ? n0 : 0) >> p.b_shift) * p.b_scale_row +
-                                                 (uint64_t)group * p.b_scale_col];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] += sum[i] * s;
-    } else {
-      acc = sum;
-    }
-  }
-  store_tile(p, acc, m, n0, half);
-}
-
-#define MO_PLAIN(name, f32_scales, wide)                                                                 \
-  extern "C" __global__ __launch_bounds__(256) void mo_fp8_product_plain##name(ProductArgs p) {          \
-    product_plain<f32_scales, wide>(p);                                                                  \
-  }
-MO_PLAIN(, false, false)
-MO_PLAIN(_f32, true, false)
-MO_PLAIN(_wide, false, true)
-MO_PLAIN(_wide_f32, true, true)
+MO_TILE(middle, Middle)
+MO_TILE(small, Small)
 
 }  // namespace

@@ -302,7 +302,8 @@ SIGNATURES: dict[str, tuple] = {
                                               _u64, _u64, _u64]),
     "mo_fp8_weight_gradient": (ctypes.c_int, [_u64, _u64, _u32, _u64, _u64, _u64, _u32, _u64, _u64, _u32, _u32, _u64,
                                               _u32, _u64, _u64, _u64]),
-    "mo_fp8_workspace_bytes": (_u64, [_u32, _u64, _u32, _u32, _u32]),
+    "mo_fp8_workspace_bytes": (_u64, [_u32, _u64, _u32, _u32, _u32, _u32, _u32]),
+    "mo_fp8_plan": (ctypes.c_int, [_u64, _u32, _u32, _u32, _u32, _u32, _P(_u32)]),
     "mo_rotary_forward": (ctypes.c_int, [_P(MoRotaryCall), _u64]),
     "mo_rotary_backward": (ctypes.c_int, [_P(MoRotaryCall), _u64, _u64, _u64]),
     "mo_rotary_workspace_bytes": (_u64, [_P(MoRotaryCall)]),

@@ -21,6 +21,7 @@ Feature sizes are multiples of 16, rows any number. A group with an infinity or 
 from __future__ import annotations
 
 import contextlib
+import ctypes
 
 import torch
 
@@ -128,9 +129,10 @@ def _output(out: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype
     return out.view(shape)
 
 
-def _workspace(op: int, rows: int, in_features: int, out_features: int, quantized: bool, device) -> tuple:
+def _workspace(op: int, rows: int, in_features: int, out_features: int, quantized: bool, kind: int, dtype: torch.dtype,
+               device) -> tuple:
     # freed to the caching allocator after the call; stream order keeps it alive for the kernels
-    nbytes = _native.load().mo_fp8_workspace_bytes(op, rows, in_features, out_features, int(quantized))
+    nbytes = _native.load().mo_fp8_workspace_bytes(op, rows, in_features, out_features, int(quantized), kind, _CODES[dtype])
     return (torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes) if nbytes else (None, 0)
 
 
@@ -275,7 +277,7 @@ def fp8_linear_forward(tokens, weight: torch.Tensor, scale: torch.Tensor, bias: 
             bias = bias.to(dtype).contiguous()
         if rows:
             space, nbytes = _workspace(_native.MO_FP8_FORWARD, rows, in_features, out_features, scales is not None,
-                                       weight.device)
+                                       kind, dtype, weight.device)
             _native.check("mo_fp8_linear_forward", lib.mo_fp8_linear_forward(
                 matrix.data_ptr(), _address(scales), code, rows, in_features, stride, weight.data_ptr(),
                 scale.data_ptr(), kind, out_features, _address(bias), result.data_ptr(), _CODES[dtype],
@@ -299,7 +301,7 @@ def fp8_linear_backward(gradient, weight: torch.Tensor, scale: torch.Tensor, *, 
         result = _output(out, (rows, in_features), dtype, weight.device)
         if rows:
             space, nbytes = _workspace(_native.MO_FP8_BACKWARD, rows, in_features, out_features, scales is not None,
-                                       weight.device)
+                                       kind, dtype, weight.device)
             _native.check("mo_fp8_linear_backward", lib.mo_fp8_linear_backward(
                 matrix.data_ptr(), _address(scales), code, rows, in_features, out_features, stride, weight.data_ptr(),
                 scale.data_ptr(), kind, result.data_ptr(), _CODES[dtype], _address(space), nbytes, _stream(weight)))
@@ -341,11 +343,23 @@ def fp8_weight_gradient(gradient, tokens, *, rows: int | None = None, dtype: tor
         result = _output(out, (out_features, in_features), dtype, dy.device)
         if not rows:
             return result.zero_()
-        space, nbytes = _workspace(_native.MO_FP8_WEIGHT, rows, in_features, out_features, quantized, dy.device)
+        space, nbytes = _workspace(_native.MO_FP8_WEIGHT, rows, in_features, out_features, quantized,
+                                   _native.MO_FP8_SCALE_E8M0, dtype, dy.device)
         _native.check("mo_fp8_weight_gradient", lib.mo_fp8_weight_gradient(
             dy.data_ptr(), _address(dy_scales), dy_code, dy_stride, x.data_ptr(), _address(x_scales), x_code, x_stride,
             rows, in_features, out_features, result.data_ptr(), _CODES[dtype], _address(space), nbytes, _stream(dy)))
     return result
+
+
+def product_plan(rows: int, cols: int, reduction: int, cus: int, *, float_scales: bool = False,
+                 dtype: torch.dtype = torch.bfloat16) -> dict:
+    """How a product ``[rows, cols]`` from a ``reduction`` runs on a device of ``cus`` CUs (``mo_fp8_plan``):
+    ``{"edge"}`` of the tile, ``"splits"`` of the reduction, ``"split_steps"`` of 128 each."""
+
+    raw = (ctypes.c_uint32 * 3)()
+    kind = _native.MO_FP8_SCALE_F32 if float_scales else _native.MO_FP8_SCALE_E8M0
+    _native.check("mo_fp8_plan", _native.load().mo_fp8_plan(rows, cols, reduction, kind, _CODES[dtype], cus, raw))
+    return dict(zip(("edge", "splits", "split_steps"), raw))
 
 
 # ---- under autograd -------------------------------------------------------------------------------

@@ -94,11 +94,32 @@ def test_the_library_refuses_before_it_looks_for_a_device() -> None:
         assert message in lib.mo_last_error(), (index, value, lib.mo_last_error())
     forward = [4096, 0, 1, 4, 64, 64, 4096, 4096, 0, 32, 0, 4096, 1, 4096, 1 << 20, 0]
     for index, value, message in [(6, 0, b"null"), (8, 2, b"scale type"), (4, 40, b"multiples"), (9, 0, b"empty"),
-                                  (11, 0, b"null"), (12, 5, b"type"), (11, 4104, b"misaligned"), (13, 0, b"workspace"),
-                                  (14, 16, b"workspace"), (13, 4100, b"workspace"), (3, 0, b"empty")]:
+                                  (11, 0, b"null"), (12, 5, b"type"), (11, 4104, b"misaligned"), (3, 0, b"empty")]:
         call = list(forward)
         call[index] = value
         assert lib.mo_fp8_linear_forward(*call) == _native.MO_E_INVALID
         assert message in lib.mo_last_error(), (index, value, lib.mo_last_error())
-    assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, 0, 64, 64, 0) == 0
-    assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, 5, 64, 64, 1) == 0
+    call = list(forward)
+    call[4], call[5], call[9] = 1 << 16, 1 << 16, 1 << 15  # 2^31 values
+    assert lib.mo_fp8_linear_forward(*call) == _native.MO_E_INVALID and b"too large" in lib.mo_last_error()
+    assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, 0, 64, 64, 0, 0, 1) == 0
+    weight = [4096, 0, 1, 32, 4096, 0, 1, 64, (1 << 23) - 127, 64, 32, 4096, 2, 4096, 1 << 40, 0]
+    assert lib.mo_fp8_weight_gradient(*weight) == _native.MO_E_INVALID and b"too many rows" in lib.mo_last_error()
+
+
+def test_plans_cover_the_reduction() -> None:
+    """Every split has work, and few rows or long reductions are shared out while large calls are not."""
+
+    for rows in (1, 77, 333, 1333, 4608, 17792, (1 << 31) - 1):
+        for cols, reduction in ((3072, 3072), (16, 17792), (24576, 3072), (3072, 24576), (80, 128), (16, 16)):
+            for cus in (32, 256):
+                for floats in (False, True):
+                    for dtype in (torch.bfloat16, torch.float32):
+                        plan = fp8.product_plan(rows, cols, reduction, cus, float_scales=floats, dtype=dtype)
+                        steps = -(-reduction // 128)
+                        assert plan["edge"] in (64, 128, 256) and 1 <= plan["splits"] <= 32
+                        assert (plan["splits"] - 1) * plan["split_steps"] < steps <= plan["splits"] * plan["split_steps"]
+                        if plan["splits"] > 1:
+                            assert plan["split_steps"] >= 2 and plan["splits"] * rows * cols * 4 <= 1 << 31
+    assert fp8.product_plan(1, 3072, 12288, 256)["splits"] > 1
+    assert fp8.product_plan(4608, 24576, 3072, 256) == {"edge": 256, "splits": 1, "split_steps": 24}
