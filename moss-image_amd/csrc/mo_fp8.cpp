@@ -188,9 +188,8 @@ uint64_t plane_bytes(const Plan& p, uint64_t rows, uint64_t cols) {
   return p.splits > 1 ? align(p.splits * rows * cols * 4) : 0;
 }
 
-// `planes`: room for plane_bytes of the plan of this call.
-int product(const Module& m, ProductArgs p, int scales, bool trans, uint64_t planes, uint64_t stream) {
-  const Plan plan = plan_of(p.m, p.n, (uint32_t)div_up(p.r, kGroup), cost_kind(scales, p.out_kind), m.cus);
+// `planes`: room for the plan's plane_bytes.
+int product(const Module& m, const Plan& plan, ProductArgs p, int scales, bool trans, uint64_t planes, uint64_t stream) {
   const TileShape& t = kTileShapes[plan.tile];
   p.splits = plan.splits, p.split_steps = plan.split_steps, p.planes = plan.splits > 1 ? (float*)planes : nullptr;
   void* params[] = {&p};
@@ -244,8 +243,9 @@ uint64_t col_bytes(uint64_t rows, uint64_t cols) {
   return align(cols * div_up(rows, kGroup) * kGroup) + align(div_up(rows, kGroup) * cols);
 }
 
-// A call's workspace: the operands it quantizes, then its planes.
+// A call's plan and its workspace: the operands it quantizes, then its planes.
 struct Room {
+  Plan plan;
   uint64_t operands, planes;
   uint64_t bytes() const { return operands + planes; }
 };
@@ -261,7 +261,8 @@ Room room_of(uint32_t op, uint64_t rows, uint64_t in_f, uint64_t out_f, bool qua
     if (op == MO_FP8_WEIGHT) r.operands = col_bytes(rows, out_f) + col_bytes(rows, in_f);
   }
   const int scales = op == MO_FP8_WEIGHT ? kScaleRows : (int)scale_kind;
-  r.planes = plane_bytes(plan_of(m, n, (uint32_t)div_up(reduction, kGroup), cost_kind(scales, out_kind), cus), m, n);
+  r.plan = plan_of(m, n, (uint32_t)div_up(reduction, kGroup), cost_kind(scales, out_kind), cus);
+  r.planes = plane_bytes(r.plan, m, n);
   return r;
 }
 
@@ -368,7 +369,7 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
     p.b_scale_row = (uint32_t)div_up(in_features, kGroup), p.b_scale_col = 1, p.b_shift = 7;
     p.bias = (const void*)bias, p.out = (void*)y, p.out_kind = y_dtype;
     p.m = rows, p.n = out_features, p.r = in_features;
-    return product(m, p, (int)scale_kind, false, workspace + room.operands, stream);
+    return product(m, room.plan, p, (int)scale_kind, false, workspace + room.operands, stream);
   });
 }
 
@@ -398,7 +399,7 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
     p.b_scale_row = 1, p.b_scale_col = (uint32_t)div_up(in_features, kGroup), p.b_shift = 7;
     p.out = (void*)dx, p.out_kind = dx_dtype;
     p.m = rows, p.n = in_features, p.r = out_features;
-    return product(m, p, (int)scale_kind, true, workspace + room.operands, stream);
+    return product(m, room.plan, p, (int)scale_kind, true, workspace + room.operands, stream);
   });
 }
 
@@ -437,7 +438,7 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     p.b_scale_row = 1, p.b_scale_col = in_features, p.b_shift = 0;
     p.out = (void*)dw, p.out_kind = dw_dtype;
     p.m = out_features, p.n = in_features, p.r = (uint32_t)padded;
-    return product(m, p, kScaleRows, false, workspace + room.operands, stream);
+    return product(m, room.plan, p, kScaleRows, false, workspace + room.operands, stream);
   });
 }
 

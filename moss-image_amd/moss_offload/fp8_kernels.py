@@ -20,8 +20,8 @@ Feature sizes are multiples of 16, rows any number. A group with an infinity or 
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -34,18 +34,17 @@ LARGEST = 448.0
 _CODES = _native.DTYPE_CODES
 
 
-def _device(tensor: torch.Tensor):
-    """The tensor's device as the current one: kernels are launched on it."""
+def _elsewhere(tensor: torch.Tensor) -> bool:
+    """Whether the tensor's device is not the current one, which kernels are launched on."""
 
-    if tensor.device.type != "cuda":
+    index = tensor.get_device()
+    if index < 0:
         raise RuntimeError("fp8 operands must be on a HIP device.")
-    if tensor.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(tensor.device)
+    return index != torch._C._cuda_getDevice()
 
 
 def _stream(tensor: torch.Tensor) -> int:
-    return torch.cuda.current_stream(tensor.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
 
 
 def _groups(size: int) -> int:
@@ -56,7 +55,8 @@ def _scales(rows: int, size: int, device) -> torch.Tensor:
     """Room for one scale for each 128 of ``size`` values of ``rows`` rows: ``[rows, groups]``, laid group by
     group (what the products read at a time is then dense)."""
 
-    return torch.empty((_groups(size), -(-rows // 16) * 16), dtype=E8M0, device=device)[:, :rows].t()
+    groups, pitch = -(-size // GROUP), -(-rows // 16) * 16
+    return torch.empty(groups * pitch, dtype=E8M0, device=device).as_strided((rows, groups), (1, pitch))
 
 
 def _plain(*operands: torch.Tensor | None) -> None:
@@ -129,11 +129,17 @@ def _output(out: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype
     return out.view(shape)
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(op: int, rows: int, in_features: int, out_features: int, quantized: bool, kind: int, code: int,
+                     device: int) -> int:
+    return _native.load().mo_fp8_workspace_bytes(op, rows, in_features, out_features, int(quantized), kind, code)
+
+
 def _workspace(op: int, rows: int, in_features: int, out_features: int, quantized: bool, kind: int, dtype: torch.dtype,
-               device) -> tuple:
+               like: torch.Tensor) -> tuple:
     # freed to the caching allocator after the call; stream order keeps it alive for the kernels
-    nbytes = _native.load().mo_fp8_workspace_bytes(op, rows, in_features, out_features, int(quantized), kind, _CODES[dtype])
-    return (torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes) if nbytes else (None, 0)
+    nbytes = _workspace_bytes(op, rows, in_features, out_features, quantized, kind, _CODES[dtype], like.get_device())
+    return (torch.empty(nbytes, dtype=torch.uint8, device=like.device), nbytes) if nbytes else (None, 0)
 
 
 def _address(tensor: torch.Tensor | None) -> int:
@@ -147,21 +153,21 @@ def _quantize(x: torch.Tensor, rows: bool, columns: bool):
     lib = _native.load()
     _plain(x)
     matrix = _rows(x, "matrix")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return _quantize(x, rows, columns)
     (m, n), device = matrix.shape, x.device
     row = column = None
-    with _device(x):
-        if rows:
-            row = (torch.empty((m, n), dtype=E4M3, device=device),
-                   _scales(m, n, device))
-        if columns:
-            column = (torch.empty((n, _groups(m) * GROUP), dtype=E4M3, device=device),
-                      _scales(n, m, device))
-        if m:
-            pointers = [t.data_ptr() if t is not None else 0 for pair in (row, column) for t in (pair or (None, None))]
-            _native.check("mo_fp8_quantize", lib.mo_fp8_quantize(
-                matrix.data_ptr(), _CODES[matrix.dtype], m, n, _stride(matrix), *pointers, _stream(x)))
-    if row is not None and x.ndim != 2:
-        row = (row[0].view(x.shape), row[1])
+    pointers = [0, 0, 0, 0]
+    if rows:
+        row = torch.empty(x.shape, dtype=E4M3, device=device), _scales(m, n, device)
+        pointers[:2] = row[0].data_ptr(), row[1].data_ptr()
+    if columns:
+        column = torch.empty((n, -(-m // GROUP) * GROUP), dtype=E4M3, device=device), _scales(n, m, device)
+        pointers[2:] = column[0].data_ptr(), column[1].data_ptr()
+    if m:
+        _native.check("mo_fp8_quantize", lib.mo_fp8_quantize(
+            matrix.data_ptr(), _CODES[matrix.dtype], m, n, _stride(matrix), *pointers, _stream(x)))
     return row, column
 
 
@@ -186,20 +192,23 @@ def fp8_quantize_both(x: torch.Tensor) -> tuple[tuple[torch.Tensor, torch.Tensor
 
 
 def fp8_quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """``(values, scales)`` of a weight ``[out, in]`` in blocks of 128 x 128."""
+    """``(values, scales)`` of a weight ``[out, in]`` in blocks of 128 x 128. (``out`` is any number here; the
+    products take multiples of 16.)"""
 
     lib = _native.load()
     _plain(weight)
-    if weight.ndim != 2 or weight.shape[0] % 16 or not weight.shape[0]:
-        raise ValueError("fp8 weight must be a matrix with features that are multiples of 16.")
+    if weight.ndim != 2 or not weight.shape[0]:
+        raise ValueError("fp8 weight must be a matrix, not empty.")
     matrix = _rows(weight, "weight")
+    if _elsewhere(weight):
+        with torch.cuda.device(weight.device):
+            return fp8_quantize_weight(weight)
     rows, cols = matrix.shape
-    with _device(weight):
-        values = torch.empty((rows, cols), dtype=E4M3, device=weight.device)
-        scales = torch.empty((_groups(rows), _groups(cols)), dtype=E8M0, device=weight.device)
-        _native.check("mo_fp8_quantize_weight", lib.mo_fp8_quantize_weight(
-            matrix.data_ptr(), _CODES[matrix.dtype], rows, cols, _stride(matrix), values.data_ptr(), scales.data_ptr(),
-            _stream(weight)))
+    values = torch.empty((rows, cols), dtype=E4M3, device=weight.device)
+    scales = torch.empty((_groups(rows), _groups(cols)), dtype=E8M0, device=weight.device)
+    _native.check("mo_fp8_quantize_weight", lib.mo_fp8_quantize_weight(
+        matrix.data_ptr(), _CODES[matrix.dtype], rows, cols, _stride(matrix), values.data_ptr(), scales.data_ptr(),
+        _stream(weight)))
     return values, scales
 
 
@@ -216,7 +225,7 @@ def fp8_decode(values: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype
         raise TypeError(f"fp8 output must be bfloat16, float16 or float32 (got {dtype}).")
     if values.shape[-1] == 0 or values.shape[-1] % 16:
         raise ValueError("fp8 values must have a last dimension that is a multiple of 16.")
-    matrix = values.reshape(-1, values.shape[-1])
+    matrix = values if values.ndim == 2 else values.reshape(-1, values.shape[-1])
     cols = matrix.shape[1] if cols is None else cols
     if not 0 <= cols <= matrix.shape[1]:
         raise ValueError("fp8_decode's cols must lie within the values.")
@@ -227,13 +236,15 @@ def fp8_decode(values: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype
     if scales.shape[0] not in (rows, _groups(rows)) or scales.shape[1] < _groups(cols) \
             or scales.get_device() != values.get_device():
         raise ValueError("fp8 scales do not fit the values.")
+    if _elsewhere(values):
+        with torch.cuda.device(values.device):
+            return fp8_decode(values, scales, dtype=dtype, cols=cols)
     out = torch.empty((*values.shape[:-1], cols), dtype=dtype, device=values.device)
-    if out.numel():
+    if rows and cols:
         kind = _native.MO_FP8_SCALE_F32 if scales.dtype == torch.float32 else _native.MO_FP8_SCALE_E8M0
-        with _device(values):
-            _native.check("mo_fp8_decode", lib.mo_fp8_decode(
-                matrix.data_ptr(), _stride(matrix), scales.data_ptr(), kind, *scales.stride(),
-                1 if scales.shape[0] == rows else GROUP, out.data_ptr(), _CODES[dtype], rows, cols, _stream(values)))
+        _native.check("mo_fp8_decode", lib.mo_fp8_decode(
+            matrix.data_ptr(), _stride(matrix), scales.data_ptr(), kind, scales.stride(0), scales.stride(1),
+            1 if scales.shape[0] == rows else GROUP, out.data_ptr(), _CODES[dtype], rows, cols, _stream(values)))
     return out
 
 
@@ -267,21 +278,23 @@ def fp8_linear_forward(tokens, weight: torch.Tensor, scale: torch.Tensor, bias: 
     matrix, scales, code, rows, stride, lead = _operand(tokens, in_features, "tokens")
     if matrix.get_device() != weight.get_device():
         raise RuntimeError("fp8 tokens and weight must be on one device.")
+    if _elsewhere(weight):
+        with torch.cuda.device(weight.device):
+            return fp8_linear_forward(tokens, weight, scale, bias, dtype=dtype, out=out)
     dtype = dtype or (torch.bfloat16 if scales is not None else matrix.dtype)
-    with _device(weight):
-        result = _output(out, (rows, out_features), dtype, weight.device)
-        if bias is not None:
-            _plain(bias)
-            if bias.shape != (out_features,) or bias.get_device() != weight.get_device():
-                raise RuntimeError(f"fp8 bias must be {out_features} values on the weight's device.")
-            bias = bias.to(dtype).contiguous()
-        if rows:
-            space, nbytes = _workspace(_native.MO_FP8_FORWARD, rows, in_features, out_features, scales is not None,
-                                       kind, dtype, weight.device)
-            _native.check("mo_fp8_linear_forward", lib.mo_fp8_linear_forward(
-                matrix.data_ptr(), _address(scales), code, rows, in_features, stride, weight.data_ptr(),
-                scale.data_ptr(), kind, out_features, _address(bias), result.data_ptr(), _CODES[dtype],
-                _address(space), nbytes, _stream(weight)))
+    result = _output(out, (rows, out_features), dtype, weight.device)
+    if bias is not None:
+        _plain(bias)
+        if bias.shape != (out_features,) or bias.get_device() != weight.get_device():
+            raise RuntimeError(f"fp8 bias must be {out_features} values on the weight's device.")
+        bias = bias.to(dtype).contiguous()
+    if rows:
+        space, nbytes = _workspace(_native.MO_FP8_FORWARD, rows, in_features, out_features, scales is not None, kind,
+                                   dtype, weight)
+        _native.check("mo_fp8_linear_forward", lib.mo_fp8_linear_forward(
+            matrix.data_ptr(), _address(scales), code, rows, in_features, stride, weight.data_ptr(), scale.data_ptr(),
+            kind, out_features, _address(bias), result.data_ptr(), _CODES[dtype], _address(space), nbytes,
+            _stream(weight)))
     return result if len(lead) == 1 else result.view(*lead, out_features)
 
 
@@ -296,15 +309,17 @@ def fp8_linear_backward(gradient, weight: torch.Tensor, scale: torch.Tensor, *, 
     matrix, scales, code, rows, stride, lead = _operand(gradient, out_features, "gradient")
     if matrix.get_device() != weight.get_device():
         raise RuntimeError("fp8 gradient and weight must be on one device.")
+    if _elsewhere(weight):
+        with torch.cuda.device(weight.device):
+            return fp8_linear_backward(gradient, weight, scale, dtype=dtype, out=out)
     dtype = dtype or (torch.bfloat16 if scales is not None else matrix.dtype)
-    with _device(weight):
-        result = _output(out, (rows, in_features), dtype, weight.device)
-        if rows:
-            space, nbytes = _workspace(_native.MO_FP8_BACKWARD, rows, in_features, out_features, scales is not None,
-                                       kind, dtype, weight.device)
-            _native.check("mo_fp8_linear_backward", lib.mo_fp8_linear_backward(
-                matrix.data_ptr(), _address(scales), code, rows, in_features, out_features, stride, weight.data_ptr(),
-                scale.data_ptr(), kind, result.data_ptr(), _CODES[dtype], _address(space), nbytes, _stream(weight)))
+    result = _output(out, (rows, in_features), dtype, weight.device)
+    if rows:
+        space, nbytes = _workspace(_native.MO_FP8_BACKWARD, rows, in_features, out_features, scales is not None, kind,
+                                   dtype, weight)
+        _native.check("mo_fp8_linear_backward", lib.mo_fp8_linear_backward(
+            matrix.data_ptr(), _address(scales), code, rows, in_features, out_features, stride, weight.data_ptr(),
+            scale.data_ptr(), kind, result.data_ptr(), _CODES[dtype], _address(space), nbytes, _stream(weight)))
     return result if len(lead) == 1 else result.view(*lead, in_features)
 
 
@@ -339,15 +354,17 @@ def fp8_weight_gradient(gradient, tokens, *, rows: int | None = None, dtype: tor
         dy_code, x_code, dy_stride, x_stride = _CODES[dy.dtype], _CODES[x.dtype], _stride(dy), _stride(x)
     if dy.get_device() != x.get_device():
         raise RuntimeError("fp8 gradient and tokens must be on one device.")
-    with _device(dy):
-        result = _output(out, (out_features, in_features), dtype, dy.device)
-        if not rows:
-            return result.zero_()
-        space, nbytes = _workspace(_native.MO_FP8_WEIGHT, rows, in_features, out_features, quantized,
-                                   _native.MO_FP8_SCALE_E8M0, dtype, dy.device)
-        _native.check("mo_fp8_weight_gradient", lib.mo_fp8_weight_gradient(
-            dy.data_ptr(), _address(dy_scales), dy_code, dy_stride, x.data_ptr(), _address(x_scales), x_code, x_stride,
-            rows, in_features, out_features, result.data_ptr(), _CODES[dtype], _address(space), nbytes, _stream(dy)))
+    if _elsewhere(dy):
+        with torch.cuda.device(dy.device):
+            return fp8_weight_gradient(gradient, tokens, rows=rows, dtype=dtype, out=out)
+    result = _output(out, (out_features, in_features), dtype, dy.device)
+    if not rows:
+        return result.zero_()
+    space, nbytes = _workspace(_native.MO_FP8_WEIGHT, rows, in_features, out_features, quantized,
+                               _native.MO_FP8_SCALE_E8M0, dtype, dy)
+    _native.check("mo_fp8_weight_gradient", lib.mo_fp8_weight_gradient(
+        dy.data_ptr(), _address(dy_scales), dy_code, dy_stride, x.data_ptr(), _address(x_scales), x_code, x_stride,
+        rows, in_features, out_features, result.data_ptr(), _CODES[dtype], _address(space), nbytes, _stream(dy)))
     return result
 
 

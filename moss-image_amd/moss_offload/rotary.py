@@ -15,9 +15,9 @@ rotary_dim / 2`` (the reference's), ``"interleaved"`` neighbours. Values past ``
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -30,16 +30,17 @@ MAX_HEAD_DIM = 512
 _CODES = _native.DTYPE_CODES
 
 
-def _device(tensor: torch.Tensor):
-    if tensor.device.type != "cuda":
+def _elsewhere(tensor: torch.Tensor) -> bool:
+    """Whether the tensor's device is not the current one, which kernels are launched on."""
+
+    index = tensor.get_device()
+    if index < 0:
         raise RuntimeError("rotary operands must be on a HIP device.")
-    if tensor.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(tensor.device)
+    return index != torch._C._cuda_getDevice()
 
 
 def _stream(tensor: torch.Tensor) -> int:
-    return torch.cuda.current_stream(tensor.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
 
 
 def _plain(*operands: torch.Tensor | None) -> None:
@@ -93,14 +94,16 @@ def rotary_table(coordinates: torch.Tensor, bands: torch.Tensor, *, amplitude: f
     if bands.get_device() != coordinates.get_device():
         raise RuntimeError("rotary coordinates and bands must be on one device.")
     coordinates, bands = coordinates.contiguous(), bands.contiguous()
+    if _elsewhere(coordinates):
+        with torch.cuda.device(coordinates.device):
+            return rotary_table(coordinates, bands, amplitude=amplitude, dtype=dtype)
     axes = coordinates.shape[-1]
     rows = coordinates.numel() // axes
-    with _device(coordinates):
-        out = torch.empty((*coordinates.shape[:-1], 2 * axes * bands.numel()), dtype=dtype, device=coordinates.device)
-        if rows:
-            _native.check("mo_rotary_table", lib.mo_rotary_table(
-                coordinates.data_ptr(), bands.data_ptr(), out.data_ptr(), _CODES[dtype], rows, axes, bands.numel(),
-                amplitude, _stream(coordinates)))
+    out = torch.empty((*coordinates.shape[:-1], 2 * axes * bands.numel()), dtype=dtype, device=coordinates.device)
+    if rows:
+        _native.check("mo_rotary_table", lib.mo_rotary_table(
+            coordinates.data_ptr(), bands.data_ptr(), out.data_ptr(), _CODES[dtype], rows, axes, bands.numel(),
+            amplitude, _stream(coordinates)))
     return out
 
 
@@ -112,16 +115,23 @@ def _heads(tensor: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
     return tensor if tensor.stride(3) == 1 else tensor.contiguous()
 
 
+_SIDE, _REST = struct.Struct("=5Q6qII"), struct.Struct("=QQ8IfI")  # mo_rotary_side; mo_rotary_call after its sides
+_NO_SIDE = bytes(_SIDE.size)
+
+
 def _call(sides, table, layout, weights, eps, backward):
-    """The call's description and what it keeps alive. ``sides``: (x or None, gradient or None) of each."""
+    """The call's description, and what it keeps alive, its outputs and weight gradients. ``sides``: (heads or
+    None, gradient or None) of queries and keys."""
 
     if layout not in LAYOUTS:
         raise ValueError(f"rotary layout must be one of {LAYOUTS}.")
-    like = next((t for side in sides for t in side if t is not None), None)
+    (q, grad_q), (k, grad_k) = sides
+    like = next((t for t in (grad_q, grad_k, q, k) if t is not None), None)
     if like is None:
         raise ValueError("rotary needs queries or keys.")
-    _plain(table, *weights, *(t for side in sides for t in side))
-    if like.dtype not in _CODES or table.dtype not in _CODES:
+    _plain(table, *weights, q, grad_q, k, grad_k)
+    code, table_code = _CODES.get(like.dtype), _CODES.get(table.dtype)
+    if code is None or table_code is None:
         raise TypeError("rotary heads and table must be bfloat16, float16 or float32.")
     if like.ndim != 4:
         raise ValueError("rotary heads must be [batch, tokens, heads, head_dim].")
@@ -136,49 +146,48 @@ def _call(sides, table, layout, weights, eps, backward):
     if table.get_device() != like.get_device():
         raise RuntimeError("rotary heads and table must be on one device.")
     table = table.contiguous()
-    call = _native.MoRotaryCall()
-    call.table, call.table_batch = table.data_ptr(), 0 if table.shape[0] == 1 else tokens * rotary_dim
-    call.dtype, call.table_dtype, call.batch, call.tokens = _CODES[like.dtype], _CODES[table.dtype], batch, tokens
-    call.head_dim, call.rotary_dim, call.interleaved, call.eps = head_dim, rotary_dim, layout == "interleaved", eps
-    kept, outs, weight_grads, weight_dtype = [table], [], [], None
-    for (x, grad), weight, side in zip(sides, weights, call.side):
+    kept, outs, weight_grads, packed, weight_dtype = [table], [], [], [], None
+    for (x, grad), weight in zip(sides, weights):
         given = grad if backward else x
         if given is None:
             outs.append(None)
             weight_grads.append(None)
+            packed.append(_NO_SIDE)
             continue
         given = _heads(given, like, "heads")
         out = torch.empty(given.shape, dtype=given.dtype, device=given.device)
-        side.heads, side.out = given.shape[2], out.data_ptr()
+        heads = given.shape[2]
+        weight_grad = None
         if weight is not None:
             if weight.shape != (head_dim,) or weight.dtype not in _CODES or weight.get_device() != like.get_device() \
                     or weight_dtype not in (None, weight.dtype):
                 raise ValueError("rotary norm weights must be [head_dim], of one floating type, on the heads' device.")
-            weight_dtype = weight.dtype
-            weight = weight.contiguous()
-            side.weight = weight.data_ptr()
-            kept.append(weight)
-        if backward:
-            side.grad = given.data_ptr()
-            side.grad_batch, side.grad_token, side.grad_head = given.stride()[:3]
-            kept.append(given)
-        weight_grad = None
-        if not backward or weight is not None:
-            if x is None:
-                raise ValueError("the norm's gradient needs the queries or keys that went in.")
-            x = _heads(x, like, "heads")
-            if x.shape != given.shape:
-                raise ValueError("rotary gradient and heads must have one shape.")
-            side.x = x.data_ptr()
-            side.x_batch, side.x_token, side.x_head = x.stride()[:3]
-            kept.append(x)
+            weight_dtype, weight = weight.dtype, weight.contiguous()
             if backward:
-                weight_grad = torch.empty_like(weight) if given.shape[2] else torch.zeros_like(weight)
-                side.weight_grad = weight_grad.data_ptr()
+                if x is None:
+                    raise ValueError("the norm's gradient needs the queries or keys that went in.")
+                x = _heads(x, like, "heads")
+                if x.shape != given.shape:
+                    raise ValueError("rotary gradient and heads must have one shape.")
+                weight_grad = torch.empty_like(weight) if heads else torch.zeros_like(weight)
+        source = x if backward and weight is not None else None if backward else given
+        kept += [given, source, weight]
+        packed.append(_SIDE.pack(
+            0 if source is None else source.data_ptr(), given.data_ptr() if backward else 0, out.data_ptr(),
+            0 if weight is None else weight.data_ptr(), 0 if weight_grad is None else weight_grad.data_ptr(),
+            *((0, 0, 0) if source is None else source.stride()[:3]), *(given.stride()[:3] if backward else (0, 0, 0)),
+            heads, 0))
         outs.append(out)
         weight_grads.append(weight_grad)
-    call.weight_dtype = _CODES[weight_dtype or torch.float32]
+    rest = _REST.pack(table.data_ptr(), 0 if table.shape[0] == 1 else tokens * rotary_dim, code, table_code,
+                      _CODES[weight_dtype or torch.float32], batch, tokens, head_dim, rotary_dim,
+                      layout == "interleaved", eps, 0)
+    call = _native.MoRotaryCall.from_buffer_copy(packed[0] + packed[1] + rest)
     return call, kept, outs, weight_grads, like
+
+
+def _any(outs) -> bool:
+    return any(out is not None and out.numel() for out in outs)
 
 
 def rotary_forward(q: torch.Tensor | None, k: torch.Tensor | None, table: torch.Tensor, *, layout: str = "half",
@@ -189,9 +198,11 @@ def rotary_forward(q: torch.Tensor | None, k: torch.Tensor | None, table: torch.
 
     lib = _native.load()
     call, _kept, outs, _, like = _call(((q, None), (k, None)), table, layout, (q_weight, k_weight), eps, False)
-    if like.shape[0] * like.shape[1] and any(o is not None and o.numel() for o in outs):
-        with _device(like):
-            _native.check("mo_rotary_forward", lib.mo_rotary_forward(ctypes.byref(call), _stream(like)))
+    if _elsewhere(like):
+        with torch.cuda.device(like.device):
+            return rotary_forward(q, k, table, layout=layout, q_weight=q_weight, k_weight=k_weight, eps=eps)
+    if _any(outs):
+        _native.check("mo_rotary_forward", lib.mo_rotary_forward(ctypes.byref(call), _stream(like)))
     return outs[0], outs[1]
 
 
@@ -205,12 +216,15 @@ def rotary_backward(grad_q: torch.Tensor | None, grad_k: torch.Tensor | None, ta
     lib = _native.load()
     call, _kept, outs, weight_grads, like = _call(((q, grad_q), (k, grad_k)), table, layout, (q_weight, k_weight), eps,
                                                   True)
-    if like.shape[0] * like.shape[1] and any(o is not None and o.numel() for o in outs):
-        with _device(like):
-            nbytes = lib.mo_rotary_workspace_bytes(ctypes.byref(call))
-            space = torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
-            _native.check("mo_rotary_backward", lib.mo_rotary_backward(
-                ctypes.byref(call), 0 if space is None else space.data_ptr(), nbytes, _stream(like)))
+    if _elsewhere(like):
+        with torch.cuda.device(like.device):
+            return rotary_backward(grad_q, grad_k, table, q, k, layout=layout, q_weight=q_weight, k_weight=k_weight,
+                                   eps=eps)
+    if _any(outs):
+        nbytes = lib.mo_rotary_workspace_bytes(ctypes.byref(call)) if q_weight is not None or k_weight is not None else 0
+        space = torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+        _native.check("mo_rotary_backward", lib.mo_rotary_backward(
+            ctypes.byref(call), 0 if space is None else space.data_ptr(), nbytes, _stream(like)))
     else:
         for grad in weight_grads:
             if grad is not None:

@@ -58,7 +58,7 @@ def test_quantizers_give_the_definition(rows, cols, dtype) -> None:
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(16, 16), (128, 256), (144, 400), (640, 48)])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (16, 16), (128, 256), (139, 400), (640, 48)])
 def test_weight_blocks_give_the_definition(rows, cols, dtype) -> None:
     w = _matrix(rows, cols, dtype) * 0.02
     values, scales = fp8.fp8_quantize_weight(w)
