@@ -22,8 +22,8 @@ namespace {
 using mo_fp8::kGroup;
 using mo_fp8::ProductArgs;
 
-enum Form { kFormRows, kFormColumns, kFormBoth, kFormWeight, kForms };
-const char* const kFormNames[kForms] = {"rows", "columns", "both", "weight"};
+enum Form { kFormRows, kFormFew, kFormColumns, kFormBoth, kFormWeight, kForms };
+const char* const kFormNames[kForms] = {"rows", "few", "columns", "both", "weight"};
 const char* const kTypeNames[3] = {"f16", "bf16", "f32"};  // by MO_DTYPE_*
 constexpr uint32_t kTypeBytes[3] = {2, 2, 4};
 
@@ -141,7 +141,9 @@ int quantize(const Module& m, Form form, uint64_t x, uint32_t dtype, uint64_t ro
   const void *X = (const void*)x, *RV = (const void*)rv, *RS = (const void*)rs, *CV = (const void*)cv,
              *CS = (const void*)cs;
   void* params[] = {&X, &rows, &cols, &stride, &RV, &RS, &CV, &CS};
-  return launch(m.quantize[form][dtype], div_up(rows, kGroup) * div_up(cols, kGroup), 256, params, stream,
+  // rows alone, fewer tiles than fill the CUs four at a time: 16 rows a workgroup
+  if (form == kFormRows && div_up(rows, kGroup) * div_up(cols, kGroup) < 4ull * m.cus) form = kFormFew;
+  return launch(m.quantize[form][dtype], div_up(rows, form == kFormFew ? 16 : kGroup) * div_up(cols, kGroup), 256, params, stream,
                 "fp8 quantize launch");
 }
 

@@ -132,13 +132,14 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
 // ---- quantizing -----------------------------------------------------------------------------------
 //
 // A workgroup takes a tile of 128 x 128 values, once, into registers: thread (g, c) holds rows 8 g to
-// 8 g + 7 of columns 8 c to 8 c + 7. A row's 16 threads are one DPP row, so its maximum takes four DPP
+// 8 g + 7 of columns 8 c to 8 c + 7 (kPer = 8; with kPer = 1, for few rows, one row, 16 a workgroup: eight times
+// the workgroups, 333 x 3072 in 3.5 us instead of 5.7). A row's 16 threads are one DPP row, so its maximum takes four DPP
 // steps; a column's maximum is taken over the thread's own rows, the four row groups of its wave, and
 // the waves through LDS. The columns' bytes are turned in LDS and leave as whole 128-byte lines.
 
 enum { kRows = 1, kColumns = 2, kBlock = 4 };
 
-template <class T, int kForm>
+template <class T, int kForm, int kPer>
 __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t rows, uint32_t cols, uint64_t stride,
                                               uint8_t* __restrict__ row_values, uint8_t* __restrict__ row_scales,
                                               uint8_t* __restrict__ col_values, uint8_t* __restrict__ col_scales) {
@@ -149,13 +150,14 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
   const uint64_t tile_r = blockIdx.x / tiles_c;
   const uint32_t tile_c = blockIdx.x % tiles_c;
   const int tid = threadIdx.x, c = tid & 15, g = tid >> 4, wave = tid >> 6;
-  const uint64_t row0 = tile_r * kGroup + 8 * g;
+  const uint64_t row0 = tile_r * 16 * kPer + kPer * g;
   const uint32_t col0 = tile_c * kGroup + 8 * c;
   const bool in_cols = col0 < cols;  // cols is a multiple of 16: a thread's eight are in or out
 
-  Bits<T> v[8];
+  static_assert(kPer == 8 || kForm == kRows, "groups down the columns take whole tiles");
+  Bits<T> v[kPer];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kPer; ++i) {
     if (in_cols && row0 + i < rows)
       v[i].load(x + (row0 + i) * stride + col0);
     else
@@ -165,7 +167,7 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
   if (kForm & kRows) {
     const uint64_t pitch = (rows + 15) & ~(uint64_t)15;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kPer; ++i) {
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i].get(j)));
@@ -183,7 +185,7 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
     }
   }
 
-  if (kForm & (kColumns | kBlock)) {
+  if constexpr ((kForm & (kColumns | kBlock)) != 0) {
     uint32_t m[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -240,17 +242,18 @@ __device__ __forceinline__ void quantize_tile(const T* __restrict__ x, uint64_t 
   }
 }
 
-#define MO_QUANTIZE(name, T, form)                                                                            \
+#define MO_QUANTIZE(name, T, form, per)                                                                            \
   extern "C" __global__ __launch_bounds__(256) void mo_fp8_quantize_##name(                                   \
       const T* x, uint64_t rows, uint32_t cols, uint64_t stride, uint8_t* row_values, uint8_t* row_scales,    \
       uint8_t* col_values, uint8_t* col_scales) {                                                             \
-    quantize_tile<T, form>(x, rows, cols, stride, row_values, row_scales, col_values, col_scales);            \
+    quantize_tile<T, form, per>(x, rows, cols, stride, row_values, row_scales, col_values, col_scales);            \
   }
 #define MO_QUANTIZE_FORMS(t, T)                     \
-  MO_QUANTIZE(rows_##t, T, kRows)                   \
-  MO_QUANTIZE(columns_##t, T, kColumns)             \
-  MO_QUANTIZE(both_##t, T, kRows | kColumns)        \
-  MO_QUANTIZE(weight_##t, T, kBlock)
+  MO_QUANTIZE(rows_##t, T, kRows, 8)                \
+  MO_QUANTIZE(few_##t, T, kRows, 1)                 \
+  MO_QUANTIZE(columns_##t, T, kColumns, 8)          \
+  MO_QUANTIZE(both_##t, T, kRows | kColumns, 8)     \
+  MO_QUANTIZE(weight_##t, T, kBlock, 8)
 MO_QUANTIZE_FORMS(f16, _Float16)
 MO_QUANTIZE_FORMS(bf16, __bf16)
 MO_QUANTIZE_FORMS(f32, float)

@@ -9,6 +9,7 @@
 #include <string>
 
 #include "../../include/moss_offload.h"
+#include "mo_layout.h"
 
 extern "C" const unsigned char mo_rotary_code[];
 
@@ -30,7 +31,6 @@ const uint32_t kVecs[4] = {1, 2, 4, 8};
 
 struct Module {
   hipModule_t module = nullptr;
-  int cus = 0;
   hipFunction_t turn[2][3][4] = {};  // [backward][type][kVecs index]; eight fp32 pairs have no kernel
   hipFunction_t weight_sum = nullptr, table = nullptr;
 };
@@ -48,8 +48,6 @@ int load_module(Module* out) {
     Module m;
     if ((e = hipModuleLoadData(&m.module, mo_rotary_code)) != hipSuccess)
       return mo::set_hip_error((int)e, "hipModuleLoadData (rotary code object)");
-    if ((e = hipDeviceGetAttribute(&m.cus, hipDeviceAttributeMultiprocessorCount, device)) != hipSuccess)
-      return mo::set_hip_error((int)e, "hipDeviceGetAttribute (CU count)");
     bool ok = (e = hipModuleGetFunction(&m.weight_sum, m.module, "mo_rotary_weight_sum")) == hipSuccess &&
               (e = hipModuleGetFunction(&m.table, m.module, "mo_rotary_table_kernel")) == hipSuccess;
     for (int back = 0; back < 2; ++back)
@@ -98,11 +96,16 @@ uint32_t pick_vec(const mo_rotary_call& c) {
   return v;
 }
 
+mo_rotary::Divisor divisor(uint32_t d) {
+  const mo::FastDiv f = mo::make_fastdiv(d);
+  return {f.d, f.m, f.s};
+}
+
 struct Plan {
   uint32_t vec, lanes, blocks[2];
 };
 
-Plan plan_of(const mo_rotary_call& c, bool backward, int cus) {
+Plan plan_of(const mo_rotary_call& c, bool backward) {
   Plan p = {};
   p.vec = pick_vec(c);
   const uint32_t held = c.head_dim / 2 / p.vec + (c.head_dim / 2 % p.vec != 0);
@@ -114,7 +117,6 @@ Plan plan_of(const mo_rotary_call& c, bool backward, int cus) {
     if (backward && c.side[i].weight && blocks > kMaxBlocks) blocks = kMaxBlocks;
     p.blocks[i] = (uint32_t)blocks;
   }
-  (void)cus;
   return p;
 }
 
@@ -156,7 +158,7 @@ int run(const mo_rotary_call* c, bool backward, uint64_t workspace, uint64_t wor
   if (int rc = check(c, backward)) return rc;
   Module m;
   if (int rc = load_module(&m)) return rc;
-  const Plan p = plan_of(*c, backward, m.cus);
+  const Plan p = plan_of(*c, backward);
   const uint64_t needed = backward ? partial_bytes(*c, p) : 0;
   if (needed && (!workspace || workspace % 256 || workspace_bytes < needed))
     return mo::set_error(MO_E_INVALID, "workspace missing, misaligned or smaller than mo_rotary_workspace_bytes");
@@ -170,7 +172,7 @@ int run(const mo_rotary_call* c, bool backward, uint64_t workspace, uint64_t wor
     d.x = (const void*)s.x, d.grad = (const void*)s.grad, d.out = (void*)s.out, d.weight = (const void*)s.weight;
     d.x_batch = s.x_batch, d.x_token = s.x_token, d.x_head = s.x_head;
     d.g_batch = s.grad_batch, d.g_token = s.grad_token, d.g_head = s.grad_head;
-    d.heads = s.heads, d.blocks = p.blocks[i];
+    d.heads = s.heads, d.blocks = p.blocks[i], d.by_heads = divisor(s.heads);
     if (backward && s.weight) {
       d.partial = (float*)at, d.weight_grad = (void*)s.weight_grad;
       at += (uint64_t)d.blocks * c->head_dim * 4;
@@ -180,6 +182,7 @@ int run(const mo_rotary_call* c, bool backward, uint64_t workspace, uint64_t wor
   a.table = (const void*)c->table, a.table_batch = c->table_batch;
   a.batch = c->batch, a.tokens = c->tokens, a.head_dim = c->head_dim, a.rotary_dim = c->rotary_dim;
   a.table_kind = c->table_dtype, a.weight_kind = c->weight_dtype, a.interleaved = c->interleaved, a.eps = c->eps;
+  a.by_tokens = divisor(c->tokens);
   uint32_t lanes = p.lanes, vec = 0;
   while (kVecs[vec] != p.vec) ++vec;
   void* params[] = {&a, &lanes};
@@ -188,7 +191,7 @@ int run(const mo_rotary_call* c, bool backward, uint64_t workspace, uint64_t wor
   if (e != hipSuccess) return mo::set_hip_error((int)e, "rotary launch");
   if (needed) {
     void* sums[] = {&a};
-    e = hipModuleLaunchKernel(m.weight_sum, (c->head_dim + 15) / 16, 2, 1, 256, 1, 1, 0, (hipStream_t)stream, sums,
+    e = hipModuleLaunchKernel(m.weight_sum, (c->head_dim + 15) / 16, 2, 1, 1024, 1, 1, 0, (hipStream_t)stream, sums,
                               nullptr);
     if (e != hipSuccess) return mo::set_hip_error((int)e, "rotary weight sum launch");
   }
@@ -203,7 +206,7 @@ uint64_t mo_rotary_workspace_bytes(const mo_rotary_call* call) {
   uint64_t bytes = 0;
   const int rc = guarded([&]() -> int {
     if (int bad = check(call, true)) return bad;
-    bytes = partial_bytes(*call, plan_of(*call, true, 0));
+    bytes = partial_bytes(*call, plan_of(*call, true));
     return 0;
   });
   return rc ? 0 : bytes;

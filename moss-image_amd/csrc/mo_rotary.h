@@ -7,6 +7,11 @@ namespace mo_rotary {
 constexpr uint32_t kMaxHead = 512;
 constexpr uint32_t kMaxBlocks = 1024;  // workgroups a side of a backward call with a norm: partial sums kept
 
+// Division of a number under 2^31 by a fixed one: (n + n m / 2^32) >> s (mo_layout.h makes m and s).
+struct Divisor {
+  uint32_t d, m, s;
+};
+
 // One side (queries or keys): tensors [batch][tokens][heads][head_dim], the last dimension dense.
 struct Side {
   const void* x;       // input (null in a backward call without a norm)
@@ -18,6 +23,7 @@ struct Side {
   int64_t x_batch, x_token, x_head;  // strides in elements
   int64_t g_batch, g_token, g_head;
   uint32_t heads, blocks;  // heads 0: no such side
+  Divisor by_heads;
 };
 
 struct Args {
@@ -28,6 +34,7 @@ struct Args {
   uint32_t table_kind, weight_kind;  // MO_DTYPE_*
   uint32_t interleaved;
   float eps;
+  Divisor by_tokens;
 };
 
 }  // namespace mo_rotary

@@ -100,10 +100,24 @@ struct Pairs {
   }
 };
 
-// Sum over `lanes` neighbouring lanes (a power of two, 1 to 64).
-__device__ __forceinline__ float sum_lanes(float v, int lanes) {
-  for (int d = 1; d < lanes; d <<= 1) v += __shfl_xor(v, d);
+// Sum over `lanes` neighbouring lanes (a power of two, 1 to 64), the same bits in each: within a row of 16 by
+// DPP (swapped neighbours, swapped pairs, mirrored halves, mirrored row), past it through the exchange unit.
+template <int kControl>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum_lanes(float v, uint32_t lanes) {
+  if (lanes > 1) v += dpp<0xB1>(v);
+  if (lanes > 2) v += dpp<0x4E>(v);
+  if (lanes > 4) v += dpp<0x141>(v);
+  if (lanes > 8) v += dpp<0x140>(v);
+  if (lanes > 16) v += __shfl_xor(v, 16);
+  if (lanes > 32) v += __shfl_xor(v, 32);
   return v;
+}
+
+__device__ __forceinline__ uint32_t divide(uint32_t n, const mo_rotary::Divisor& by) {
+  return (__umulhi(by.m, n) + n) >> by.s;
 }
 
 // Lanes of a head (a power of two) and the pairs a lane holds: kVec at a time, kIter times.
@@ -137,8 +151,8 @@ __device__ __forceinline__ void rotary(const Args& a, uint32_t lanes) {
   for (uint32_t first = blockIdx.x * per; first < rows; first += step) {
     const uint32_t row = first + threadIdx.x / lanes;
     const bool live = row < rows;
-    const uint32_t token = live ? row / side.heads : 0, head = live ? row % side.heads : 0;
-    const uint32_t b = token / a.tokens, t = token % a.tokens;
+    const uint32_t token = live ? divide(row, side.by_heads) : 0, head = live ? row - token * side.heads : 0;
+    const uint32_t b = divide(token, a.by_tokens), t = token - b * a.tokens;
     const T* x = (const T*)side.x + (int64_t)b * side.x_batch + (int64_t)t * side.x_token + (int64_t)head * side.x_head;
     const T* g = (const T*)side.grad + (int64_t)b * side.g_batch + (int64_t)t * side.g_token +
                  (int64_t)head * side.g_head;
@@ -256,19 +270,22 @@ MO_ROTARY(float, f32, 1)
 MO_ROTARY(float, f32, 2)
 MO_ROTARY(float, f32, 4)
 
-// The norm weights' gradients: the workgroups' sums of 16 values a workgroup, in a fixed order.
-extern "C" __global__ __launch_bounds__(256) void mo_rotary_weight_sum(Args a) {
-  __shared__ float sums[16][17];
+// The norm weights' gradients: the workgroups' sums of 16 values a workgroup, in a fixed order, 64 runs of
+// them side by side and then the runs.
+extern "C" __global__ __launch_bounds__(1024) void mo_rotary_weight_sum(Args a) {
+  __shared__ float sums[64][17];
   const Side& side = a.side[blockIdx.y];
   if (!side.weight_grad) return;
   const uint32_t e = blockIdx.x * 16 + threadIdx.x % 16, part = threadIdx.x / 16;
   float total = 0.0f;
-  if (e < a.head_dim)
-    for (uint32_t i = part; i < side.blocks; i += 16) total += side.partial[(uint64_t)i * a.head_dim + e];
+  if (e < a.head_dim) {
+#pragma unroll 8
+    for (uint32_t i = part; i < side.blocks; i += 64) total += side.partial[(uint64_t)i * a.head_dim + e];
+  }
   sums[part][threadIdx.x % 16] = total;
   __syncthreads();
   if (part || e >= a.head_dim) return;
-  for (int i = 1; i < 16; ++i) total += sums[i][threadIdx.x];
+  for (int i = 1; i < 64; ++i) total += sums[i][threadIdx.x];
   if (a.weight_kind == kF32)
     ((float*)side.weight_grad)[e] = total;
   else if (a.weight_kind == kBF16)

@@ -38,7 +38,7 @@ def _check_rows(values, scales, x):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 16), (2, 128), (77, 144), (128, 64), (129, 272), (300, 1040), (512, 640)])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (2, 128), (77, 144), (128, 64), (129, 272), (300, 1040), (512, 640), (4097, 4128)])
 def test_quantizers_give_the_definition(rows, cols, dtype) -> None:
     x = _matrix(rows, cols, dtype)
     x[rows // 2] = 0

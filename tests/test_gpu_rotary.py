@@ -59,7 +59,7 @@ def _close(got, exact, size, dtype, steps):
 # batch, tokens, query heads, key heads, head_dim, rotary_dim
 SHAPES = [(1, 1, 1, 1, 2, 2), (2, 3, 5, 1, 6, 2), (1, 7, 3, 3, 8, 8), (3, 5, 2, 4, 10, 6), (1, 33, 4, 2, 64, 64),
           (2, 17, 8, 2, 80, 40), (1, 130, 3, 3, 96, 48), (2, 65, 24, 24, 128, 128), (16, 1, 32, 8, 128, 64),
-          (1, 9, 2, 2, 256, 250), (1, 5, 3, 1, 512, 512), (1, 6, 2, 1, 510, 254), (1, 600, 7, 7, 128, 96)]
+          (1, 9, 2, 2, 256, 250), (1, 5, 3, 1, 512, 512), (1, 6, 2, 1, 510, 254), (1, 600, 7, 7, 128, 96), (2, 1100, 12, 4, 128, 96), (1, 2100, 8, 8, 40, 24)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
