@@ -600,9 +600,10 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
 uint64_t mo_fp8_workspace_bytes(uint32_t op, uint64_t rows, uint32_t in_features, uint32_t out_features,
                                 uint32_t quantized, uint32_t scale_kind, uint32_t out_dtype);
 
-/* The plan of a product [rows][cols] from a `reduction` on a device of `cus` CUs, host only: plan[0..2] = the
- * tile's edge, splits (workgroups a tile), groups of 128 of the reduction a split. The same call gives the
- * same bits every time. For tests and tools. */
+/* The launches of a product [rows][cols] from a `reduction` on a device of `cus` CUs, host only, first rows
+ * first: plan[4 i .. 4 i + 3] of launch i < 2 = its rows (0: no such launch), the tile's edge, splits (workgroups
+ * a tile), groups of 128 of the reduction a split. The same call gives the same bits every time. For tests
+ * and tools. */
 int mo_fp8_plan(uint64_t rows, uint32_t cols, uint32_t reduction, uint32_t scale_kind, uint32_t out_dtype, uint32_t cus,
                 uint32_t* plan);
 

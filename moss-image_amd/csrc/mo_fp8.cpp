@@ -53,8 +53,9 @@ constexpr TileShape kTileShapes[kTiles] = {
     {"middle", 128, 256, 2, {{4.1, 0.63, 0.54, 0.91}, {4.5, 0.46, 0.78, 1.19}, {4.5, 0.19, 0.91, 1.64}}},
     {"small", 64, 256, 4, {{3.1, 0.31, 0.32, 0.92}, {3.2, 0.32, 0.37, 1.00}, {3.2, 0.19, 0.44, 1.21}}},
 };
-// The sum of a split call's planes: fixed, a plane, a MB of planes.
-constexpr double kSumFixed = 1.1, kSumPlane = 0.26, kSumMb = 0.32;
+// The sum of a split call's planes: fixed (1.1 on the GPU; the launch takes the host 3.4, which calls this short
+// wait for), a plane, a MB of planes.
+constexpr double kSumFixed = 3.5, kSumPlane = 0.26, kSumMb = 0.32;
 constexpr uint32_t kMaxSplits = 32, kMinSplitSteps = 2;
 constexpr uint64_t kMaxPlanes = 1ull << 31;  // bytes
 
@@ -147,9 +148,15 @@ int quantize(const Module& m, Form form, uint64_t x, uint32_t dtype, uint64_t ro
                 "fp8 quantize launch");
 }
 
-struct Plan {
+// A product's launches: rows [row0, row0 + rows) on `tile`, the reduction in `splits` of `split_steps` groups.
+struct Part {
+  uint64_t row0, rows;
   int tile;
   uint32_t splits, split_steps;
+};
+struct Plan {
+  int parts;
+  Part part[2];
 };
 
 // Modelled time (us) of a call whose reduction is shared out over `splits` workgroups a tile, `per` steps each.
@@ -164,9 +171,10 @@ double cost_of(const TileShape& t, const Cost& c, uint64_t rows, uint64_t cols, 
   return us;
 }
 
-Plan plan_of(uint64_t rows, uint64_t cols, uint32_t steps, int kind, int cus) {
-  Plan best{0, 1, steps};
-  double best_us = 0;
+// The cheapest tile and splits for `rows` rows from row0 on; *us: the modelled time.
+Part part_of(uint64_t row0, uint64_t rows, uint64_t cols, uint32_t steps, int kind, int cus, double* us) {
+  Part best{row0, rows, 0, 1, steps};
+  *us = 0;
   for (int i = 0; i < kTiles; ++i) {
     const TileShape& t = kTileShapes[i];
     uint32_t tried = 0;
@@ -175,32 +183,60 @@ Plan plan_of(uint64_t rows, uint64_t cols, uint32_t steps, int kind, int cus) {
       const uint32_t per = (uint32_t)div_up(steps, want), splits = (uint32_t)div_up(steps, per);
       if (splits == tried) continue;
       tried = splits;
-      const double us = cost_of(t, t.cost[kind], rows, cols, splits, per, cus);
-      if (best_us == 0 || us < best_us) best = Plan{i, splits, per}, best_us = us;
+      const double c = cost_of(t, t.cost[kind], rows, cols, splits, per, cus);
+      if (*us == 0 || c < *us) best = Part{row0, rows, i, splits, per}, *us = c;
     }
   }
   return best;
+}
+
+// One launch, or two: the rows that fill whole rounds of the CUs with large tiles, and the rest on what suits
+// them. A last round that few tiles are left for costs as much as a full one (17792 rows of 3072 from 12288 are
+// 840 tiles, 3.3 rounds).
+Plan plan_of(uint64_t rows, uint64_t cols, uint32_t steps, int kind, int cus) {
+  double whole;
+  Plan plan{1, {part_of(0, rows, cols, steps, kind, cus, &whole), {}}};
+  const TileShape& t = kTileShapes[0];
+  const uint64_t tiles_m = div_up(rows, t.edge), tiles_n = div_up(cols, t.edge);
+  const uint64_t rounds = tiles_m * tiles_n / (uint64_t)cus, fill = rounds * (uint64_t)cus / tiles_n;
+  if (fill == 0 || fill >= tiles_m) return plan;
+  double rest;
+  const uint64_t head = fill * t.edge;
+  const Part tail = part_of(head, rows - head, cols, steps, kind, cus, &rest);
+  if (cost_of(t, t.cost[kind], head, cols, 1, steps, cus) + rest < whole)
+    plan = Plan{2, {Part{0, head, 0, 1, steps}, tail}};
+  return plan;
 }
 
 int cost_kind(int scales, uint32_t out_kind) {
   return out_kind == MO_DTYPE_F32 ? kCostWide : scales == kScaleFloats ? kCostFloats : kCostNarrow;
 }
 
-uint64_t plane_bytes(const Plan& p, uint64_t rows, uint64_t cols) {
-  return p.splits > 1 ? align(p.splits * rows * cols * 4) : 0;
+uint64_t plane_bytes(const Plan& p, uint64_t cols) {  // only the last part is split
+  const Part& last = p.part[p.parts - 1];
+  return last.splits > 1 ? align(last.splits * last.rows * cols * 4) : 0;
 }
 
 // `planes`: room for the plan's plane_bytes.
-int product(const Module& m, const Plan& plan, ProductArgs p, int scales, bool trans, uint64_t planes, uint64_t stream) {
-  const TileShape& t = kTileShapes[plan.tile];
-  p.splits = plan.splits, p.split_steps = plan.split_steps, p.planes = plan.splits > 1 ? (float*)planes : nullptr;
-  void* params[] = {&p};
-  if (int rc = launch(m.product[plan.tile][scales][p.out_kind == MO_DTYPE_F32][trans],
-                      div_up(p.m, t.edge) * div_up(p.n, t.edge) * plan.splits, t.threads, params, stream,
-                      "fp8 product launch"))
-    return rc;
-  if (plan.splits == 1) return 0;
-  return launch(m.sum, div_up(p.m * p.n / 4, 256), 256, params, stream, "fp8 plane sum launch");
+int product(const Module& m, const Plan& plan, const ProductArgs& whole, int scales, bool trans, uint64_t planes,
+            uint64_t stream) {
+  for (int i = 0; i < plan.parts; ++i) {
+    const Part& part = plan.part[i];
+    const TileShape& t = kTileShapes[part.tile];
+    ProductArgs p = whole;
+    p.a += part.row0 * p.a_pitch, p.a_scales += part.row0;
+    p.out = (uint8_t*)p.out + part.row0 * p.n * kTypeBytes[p.out_kind];
+    p.m = part.rows, p.splits = part.splits, p.split_steps = part.split_steps;
+    p.planes = part.splits > 1 ? (float*)planes : nullptr;
+    void* params[] = {&p};
+    if (int rc = launch(m.product[part.tile][scales][p.out_kind == MO_DTYPE_F32][trans],
+                        div_up(p.m, t.edge) * div_up(p.n, t.edge) * part.splits, t.threads, params, stream,
+                        "fp8 product launch"))
+      return rc;
+    if (part.splits == 1) continue;
+    if (int rc = launch(m.sum, div_up(p.m * p.n / 4, 256), 256, params, stream, "fp8 plane sum launch")) return rc;
+  }
+  return 0;
 }
 
 int check_weight(uint64_t w, uint64_t scale, uint32_t kind, uint32_t in_f, uint32_t out_f) {
@@ -264,7 +300,7 @@ Room room_of(uint32_t op, uint64_t rows, uint64_t in_f, uint64_t out_f, bool qua
   }
   const int scales = op == MO_FP8_WEIGHT ? kScaleRows : (int)scale_kind;
   r.plan = plan_of(m, n, (uint32_t)div_up(reduction, kGroup), cost_kind(scales, out_kind), cus);
-  r.planes = plane_bytes(r.plan, m, n);
+  r.planes = plane_bytes(r.plan, n);
   return r;
 }
 
@@ -294,7 +330,12 @@ int mo_fp8_plan(uint64_t rows, uint32_t cols, uint32_t reduction, uint32_t scale
     return mo::set_error(MO_E_INVALID, "empty shape, or too many rows");
   if (scale_kind > MO_FP8_SCALE_F32 || out_dtype > MO_DTYPE_F32) return mo::set_error(MO_E_INVALID, "unknown type");
   const Plan p = plan_of(rows, cols, (uint32_t)div_up(reduction, kGroup), cost_kind((int)scale_kind, out_dtype), (int)cus);
-  plan[0] = kTileShapes[p.tile].edge, plan[1] = p.splits, plan[2] = p.split_steps;
+  for (int i = 0; i < 2; ++i) {
+    const Part& part = p.part[i];
+    const bool on = i < p.parts;
+    plan[4 * i] = on ? (uint32_t)part.rows : 0, plan[4 * i + 1] = on ? kTileShapes[part.tile].edge : 0;
+    plan[4 * i + 2] = on ? part.splits : 0, plan[4 * i + 3] = on ? part.split_steps : 0;
+  }
   return 0;
 }
 

@@ -369,14 +369,15 @@ def fp8_weight_gradient(gradient, tokens, *, rows: int | None = None, dtype: tor
 
 
 def product_plan(rows: int, cols: int, reduction: int, cus: int, *, float_scales: bool = False,
-                 dtype: torch.dtype = torch.bfloat16) -> dict:
+                 dtype: torch.dtype = torch.bfloat16) -> list[dict]:
     """How a product ``[rows, cols]`` from a ``reduction`` runs on a device of ``cus`` CUs (``mo_fp8_plan``):
-    ``{"edge"}`` of the tile, ``"splits"`` of the reduction, ``"split_steps"`` of 128 each."""
+    one or two launches, each ``{"rows", "edge"}`` of its tile, ``"splits"`` of the reduction and
+    ``"split_steps"`` of 128 each."""
 
-    raw = (ctypes.c_uint32 * 3)()
+    raw = (ctypes.c_uint32 * 8)()
     kind = _native.MO_FP8_SCALE_F32 if float_scales else _native.MO_FP8_SCALE_E8M0
     _native.check("mo_fp8_plan", _native.load().mo_fp8_plan(rows, cols, reduction, kind, _CODES[dtype], cus, raw))
-    return dict(zip(("edge", "splits", "split_steps"), raw))
+    return [dict(zip(("rows", "edge", "splits", "split_steps"), raw[4 * i : 4 * i + 4])) for i in range(2) if raw[4 * i]]
 
 
 # ---- under autograd -------------------------------------------------------------------------------

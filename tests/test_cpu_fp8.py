@@ -116,9 +116,15 @@ def test_plans_cover_the_reduction() -> None:
                     for dtype in (torch.bfloat16, torch.float32):
                         plan = fp8.product_plan(rows, cols, reduction, cus, float_scales=floats, dtype=dtype)
                         steps = -(-reduction // 128)
-                        assert plan["edge"] in (64, 128, 256) and 1 <= plan["splits"] <= 32
-                        assert (plan["splits"] - 1) * plan["split_steps"] < steps <= plan["splits"] * plan["split_steps"]
-                        if plan["splits"] > 1:
-                            assert plan["split_steps"] >= 2 and plan["splits"] * rows * cols * 4 <= 1 << 31
-    assert fp8.product_plan(1, 3072, 12288, 256)["splits"] > 1
-    assert fp8.product_plan(4608, 24576, 3072, 256) == {"edge": 256, "splits": 1, "split_steps": 24}
+                        assert sum(part["rows"] for part in plan) == rows
+                        for part in plan:
+                            assert part["edge"] in (64, 128, 256) and 1 <= part["splits"] <= 32
+                            covered = part["splits"] * part["split_steps"]
+                            assert covered - part["split_steps"] < steps <= covered
+                            if part["splits"] > 1:
+                                assert part["split_steps"] >= 2 and part["splits"] * part["rows"] * cols * 4 <= 1 << 31
+                        if len(plan) == 2:  # whole rounds of large tiles first
+                            assert plan[0]["edge"] == 256 and plan[0]["splits"] == 1 and plan[0]["rows"] % 256 == 0
+    assert fp8.product_plan(1, 3072, 12288, 256)[0]["splits"] > 1
+    assert fp8.product_plan(4608, 24576, 3072, 256) == [{"rows": 4608, "edge": 256, "splits": 1, "split_steps": 24}]
+    assert [part["rows"] for part in fp8.product_plan(17792, 3072, 12288, 256)] == [16384, 1408]

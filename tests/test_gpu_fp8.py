@@ -215,6 +215,26 @@ def test_weight_gradient_matches_64_bits(rows, in_features, out_features) -> Non
         assert torch.equal(fp8.fp8_weight_gradient(*pairs, rows=rows, dtype=out), got)
 
 
+@pytest.mark.parametrize("kind", ["power", "float32"])
+def test_calls_in_two_launches_match_64_bits(kind) -> None:
+    """Rows past whole rounds of large tiles go to a second launch, its reduction split."""
+
+    rows, in_features, out_features = 17792 - 5, 6144, 3072 - 16
+    cus = torch.cuda.get_device_properties(DEV).multi_processor_count
+    plan = fp8.product_plan(rows, out_features, in_features, cus, float_scales=kind == "float32")
+    assert len(plan) == 2
+    weight, scale = _weight_of(out_features, in_features, kind, seed=3)
+    tokens = _matrix(rows, in_features, torch.bfloat16, seed=1)
+    bias = _matrix(1, out_features, torch.bfloat16, seed=2)[0]
+    got = fp8.fp8_linear_forward(tokens, weight, scale, bias)
+    b = model.decoded(weight, scale).t().contiguous()
+    one = torch.ones(512, 1, device=DEV, dtype=torch.float64)
+    edge = plan[0]["rows"]
+    for part in (slice(0, 512), slice(edge - 256, edge + 256), slice(rows - 512, rows)):
+        a = model.read_back(tokens[part])
+        _within(got[part], a @ b + bias.double(), torch.cat((a, one), 1), torch.cat((b, bias.double()[None]), 0))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_hot_operands_place_every_element(dtype) -> None:
     """The identity through the product reads the weight back, each element in its place, both ways."""
