@@ -9,6 +9,7 @@
 #include <string>
 
 #include "../../include/moss_offload.h"
+#include "mo_layout.h"
 
 extern "C" const unsigned char mo_fp8_code[];
 
@@ -381,8 +382,12 @@ int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t sca
     const void *V = (const void*)values, *S = (const void*)scales;
     void* O = (void*)out;
     uint32_t shift = block_rows == 1 ? 0 : 7;
-    void* params[] = {&V, &pitch, &S, &scale_kind, &scale_row, &scale_col, &shift, &O, &dtype, &rows, &cols};
-    return launch(m.decode, div_up(rows * div_up(cols, 16), 256), 256, params, stream, "fp8 decode launch");
+    const uint32_t across = (uint32_t)div_up(cols, 8);
+    const uint64_t total = rows * across;
+    const mo::FastDiv f = mo::make_fastdiv(across);
+    mo_fp8::Divisor chunks = {f.d, total + 255 < (1ull << 31) ? f.m : 0u, f.s};
+    void* params[] = {&V, &pitch, &S, &scale_kind, &scale_row, &scale_col, &shift, &O, &dtype, &rows, &cols, &chunks};
+    return launch(m.decode, div_up(total, 256), 256, params, stream, "fp8 decode launch");
   });
 }
 

@@ -7,6 +7,11 @@ namespace mo_fp8 {
 constexpr uint32_t kGroup = 128;                   // values that share a scale
 constexpr uint32_t kF16 = 0, kBF16 = 1, kF32 = 2;  // MO_DTYPE_*
 
+// Division of a number under 2^31 by a fixed one: (n + n m / 2^32) >> s (mo_layout.h makes m and s).
+struct Divisor {
+  uint32_t d, m, s;
+};
+
 // C[m][n] = sum_k A[m][k] B[n][k] under their scales (+ bias[n]); pitches in bytes, scale strides in
 // elements. B's scale of (n, group) is at (n >> b_shift) * b_scale_row + group * b_scale_col.
 struct ProductArgs {

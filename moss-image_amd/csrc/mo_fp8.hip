@@ -284,39 +284,51 @@ __device__ __forceinline__ float load1(const void* base, uint64_t at, uint32_t k
                                                                  : (float)((const _Float16*)base)[at];
 }
 
-// One lane reads 16 values and their scale and writes 16 products: bound by memory.
+// One lane reads eight values and their scale and writes eight products, 16 bytes (or twice that) in a row with
+// its neighbours': bound by memory. d: chunks of eight in a row, and its divisor while all chunks are under
+// 2^31 (m 0: a 64-bit division). Output rows that are not whole chunks go out value by value.
 extern "C" __global__ __launch_bounds__(256) void mo_fp8_decode_kernel(
     const uint8_t* __restrict__ values, uint64_t pitch, const void* __restrict__ scales, uint32_t f32_scales,
     uint64_t scale_row, uint64_t scale_col, uint32_t shift, void* __restrict__ out, uint32_t kind, uint64_t rows,
-    uint32_t cols) {
-  const uint32_t chunks = (cols + 15) / 16;
+    uint32_t cols, mo_fp8::Divisor chunks) {
   const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  const uint64_t row = at / chunks;
-  const uint32_t col = (uint32_t)(at % chunks) * 16;
+  const uint64_t row = chunks.m ? (__umulhi(chunks.m, (uint32_t)at) + (uint32_t)at) >> chunks.s : at / chunks.d;
+  const uint32_t col = (uint32_t)(at - row * chunks.d) * 8;
   if (row >= rows) return;
-  const u32x4 w = *(const u32x4*)(values + row * pitch + col);
+  const u32x2 w = *(const u32x2*)(values + row * pitch + col);
   const uint64_t s = (row >> shift) * scale_row + col / kGroup * scale_col;
   const float scale = f32_scales ? ((const float*)scales)[s] : scale_value(((const uint8_t*)scales)[s]);
-  const bool whole = col + 16 <= cols && cols % 4 == 0;
+  float v[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
     const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-    const f32x4 v = {lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
-    if (whole) {
-      store4(out, row * cols + col + 4 * i, v, kind);
-    } else {
-      for (int j = 0; j < 4; ++j) {
-        if (col + 4 * i + j >= cols) break;
-        const uint64_t o = row * cols + col + 4 * i + j;
-        if (kind == kF32)
-          ((float*)out)[o] = v[j];
-        else if (kind == kBF16)
-          ((__bf16*)out)[o] = (__bf16)v[j];
-        else
-          ((_Float16*)out)[o] = (_Float16)v[j];
-      }
+    v[4 * i] = lo[0] * scale, v[4 * i + 1] = lo[1] * scale, v[4 * i + 2] = hi[0] * scale, v[4 * i + 3] = hi[1] * scale;
+  }
+  const uint64_t to = row * cols + col;
+  if (cols % 8) {
+    for (uint32_t j = 0; j < 8 && col + j < cols; ++j) {
+      if (kind == kF32)
+        ((float*)out)[to + j] = v[j];
+      else if (kind == kBF16)
+        ((__bf16*)out)[to + j] = (__bf16)v[j];
+      else
+        ((_Float16*)out)[to + j] = (_Float16)v[j];
     }
+  } else if (kind == kF32) {
+    *(f32x4*)((float*)out + to) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)((float*)out + to + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else if (kind == kBF16) {
+    bf16x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
+    *(bf16x8*)((__bf16*)out + to) = o;
+  } else {
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    f16x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (_Float16)v[j];
+    *(f16x8*)((_Float16*)out + to) = o;
   }
 }
 
