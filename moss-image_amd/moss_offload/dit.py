@@ -12,6 +12,10 @@ forwards with the offload context around the traversal (:439-544), and selective
 checkpointing (:672-710, :780-789). LoRA follows ``training/lora.py:21-86`` and the int8
 weight-only base follows ``training/quantization.py:23-131`` (eager dequantisation).
 
+Two ways of running the blocks that the reference does not have, both off until asked for: a base
+in 8-bit floating point (``quantize_joint_linears_fp8``) and fused head norms and rotary positions
+(``configure_rotary``).
+
 It is test and benchmark harness code: random-initialised weights, synthetic inputs.
 """
 
@@ -92,6 +96,18 @@ def attention(query, key, value, rope, heads, cu_seqlens=None, seq_lengths=None)
     return mixed.transpose(1, 2).flatten(2)
 
 
+def attention_fused(query, key, value, rope, heads, q_norm, k_norm, cu_seqlens=None, seq_lengths=None):
+    """``attention`` on queries and keys before their head norms: norms and turns in one launch."""
+
+    from .rotary import rotary
+
+    query, key = (t.unflatten(-1, (heads, -1)) for t in (query, key))
+    query, key = rotary(query, key, rope, q_weight=q_norm.weight, k_weight=k_norm.weight)
+    value = value.unflatten(-1, (heads, -1)).transpose(1, 2)
+    mixed = _attention_core(query.transpose(1, 2), key.transpose(1, 2), value, cu_seqlens, seq_lengths)
+    return mixed.transpose(1, 2).flatten(2)
+
+
 def rope_coordinates(images, text_length: int, device) -> torch.Tensor:
     """``(r, t, h, w)`` per token: image grids (centred), then text (reference model.py:94-133)."""
 
@@ -143,6 +159,8 @@ def _linear_dtype(module: nn.Module) -> torch.dtype:
 class TextBlock(nn.Module):
     """Text adapter block with fused qkv (reference model.py:175-215)."""
 
+    rotary = "composed"
+
     def __init__(self, dim: int, ffn_dim: int, heads: int) -> None:
         super().__init__()
         self.heads = heads
@@ -155,9 +173,13 @@ class TextBlock(nn.Module):
 
     def forward(self, tokens, rope, cu_seqlens=None):
         query, key, value = self.qkv(self.norm1(tokens)).chunk(3, -1)
-        query = self.q_norm(query.unflatten(-1, (self.heads, -1))).flatten(2)
-        key = self.k_norm(key.unflatten(-1, (self.heads, -1))).flatten(2)
-        tokens = tokens + self.proj(attention(query, key, value, rope, self.heads, cu_seqlens))
+        if self.rotary == "hip":
+            mixed = attention_fused(query, key, value, rope, self.heads, self.q_norm, self.k_norm, cu_seqlens)
+        else:
+            query = self.q_norm(query.unflatten(-1, (self.heads, -1))).flatten(2)
+            key = self.k_norm(key.unflatten(-1, (self.heads, -1))).flatten(2)
+            mixed = attention(query, key, value, rope, self.heads, cu_seqlens)
+        tokens = tokens + self.proj(mixed)
         hidden = self.norm2(tokens)
         return tokens + self.ffn_down(situ(self.ffn_up(hidden), self.ffn_gate(hidden)))
 
@@ -205,6 +227,8 @@ class Block(nn.Module):
     per block instead of SiTU's six intermediates).
     """
 
+    rotary = "composed"
+
     def __init__(self, dim: int, ffn_dim: int, heads: int, mlp: str = "situ") -> None:
         super().__init__()
         if mlp not in MLP_VARIANTS:
@@ -227,9 +251,13 @@ class Block(nn.Module):
         hidden = hidden + _condition_for_tokens(shift_attn, index)
         weight_dtype = _linear_dtype(self.proj["q"])
         hidden = hidden.to(weight_dtype)
-        query = self.q_norm(self.proj["q"](hidden).unflatten(-1, (self.heads, -1))).flatten(2)
-        key = self.k_norm(self.proj["k"](hidden).unflatten(-1, (self.heads, -1))).flatten(2)
-        attended = attention(query, key, self.proj["v"](hidden), rope, self.heads, cu_seqlens, seq_lengths)
+        if self.rotary == "hip":
+            attended = attention_fused(self.proj["q"](hidden), self.proj["k"](hidden), self.proj["v"](hidden), rope,
+                                       self.heads, self.q_norm, self.k_norm, cu_seqlens, seq_lengths)
+        else:
+            query = self.q_norm(self.proj["q"](hidden).unflatten(-1, (self.heads, -1))).flatten(2)
+            key = self.k_norm(self.proj["k"](hidden).unflatten(-1, (self.heads, -1))).flatten(2)
+            attended = attention(query, key, self.proj["v"](hidden), rope, self.heads, cu_seqlens, seq_lengths)
         tokens = tokens + self.proj["o"](attended) * _condition_for_tokens(gate_attn, index)
         hidden = self.norm2(tokens)
         hidden = hidden * (1 + _condition_for_tokens(scale_ffn, index))
@@ -240,6 +268,21 @@ class Block(nn.Module):
             up, gate = self.proj["ffn_up_gate"](hidden.to(weight_dtype)).chunk(2, -1)
             activated = situ(up, gate)
         return tokens + self.proj["ffn_down"](activated) * _condition_for_tokens(gate_ffn, index)
+
+
+ROTARY_BACKENDS = ("composed", "hip")
+
+
+def configure_rotary(model: nn.Module, backend: str) -> int:
+    """How every block norms and turns its queries and keys: ``composed`` (the reference's operations,
+    the default) or ``hip`` (``moss_offload.rotary``, fp32 inside and rounded once). Returns the blocks set."""
+
+    if backend not in ROTARY_BACKENDS:
+        raise ValueError(f"rotary backend must be one of {ROTARY_BACKENDS}")
+    blocks = [module for module in model.modules() if isinstance(module, (Block, TextBlock))]
+    for block in blocks:
+        block.rotary = backend
+    return len(blocks)
 
 
 class RoPE(nn.Module):
@@ -555,6 +598,42 @@ class FrozenInt8Linear(nn.Module):
                                          self.quantized_backend)
 
 
+class FrozenFp8Linear(nn.Module):
+    """A frozen base linear in 8-bit floating point: e4m3 weights with a scale for each block of 128 x 128
+    (e8m0, or float32 from elsewhere), tokens quantized on the way in, no bias; the input gradient alone.
+    Features are multiples of 16. The reference's quantized bases are int8."""
+
+    def __init__(self, weight: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> None:
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self.register_buffer("weight_fp8", weight)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("_dtype_anchor", torch.empty(0, device=weight.device, dtype=dtype), persistent=False)
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, dtype: torch.dtype | None = None) -> "FrozenFp8Linear":
+        from .fp8_kernels import fp8_quantize_weight
+
+        return cls(*fp8_quantize_weight(weight.detach()), dtype or weight.dtype)
+
+    @property
+    def compute_dtype(self):
+        return self._dtype_anchor.dtype
+
+    def _apply(self, fn, recurse=True):
+        # a cast of the model changes the compute dtype; weights and scales stay in their formats
+        weight, scale = self.weight_fp8, self.weight_scale
+        result = super()._apply(fn, recurse=recurse)
+        device = self._dtype_anchor.device
+        self.weight_fp8, self.weight_scale = weight.to(device), scale.to(device)
+        return result
+
+    def forward(self, tokens):
+        from .fp8_kernels import fp8_linear
+
+        return fp8_linear(tokens.to(self.compute_dtype), self.weight_fp8, self.weight_scale, dtype=self.compute_dtype)
+
+
 def configure_quantized_backend(model: nn.Module, backend: str) -> list[str]:
     """Set the backend of every frozen int8 module; return their names (quantization.py:134-144)."""
 
@@ -576,7 +655,7 @@ def joint_linear_names(model: MOSSImageTransformer) -> list[str]:
     return [
         name
         for name, module in model.named_modules()
-        if isinstance(module, (nn.Linear, FrozenInt8Linear)) and name.startswith("layers.")
+        if isinstance(module, (nn.Linear, FrozenInt8Linear, FrozenFp8Linear)) and name.startswith("layers.")
     ]
 
 
@@ -632,6 +711,15 @@ def quantize_joint_linears(model: MOSSImageTransformer, generator: torch.Generat
         weight = torch.randint(-127, 128, (out_features, in_features), dtype=torch.int8, device=device, generator=generator)
         scale = torch.empty(out_features, dtype=torch.float16, device=device).uniform_(0.001, 0.02, generator=generator)
         _replace(model, name, FrozenInt8Linear(weight, scale.float(), dtype))
+    return names
+
+
+def quantize_joint_linears_fp8(model: MOSSImageTransformer) -> list[str]:
+    """Replace joint-block linears by ``FrozenFp8Linear`` of their own weights (on a HIP device)."""
+
+    names = [name for name in joint_linear_names(model) if isinstance(model.get_submodule(name), nn.Linear)]
+    for name in names:
+        _replace(model, name, FrozenFp8Linear.from_weight(model.get_submodule(name).weight))
     return names
 
 
