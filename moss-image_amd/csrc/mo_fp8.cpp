@@ -38,6 +38,7 @@ const char* const kScaleNames[3] = {"bytes", "floats", "rows"};
 // with all that fit. Fitted to 12 400 timed calls (110 shapes of 1 to 17 792 rows, every tile, 1 to 32
 // splits, eight kinds of operands, replayed back to back): the model's choice takes 1 % longer than the
 // fastest one on average, 4 % at the ninetieth percentile, 31 % at worst (199 rows of 3072 from 24576).
+// Those three were taken with 1.1 us as a sum's fixed part, before the host's launch was counted in.
 struct Cost {
   double fixed, again, alone, together;
 };

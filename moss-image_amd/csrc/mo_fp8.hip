@@ -135,7 +135,8 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
 // 8 g + 7 of columns 8 c to 8 c + 7 (kPer = 8; with kPer = 1, for few rows, one row, 16 a workgroup: eight times
 // the workgroups, 333 x 3072 in 3.5 us instead of 5.7). A row's 16 threads are one DPP row, so its maximum takes four DPP
 // steps; a column's maximum is taken over the thread's own rows, the four row groups of its wave, and
-// the waves through LDS. The columns' bytes are turned in LDS and leave as whole 128-byte lines.
+// the waves through LDS. Bound by memory: 17792 x 12288 bf16 both ways in 162 us (5.4 TB/s read and written), rows
+// alone 119 (5.5), columns alone 123. The columns' bytes are turned in LDS and leave as whole 128-byte lines.
 
 enum { kRows = 1, kColumns = 2, kBlock = 4 };
 
@@ -285,7 +286,7 @@ __device__ __forceinline__ float load1(const void* base, uint64_t at, uint32_t k
 }
 
 // One lane reads eight values and their scale and writes eight products, 16 bytes (or twice that) in a row with
-// its neighbours': bound by memory. d: chunks of eight in a row, and its divisor while all chunks are under
+// its neighbours': bound by memory, 17792 x 12288 to bf16 in 115 us (5.7 TB/s). d: chunks of eight in a row, and its divisor while all chunks are under
 // 2^31 (m 0: a 64-bit division). Output rows that are not whole chunks go out value by value.
 extern "C" __global__ __launch_bounds__(256) void mo_fp8_decode_kernel(
     const uint8_t* __restrict__ values, uint64_t pitch, const void* __restrict__ scales, uint32_t f32_scales,
@@ -362,6 +363,9 @@ extern "C" __global__ __launch_bounds__(256) void mo_fp8_decode_kernel(
 // 2^-126 count as zero, an infinite one as NaN.
 //
 // kWide (fp32 outputs): operands decoded to bf16 in registers, the power-of-two scales with them.
+// Large tile, 8192 x 8192 from 8192: 418 to 425 us, 2.6 PFLOP/s; the instructions alone reach 3.84 on such bytes,
+// held to 1.9 GHz by power, and are busy 66 % of the cycles here. Eight waves of 128 x 64 with the scales group by
+// group: 404 us at best, four waves of 128 x 128 without 490. fp32 scales: 16384 rows of 3072 from 12288 604 us.
 // Tiles are numbered in groups of kGroupM row tiles and then by XCD, so that the workgroups of one XCD
 // (blockIdx % 8) share rows and columns in its L2 (groups of 4, 8, 16 row tiles: 4608 rows of 24576 from 3072
 // 318, 325, 346 us; the other large calls differ by 1 %).

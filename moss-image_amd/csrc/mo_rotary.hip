@@ -12,7 +12,9 @@
 // type after every step. Bound by memory: one read and one write of the heads a direction (two reads and
 // one write backward with a norm), and the table from cache for all but one head of a token. So each lane
 // moves 16 bytes at a time: a head's row is shared out over the lanes of a part of a wave, kVec pairs a
-// lane, and the row's sums are taken by lane exchanges.
+// lane, and the row's sums are taken by lane exchanges. 4608 tokens, 24 heads of 128, bf16, both sides with norms: forward
+// 30.6 us (3.7 TB/s), backward 52.6 (3.2) and 4 for the weights' sums. Four heads a lane, which reads the angles once:
+// 44 and 77.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -295,7 +297,8 @@ extern "C" __global__ __launch_bounds__(1024) void mo_rotary_weight_sum(Args a) 
 }
 
 // Sines and cosines of coordinate x band, the product rounded to fp32 as the composed form rounds it, times
-// the amplitude: out[t] = axes * bands sines, then as many cosines. One lane an angle.
+// the amplitude: out[t] = axes * bands sines, then as many cosines. One lane an angle;
+// 4.0 us for 4608 rows of 64 angles, 2.0 for a few: a launch.
 extern "C" __global__ __launch_bounds__(256) void mo_rotary_table_kernel(const float* __restrict__ coordinates,
                                                                          const float* __restrict__ bands,
                                                                          void* __restrict__ out, uint64_t rows,

@@ -110,7 +110,9 @@ def _pair(pair: tuple[torch.Tensor, torch.Tensor], features: int, what: str) -> 
     if scales.shape != (rows, groups) or scales.get_device() != values.get_device():
         raise RuntimeError(f"quantized fp8 {what} must have one scale for each 128 values of a row, on its device.")
     if rows and (scales.stride(0) != 1 or groups > 1 and scales.stride(1) != -(-rows // 16) * 16
-                 or scales.data_ptr() % 4):
+                 or scales.data_ptr() % 4
+                 # a row's end is read in whole words
+                 or scales.untyped_storage().nbytes() - scales.storage_offset() < groups * (-(-rows // 16) * 16)):
         laid = _scales(rows, features, scales.device)
         laid.view(torch.uint8).copy_(scales.view(torch.uint8))
         scales = laid

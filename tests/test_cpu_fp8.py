@@ -128,3 +128,16 @@ def test_plans_cover_the_reduction() -> None:
     assert fp8.product_plan(1, 3072, 12288, 256)[0]["splits"] > 1
     assert fp8.product_plan(4608, 24576, 3072, 256) == [{"rows": 4608, "edge": 256, "splits": 1, "split_steps": 24}]
     assert [part["rows"] for part in fp8.product_plan(17792, 3072, 12288, 256)] == [16384, 1408]
+
+
+@pytest.mark.parametrize("rows", [1, 5, 16, 17])
+@pytest.mark.parametrize("spare", [0, 2])
+def test_tight_scales_are_laid_out_again(rows, spare):
+    from moss_offload import fp8_kernels
+
+    room = torch.arange(rows + spare, dtype=torch.uint8).add(100)
+    tight = room.view(torch.float8_e8m0fnu)[:rows].unsqueeze(1)
+    values = torch.zeros(rows, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    scales = fp8_kernels._pair((values, tight), 128, "tokens")[1]
+    assert scales.untyped_storage().nbytes() - scales.storage_offset() >= -(-rows // 16) * 16
+    assert torch.equal(scales.view(torch.uint8), tight.view(torch.uint8))
