@@ -406,7 +406,9 @@ class _FrozenFunction(torch.autograd.Function):
 
 class _TrainedFunction(torch.autograd.Function):
     """A weight in training: quantized for the call; the tokens are kept in 8 bits, turned for the weight
-    gradient (half the bytes that a bfloat16 linear keeps), and the weight's 8 bits for the input gradient."""
+    gradient (half the bytes that a bfloat16 linear keeps), and the weight's 8 bits for the input gradient.
+    What is kept carries no graph, while the tokens' gradient depends on the weight and the weight's on the
+    tokens: where both are wanted, a backward that should build a graph is refused."""
 
     @staticmethod
     def forward(ctx, tokens, weight, bias, dtype):
@@ -414,6 +416,7 @@ class _TrainedFunction(torch.autograd.Function):
         ctx.input_dtype, ctx.weight_dtype = tokens.dtype, weight.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.rows = tokens.shape[:-1].numel()
+        ctx.both = ctx.needs_input_grad[0] and ctx.needs_input_grad[1]
         if ctx.needs_input_grad[1]:
             tokens, columns = fp8_quantize_both(tokens)
         else:
@@ -423,6 +426,8 @@ class _TrainedFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gradient):
+        if ctx.both and torch.is_grad_enabled():
+            raise RuntimeError("fp8_linear has no second derivatives for a weight in training (create_graph=True).")
         values, scale, *columns = ctx.saved_tensors
         tokens = weight = bias = None
         if ctx.needs_input_grad[2]:

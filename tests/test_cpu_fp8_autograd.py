@@ -1,0 +1,70 @@
+"""``fp8_linear`` under autograd on the CPU: the library's calls are taken by a stand-in that computes nothing, so
+what is checked is which calls are made, what they are given, and what autograd makes of them."""
+
+from __future__ import annotations
+
+from collections import Counter
+
+import pytest
+import torch
+
+from moss_offload import fp8_kernels as fp8
+
+
+class _Library:
+    """Every entry point: counts the call and keeps its last arguments."""
+
+    def __init__(self):
+        self.calls, self.last = Counter(), {}
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls[name] += 1
+            self.last[name] = args
+            return 256 if name.endswith("_bytes") else 0
+
+        return call
+
+
+@pytest.fixture
+def library(monkeypatch):
+    library = _Library()
+    monkeypatch.setattr(fp8._native, "load", lambda: library)
+    monkeypatch.setattr(fp8, "_elsewhere", lambda tensor: False)
+    monkeypatch.setattr(fp8, "_stream", lambda tensor: 0)
+    fp8._workspace_bytes.cache_clear()
+    yield library
+    fp8._workspace_bytes.cache_clear()
+
+
+def _operands(*lead, dtype=torch.float32):
+    return torch.zeros(*lead, 144, dtype=dtype).requires_grad_(), torch.zeros(32, 144).requires_grad_()
+
+
+# ---- second derivatives ---------------------------------------------------------------------------
+
+
+def test_a_graph_through_a_trained_weights_backward_is_refused(library) -> None:
+    """The incoming gradient of a sum needs no graph, but the tokens' gradient depends on the weight: a penalty on
+    it would lose its term in the weight's gradient."""
+
+    for wanted in (0, 1, (0, 1)):
+        leaves = _operands(5)
+        y = fp8.fp8_linear(*leaves)
+        inputs = [leaves[i] for i in (wanted if isinstance(wanted, tuple) else (wanted,))]
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(y.sum(), inputs, create_graph=True)
+    tokens, master = _operands(5)
+    with pytest.raises(RuntimeError):
+        fp8.fp8_linear(tokens, master).square().sum().backward(create_graph=True)
+
+
+def test_first_derivatives_and_constant_ones_are_not(library) -> None:
+    tokens, master = _operands(5)
+    grads = torch.autograd.grad(fp8.fp8_linear(tokens, master).sum(), [tokens, master])
+    assert [g.shape for g in grads] == [tokens.shape, master.shape]
+    # nothing that the gradient depends on wants one
+    (grad,) = torch.autograd.grad(fp8.fp8_linear(tokens, master.detach()).sum(), [tokens], create_graph=True)
+    assert not grad.requires_grad
+    (grad,) = torch.autograd.grad(fp8.fp8_linear(tokens.detach(), master).sum(), [master], create_graph=True)
+    assert not grad.requires_grad
