@@ -61,7 +61,8 @@ def _scales(rows: int, size: int, device) -> torch.Tensor:
 
 def _plain(*operands: torch.Tensor | None) -> None:
     if not _by_address(*operands):
-        raise RuntimeError("fp8 operands must be plain tensors without a graph or a tangent; fp8_linear has a gradient.")
+        raise RuntimeError("fp8 operands must be plain tensors without a graph or a tangent; fp8_linear has a gradient "
+                           "(none for a block-scaled weight or its scales).")
 
 
 def _rows(tensor: torch.Tensor, what: str) -> torch.Tensor:
@@ -86,6 +87,7 @@ def _stride(matrix: torch.Tensor) -> int:
 def _weight(weight: torch.Tensor, scale: torch.Tensor) -> int:
     """The scale kind of a block-scaled weight, after its checks: every kernel takes it by address."""
 
+    _plain(weight, scale)
     if weight.ndim != 2 or weight.dtype != E4M3 or not weight.is_contiguous() or weight.data_ptr() % 16:
         raise RuntimeError("fp8 weight must be a contiguous, 16-byte aligned float8_e4m3fn matrix.")
     if weight.shape[0] % 16 or weight.shape[1] % 16 or not weight.numel():
@@ -446,11 +448,13 @@ class _TrainedFunction(torch.autograd.Function):
 
 def fp8_linear(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, *, dtype: torch.dtype | None = None) -> torch.Tensor:
-    """A linear in 8-bit floating point with its gradients. With ``scale``: a frozen block-scaled weight.
+    """A linear in 8-bit floating point with its gradients. With ``scale``: a frozen block-scaled weight; one that
+    wants a gradient, or whose scales do, is refused.
     Without: ``weight`` is ``[out, in]`` in bfloat16, float16 or float32, quantized for the call, and gets
     a gradient of its own type. ``dtype``: the result's (the tokens' own)."""
 
     dtype = dtype or tokens.dtype
     if scale is not None:
+        _plain(weight, scale)  # seen here: inside the function grad mode is off
         return _FrozenFunction.apply(tokens, weight, scale, bias, dtype)
     return _TrainedFunction.apply(tokens, weight, bias, dtype)

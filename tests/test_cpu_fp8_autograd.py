@@ -68,3 +68,44 @@ def test_first_derivatives_and_constant_ones_are_not(library) -> None:
     assert not grad.requires_grad
     (grad,) = torch.autograd.grad(fp8.fp8_linear(tokens.detach(), master).sum(), [master], create_graph=True)
     assert not grad.requires_grad
+
+
+# ---- a frozen weight ------------------------------------------------------------------------------
+
+
+def _frozen():
+    return torch.zeros(32, 144).to(torch.float8_e4m3fn), torch.ones(1, 2)
+
+
+def test_a_frozen_weight_or_scale_that_wants_a_gradient_is_refused(library) -> None:
+    """Both go to the kernels by address: a learnable scale would get no gradient."""
+
+    weight, scale = _frozen()
+    tokens, gradient = torch.zeros(4, 144), torch.zeros(4, 32)
+    learnt = scale.clone().requires_grad_()
+    calls = [
+        (fp8.fp8_linear_forward, (tokens, weight, learnt)),
+        (fp8.fp8_linear_backward, (gradient, weight, learnt)),
+        (fp8.fp8_linear, (tokens, weight, learnt)),
+        (fp8.fp8_linear, (tokens.clone().requires_grad_(), weight, learnt)),
+        (fp8.fp8_linear, (tokens, weight, (2 * learnt))),
+        (fp8.fp8_linear, (tokens, weight.clone().requires_grad_(), scale)),
+        (fp8.fp8_linear_forward, (tokens, weight.clone().requires_grad_(), scale)),
+    ]
+    for call, operands in calls:
+        with pytest.raises(RuntimeError, match="graph"):
+            call(*operands)
+    assert not library.calls
+    with torch.no_grad():  # no graph is wanted
+        fp8.fp8_linear(tokens, weight, learnt)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(scale, torch.ones_like(scale))
+        with pytest.raises(RuntimeError, match="graph"):
+            fp8.fp8_linear_forward(tokens, weight, dual)
+
+
+def test_a_frozen_weight_gives_the_tokens_their_gradient(library) -> None:
+    weight, scale = _frozen()
+    tokens = torch.zeros(4, 144).requires_grad_()
+    (grad,) = torch.autograd.grad(fp8.fp8_linear(tokens, weight, scale).sum(), [tokens])
+    assert grad.shape == tokens.shape and library.calls["mo_fp8_linear_backward"] == 1
