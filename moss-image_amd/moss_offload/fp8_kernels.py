@@ -105,10 +105,10 @@ def _pair(pair: tuple[torch.Tensor, torch.Tensor], features: int, what: str) -> 
     values, scales = pair
     if values.dtype != E4M3 or scales.dtype != E8M0 or values.ndim < 2 or values.shape[-1] != features:
         raise RuntimeError(f"quantized fp8 {what} must be float8_e4m3fn of {features} features with float8_e8m0fnu scales.")
-    values = values.reshape(-1, features).contiguous()
+    rows, groups = values.shape[:-1].numel(), _groups(features)
+    values = values.reshape(rows, features).contiguous()  # the rows of no tokens hold nothing: -1 would be ambiguous
     if values.data_ptr() % 16:
         values = values.clone()
-    rows, groups = values.shape[0], _groups(features)
     if scales.shape != (rows, groups) or scales.get_device() != values.get_device():
         raise RuntimeError(f"quantized fp8 {what} must have one scale for each 128 values of a row, on its device.")
     if rows and (scales.stride(0) != 1 or groups > 1 and scales.stride(1) != -(-rows // 16) * 16

@@ -109,3 +109,29 @@ def test_a_frozen_weight_gives_the_tokens_their_gradient(library) -> None:
     tokens = torch.zeros(4, 144).requires_grad_()
     (grad,) = torch.autograd.grad(fp8.fp8_linear(tokens, weight, scale).sum(), [tokens])
     assert grad.shape == tokens.shape and library.calls["mo_fp8_linear_backward"] == 1
+
+
+# ---- no tokens ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lead", [(0,), (2, 0), (0, 3)])
+@pytest.mark.parametrize("trained", [False, True])
+def test_no_tokens_have_gradients_without_a_launch(library, lead, trained) -> None:
+    tokens, master = _operands(*lead)
+    bias = torch.zeros(32).requires_grad_()
+    operands = (tokens, master, None, bias) if trained else (tokens, *_frozen(), bias)
+    y = fp8.fp8_linear(*operands)
+    assert y.shape == (*lead, 32)
+    wanted = [tokens, bias, *([master] if trained else [])]
+    grads = torch.autograd.grad(y.sum(), wanted)
+    assert [g.shape for g in grads] == [t.shape for t in wanted]
+    assert not any(g.any() for g in grads)
+    assert not [name for name in library.calls if "linear" in name or "gradient" in name]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_tokens_weight_gradient_of_pairs_is_zero(library, dtype) -> None:
+    pairs = [fp8.fp8_quantize_columns(torch.zeros(0, features)) for features in (32, 144)]
+    out = torch.ones(32, 144, dtype=dtype)
+    got = fp8.fp8_weight_gradient(*pairs, rows=0, dtype=dtype, out=out)
+    assert got.data_ptr() == out.data_ptr() and not out.any()
