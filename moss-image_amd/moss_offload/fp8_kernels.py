@@ -103,7 +103,7 @@ def _pair(pair: tuple[torch.Tensor, torch.Tensor], features: int, what: str) -> 
     """A quantized operand as the kernels read it: dense rows, scales group by group."""
 
     values, scales = pair
-    if values.dtype != E4M3 or scales.dtype != E8M0 or values.ndim < 2 or values.shape[-1] != features:
+    if values.dtype != E4M3 or scales.dtype != E8M0 or values.ndim < 1 or values.shape[-1] != features:
         raise RuntimeError(f"quantized fp8 {what} must be float8_e4m3fn of {features} features with float8_e8m0fnu scales.")
     rows, groups = values.shape[:-1].numel(), _groups(features)
     values = values.reshape(rows, features).contiguous()  # the rows of no tokens hold nothing: -1 would be ambiguous
@@ -176,8 +176,8 @@ def _quantize(x: torch.Tensor, rows: bool, columns: bool):
 
 
 def fp8_quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """``(values, scales)`` of a matrix (or rows of any leading shape) in groups of 128 along its rows:
-    values of ``x``'s shape, one scale ``[rows, ceil(cols / 128)]``."""
+    """``(values, scales)`` of a matrix (or rows of any leading shape, or one row) in groups of 128 along its
+    rows: values of ``x``'s shape, one scale ``[rows, ceil(cols / 128)]``."""
 
     return _quantize(x, True, False)[0]
 
@@ -223,7 +223,7 @@ def fp8_decode(values: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype
 
     lib = _native.load()
     _plain(values, scales)
-    if values.dtype != E4M3 or values.ndim < 2 or scales.dtype not in (E8M0, torch.float32) or scales.ndim != 2:
+    if values.dtype != E4M3 or values.ndim < 1 or scales.dtype not in (E8M0, torch.float32) or scales.ndim != 2:
         raise TypeError("fp8_decode takes float8_e4m3fn values with float8_e8m0fnu or float32 scales.")
     if dtype not in _CODES:
         raise TypeError(f"fp8 output must be bfloat16, float16 or float32 (got {dtype}).")
@@ -387,6 +387,10 @@ def product_plan(rows: int, cols: int, reduction: int, cus: int, *, float_scales
 # ---- under autograd -------------------------------------------------------------------------------
 
 
+def _bias_gradient(gradient: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return gradient.reshape(-1, gradient.shape[-1]).sum(0, dtype=torch.float32).to(dtype)
+
+
 class _FrozenFunction(torch.autograd.Function):
     """A frozen weight: saves the weight and its scales, which are the module's own buffers."""
 
@@ -402,7 +406,7 @@ class _FrozenFunction(torch.autograd.Function):
         weight, scale = ctx.saved_tensors
         wanted, bias_wanted = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
         tokens = fp8_linear_backward(gradient, weight, scale, dtype=ctx.input_dtype) if wanted else None
-        bias = gradient.flatten(0, -2).sum(0, dtype=torch.float32).to(ctx.bias_dtype) if bias_wanted else None
+        bias = _bias_gradient(gradient, ctx.bias_dtype) if bias_wanted else None
         return tokens, None, None, bias, None
 
 
@@ -433,7 +437,7 @@ class _TrainedFunction(torch.autograd.Function):
         values, scale, *columns = ctx.saved_tensors
         tokens = weight = bias = None
         if ctx.needs_input_grad[2]:
-            bias = gradient.flatten(0, -2).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+            bias = _bias_gradient(gradient, ctx.bias_dtype)
         rows, turned = gradient, None
         if ctx.needs_input_grad[0] and ctx.needs_input_grad[1]:
             rows, turned = fp8_quantize_both(gradient)

@@ -135,3 +135,30 @@ def test_no_tokens_weight_gradient_of_pairs_is_zero(library, dtype) -> None:
     out = torch.ones(32, 144, dtype=dtype)
     got = fp8.fp8_weight_gradient(*pairs, rows=0, dtype=dtype, out=out)
     assert got.data_ptr() == out.data_ptr() and not out.any()
+
+
+# ---- a vector of tokens ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("trained", [False, True])
+def test_a_vector_of_tokens_is_one_row(library, trained, biased) -> None:
+    tokens, master = _operands()
+    bias = torch.zeros(32).requires_grad_() if biased else None
+    operands = (tokens, master, None, bias) if trained else (tokens, *_frozen(), bias)
+    y = fp8.fp8_linear(*operands)
+    assert y.shape == (32,)
+    wanted = [tokens, *([bias] if biased else []), *([master] if trained else [])]
+    grads = torch.autograd.grad(y.sum(), wanted)
+    assert [g.shape for g in grads] == [t.shape for t in wanted]
+    if biased:
+        assert torch.equal(grads[1], torch.ones(32))
+    assert library.last["mo_fp8_linear_backward"][3] == 1
+    assert not trained or library.last["mo_fp8_weight_gradient"][8] == 1
+
+
+def test_a_vectors_pair_is_taken_and_read_back(library) -> None:
+    pair = fp8.fp8_quantize_rows(torch.zeros(144))
+    assert pair[0].shape == (144,) and pair[1].shape == (1, 2)
+    assert fp8.fp8_linear_forward(pair, *_frozen()).shape == (32,)
+    assert fp8.fp8_decode(*pair).shape == (144,)
