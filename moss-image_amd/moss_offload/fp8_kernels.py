@@ -417,8 +417,10 @@ class _TrainedFunction(torch.autograd.Function):
     tokens: where both are wanted, a backward that should build a graph is refused."""
 
     @staticmethod
-    def forward(ctx, tokens, weight, bias, dtype):
+    def forward(ctx, tokens, weight, bias, dtype, graph):
         values, scale = fp8_quantize_weight(weight)
+        if not graph:  # needs_input_grad is set all the same
+            return fp8_linear_forward(tokens, values, scale, bias, dtype=dtype)
         ctx.input_dtype, ctx.weight_dtype = tokens.dtype, weight.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.rows = tokens.shape[:-1].numel()
@@ -447,7 +449,7 @@ class _TrainedFunction(torch.autograd.Function):
             tokens = fp8_linear_backward(rows, values, scale, dtype=ctx.input_dtype)
         if ctx.needs_input_grad[1]:
             weight = fp8_weight_gradient(turned, tuple(columns), rows=ctx.rows, dtype=ctx.weight_dtype)
-        return tokens, weight, bias, None
+        return tokens, weight, bias, None, None
 
 
 def fp8_linear(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor | None = None,
@@ -461,4 +463,4 @@ def fp8_linear(tokens: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor |
     if scale is not None:
         _plain(weight, scale)  # seen here: inside the function grad mode is off
         return _FrozenFunction.apply(tokens, weight, scale, bias, dtype)
-    return _TrainedFunction.apply(tokens, weight, bias, dtype)
+    return _TrainedFunction.apply(tokens, weight, bias, dtype, torch.is_grad_enabled())

@@ -162,3 +162,23 @@ def test_a_vectors_pair_is_taken_and_read_back(library) -> None:
     assert pair[0].shape == (144,) and pair[1].shape == (1, 2)
     assert fp8.fp8_linear_forward(pair, *_frozen()).shape == (32,)
     assert fp8.fp8_decode(*pair).shape == (144,)
+
+
+# ---- without a graph ------------------------------------------------------------------------------
+
+
+def test_evaluation_on_a_trained_weight_makes_no_columns(library) -> None:
+    """The transposed copy is the weight gradient's alone."""
+
+    tokens, master = _operands(5)
+    bias = torch.zeros(32).requires_grad_()
+    for mode in (torch.no_grad, torch.inference_mode):
+        library.calls.clear()
+        with mode():
+            y = fp8.fp8_linear(tokens, master, None, bias)
+        assert y.shape == (5, 32) and not y.requires_grad
+        assert library.calls["mo_fp8_linear_forward"] == library.calls["mo_fp8_quantize_weight"] == 1
+        assert not library.calls["mo_fp8_quantize"]
+    with torch.enable_grad():
+        fp8.fp8_linear(tokens, master, None, bias)
+    assert library.calls["mo_fp8_quantize"] == 1 and library.last["mo_fp8_quantize"][7]
