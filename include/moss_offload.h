@@ -596,7 +596,9 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
 
 /* Bytes of a call's workspace on the current device: the operands it quantizes, and the fp32 planes of a
  * reduction that its plan shares out over workgroups. `quantized`: the operands are given so; out_dtype: the
- * result's. */
+ * result's. 0: none is needed, or no call takes these arguments. MO_FP8_NO_SIZE: the device could not be asked
+ * (mo_last_error). */
+#define MO_FP8_NO_SIZE UINT64_MAX
 uint64_t mo_fp8_workspace_bytes(uint32_t op, uint64_t rows, uint32_t in_features, uint32_t out_features,
                                 uint32_t quantized, uint32_t scale_kind, uint32_t out_dtype);
 

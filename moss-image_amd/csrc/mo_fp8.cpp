@@ -313,7 +313,7 @@ extern "C" {
 uint64_t mo_fp8_workspace_bytes(uint32_t op, uint64_t rows, uint32_t in_features, uint32_t out_features,
                                 uint32_t quantized, uint32_t scale_kind, uint32_t out_dtype) {
   if (op > MO_FP8_WEIGHT || rows == 0 || rows >= (1ull << 31) || in_features == 0 || out_features == 0 ||
-      scale_kind > MO_FP8_SCALE_F32 || out_dtype > MO_DTYPE_F32)
+      in_features > (1u << 20) || out_features > (1u << 20) || scale_kind > MO_FP8_SCALE_F32 || out_dtype > MO_DTYPE_F32)
     return 0;
   uint64_t bytes = 0;
   const int rc = guarded([&]() -> int {
@@ -322,7 +322,7 @@ uint64_t mo_fp8_workspace_bytes(uint32_t op, uint64_t rows, uint32_t in_features
     bytes = room_of(op, rows, in_features, out_features, quantized != 0, scale_kind, out_dtype, m.cus).bytes();
     return 0;
   });
-  return rc ? 0 : bytes;
+  return rc ? MO_FP8_NO_SIZE : bytes;
 }
 
 int mo_fp8_plan(uint64_t rows, uint32_t cols, uint32_t reduction, uint32_t scale_kind, uint32_t out_dtype, uint32_t cus,

@@ -42,6 +42,7 @@ MO_FP8_SCALE_F32 = 1
 MO_FP8_FORWARD = 0
 MO_FP8_BACKWARD = 1
 MO_FP8_WEIGHT = 2
+MO_FP8_NO_SIZE = (1 << 64) - 1
 
 DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # MO_DTYPE_*
 

@@ -136,7 +136,11 @@ def _output(out: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(op: int, rows: int, in_features: int, out_features: int, quantized: bool, kind: int, code: int,
                      device: int) -> int:
-    return _native.load().mo_fp8_workspace_bytes(op, rows, in_features, out_features, int(quantized), kind, code)
+    lib = _native.load()
+    nbytes = lib.mo_fp8_workspace_bytes(op, rows, in_features, out_features, int(quantized), kind, code)
+    if nbytes == _native.MO_FP8_NO_SIZE:  # an exception is not cached: the next call asks again
+        raise _native.EngineError("mo_fp8_workspace_bytes", -1, lib.mo_last_error().decode(errors="replace"))
+    return nbytes
 
 
 def _workspace(op: int, rows: int, in_features: int, out_features: int, quantized: bool, kind: int, dtype: torch.dtype,

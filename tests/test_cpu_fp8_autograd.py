@@ -8,7 +8,7 @@ from collections import Counter
 import pytest
 import torch
 
-from moss_offload import fp8_kernels as fp8
+from moss_offload import _native, fp8_kernels as fp8
 
 
 class _Library:
@@ -182,3 +182,30 @@ def test_evaluation_on_a_trained_weight_makes_no_columns(library) -> None:
     with torch.enable_grad():
         fp8.fp8_linear(tokens, master, None, bias)
     assert library.calls["mo_fp8_quantize"] == 1 and library.last["mo_fp8_quantize"][7]
+
+
+# ---- workspaces -----------------------------------------------------------------------------------
+
+
+def test_a_workspace_that_could_not_be_sized_is_asked_for_again(library) -> None:
+    weight, scale = _frozen()
+    tokens = torch.zeros(4, 144)
+    answers = [_native.MO_FP8_NO_SIZE, 4096]
+    library.mo_fp8_workspace_bytes = lambda *args: answers.pop(0)
+    library.mo_last_error = lambda: b"no device"
+    with pytest.raises(_native.EngineError, match="no device"):
+        fp8.fp8_linear_forward(tokens, weight, scale)
+    assert not library.calls["mo_fp8_linear_forward"]
+    for _ in range(2):  # and kept then
+        fp8.fp8_linear_forward(tokens, weight, scale)
+        assert library.last["mo_fp8_linear_forward"][14] == 4096
+    assert not answers
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="asks a library without a device")
+def test_the_library_tells_a_failure_from_no_room() -> None:
+    lib = _native.load()
+    assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, 4, 144, 32, 1, 0, 1) == _native.MO_FP8_NO_SIZE
+    assert lib.mo_last_error()
+    for sizes in ((4, 144, 1 << 21), (4, 1 << 21, 32), (4, 0, 32), (1 << 31, 144, 32)):
+        assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, *sizes, 0, 0, 1) == 0
