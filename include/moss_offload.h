@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MO_ABI_VERSION 24
+#define MO_ABI_VERSION 25
 #define MO_MAX_DIMS 8
 
 /* Error codes outside the hipError_t range. */
@@ -550,6 +550,7 @@ int mo_int8_strip_plan(uint32_t rows, uint32_t cols, uint32_t reduction, uint32_
  * (below). */
 enum { MO_FP8_SCALE_E8M0 = 0, MO_FP8_SCALE_F32 = 1 };
 enum { MO_FP8_FORWARD = 0, MO_FP8_BACKWARD = 1, MO_FP8_WEIGHT = 2 };
+enum { MO_FP8_BIAS_F32 = 0x100 };
 
 /* x[rows][cols] (rows `row_stride` elements apart) in groups along its rows and / or its columns (0 for
  * the pair that is not wanted), in one reading:
@@ -574,7 +575,8 @@ int mo_fp8_decode(uint64_t values, uint64_t pitch, uint64_t scales, uint32_t sca
 /* y[rows][out] = x . w^T (+ bias), fp32 sums, on the scaled f8f6f4 matrix instructions. x: a matrix of
  * `dtype` that the call quantizes along its rows, or (x_scales not 0) row_values and row_scales of
  * mo_fp8_quantize. w: e4m3 [out][in], w_scale [ceil(out / 128)][ceil(in / 128)], E8M0 or any fp32. bias:
- * [out] in y's type, or 0. `workspace`: 256-byte aligned, at least mo_fp8_workspace_bytes(MO_FP8_FORWARD,
+ * [out] in y's type, or in fp32 where y_dtype has the bit MO_FP8_BIAS_F32, or 0; it is added to the fp32 sum,
+ * which is rounded once. `workspace`: 256-byte aligned, at least mo_fp8_workspace_bytes(MO_FP8_FORWARD,
  * rows, in, out, x_scales != 0, scale_kind, y_dtype) bytes. */
 int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_t rows, uint32_t in_features,
                           uint64_t row_stride, uint64_t w, uint64_t w_scale, uint32_t scale_kind,

@@ -255,10 +255,10 @@ int check_weight(uint64_t w, uint64_t scale, uint32_t kind, uint32_t in_f, uint3
   return 0;
 }
 
-int check_output(uint64_t out, uint32_t dtype, uint64_t bias) {
+int check_output(uint64_t out, uint32_t dtype, uint64_t bias = 0, uint32_t bias_dtype = 0) {
   if (!out) return mo::set_error(MO_E_INVALID, "null output pointer");
   if (dtype > MO_DTYPE_F32) return mo::set_error(MO_E_INVALID, "unknown output type");
-  if (out % 16 || bias % kTypeBytes[dtype]) return mo::set_error(MO_E_INVALID, "misaligned output or bias pointer");
+  if (out % 16 || bias % kTypeBytes[bias_dtype]) return mo::set_error(MO_E_INVALID, "misaligned output or bias pointer");
   return 0;
 }
 
@@ -399,7 +399,10 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
   return guarded([&]() -> int {
     if (int rc = check_weight(w, w_scale, scale_kind, in_features, out_features)) return rc;
     if (int rc = check_operand(x, x_scales, dtype, rows, in_features, row_stride)) return rc;
-    if (int rc = check_output(y, y_dtype, bias)) return rc;
+    const bool wide_bias = y_dtype & MO_FP8_BIAS_F32;
+    y_dtype &= ~(uint32_t)MO_FP8_BIAS_F32;
+    const uint32_t bias_dtype = wide_bias ? (uint32_t)MO_DTYPE_F32 : y_dtype > MO_DTYPE_F32 ? 0 : y_dtype;
+    if (int rc = check_output(y, y_dtype, bias, bias_dtype)) return rc;
     Module m;
     if (int rc = load_module(&m)) return rc;
     const Room room =
@@ -416,7 +419,7 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
     p.a_scale_pitch = (uint32_t)scale_pitch(rows);
     p.b = (const uint8_t*)w, p.b_scales = (const void*)w_scale, p.b_pitch = in_features;
     p.b_scale_row = (uint32_t)div_up(in_features, kGroup), p.b_scale_col = 1, p.b_shift = 7;
-    p.bias = (const void*)bias, p.out = (void*)y, p.out_kind = y_dtype;
+    p.bias = (const void*)bias, p.bias_kind = bias_dtype, p.out = (void*)y, p.out_kind = y_dtype;
     p.m = rows, p.n = out_features, p.r = in_features;
     return product(m, room.plan, p, (int)scale_kind, false, workspace + room.operands, stream);
   });
@@ -429,7 +432,7 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
   return guarded([&]() -> int {
     if (int rc = check_weight(w, w_scale, scale_kind, in_features, out_features)) return rc;
     if (int rc = check_operand(dy, dy_scales, dtype, rows, out_features, row_stride)) return rc;
-    if (int rc = check_output(dx, dx_dtype, 0)) return rc;
+    if (int rc = check_output(dx, dx_dtype)) return rc;
     Module m;
     if (int rc = load_module(&m)) return rc;
     const Room room =
@@ -463,7 +466,7 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     if (!dy_scales != !x_scales) return mo::set_error(MO_E_INVALID, "both operands are quantized, or neither");
     if (int rc = check_operand(dy, dy_scales, dy_dtype, rows, out_features, dy_stride)) return rc;
     if (int rc = check_operand(x, x_scales, x_dtype, rows, in_features, x_stride)) return rc;
-    if (int rc = check_output(dw, dw_dtype, 0)) return rc;
+    if (int rc = check_output(dw, dw_dtype)) return rc;
     const uint64_t padded = div_up(rows, kGroup) * kGroup;
     if (padded * 256 >= (1ull << 31))  // 32-bit buffer offsets over a tile's rows
       return mo::set_error(MO_E_INVALID, "too many rows for one weight gradient (2^23 - 128 at most)");

@@ -19,12 +19,12 @@ struct ProductArgs {
   const uint8_t* b;
   const uint8_t* a_scales;  // one byte a row and group: group * a_scale_pitch + row
   const void* b_scales;     // bytes, or fp32 for the f32 kernels (then b_shift is 7)
-  const void* bias;         // in out's type, or null
+  const void* bias;         // of bias_kind, or null
   void* out;                // [m][n]
   uint64_t m, a_pitch, b_pitch;
   uint32_t n, r;
   uint32_t a_scale_pitch, b_scale_row, b_scale_col, b_shift;
-  uint32_t out_kind;
+  uint32_t out_kind, bias_kind;
   // the reduction shared out over workgroups: each takes split_steps groups of it and leaves fp32 sums in its
   // plane, [splits][m][n]; out and bias are then the sum kernel's. splits 1: planes is null
   uint32_t splits, split_steps;

@@ -678,7 +678,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p) {
             if (last && p.bias) {
               const uint32_t n = n_line + 32 * j + 8 * q + 4 * half;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[e] += n < p.n ? load1(p.bias, n + e, p.out_kind) : 0.0f;
+              for (int e = 0; e < 4; ++e) o[e] += n < p.n ? load1(p.bias, n + e, p.bias_kind) : 0.0f;
             }
             if (kBytes == 4) {
               *(MO_LDS f32x4*)(own + lr * kLine + 16 * ((2 * q + half) ^ (lr % kPieces))) = o;
@@ -723,7 +723,7 @@ extern "C" __global__ __launch_bounds__(256) void mo_fp8_plane_sum(ProductArgs p
   if (p.bias) {
     const uint32_t n = (uint32_t)(at % p.n);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += load1(p.bias, n + e, p.out_kind);
+    for (int e = 0; e < 4; ++e) v[e] += load1(p.bias, n + e, p.bias_kind);
   }
   store4(p.out, at, v, p.out_kind);
 }

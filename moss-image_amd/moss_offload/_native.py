@@ -15,7 +15,7 @@ import torch  # noqa: F401  (must be imported before the library, see module doc
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmoss_offload.so"
 
-MO_ABI_VERSION = 24
+MO_ABI_VERSION = 25
 MO_MAX_DIMS = 8
 
 MO_E_INVALID = 1001
@@ -42,6 +42,7 @@ MO_FP8_SCALE_F32 = 1
 MO_FP8_FORWARD = 0
 MO_FP8_BACKWARD = 1
 MO_FP8_WEIGHT = 2
+MO_FP8_BIAS_F32 = 0x100
 MO_FP8_NO_SIZE = (1 << 64) - 1
 
 DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # MO_DTYPE_*

@@ -277,8 +277,8 @@ def fp8_linear_forward(tokens, weight: torch.Tensor, scale: torch.Tensor, bias: 
                        dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``Q(tokens) @ decode(weight, scale).T (+ bias)``. ``tokens``: ``[..., in]``, quantized along its rows,
     or the pair that ``fp8_quantize_rows`` gives. ``weight``: e4m3 ``[out, in]``; ``scale``: one for each
-    128 x 128 block, e8m0 or float32. ``dtype``: the result's (the tokens' own; bfloat16 for a pair). The
-    result has no graph: ``fp8_linear`` has one."""
+    128 x 128 block, e8m0 or float32. ``bias``: ``[out]`` of any floating type, added to the float32 sum. ``dtype``:
+    the result's (the tokens' own; bfloat16 for a pair). The result has no graph: ``fp8_linear`` has one."""
 
     lib = _native.load()
     kind = _weight(weight, scale)
@@ -291,18 +291,20 @@ def fp8_linear_forward(tokens, weight: torch.Tensor, scale: torch.Tensor, bias: 
             return fp8_linear_forward(tokens, weight, scale, bias, dtype=dtype, out=out)
     dtype = dtype or (torch.bfloat16 if scales is not None else matrix.dtype)
     result = _output(out, (rows, out_features), dtype, weight.device)
+    kinds = _CODES[dtype]
     if bias is not None:
         _plain(bias)
         if bias.shape != (out_features,) or bias.get_device() != weight.get_device():
             raise RuntimeError(f"fp8 bias must be {out_features} values on the weight's device.")
-        bias = bias.to(dtype).contiguous()
+        # added in fp32, before the one rounding: another type than the result's goes in as float32
+        bias = (bias if bias.dtype == dtype else bias.float()).contiguous()
+        kinds |= _native.MO_FP8_BIAS_F32 if bias.dtype == torch.float32 else 0
     if rows:
         space, nbytes = _workspace(_native.MO_FP8_FORWARD, rows, in_features, out_features, scales is not None, kind,
                                    dtype, weight)
         _native.check("mo_fp8_linear_forward", lib.mo_fp8_linear_forward(
             matrix.data_ptr(), _address(scales), code, rows, in_features, stride, weight.data_ptr(), scale.data_ptr(),
-            kind, out_features, _address(bias), result.data_ptr(), _CODES[dtype], _address(space), nbytes,
-            _stream(weight)))
+            kind, out_features, _address(bias), result.data_ptr(), kinds, _address(space), nbytes, _stream(weight)))
     return result if len(lead) == 1 else result.view(*lead, out_features)
 
 

@@ -209,3 +209,30 @@ def test_the_library_tells_a_failure_from_no_room() -> None:
     assert lib.mo_last_error()
     for sizes in ((4, 144, 1 << 21), (4, 1 << 21, 32), (4, 0, 32), (1 << 31, 144, 32)):
         assert lib.mo_fp8_workspace_bytes(_native.MO_FP8_FORWARD, *sizes, 0, 0, 1) == 0
+
+
+# ---- biases ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bias_dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_bias_goes_to_the_kernel_unrounded(library, dtype, bias_dtype) -> None:
+    weight, scale = _frozen()
+    bias = torch.ones(32, dtype=bias_dtype)
+    fp8.fp8_linear_forward(torch.zeros(4, 144, dtype=dtype), weight, scale, bias)
+    address, kinds = (library.last["mo_fp8_linear_forward"][i] for i in (10, 12))
+    assert kinds & 0xFF == _native.DTYPE_CODES[dtype]
+    if bias_dtype == dtype:
+        assert address == bias.data_ptr()
+    assert bool(kinds & _native.MO_FP8_BIAS_F32) == (bias_dtype != dtype or bias_dtype == torch.float32)
+
+
+def test_the_library_takes_a_float32_bias_by_its_alignment() -> None:
+    lib = _native.load()
+    for kinds, bias, message in [(1, 4098, None), (1 | _native.MO_FP8_BIAS_F32, 4098, b"bias"), (1, 4097, b"bias"),
+                                 (1 | _native.MO_FP8_BIAS_F32, 4100, None), (7 | _native.MO_FP8_BIAS_F32, 4096, b"type")]:
+        # one that passes ends at the device or at the workspace of no bytes
+        call = [4096, 0, 1, 4, 64, 64, 4096, 4096, 0, 32, bias, 4096, kinds, 4096, 0, 0]
+        status = lib.mo_fp8_linear_forward(*call)
+        assert status != 0
+        assert (message in lib.mo_last_error()) if message else (b"bias" not in lib.mo_last_error()), (kinds, bias)
