@@ -84,7 +84,8 @@ uint32_t pick_vec(const mo_rotary_call& c) {
   const uint32_t size = kTypeBytes[c.dtype], table = kTypeBytes[c.table_dtype], weight = kTypeBytes[c.weight_dtype];
   uint32_t v = 16 / size;
   for (; v > 1; v /= 2) {
-    bool ok = c.rotary_dim / 2 % v == 0 && (c.head_dim - c.rotary_dim) / 2 % v == 0 && fits(c.table, v * table);
+    bool ok = c.rotary_dim / 2 % v == 0 && (c.head_dim - c.rotary_dim) / 2 % v == 0 && fits(c.table, v * table) &&
+              c.table_batch % v == 0;
     for (const mo_rotary_side& s : c.side) {
       if (!s.heads) continue;
       for (int64_t stride : {s.x_batch, s.x_token, s.x_head}) ok = ok && (!s.x || stride % v == 0);
