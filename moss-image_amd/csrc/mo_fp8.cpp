@@ -418,7 +418,7 @@ int mo_fp8_linear_forward(uint64_t x, uint64_t x_scales, uint32_t dtype, uint64_
     p.a = (const uint8_t*)x, p.a_scales = (const uint8_t*)x_scales, p.a_pitch = in_features;
     p.a_scale_pitch = (uint32_t)scale_pitch(rows);
     p.b = (const uint8_t*)w, p.b_scales = (const void*)w_scale, p.b_pitch = in_features;
-    p.b_scale_row = (uint32_t)div_up(in_features, kGroup), p.b_scale_col = 1, p.b_shift = 7;
+    p.b_scale_row = (uint32_t)div_up(in_features, kGroup), p.b_scale_col = 1;
     p.bias = (const void*)bias, p.bias_kind = bias_dtype, p.out = (void*)y, p.out_kind = y_dtype;
     p.m = rows, p.n = out_features, p.r = in_features;
     return product(m, room.plan, p, (int)scale_kind, false, workspace + room.operands, stream);
@@ -448,7 +448,7 @@ int mo_fp8_linear_backward(uint64_t dy, uint64_t dy_scales, uint32_t dtype, uint
     p.a = (const uint8_t*)dy, p.a_scales = (const uint8_t*)dy_scales, p.a_pitch = out_features;
     p.a_scale_pitch = (uint32_t)scale_pitch(rows);
     p.b = (const uint8_t*)w, p.b_scales = (const void*)w_scale, p.b_pitch = in_features;  // as stored
-    p.b_scale_row = 1, p.b_scale_col = (uint32_t)div_up(in_features, kGroup), p.b_shift = 7;
+    p.b_scale_row = 1, p.b_scale_col = (uint32_t)div_up(in_features, kGroup);
     p.out = (void*)dx, p.out_kind = dx_dtype;
     p.m = rows, p.n = in_features, p.r = out_features;
     return product(m, room.plan, p, (int)scale_kind, true, workspace + room.operands, stream);
@@ -487,7 +487,7 @@ int mo_fp8_weight_gradient(uint64_t dy, uint64_t dy_scales, uint32_t dy_dtype, u
     p.a = (const uint8_t*)dy, p.a_scales = (const uint8_t*)dy_scales, p.a_pitch = padded;
     p.a_scale_pitch = out_features;
     p.b = (const uint8_t*)x, p.b_scales = (const void*)x_scales, p.b_pitch = padded;
-    p.b_scale_row = 1, p.b_scale_col = in_features, p.b_shift = 0;
+    p.b_scale_col = in_features;  // one scale a row
     p.out = (void*)dw, p.out_kind = dw_dtype;
     p.m = out_features, p.n = in_features, p.r = (uint32_t)padded;
     return product(m, room.plan, p, kScaleRows, false, workspace + room.operands, stream);
