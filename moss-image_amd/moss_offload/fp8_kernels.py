@@ -238,7 +238,8 @@ def fp8_decode(values: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype
     if not 0 <= cols <= matrix.shape[1]:
         raise ValueError("fp8_decode's cols must lie within the values.")
     rows = matrix.shape[0]
-    if matrix.stride(1) != 1 or (rows > 1 and matrix.stride(0) % 16) or matrix.data_ptr() % 16:
+    if matrix.stride(1) != 1 or (rows > 1 and (matrix.stride(0) < matrix.shape[1] or matrix.stride(0) % 16)) \
+            or matrix.data_ptr() % 16:
         matrix = matrix.contiguous()
         matrix = matrix.clone() if matrix.data_ptr() % 16 else matrix
     if scales.shape[0] not in (rows, _groups(rows)) or scales.shape[1] < _groups(cols) \

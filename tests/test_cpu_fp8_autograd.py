@@ -236,3 +236,20 @@ def test_the_library_takes_a_float32_bias_by_its_alignment() -> None:
         status = lib.mo_fp8_linear_forward(*call)
         assert status != 0
         assert (message in lib.mo_last_error()) if message else (b"bias" not in lib.mo_last_error()), (kinds, bias)
+
+
+# ---- reading back ---------------------------------------------------------------------------------
+
+
+def test_values_whose_rows_overlap_are_copied_to_be_read_back(library) -> None:
+    """The kernel takes rows a row's length apart or more."""
+
+    row = torch.zeros(1, 144).to(torch.float8_e4m3fn)
+    windows = torch.zeros(400).to(torch.float8_e4m3fn).as_strided((4, 144), (16, 1))
+    for values in (row.expand(4, -1), windows, row.expand(2, 3, 144).flatten(0, 1)):
+        scales = torch.ones(values.shape[0], 2)
+        assert fp8.fp8_decode(values, scales).shape == values.shape
+        assert library.last["mo_fp8_decode"][1] == 144
+    apart = torch.zeros(4, 160).to(torch.float8_e4m3fn)[:, :144]
+    fp8.fp8_decode(apart, torch.ones(4, 2))
+    assert library.last["mo_fp8_decode"][:2] == (apart.data_ptr(), 160)
