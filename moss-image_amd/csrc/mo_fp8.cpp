@@ -36,9 +36,10 @@ const char* const kScaleNames[3] = {"bytes", "floats", "rows"};
 // in us, for 16-bit outputs, 16-bit outputs with fp32 block scales, and fp32 outputs: a call's fixed part, what
 // a further round of workgroups adds of it, and a step of 128 of the reduction with one workgroup on a CU and
 // with all that fit. Fitted to 12 400 timed calls (110 shapes of 1 to 17 792 rows, every tile, 1 to 32
-// splits, eight kinds of operands, replayed back to back): the model's choice takes 1 % longer than the
-// fastest one on average, 4 % at the ninetieth percentile, 31 % at worst (199 rows of 3072 from 24576).
-// Those three were taken with 1.1 us as a sum's fixed part, before the host's launch was counted in.
+// splits, eight kinds of operands, replayed back to back). Of the launches timed for a shape, the one that these
+// numbers choose takes 1 % longer than the fastest on average, 4 % at the ninetieth percentile, 29 % at worst (199
+// rows of 3072 from 24576), a split call's time with the 2.4 us that kSumFixed counts for the host. Inputs that come
+// from memory take longer than replays do: 3072 x 3072 fp32 from 1333 is 34 here and 44 in a program's trace.
 struct Cost {
   double fixed, again, alone, together;
 };

@@ -15,10 +15,11 @@
 //
 // What the matrix instructions on e4m3 add is not exact to fp32: of neighbouring products inside one
 // instruction, bits under about 2^-15 of the largest are dropped (measured: 65536 + 1 gives 65536, and
-// Gaussian operands come out 1.5e-5 off, in the scaled, the unscaled and the 16-deep form alike). That is
-// a hundredth of a bf16 rounding and a tenth of an fp16 one, and stays for 16-bit outputs. An fp32 output
-// is asked for its fp32 sums: those kernels decode the operands to bf16, which is exact, and use the bf16
-// instructions (half the rate, 6e-8 off).
+// Gaussian operands come out 1.5e-5 off, in the scaled, the unscaled and the 16-deep form alike). There, that
+// is a hundredth of a bf16 rounding and a tenth of an fp16 one, and stays for 16-bit outputs; where products of
+// a strong channel cancel, what is lost is relative to them and can be more than the output's own rounding. An
+// fp32 output is asked for its fp32 sums: those kernels decode the operands to bf16, exact for values from
+// 2^-126 on, and use the bf16 instructions (half the rate, 6e-8 off).
 //
 // A group with an infinity or a NaN gets the scale byte 255, which reads back as NaN throughout and
 // makes NaN of every output that it takes part in.

@@ -13,7 +13,7 @@
 // one write backward with a norm), and the table from cache for all but one head of a token. So each lane
 // moves 16 bytes at a time: a head's row is shared out over the lanes of a part of a wave, kVec pairs a
 // lane, and the row's sums are taken by lane exchanges. 4608 tokens, 24 heads of 128, bf16, both sides with norms: forward
-// 30.6 us (3.7 TB/s), backward 52.6 (3.2) and 4 for the weights' sums. Four heads a lane, which reads the angles once:
+// 30 to 31 us (3.7 TB/s), backward 51 to 53 (3.2) and 4 for the weights' sums. Four heads a lane, which reads the angles once:
 // 44 and 77.
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -97,7 +97,8 @@ def attention(query, key, value, rope, heads, cu_seqlens=None, seq_lengths=None)
 
 
 def attention_fused(query, key, value, rope, heads, q_norm, k_norm, cu_seqlens=None, seq_lengths=None):
-    """``attention`` on queries and keys before their head norms: norms and turns in one launch."""
+    """``attention`` on queries and keys before their head norms: norms and turns in one launch. The norms' weights
+    are read and their modules not called, so hooks on those do not run."""
 
     from .rotary import rotary
 

@@ -12,7 +12,8 @@ Three products share them (``csrc/mo_fp8.hip``), fp32 sums, each rounded once to
 - ``fp8_linear_backward``: ``Q(gradient) @ W``, the gradient quantized along its rows;
 - ``fp8_weight_gradient``: ``Q(gradient).T @ Q(tokens)``, both quantized along the tokens.
 
-``fp8_linear`` puts them under autograd, for a frozen weight or for one in training. The reference has no
+``fp8_linear`` puts them under autograd, for a frozen weight or for one in training (first derivatives; a
+backward that should build a graph through a weight in training raises). The reference has no
 floating-point 8-bit base; its int8 one (``training/quantization.py:23-131``) is ``quant_kernels`` here.
 
 Feature sizes are multiples of 16, rows any number. A group with an infinity or a NaN reads back as NaN.

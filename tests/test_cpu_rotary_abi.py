@@ -1,12 +1,14 @@
-"""The rotary calls' C ABI without a device: which lanes a call gets, seen in the size of its partial sums."""
+"""The rotary calls without a device: which lanes a call gets through the C ABI, seen in the size of its partial sums,
+and what autograd refuses."""
 
 from __future__ import annotations
 
 import ctypes
 
 import pytest
+import torch
 
-from moss_offload import _native
+from moss_offload import _native, rotary
 
 
 def _lanes(**fields) -> int:
@@ -44,3 +46,24 @@ def test_every_other_stride_is_part_of_the_alignment() -> None:
         assert _lanes(**{name: 8001}) == 8 and _lanes(**{name: 8008}) == 1
     for name in ("x", "grad", "out"):
         assert _lanes(**{name: 4098}) == 8 and _lanes(**{name: 4104}) == 2
+
+
+def test_a_graph_through_the_norms_backward_is_refused(monkeypatch) -> None:
+    """The gradients of heads and norm weights depend on both; without a norm the turn is linear in its gradient."""
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 256 if name.endswith("_bytes") else 0
+
+    monkeypatch.setattr(rotary._native, "load", Library)
+    monkeypatch.setattr(rotary, "_elsewhere", lambda tensor: False)
+    monkeypatch.setattr(rotary, "_stream", lambda tensor: 0)
+    q, table, weight = torch.zeros(1, 3, 2, 8).requires_grad_(), torch.zeros(1, 3, 8), torch.ones(8).requires_grad_()
+    for wanted, heads, scale in (([q], q, weight.detach()), ([weight], q.detach(), weight), ([q, weight], q, weight)):
+        out = rotary.rotary(heads, None, table, q_weight=scale)[0]
+        with pytest.raises(RuntimeError, match="graph"):
+            torch.autograd.grad(out.sum(), wanted, create_graph=True)
+        grads = torch.autograd.grad(rotary.rotary(heads, None, table, q_weight=scale)[0].sum(), wanted)
+        assert [g.shape for g in grads] == [t.shape for t in wanted]
+    (grad,) = torch.autograd.grad(rotary.rotary(q, None, table)[0].sum(), [q], create_graph=True)
+    assert not grad.requires_grad
