@@ -622,11 +622,13 @@ class FrozenFp8Linear(nn.Module):
         return self._dtype_anchor.dtype
 
     def _apply(self, fn, recurse=True):
-        # a cast of the model changes the compute dtype; weights and scales stay in their formats
-        weight, scale = self.weight_fp8, self.weight_scale
+        # a cast of the model changes the compute dtype; weights and scales stay in their formats. What kept its
+        # format is the call's own result: moved once
+        before = {name: getattr(self, name) for name in ("weight_fp8", "weight_scale")}
         result = super()._apply(fn, recurse=recurse)
-        device = self._dtype_anchor.device
-        self.weight_fp8, self.weight_scale = weight.to(device), scale.to(device)
+        for name, tensor in before.items():
+            if getattr(self, name).dtype != tensor.dtype:
+                setattr(self, name, tensor.to(self._dtype_anchor.device))
         return result
 
     def forward(self, tokens):
