@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MO_ABI_VERSION 25
+#define MO_ABI_VERSION 26
 #define MO_MAX_DIMS 8
 
 /* Error codes outside the hipError_t range. */
@@ -648,6 +648,97 @@ uint64_t mo_rotary_workspace_bytes(const mo_rotary_call* call);
  * `amplitude`; coordinates fp32 [rows][axes], bands fp32. */
 int mo_rotary_table(uint64_t coordinates, uint64_t bands, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t axes,
                     uint32_t n_bands, float amplitude, uint64_t stream);
+
+/* ---- norms with a modulation for each sample (training/model.py:154-172, 291-314) --------- */
+
+/* out = ((x - mean) / sqrt(variance + eps) * weight + bias) * (1 + scale_s) + shift_s for each row of x
+ * [rows][dim], s the row's sample; not `layer`: the mean is taken as 0 (an RMS norm). fp32 inside, each result
+ * rounded once. Outputs are dense. 0 stands for what is not there. */
+typedef struct mo_norm_call {
+  uint64_t x;            /* [rows][dim] of `dtype`; backward also 8-bit values (mo_keep_pack) */
+  uint64_t x_exponents;  /* backward: their exponents, or 0 */
+  uint64_t grad;         /* backward: the output's gradient [rows][dim] */
+  uint64_t out;          /* forward: the output; backward: the input's gradient */
+  uint64_t stats;        /* fp32 [rows][2]: mean and 1 / sqrt(..): written forward (or 0), read backward */
+  uint64_t weight, bias; /* [dim] of weight_dtype */
+  uint64_t scale, shift; /* [samples][dim] of scale_dtype */
+  uint64_t kept, kept_exponents; /* forward: x in 8 bits, as mo_keep_pack writes it */
+  uint64_t weight_grad, bias_grad, scale_grad, shift_grad; /* backward, of their tensors' types */
+  uint64_t cu;           /* int64 [samples + 1]: sample s has rows cu[s] to cu[s + 1] - 1, in order; rows in no
+                          * sample give zeros and take part in nothing. 0: rows / samples each */
+  uint64_t rows, x_stride, grad_stride, scale_stride, shift_stride; /* between rows, in elements */
+  uint32_t samples;      /* 0 without scale and shift */
+  uint32_t dim, dtype, weight_dtype, scale_dtype, layer;
+  float eps;
+  uint32_t reserved;
+} mo_norm_call;
+
+int mo_norm_forward(const mo_norm_call* call, uint64_t stream);
+/* `workspace`: 256-byte aligned, mo_norm_workspace_bytes(call) bytes (the gradients' partial sums, added in a
+ * fixed order). */
+int mo_norm_backward(const mo_norm_call* call, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream);
+uint64_t mo_norm_workspace_bytes(const mo_norm_call* call);
+
+/* ---- activations in 8 bits ----------------------------------------------------------------- */
+
+/* x[rows][cols] (rows `row_stride` elements apart) in groups of 32 along its rows: e the smallest integer >= -126
+ * with max |x| <= 127 2^e, values[rows][ceil(cols / 32) * 32] = round(x 2^-e) (half to even, zero past cols),
+ * exponents[rows][ceil(cols / 32)] = e + 127. A group with an infinity or a NaN: zeros and 255, which reads back as
+ * NaN. |value| is at most 63 where 64 2^e is past the type's largest. */
+int mo_keep_pack(uint64_t x, uint32_t dtype, uint64_t rows, uint32_t cols, uint64_t row_stride, uint64_t values,
+                 uint64_t exponents, uint64_t stream);
+/* out[rows][cols] = value 2^e, rounded to `dtype`. */
+int mo_keep_restore(uint64_t values, uint64_t exponents, uint64_t out, uint32_t dtype, uint64_t rows, uint32_t cols,
+                    uint64_t row_stride, uint64_t stream);
+
+/* ---- gated activation (training/model.py:27-38) -------------------------------------------- */
+
+/* out = act(gate) cap(up) for [rows][cols] each: SiTU (4 tanh(g / 4) sigmoid(g), 25 tanh(u / 25)) or `silu` (g
+ * sigmoid(g), u). Strides in elements, those of what is in 8 bits in bytes. */
+typedef struct mo_gated_call {
+  uint64_t up, gate;                           /* backward also 8-bit values */
+  uint64_t up_exponents, gate_exponents;       /* backward: their exponents, or 0 */
+  uint64_t grad;                               /* backward: the output's gradient */
+  uint64_t out;                                /* forward: the output; backward: up's gradient */
+  uint64_t out_gate;                           /* backward: gate's gradient, rows out_stride apart too */
+  uint64_t kept_up, kept_gate;                 /* forward: up and gate in 8 bits, or 0 */
+  uint64_t kept_up_exponents, kept_gate_exponents;
+  uint64_t rows, up_stride, gate_stride, grad_stride, out_stride;
+  uint64_t values_stride, exponents_stride;    /* of whichever is in 8 bits */
+  uint32_t cols, dtype, silu, reserved;
+} mo_gated_call;
+
+int mo_gated_forward(const mo_gated_call* call, uint64_t stream);
+int mo_gated_backward(const mo_gated_call* call, uint64_t stream);
+
+/* ---- low-rank adapters beside a shared projection (training/lora.py:60-86, for many requests) ---- */
+
+/* hidden = x a_i^T, y = result + factor scale_i hidden b_i^T, i the adapter of the row's request; a row without one
+ * passes the result on. fp32 sums, y rounded once. */
+typedef struct mo_adapters_call {
+  uint64_t x;              /* [rows][in] of `dtype`; backward, wanted for da alone, also 8-bit values (mo_keep_pack) */
+  uint64_t x_exponents;    /* backward: their exponents, or 0 */
+  uint64_t result, y;      /* forward: [rows][out]; y dense, it may be the result */
+  uint64_t a, b;           /* [adapters][rank][in], [adapters][out][rank], dense */
+  uint64_t scale;          /* fp32 [adapters], or 0: 1 */
+  uint64_t cu;             /* int64 [requests + 1]: request s has rows cu[s] to cu[s + 1] - 1, in order; rows in none
+                            * have no adapter. 0: rows / requests each */
+  uint64_t index;          /* int64 [requests]: its adapter; a number outside [0, adapters): none. 0: the request's
+                            * own number, or 0 where there is one adapter */
+  uint64_t hidden;         /* fp32 [rows][rank]: written forward, read backward */
+  uint64_t grad, add;      /* backward: y's gradient [rows][out]; [rows][in] to be added to dx, or 0 */
+  uint64_t dx, da, db;     /* backward, dense, or 0: not wanted. An adapter that no row has gets zeros */
+  uint64_t rows, x_stride, result_stride, grad_stride, add_stride; /* strides in elements */
+  uint32_t requests, adapters, rank, in_features, out_features, dtype; /* rank 1 to 128 */
+  float factor;            /* times every scale */
+  uint32_t reserved;
+} mo_adapters_call;
+
+/* `workspace`: 256-byte aligned, mo_adapters_workspace_bytes(call, backward) bytes. The same call gives the same bits
+ * every time. */
+int mo_adapters_forward(const mo_adapters_call* call, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream);
+int mo_adapters_backward(const mo_adapters_call* call, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream);
+uint64_t mo_adapters_workspace_bytes(const mo_adapters_call* call, uint32_t backward);
 
 /* ---- host gradient accumulation (training/fused_adafactor.py:327-369) -------------------- */
 

@@ -1,0 +1,141 @@
+// The gated activation between the two products of a feed-forward, and activations in 8 bits, for gfx950.
+//
+//   out = act(g) cap(u):  SiTU  act = 4 tanh(g / 4) s, cap = 25 tanh(u / 25), s = 1 / (1 + exp(-g))
+//                         SiLU  act = g s, cap = u
+//   backward, d the output's gradient:  d u = d act cap', d g = d cap act'
+//                         SiTU  act' = (1 - t^2) s + 4 t s (1 - s), t = tanh(g / 4); cap' = 1 - tanh(u / 25)^2
+//                         SiLU  act' = s (1 + g (1 - s)), cap' = 1
+// (the reference's SiTU-GLU: model.py:27-38.)
+//
+// fp32 inside, each result rounded once.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mo_block.h"
+#include "mo_keep.h"
+
+namespace {
+
+using mo_block::GatedArgs;
+using mo_block::KeepArgs;
+using namespace mo_keep;
+
+__device__ __forceinline__ uint32_t divide(uint32_t n, const mo_block::Divisor& by) {
+  return (__umulhi(by.m, n) + n) >> by.s;
+}
+
+__device__ __forceinline__ float tanh_of(float x) { return tanhf(x); }
+__device__ __forceinline__ float sigmoid_of(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// A lane's place: row, first column, how many of its 8 are in the row, its group and whether it has a row at all.
+struct Spot {
+  uint32_t row, at, n;
+  bool live;
+  __device__ __forceinline__ Spot(uint32_t rows, uint32_t cols, uint32_t lanes, const mo_block::Divisor& by) {
+    const uint32_t item = blockIdx.x * 256 + threadIdx.x;
+    row = divide(item, by);
+    at = (item - row * lanes) * 8;
+    live = row < rows;
+    n = live && at < cols ? min(8u, cols - at) : 0;
+  }
+};
+
+template <class T>
+__device__ __forceinline__ void load_row(float (&to)[8], const void* base, uint64_t stride, const Spot& s) {
+  widen(to, load8((const T*)base + (s.n ? s.row * stride + s.at : 0), s.n));
+}
+template <class T>
+__device__ __forceinline__ void write_kept(const float (&v)[8], int8_t* values, uint8_t* exponents, uint64_t stride,
+                                           uint64_t exponents_stride, const Spot& s) {
+  uint32_t exponent;
+  const uint2 q = encode<T>(v, exponent);
+  if (!s.live) return;
+  *(uint2*)(values + s.row * stride + s.at) = q;
+  if (s.at % kGroup == 0) exponents[s.row * exponents_stride + s.at / kGroup] = (uint8_t)exponent;
+}
+__device__ __forceinline__ void read_kept(float (&to)[8], const void* values, const uint8_t* exponents, uint64_t stride,
+                                          uint64_t exponents_stride, const Spot& s) {
+  uint2 q = {0, 0};
+  uint32_t exponent = 0;
+  if (s.live) {
+    q = *(const uint2*)((const int8_t*)values + s.row * stride + s.at);
+    exponent = exponents[s.row * exponents_stride + s.at / kGroup];
+  }
+  decode(to, q, exponent);
+}
+
+template <class T, bool kKeep>
+__device__ __forceinline__ void forward(const GatedArgs& a) {
+  const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
+  float u[8], g[8];
+  load_row<T>(u, a.up, a.up_stride, s);
+  load_row<T>(g, a.gate, a.gate_stride, s);
+  if (kKeep) {
+    write_kept<T>(u, a.kept_up, a.kept_up_exponents, a.values_stride, a.exponents_stride, s);
+    write_kept<T>(g, a.kept_gate, a.kept_gate_exponents, a.values_stride, a.exponents_stride, s);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float gate = sigmoid_of(g[i]);
+    u[i] = a.silu ? u[i] * (g[i] * gate) : 4.0f * tanh_of(g[i] * 0.25f) * gate * (25.0f * tanh_of(u[i] * 0.04f));
+  }
+  if (s.n) store8((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
+}
+
+template <class T, bool kKept>
+__device__ __forceinline__ void backward(const GatedArgs& a) {
+  const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
+  float u[8], g[8], d[8];
+  if (kKept) {
+    read_kept(u, a.up, a.up_exponents, a.values_stride, a.exponents_stride, s);
+    read_kept(g, a.gate, a.gate_exponents, a.values_stride, a.exponents_stride, s);
+  } else {
+    load_row<T>(u, a.up, a.up_stride, s);
+    load_row<T>(g, a.gate, a.gate_stride, s);
+  }
+  load_row<T>(d, a.grad, a.grad_stride, s);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float gate = sigmoid_of(g[i]);
+    float act, slope, cap, cap_slope;
+    if (a.silu) {
+      act = g[i] * gate, slope = gate * (1.0f + g[i] * (1.0f - gate)), cap = u[i], cap_slope = 1.0f;
+    } else {
+      const float t = tanh_of(g[i] * 0.25f), c = tanh_of(u[i] * 0.04f);
+      act = 4.0f * t * gate, slope = (1.0f - t * t) * gate + act * (1.0f - gate), cap = 25.0f * c, cap_slope = 1.0f - c * c;
+    }
+    u[i] = d[i] * act * cap_slope;
+    g[i] = d[i] * cap * slope;
+  }
+  if (!s.n) return;
+  store8((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
+  store8((T*)a.out_gate + s.row * a.out_stride + s.at, g, s.n);
+}
+
+template <class T>
+__device__ __forceinline__ void pack(const KeepArgs& a) {
+  const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
+  float v[8];
+  load_row<T>(v, a.x, a.stride, s);
+  write_kept<T>(v, a.values, a.exponents, (uint64_t)a.groups * kGroup, a.groups, s);
+}
+template <class T>
+__device__ __forceinline__ void restore(const KeepArgs& a) {
+  const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
+  float v[8];
+  read_kept(v, a.values, a.exponents, (uint64_t)a.groups * kGroup, a.groups, s);
+  if (s.n) store8((T*)a.out + s.row * a.stride + s.at, v, s.n);
+}
+
+#define MO_GATED(T, t)                                                                                               \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_##t(GatedArgs a) { forward<T, false>(a); }      \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_keep_##t(GatedArgs a) { forward<T, true>(a); }  \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_backward_##t(GatedArgs a) { backward<T, false>(a); }    \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_backward_kept_##t(GatedArgs a) { backward<T, true>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void mo_keep_pack_##t(KeepArgs a) { pack<T>(a); }                     \
+  extern "C" __global__ __launch_bounds__(256) void mo_keep_restore_##t(KeepArgs a) { restore<T>(a); }
+MO_GATED(_Float16, f16)
+MO_GATED(__bf16, bf16)
+MO_GATED(float, f32)
+
+}  // namespace

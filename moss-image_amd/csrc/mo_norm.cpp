@@ -1,0 +1,154 @@
+// Host side of the norms (csrc/mo_norm.hip): argument checks, how rows are shared out, launches. C ABI: mo_norm_*.
+#include "mo_block.h"
+#include "mo_layout.h"
+#include "mo_module.h"
+
+extern "C" const unsigned char mo_norm_code[];
+
+namespace {
+
+using mo_block::NormArgs;
+
+const char* const kTypeNames[3] = {"f16", "bf16", "f32"};  // by MO_DTYPE_*
+constexpr uint32_t kTypeBytes[3] = {2, 2, 4};
+
+mo::Kernels& kernels() {
+  static mo::Kernels k(mo_norm_code);
+  return k;
+}
+
+uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+// How a call's rows are shared out: `lanes` of 8 values (kIter times) a row, `per` rows side by side in a workgroup,
+// `chunk` rows one after the other.
+struct Plan {
+  uint32_t lanes, per, chunk, iter, groups;
+  uint64_t slots;  // backward: pairs of a group of rows and a sample that have a place for sums
+};
+
+Plan plan_of(const mo_norm_call& c, bool backward) {
+  Plan p = {};
+  const uint64_t held = div_up(c.dim, 8);
+  p.iter = held > 1024 ? 2 : 1;
+  p.lanes = (uint32_t)div_up(div_up(held, p.iter), 64) * 64;
+  p.per = p.lanes == 64 ? 4 : 1;
+  // forward: enough workgroups for several on every CU; backward: each leaves sums of dim values, so fewer
+  const uint64_t most = backward ? 1024 : 2048;
+  p.chunk = (uint32_t)div_up(c.rows, most * p.per);
+  p.groups = (uint32_t)div_up(c.rows, p.chunk);
+  p.slots = (uint64_t)p.groups + (c.samples ? c.samples - 1 : 0);
+  return p;
+}
+
+uint32_t pitch_of(const mo_norm_call& c) { return (c.dim + 7) / 8 * 8; }
+bool wants_sums(const mo_norm_call& c) { return c.weight_grad || c.bias_grad || c.scale_grad || c.shift_grad; }
+bool wants_sample_sums(const mo_norm_call& c) { return c.samples > 1 && (c.weight_grad || c.bias_grad); }
+
+uint64_t workspace_bytes(const mo_norm_call& c, const Plan& p) {
+  uint64_t floats = 0;
+  if (wants_sums(c)) floats += p.slots * 2 * pitch_of(c);
+  if (wants_sample_sums(c)) floats += (uint64_t)c.samples * 2 * pitch_of(c);
+  return (floats * 4 + 255) & ~uint64_t(255);
+}
+
+int check(const mo_norm_call* c, bool backward) {
+  auto bad = [](const char* what) { return mo::set_error(MO_E_INVALID, what); };
+  if (!c) return bad("null call");
+  if (c->dtype > MO_DTYPE_F32 || c->weight_dtype > MO_DTYPE_F32 || c->scale_dtype > MO_DTYPE_F32)
+    return bad("unknown element type");
+  if (c->rows == 0 || c->rows >= (1ull << 31) || c->dim == 0 || c->dim > mo_block::kMaxDim)
+    return bad("rows must be 1 to 2^31 - 1 and dim 1 to 16384");
+  const uint32_t size = kTypeBytes[c->dtype];
+  if (!c->x || !c->out || c->out % size) return bad("null or misaligned rows");
+  if (c->x_exponents ? !backward || c->x % 8 != 0 : c->x % size != 0) return bad("misaligned input");
+  if (c->rows > 1 && !c->x_exponents && c->x_stride < c->dim) return bad("rows of the input overlap");
+  const bool modulated = c->scale || c->shift;
+  if (modulated != (c->samples != 0)) return bad("samples go with a scale or a shift");
+  if (c->samples >= (1u << 16)) return bad("too many samples (2^16 or more)");
+  if (c->cu ? !modulated || c->cu % 8 != 0 : modulated && c->rows % c->samples != 0)
+    return bad("samples' rows must be given, or the same number for each");
+  for (uint64_t p : {c->weight, c->bias, c->weight_grad, c->bias_grad})
+    if (p % kTypeBytes[c->weight_dtype]) return bad("misaligned weight");
+  for (uint64_t p : {c->scale, c->shift, c->scale_grad, c->shift_grad})
+    if (p % kTypeBytes[c->scale_dtype]) return bad("misaligned modulation");
+  if (c->stats % 4) return bad("misaligned statistics");
+  if (!backward) {
+    if ((c->kept != 0) != (c->kept_exponents != 0) || c->kept % 8) return bad("both the 8-bit values and their exponents");
+    return 0;
+  }
+  if (!c->grad || c->grad % size || !c->stats) return bad("the gradient and the forward pass's statistics are needed");
+  if (c->rows > 1 && c->grad_stride < c->dim) return bad("rows of the gradient overlap");
+  if ((c->weight_grad && !c->weight) || (c->bias_grad && !c->bias) || (c->scale_grad && !c->scale) ||
+      (c->shift_grad && !c->shift))
+    return bad("a gradient of what is not there");
+  return 0;
+}
+
+int run(const mo_norm_call* c, bool backward, uint64_t workspace, uint64_t bytes, uint64_t stream) {
+  if (int rc = check(c, backward)) return rc;
+  const Plan p = plan_of(*c, backward);
+  const uint64_t needed = backward ? workspace_bytes(*c, p) : 0;
+  if (needed && (!workspace || workspace % 256 || bytes < needed))
+    return mo::set_error(MO_E_INVALID, "workspace missing, misaligned or smaller than mo_norm_workspace_bytes");
+  NormArgs a = {};
+  a.x = (const void*)c->x, a.x_exponents = (const uint8_t*)c->x_exponents, a.grad = (const void*)c->grad;
+  a.out = (void*)c->out, a.stats = (float*)c->stats;
+  a.weight = (const void*)c->weight, a.bias = (const void*)c->bias;
+  a.scale = (const void*)c->scale, a.shift = (const void*)c->shift;
+  a.cu = (const int64_t*)c->cu;
+  if (!backward) a.kept = (int8_t*)c->kept, a.kept_exponents = (uint8_t*)c->kept_exponents;
+  a.x_stride = c->rows > 1 ? c->x_stride : c->dim, a.grad_stride = c->rows > 1 ? c->grad_stride : c->dim;
+  a.scale_stride = c->scale_stride, a.shift_stride = c->shift_stride;
+  a.rows = (uint32_t)c->rows, a.dim = c->dim, a.samples = c->samples;
+  a.groups = (c->dim + 31) / 32, a.pitch = pitch_of(*c);
+  a.lanes = p.lanes, a.per = p.per, a.chunk = p.chunk;
+  a.weight_kind = c->weight_dtype, a.scale_kind = c->scale_dtype, a.layer = c->layer, a.eps = c->eps;
+  const uint32_t share = c->samples && !c->cu ? (uint32_t)(c->rows / c->samples) : 1;
+  const mo::FastDiv f = mo::make_fastdiv(share);
+  a.by_share = {f.d, f.m, f.s};
+  if (backward) {
+    a.weight_grad = (void*)c->weight_grad, a.bias_grad = (void*)c->bias_grad;
+    a.scale_grad = (void*)c->scale_grad, a.shift_grad = (void*)c->shift_grad;
+    if (wants_sums(*c)) a.partial = (float*)workspace;
+    if (wants_sample_sums(*c)) a.sample_sums = (float*)workspace + p.slots * 2 * a.pitch;
+  }
+  const std::string name = std::string("mo_norm_") + (backward ? "backward_" : "forward_") +
+                           (backward ? (a.x_exponents ? "kept_" : "") : (a.kept ? "keep_" : "")) + kTypeNames[c->dtype] +
+                           "_" + std::to_string(p.iter);
+  hipFunction_t kernel;
+  if (int rc = kernels().get(name, &kernel)) return rc;
+  void* params[] = {&a};
+  if (int rc = mo::launch(kernel, (uint32_t)div_up(p.groups, p.per), 1, 1, p.lanes * p.per, stream, params, "norm launch"))
+    return rc;
+  if (!a.partial) return 0;
+  if (int rc = kernels().get("mo_norm_sums", &kernel)) return rc;
+  if (int rc = mo::launch(kernel, (c->dim + 31) / 32, c->samples ? c->samples : 1, 1, 1024, stream, params, "norm sums launch"))
+    return rc;
+  if (!a.sample_sums) return 0;
+  if (int rc = kernels().get("mo_norm_sample_sums", &kernel)) return rc;
+  return mo::launch(kernel, (c->dim + 255) / 256, 1, 1, 256, stream, params, "norm sums launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t mo_norm_workspace_bytes(const mo_norm_call* call) {
+  uint64_t bytes = 0;
+  const int rc = mo::guarded([&]() -> int {
+    if (int bad = check(call, true)) return bad;
+    bytes = workspace_bytes(*call, plan_of(*call, true));
+    return 0;
+  });
+  return rc ? 0 : bytes;
+}
+
+int mo_norm_forward(const mo_norm_call* call, uint64_t stream) {
+  return mo::guarded([&]() -> int { return run(call, false, 0, 0, stream); });
+}
+
+int mo_norm_backward(const mo_norm_call* call, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream) {
+  return mo::guarded([&]() -> int { return run(call, true, workspace, workspace_bytes, stream); });
+}
+
+}  // extern "C"

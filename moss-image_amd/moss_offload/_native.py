@@ -15,7 +15,7 @@ import torch  # noqa: F401  (must be imported before the library, see module doc
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmoss_offload.so"
 
-MO_ABI_VERSION = 25
+MO_ABI_VERSION = 26
 MO_MAX_DIMS = 8
 
 MO_E_INVALID = 1001
@@ -198,6 +198,35 @@ class MoRotaryCall(ctypes.Structure):
     ] + [("eps", ctypes.c_float), ("reserved", ctypes.c_uint32)]
 
 
+class MoNormCall(ctypes.Structure):
+    _fields_ = [
+        (name, ctypes.c_uint64)
+        for name in ("x", "x_exponents", "grad", "out", "stats", "weight", "bias", "scale", "shift", "kept",
+                     "kept_exponents", "weight_grad", "bias_grad", "scale_grad", "shift_grad", "cu", "rows", "x_stride",
+                     "grad_stride", "scale_stride", "shift_stride")
+    ] + [(name, ctypes.c_uint32) for name in ("samples", "dim", "dtype", "weight_dtype", "scale_dtype", "layer")] + [
+        ("eps", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
+class MoGatedCall(ctypes.Structure):
+    _fields_ = [
+        (name, ctypes.c_uint64)
+        for name in ("up", "gate", "up_exponents", "gate_exponents", "grad", "out", "out_gate", "kept_up", "kept_gate",
+                     "kept_up_exponents", "kept_gate_exponents", "rows", "up_stride", "gate_stride", "grad_stride",
+                     "out_stride", "values_stride", "exponents_stride")
+    ] + [(name, ctypes.c_uint32) for name in ("cols", "dtype", "silu", "reserved")]
+
+
+class MoAdaptersCall(ctypes.Structure):
+    _fields_ = [
+        (name, ctypes.c_uint64)
+        for name in ("x", "x_exponents", "result", "y", "a", "b", "scale", "cu", "index", "hidden", "grad", "add", "dx",
+                     "da", "db", "rows", "x_stride", "result_stride", "grad_stride", "add_stride")
+    ] + [(name, ctypes.c_uint32)
+         for name in ("requests", "adapters", "rank", "in_features", "out_features", "dtype")] + [
+        ("factor", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
 class EngineError(RuntimeError):
     """A non-zero status from the engine library, with its message."""
 
@@ -310,6 +339,16 @@ SIGNATURES: dict[str, tuple] = {
     "mo_rotary_backward": (ctypes.c_int, [_P(MoRotaryCall), _u64, _u64, _u64]),
     "mo_rotary_workspace_bytes": (_u64, [_P(MoRotaryCall)]),
     "mo_rotary_table": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u32, _u32, ctypes.c_float, _u64]),
+    "mo_norm_forward": (ctypes.c_int, [_P(MoNormCall), _u64]),
+    "mo_norm_backward": (ctypes.c_int, [_P(MoNormCall), _u64, _u64, _u64]),
+    "mo_norm_workspace_bytes": (_u64, [_P(MoNormCall)]),
+    "mo_keep_pack": (ctypes.c_int, [_u64, _u32, _u64, _u32, _u64, _u64, _u64, _u64]),
+    "mo_keep_restore": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u32, _u64, _u64]),
+    "mo_gated_forward": (ctypes.c_int, [_P(MoGatedCall), _u64]),
+    "mo_gated_backward": (ctypes.c_int, [_P(MoGatedCall), _u64]),
+    "mo_adapters_forward": (ctypes.c_int, [_P(MoAdaptersCall), _u64, _u64, _u64]),
+    "mo_adapters_backward": (ctypes.c_int, [_P(MoAdaptersCall), _u64, _u64, _u64]),
+    "mo_adapters_workspace_bytes": (_u64, [_P(MoAdaptersCall), _u32]),
 }
 
 _lock = threading.Lock()
