@@ -7,25 +7,63 @@
 namespace mo_adapters {
 
 constexpr uint32_t kMaxRank = 128;
+constexpr uint32_t kMaxSplits = 64;   // of the rows of a weight's gradient: a bit each in a mask
+constexpr uint32_t kOuterCols = 128;  // columns a workgroup of a weight's gradient
 
-struct Args {
-  const void* x;               // [rows][in] of the call's type, or 8-bit values [rows][groups * 32]
-  const uint8_t* x_exponents;  // [rows][groups], or null
-  const void* result;          // forward: [rows][out], the shared projection's
-  void* y;                     // forward: [rows][out]
-  const void *a, *b;           // [adapters][rank][in], [adapters][out][rank]
-  const float* scale;          // [adapters], or null: 1; times factor
-  const int64_t* cu;           // [requests + 1], or null: rows / requests each
-  const int64_t* index;        // [requests]: the adapter of each, any other number: none; null: 0, or the request's own
-  float* hidden;               // [rows][rank]: x a^T
-  const void* grad;            // backward: [rows][out]
-  const void* add;             // [rows][in] or null
-  void *dx, *da, *db;
-  float* back;                 // [rows][rank]: scale grad b
-  uint64_t x_stride, result_stride, grad_stride, add_stride;  // elements between rows
-  uint32_t rows, requests, adapters, rank, in, out, groups;
+// Which rows have which adapter.
+struct Requests {
+  const int64_t* cu;      // [requests + 1], or null: rows / requests each
+  const int64_t* index;   // [requests]: the adapter of each, any other number: none; null: 0, or the request's own
+  const float* scale;     // [adapters], or null: 1; times factor
   float factor;
-  mo_block::Divisor by_share;  // rows a request, where cu is null
+  uint32_t rows, requests, adapters, rank, share;
+};
+
+// to[row][j] = sum over the features of x[row][k] w_i[j][k].
+struct Shrink {
+  Requests by;
+  const void* x;          // [rows][features]
+  const void* w;          // [adapters][rank][features]
+  float* to;              // [splits][rows][rank]
+  uint64_t x_stride;
+  uint32_t features, span;  // features a split, a multiple of 64
+  uint32_t scaled;        // times the adapter's scale
+};
+
+// to[row][n] = base[row][n] + s sum over the rank of h[row][j] v_i[n][j], h the sum of its splits.
+struct Expand {
+  Requests by;
+  const float* h;         // [splits][rows][rank]
+  float* h_sum;           // [rows][rank], where there are several splits
+  const void* v;          // [adapters][features][rank]
+  const void* base;       // [rows][features], or null: 0
+  void* to;
+  uint64_t base_stride;
+  uint32_t features, splits, cols;  // columns a wave
+  uint32_t scaled;
+};
+
+// One gradient of a weight: sum over an adapter's rows of narrow[row][j] wide[row][c].
+struct Side {
+  const void* wide;          // [rows][cols], or 8-bit values [rows][groups * 32]
+  const uint8_t* exponents;  // [rows][groups], or null
+  const float* narrow;       // [rows][rank]
+  float* planes;             // [splits][adapters][cols * rank] sums over a split's rows, where there are several
+  void* to;                  // [adapters][rank][cols], or turned: [adapters][cols][rank]; null: not wanted
+  uint64_t stride;
+  uint32_t cols, groups, tiles, splits, span;  // span: rows a split, a multiple of 32
+  uint32_t turned, scaled;
+};
+struct Outer {
+  Requests by;
+  Side side[2];
+};
+
+// Copies of both weights, each [adapters] matrices turned.
+struct Turn {
+  const void* from[2];
+  void* to[2];
+  uint32_t rows[2], cols[2], tiles[2];  // of `from`; tiles of 32 x 32, 0: not wanted
 };
 
 }  // namespace mo_adapters
