@@ -728,7 +728,8 @@ typedef struct mo_adapters_call {
   uint64_t hidden;         /* fp32 [rows][rank]: written forward, read backward */
   uint64_t grad, add;      /* backward: y's gradient [rows][out]; [rows][in] to be added to dx, or 0 */
   uint64_t dx, da, db;     /* backward, dense, or 0: not wanted. An adapter that no row has gets zeros */
-  uint64_t rows, x_stride, result_stride, grad_stride, add_stride; /* strides in elements */
+  uint64_t rows;           /* under 2^26 */
+  uint64_t x_stride, result_stride, grad_stride, add_stride; /* strides in elements, up to 2^22 */
   uint32_t requests, adapters, rank, in_features, out_features, dtype; /* rank 1 to 128 */
   float factor;            /* times every scale */
   uint32_t reserved;

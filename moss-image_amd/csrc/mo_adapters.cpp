@@ -13,8 +13,8 @@ using mo_adapters::Requests;
 const char* const kTypeNames[3] = {"f16", "bf16", "f32"};  // by MO_DTYPE_*
 constexpr uint32_t kTypeBytes[3] = {2, 2, 4};
 
-// Workgroups that a launch aims at: four, four and three for each of 256 CUs.
-constexpr uint64_t kShrinkGroups = 1024, kExpandGroups = 1024, kOuterGroups = 768;
+// Workgroups that a launch aims at: four and three for each of 256 CUs.
+constexpr uint64_t kExpandGroups = 1024, kOuterGroups = 768;
 
 mo::Kernels& kernels() {
   static mo::Kernels k(mo_adapters_code);
@@ -26,7 +26,11 @@ int check(const mo_adapters_call* c, bool backward) {
   if (!c) return bad("null call");
   if (c->dtype > MO_DTYPE_F32) return bad("unknown element type");
   const uint32_t size = kTypeBytes[c->dtype];
-  if (c->rows == 0 || c->rows >= (1ull << 31) - 65536) return bad("no rows, or too many");
+  // a lane's offsets from its wave's address have 31 bits: 31 rows of the tokens, and a whole matrix of an adapter
+  if (c->rows == 0 || c->rows >= mo_adapters::kMaxRows) return bad("rows must be 1 to 2^26 - 1");
+  if (c->rows > 1 && (c->x_stride > mo_adapters::kMaxStride || c->result_stride > mo_adapters::kMaxStride ||
+                      c->grad_stride > mo_adapters::kMaxStride || c->add_stride > mo_adapters::kMaxStride))
+    return bad("rows are more than 2^22 elements apart");
   if (c->in_features == 0 || c->in_features > (1u << 20) || c->out_features == 0 || c->out_features > (1u << 20))
     return bad("features must be 1 to 2^20");
   if (c->rank == 0 || c->rank > mo_adapters::kMaxRank) return bad("rank must be 1 to 128");
@@ -51,13 +55,27 @@ int check(const mo_adapters_call* c, bool backward) {
   return 0;
 }
 
+// The distance between rows; of one row, its length.
+uint64_t stride_of(const mo_adapters_call& c, uint64_t stride, uint32_t features) { return c.rows > 1 ? stride : features; }
+
 uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 uint64_t round_up(uint64_t a, uint64_t b) { return div_up(a, b) * b; }
 template <class N>
 N between(N low, N value, N high) { return value < low ? low : value > high ? high : value; }
 
-// Rows a tile and splits of the features of a shrink. Short requests take tiles of 16 rows, whose other rows would be
-// empty; the features are shared out until there are some workgroups for every CU, 256 features each at least.
+// Whether eight neighbouring values can be read at once: features and rank are multiples of eight and every row lies on
+// the 4-byte grid. Other calls have kernels that read value by value.
+bool odd(const mo_adapters_call& c) {
+  const uint64_t size = kTypeBytes[c.dtype];
+  uint64_t off = (c.in_features | c.out_features | c.rank) % 8;
+  for (uint64_t p : {c.x_exponents ? 0 : c.x, c.result, c.y, c.a, c.b, c.grad, c.add, c.dx, c.da, c.db}) off |= p % 4;
+  if (c.rows > 1)
+    for (uint64_t s : {c.x_exponents ? 0 : c.x_stride, c.result_stride, c.grad_stride, c.add_stride}) off |= s * size % 4;
+  return off != 0;
+}
+
+// Rows a tile and splits of the features of a shrink: tiles of 16 rows where those are few or the requests short (the
+// other rows would be empty), and splits until there are four workgroups for every CU, 1024 features each at least.
 struct ShrinkPlan {
   uint32_t ranks, tiles, splits, span;
   uint64_t slots;
@@ -65,16 +83,16 @@ struct ShrinkPlan {
 ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
   ShrinkPlan p = {};
   p.ranks = c.rank <= 16 ? 1 : c.rank <= 32 ? 2 : c.rank <= 64 ? 4 : 8;
-  p.tiles = p.ranks < 8 && c.rows >= 32ull * c.requests ? 2 : 1;
+  p.tiles = !odd(c) && c.dtype == MO_DTYPE_BF16 && p.ranks < 8 && c.rows >= 32ull * c.requests && c.rows >= (p.ranks > 1 ? 4096 : 8192) ? 2 : 1;
   const uint64_t tiles = div_up(c.rows, p.tiles * 16);
-  const uint64_t splits = between<uint64_t>(1, div_up(kShrinkGroups, tiles), 8);
-  p.span = (uint32_t)round_up(div_up(features, splits), 256);
+  const uint64_t splits = between<uint64_t>(1, between<uint64_t>(1, div_up(1024, tiles), div_up(features, 1024)), 8);
+  p.span = (uint32_t)round_up(div_up(features, splits), 1024);
   p.splits = (uint32_t)div_up(features, p.span);
   p.slots = tiles + c.requests + 1;
   return p;
 }
 
-// Rows a tile and columns a wave of an expand: as many as leave some workgroups for every CU.
+// Rows a tile and columns a workgroup of an expand: as many as leave some workgroups for every CU.
 struct ExpandPlan {
   uint32_t rank, tiles, cols;
   uint64_t slots;
@@ -82,28 +100,30 @@ struct ExpandPlan {
 ExpandPlan expand_plan(const mo_adapters_call& c, uint32_t features) {
   ExpandPlan p = {};
   p.rank = c.rank <= 16 ? 16 : c.rank <= 32 ? 32 : c.rank <= 64 ? 64 : 128;
-  p.tiles = p.rank < 128 && c.rows >= 64ull * c.requests ? 4 : 1;
+  p.tiles = !odd(c) && p.rank < 128 && c.rows >= 32ull * c.requests ? 2 : 1;
   const uint64_t tiles = div_up(c.rows, p.tiles * 16);
-  p.cols = (uint32_t)round_up(between<uint64_t>(1, tiles * features / (4 * kExpandGroups), 512), 32);
+  p.cols = (uint32_t)round_up(between<uint64_t>(1, tiles * features / kExpandGroups, 4096), 512);
   p.slots = tiles + c.requests + 1;
   return p;
 }
 
-// Splits of the rows of a weight's gradient: some workgroups for every CU again, 128 rows each at least.
-void share_rows(const mo_adapters_call& c, mo_adapters::Side* side, uint32_t cols) {
-  side->cols = cols;
-  side->tiles = (uint32_t)div_up(cols, mo_adapters::kOuterCols);
-  const uint64_t used = c.adapters < c.requests ? c.adapters : c.requests;
-  uint64_t splits = div_up(kOuterGroups, side->tiles * used);
-  splits = between<uint64_t>(1, splits, div_up(c.rows, 128));
+// Splits of the rows of the weights' gradients, the same for both: some workgroups for every CU again, 128 rows each at
+// least, and no more planes than 256 MB hold.
+void share_rows(const mo_adapters_call& c, mo_adapters::Side* a, mo_adapters::Side* b) {
+  a->cols = c.da ? c.in_features : 0, b->cols = c.db ? c.out_features : 0;
+  a->tiles = (uint32_t)div_up(a->cols, mo_adapters::kOuterCols), b->tiles = (uint32_t)div_up(b->cols, mo_adapters::kOuterCols);
+  const uint64_t plane = 4ull * c.adapters * c.rank * (a->cols + b->cols);
+  uint64_t splits = between<uint64_t>(1, div_up(kOuterGroups, a->tiles + b->tiles), div_up(c.rows, 128));
+  const uint64_t held = (256u << 20) / plane;
+  splits = between<uint64_t>(1, splits, held ? held : 1);
   if (splits > mo_adapters::kMaxSplits) splits = mo_adapters::kMaxSplits;
-  side->span = (uint32_t)round_up(div_up(c.rows, splits), 32);
-  side->splits = (uint32_t)div_up(c.rows, side->span);
+  a->span = b->span = (uint32_t)round_up(div_up(c.rows, splits), 32);
+  a->splits = b->splits = (uint32_t)div_up(c.rows, a->span);
 }
 
 // Where what a call needs for itself lies in its workspace.
 struct Room {
-  uint64_t back, planes, turned_a, turned_b, da, db, bytes;  // offsets
+  uint64_t back, planes, turned_a, turned_b, turned_hidden, turned_back, da, db, bytes;  // offsets
 };
 Room room_of(const mo_adapters_call& c, bool backward) {
   Room r = {};
@@ -113,6 +133,7 @@ Room room_of(const mo_adapters_call& c, bool backward) {
     return at;
   };
   const uint64_t between_bytes = c.rows * c.rank * 4, size = kTypeBytes[c.dtype];
+  const uint64_t turned = round_up(c.rows, 32) * c.rank * 4;  // one fp32 or two bfloat16, in whole steps of 32 rows
   if (!backward) {
     const ShrinkPlan p = shrink_plan(c, c.in_features);
     if (p.splits > 1) r.planes = take(p.splits * between_bytes);
@@ -120,51 +141,44 @@ Room room_of(const mo_adapters_call& c, bool backward) {
   }
   if (c.dx || c.da) {
     const ShrinkPlan p = shrink_plan(c, c.out_features);
-    r.back = take(between_bytes);
-    if (p.splits > 1) r.planes = take(p.splits * between_bytes);
+    r.planes = take(p.splits * between_bytes);
     r.turned_b = take((uint64_t)c.adapters * c.rank * c.out_features * size);
   }
   if (c.dx) r.turned_a = take((uint64_t)c.adapters * c.rank * c.in_features * size);
-  mo_adapters::Side side = {};
-  if (c.da) {
-    share_rows(c, &side, c.in_features);
-    if (side.splits > 1) r.da = take(4ull * side.splits * c.adapters * c.rank * c.in_features);
-  }
-  if (c.db) {
-    share_rows(c, &side, c.out_features);
-    if (side.splits > 1) r.db = take(4ull * side.splits * c.adapters * c.rank * c.out_features);
+  if (c.da) r.turned_back = take(turned);
+  if (c.db) r.turned_hidden = take(turned);
+  if (c.da || c.db) {
+    mo_adapters::Side a = {}, b = {};
+    share_rows(c, &a, &b);
+    if (c.da && a.splits > 1) r.da = take(4ull * a.splits * c.adapters * c.rank * c.in_features);
+    if (c.db && b.splits > 1) r.db = take(4ull * b.splits * c.adapters * c.rank * c.out_features);
   }
   return r;
 }
 
-int start(const std::string& name, uint64_t gx, uint64_t gy, uint64_t gz, void* args, uint64_t stream) {
+int start(const std::string& name, uint64_t gx, uint64_t gy, uint64_t gz, void* args, uint64_t stream, uint32_t threads = 256) {
   if (gx >= (1ull << 31) || gy >= (1u << 16) || gz > (1u << 16)) return mo::set_error(MO_E_INVALID, "too many values");
   hipFunction_t kernel;
   if (int rc = kernels().get("mo_adapters_" + name, &kernel)) return rc;
   void* params[] = {args};
-  return mo::launch(kernel, (uint32_t)gx, (uint32_t)gy, (uint32_t)gz, 256, stream, params, "adapters launch");
+  return mo::launch(kernel, (uint32_t)gx, (uint32_t)gy, (uint32_t)gz, threads, stream, params, "adapters launch");
 }
 
 int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t stride, uint64_t w, uint32_t features, uint64_t to,
-           uint64_t planes, bool scaled, uint64_t stream) {
+           bool scaled, uint64_t stream) {
   const ShrinkPlan p = shrink_plan(c, features);
   mo_adapters::Shrink a = {};
-  a.by = by, a.x = (const void*)x, a.w = (const void*)w, a.to = (float*)(p.splits > 1 ? planes : to);
+  a.by = by, a.x = (const void*)x, a.w = (const void*)w, a.to = (float*)to;
   a.x_stride = stride, a.features = features, a.span = p.span, a.scaled = scaled;
-  return start(std::string("shrink_") + kTypeNames[c.dtype] + "_" + std::to_string(p.ranks) + "_" + std::to_string(p.tiles),
-               p.slots, p.splits, 1, &a, stream);
+  return start(std::string("shrink_") + kTypeNames[c.dtype] + "_" + std::to_string(p.ranks) + (odd(c) ? "_odd" : p.tiles == 2 ? "_2" : "_1"),
+               p.slots, p.splits, 1, &a, stream, 512);
 }
 
-// `splits` > 1: h's, with their sum left at `h`.
-int expand(const mo_adapters_call& c, const Requests& by, uint64_t h, uint64_t planes, uint32_t splits, uint64_t v, uint64_t base,
-           uint64_t stride, uint64_t to, uint32_t features, bool scaled, uint64_t stream) {
-  const ExpandPlan p = expand_plan(c, features);
-  mo_adapters::Expand a = {};
-  a.by = by, a.h = (const float*)(splits > 1 ? planes : h), a.h_sum = splits > 1 ? (float*)h : nullptr;
-  a.v = (const void*)v, a.base = (const void*)base, a.to = (void*)to, a.base_stride = stride;
-  a.features = features, a.splits = splits, a.cols = p.cols, a.scaled = scaled;
-  return start(std::string("expand_") + kTypeNames[c.dtype] + "_" + std::to_string(p.rank) + "_" + std::to_string(p.tiles),
-               p.slots, div_up(features, 4 * p.cols), 1, &a, stream);
+int expand(const mo_adapters_call& c, mo_adapters::Expand& a, uint64_t stream) {
+  const ExpandPlan p = expand_plan(c, a.features);
+  a.cols = p.cols;
+  return start(std::string("expand_") + kTypeNames[c.dtype] + "_" + std::to_string(p.rank) + (odd(c) ? "_odd" : p.tiles == 2 ? "_2" : "_1"),
+               p.slots, div_up(a.features, p.cols), 1, &a, stream);
 }
 
 int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_t bytes, uint64_t stream) {
@@ -178,62 +192,60 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
   by.rows = (uint32_t)c.rows, by.requests = c.requests, by.adapters = c.adapters, by.rank = c.rank;
   by.share = c.cu ? 0 : (uint32_t)(c.rows / c.requests);
   const uint64_t planes = workspace + room.planes;
-  if (!backward) {
-    if (int rc = shrink(c, by, c.x, c.x_stride, c.a, c.in_features, c.hidden, planes, false, stream)) return rc;
-    return expand(c, by, c.hidden, planes, shrink_plan(c, c.in_features).splits, c.b, c.result, c.result_stride, c.y,
-                  c.out_features, true, stream);
-  }
-  const uint64_t back = workspace + room.back;
   const char* type = kTypeNames[c.dtype];
+  mo_adapters::Expand e = {};
+  e.by = by;
+  if (!backward) {
+    e.splits = shrink_plan(c, c.in_features).splits;
+    const uint64_t to = e.splits > 1 ? planes : c.hidden;
+    if (int rc = shrink(c, by, c.x, stride_of(c, c.x_stride, c.in_features), c.a, c.in_features, to, false, stream)) return rc;
+    e.h = (const float*)to, e.h_sum = e.splits > 1 ? (float*)c.hidden : nullptr;
+    e.v = (const void*)c.b, e.base = (const void*)c.result, e.base_stride = stride_of(c, c.result_stride, c.out_features), e.to = (void*)c.y;
+    e.features = c.out_features, e.scaled = 1;
+    return expand(c, e, stream);
+  }
+  mo_adapters::Turn t = {};
+  t.adapters = c.adapters, t.count = by.rows, t.rank = c.rank;
+  auto turned = [&](int i, uint64_t from, uint64_t to, uint32_t rows, uint32_t cols) {
+    t.from[i] = (const void*)from, t.to[i] = (void*)to, t.rows[i] = rows, t.cols[i] = cols;
+    t.tiles[i] = (uint32_t)(div_up(rows, 32) * div_up(cols, 32));
+  };
+  if (c.dx || c.da) turned(0, c.b, workspace + room.turned_b, c.out_features, c.rank);
+  if (c.dx) turned(1, c.a, workspace + room.turned_a, c.rank, c.in_features);
+  const uint64_t narrow = div_up(c.rows, 32) * div_up(c.rank, 32);
+  if (c.db) t.narrow = (const float*)c.hidden, t.turned = (void*)(workspace + room.turned_hidden), t.splits = 1;
+  const uint64_t weights = (uint64_t)t.tiles[0] + t.tiles[1];
+  if (int rc = start(std::string("turn_") + type, weights + (c.db ? narrow : 0), weights ? c.adapters : 1, 1, &t, stream)) return rc;
   if (c.dx || c.da) {
-    mo_adapters::Turn t = {};
-    auto side = [&](int i, uint64_t from, uint64_t to, uint32_t rows, uint32_t cols) {
-      t.from[i] = (const void*)from, t.to[i] = (void*)to, t.rows[i] = rows, t.cols[i] = cols;
-      t.tiles[i] = (uint32_t)(div_up(rows, 32) * div_up(cols, 32));
-    };
-    side(0, c.b, workspace + room.turned_b, c.out_features, c.rank);
-    if (c.dx) side(1, c.a, workspace + room.turned_a, c.rank, c.in_features);
-    if (int rc = start(std::string("turn_") + type, (uint64_t)t.tiles[0] + t.tiles[1], c.adapters, 1, &t, stream)) return rc;
+    if (int rc = shrink(c, by, c.grad, stride_of(c, c.grad_stride, c.out_features), workspace + room.turned_b, c.out_features, planes, true, stream)) return rc;
     const uint32_t splits = shrink_plan(c, c.out_features).splits;
-    if (int rc = shrink(c, by, c.grad, c.grad_stride, workspace + room.turned_b, c.out_features, back, planes, true, stream))
-      return rc;
     if (c.dx) {
-      if (int rc = expand(c, by, back, planes, splits, workspace + room.turned_a, c.add, c.add_stride, c.dx, c.in_features, false,
-                          stream))
-        return rc;
-    } else if (splits > 1) {
-      hipFunction_t kernel;
-      if (int rc = kernels().get("mo_adapters_sum", &kernel)) return rc;
-      const float* from = (const float*)planes;
-      float* to = (float*)back;
-      uint64_t count = c.rows * c.rank;
-      uint32_t parts = splits;
-      void* params[] = {&from, &to, &count, &parts};
-      if (int rc = mo::launch(kernel, (uint32_t)div_up(count, 256), 1, 1, 256, stream, params, "adapters launch")) return rc;
+      e.splits = splits, e.h = (const float*)planes, e.turned = c.da ? (void*)(workspace + room.turned_back) : nullptr;
+      e.v = (const void*)(workspace + room.turned_a), e.base = (const void*)c.add, e.base_stride = stride_of(c, c.add_stride, c.in_features);
+      e.to = (void*)c.dx, e.features = c.in_features;
+      if (int rc = expand(c, e, stream)) return rc;
+    } else {
+      t.tiles[0] = t.tiles[1] = 0;
+      t.narrow = (const float*)planes, t.turned = (void*)(workspace + room.turned_back), t.splits = splits;
+      if (int rc = start(std::string("turn_") + type, narrow, 1, 1, &t, stream)) return rc;
     }
   }
   if (!c.da && !c.db) return 0;
   mo_adapters::Outer o = {};
   o.by = by;
-  if (c.da) {
-    mo_adapters::Side& s = o.side[0];
-    share_rows(c, &s, c.in_features);
-    s.wide = (const void*)c.x, s.exponents = (const uint8_t*)c.x_exponents, s.narrow = (const float*)back;
-    s.planes = (float*)(workspace + room.da), s.to = (void*)c.da, s.stride = c.x_stride, s.groups = (c.in_features + 31) / 32;
-  }
-  if (c.db) {
-    mo_adapters::Side& s = o.side[1];
-    share_rows(c, &s, c.out_features);
-    s.wide = (const void*)c.grad, s.narrow = (const float*)c.hidden, s.planes = (float*)(workspace + room.db), s.to = (void*)c.db;
-    s.stride = c.grad_stride, s.turned = 1, s.scaled = 1;
-  }
+  mo_adapters::Side &a = o.side[0], &b = o.side[1];
+  share_rows(c, &a, &b);
+  a.wide = (const void*)c.x, a.exponents = (const uint8_t*)c.x_exponents, a.narrow = (const void*)(workspace + room.turned_back);
+  a.planes = (float*)(workspace + room.da), a.to = (void*)c.da, a.stride = stride_of(c, c.x_stride, c.in_features), a.groups = (c.in_features + 31) / 32;
+  b.wide = (const void*)c.grad, b.narrow = (const void*)(workspace + room.turned_hidden);
+  b.planes = (float*)(workspace + room.db), b.to = (void*)c.db, b.stride = stride_of(c, c.grad_stride, c.out_features);
+  b.turned = 1, b.scaled = 1;
   const uint32_t ranks = c.rank <= 16 ? 1 : c.rank <= 32 ? 2 : 4;
-  const uint32_t most = o.side[0].splits > o.side[1].splits ? o.side[0].splits : o.side[1].splits;
-  if (int rc = start(std::string("outer_") + type + "_" + std::to_string(ranks), (uint64_t)o.side[0].tiles + o.side[1].tiles, most,
+  if (int rc = start(std::string("outer_") + type + "_" + std::to_string(ranks) + (odd(c) ? "_odd" : ""), (uint64_t)a.tiles + b.tiles, a.splits,
                      (uint64_t)c.adapters * div_up(c.rank, ranks * 16), &o, stream))
     return rc;
-  if (most <= 1) return 0;
-  const uint64_t size = (uint64_t)c.rank * (c.in_features > c.out_features ? c.in_features : c.out_features);
+  if (a.splits == 1) return 0;
+  const uint64_t size = (uint64_t)c.rank * (a.cols > b.cols ? a.cols : b.cols);
   return start(std::string("join_") + type, div_up(size, 1024), c.adapters, 2, &o, stream);
 }
 

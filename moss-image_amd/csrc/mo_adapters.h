@@ -7,6 +7,8 @@
 namespace mo_adapters {
 
 constexpr uint32_t kMaxRank = 128;
+constexpr uint64_t kMaxRows = 1ull << 26;    // less
+constexpr uint64_t kMaxStride = 1ull << 22;  // elements between rows
 constexpr uint32_t kMaxSplits = 64;   // of the rows of a weight's gradient: a bit each in a mask
 constexpr uint32_t kOuterCols = 128;  // columns a workgroup of a weight's gradient
 
@@ -26,7 +28,7 @@ struct Shrink {
   const void* w;          // [adapters][rank][features]
   float* to;              // [splits][rows][rank]
   uint64_t x_stride;
-  uint32_t features, span;  // features a split, a multiple of 64
+  uint32_t features, span;  // features a split, a multiple of 128
   uint32_t scaled;        // times the adapter's scale
 };
 
@@ -34,12 +36,13 @@ struct Shrink {
 struct Expand {
   Requests by;
   const float* h;         // [splits][rows][rank]
-  float* h_sum;           // [rows][rank], where there are several splits
+  float* h_sum;           // [rows][rank] or null
+  void* turned;           // h turned, for an outer, or null
   const void* v;          // [adapters][features][rank]
   const void* base;       // [rows][features], or null: 0
   void* to;
   uint64_t base_stride;
-  uint32_t features, splits, cols;  // columns a wave
+  uint32_t features, splits, cols;  // columns a workgroup, a multiple of 512
   uint32_t scaled;
 };
 
@@ -47,7 +50,7 @@ struct Expand {
 struct Side {
   const void* wide;          // [rows][cols], or 8-bit values [rows][groups * 32]
   const uint8_t* exponents;  // [rows][groups], or null
-  const float* narrow;       // [rows][rank]
+  const void* narrow;        // turned: [rows / 8][parts][rank][8]
   float* planes;             // [splits][adapters][cols * rank] sums over a split's rows, where there are several
   void* to;                  // [adapters][rank][cols], or turned: [adapters][cols][rank]; null: not wanted
   uint64_t stride;
@@ -59,11 +62,15 @@ struct Outer {
   Side side[2];
 };
 
-// Copies of both weights, each [adapters] matrices turned.
+// Copies of both weights, each [adapters] matrices turned, and of a narrow matrix for an outer: the sum of its splits,
+// turned, [rows / 8][parts][rank][8].
 struct Turn {
   const void* from[2];
   void* to[2];
   uint32_t rows[2], cols[2], tiles[2];  // of `from`; tiles of 32 x 32, 0: not wanted
+  const float* narrow;                  // [splits][count][rank]
+  void* turned;
+  uint32_t adapters, count, rank, splits;
 };
 
 }  // namespace mo_adapters

@@ -31,6 +31,51 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kNone = 0xffffffffu;
 
+// A part of memory that all lanes share: its address stays in scalar registers, a lane has 32-bit offsets (the host keeps
+// rows near enough for that), and what a lane should not read or write it asks for past the end, where reads
+// give zeros and writes are dropped. Odd sizes, or addresses off the 4-byte grid, go value by value.
+constexpr uint32_t kNowhere = 0x80000000u;  // no window is as long
+
+template <class T, bool kOdd>
+struct Window {
+  T* at;
+  __amdgpu_buffer_rsrc_t buffer;
+  // `count` elements from `p`
+  __device__ __forceinline__ Window(const T* p, uint32_t count)
+      : at(const_cast<T*>(p)),
+        buffer(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, (int)(count * sizeof(T)), 0x00020000)) {}
+  // the first n (8 or 0, unless kOdd) of eight elements, `shared` + `own` from the beginning; the rest are zero
+  __device__ __forceinline__ Eight<T> read(uint32_t shared, uint32_t own, uint32_t n) const {
+    if (kOdd) return load8<true>(at + shared + (n ? own : 0), n);
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    Words words[sizeof(Eight<T>) / 16];
+    const uint32_t offset = n ? own * (uint32_t)sizeof(T) : kNowhere;
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(Eight<T>) / 16; ++i)
+      words[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer, offset + i * 16, shared * (uint32_t)sizeof(T), 0);
+    return __builtin_bit_cast(Eight<T>, words);
+  }
+  __device__ __forceinline__ void write(const float (&v)[8], uint32_t shared, uint32_t own, uint32_t n) const {
+    if (kOdd) {
+      store8<true>(at + shared + (n ? own : 0), v, n);
+      return;
+    }
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    Eight<T> e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e.v[i] = (T)v[i];
+    struct All {
+      Words words[sizeof(Eight<T>) / 16];
+    };
+    const All all = __builtin_bit_cast(All, e);
+    const uint32_t offset = n ? own * (uint32_t)sizeof(T) : kNowhere;
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(Eight<T>) / 16; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(all.words[i], buffer, offset + i * 16, shared * (uint32_t)sizeof(T), 0);
+  }
+};
+__device__ __forceinline__ uint32_t wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+
 // ---- operands of the matrix instructions: eight values a lane, 32 of the reduced dimension a fragment ----
 
 struct Eight32 {
@@ -41,11 +86,12 @@ template <class T>
 struct Path {  // fp32 instructions: lane (i, k) has values k * 8 to k * 8 + 7, one instruction for each of the eight
   typedef Eight32 Fragment;
   static constexpr int kParts = 1;
-  static __device__ __forceinline__ Fragment load(const T* p, uint32_t n) {
+  static __device__ __forceinline__ Fragment of(const Eight<T>& v) {
     Fragment f;
-    widen(f.v, load8(p, n));
+    widen(f.v, v);
     return f;
   }
+  typedef float Narrow;
   static __device__ __forceinline__ Fragment part(const float (&v)[8], int) {
     Fragment f;
 #pragma unroll
@@ -77,9 +123,8 @@ template <>
 struct Path<__bf16> {
   typedef bf16x8 Fragment;
   static constexpr int kParts = 2;
-  static __device__ __forceinline__ Fragment load(const __bf16* p, uint32_t n) {
-    return __builtin_bit_cast(Fragment, load8(p, n));
-  }
+  static __device__ __forceinline__ Fragment of(const Eight<__bf16>& v) { return __builtin_bit_cast(Fragment, v); }
+  typedef __bf16 Narrow;
   // The upper half of an fp32 number (cut, so that nothing overflows), and the rest of it rounded to the nearest. What
   // is not finite has no rest.
   static __device__ __forceinline__ Fragment part(const float (&v)[8], int which) {
@@ -154,161 +199,217 @@ __device__ __forceinline__ Tile tile_of(const Requests& by, uint32_t slot) {
   low = __builtin_amdgcn_readfirstlane(low);
   const uint32_t first = (slot - low) * kRows;
   Tile t;
-  t.low = max(border(low), first);
-  t.high = min(border(low + 1), first + kRows);
-  t.adapter = low == 0 || low == pieces - 1 ? kNone : adapter_of(by, low - 1);
+  t.low = __builtin_amdgcn_readfirstlane(max(border(low), first));
+  t.high = __builtin_amdgcn_readfirstlane(min(border(low + 1), first + kRows));
+  t.adapter = __builtin_amdgcn_readfirstlane(low == 0 || low == pieces - 1 ? kNone : adapter_of(by, low - 1));
   return t;
 }
 
 // ---- shrink ------------------------------------------------------------------------------------------
 
-// A workgroup has kTiles * 16 rows, all ranks and one split of the features; its waves take 64 features in turn and add
-// up through LDS. The rows are the instruction's columns, so a lane ends with four neighbouring ranks of a row.
-template <class T, int kRanks, int kTiles>
+// A workgroup has kTiles * 16 rows, all ranks and one split of the features; its eight waves take 128 features in turn and
+// add up through LDS. A wave reads 256 bytes of each row side by side (64 bytes a row, as the instructions want them, came
+// at 4.2 TB/s where this comes at 5.4) and turns them through its own part of LDS, eight values at a time; those of
+// row r lie at (place ^ r), so that neither writing nor reading meets a bank twice. The rows are the instruction's
+// columns, so a lane ends with four neighbouring ranks of a row. Nothing is loaded ahead: sixteen waves a CU are enough.
+template <class T, int kRanks, int kTiles, bool kOdd>
 __device__ __forceinline__ void shrink(const Shrink& a) {
   typedef Path<T> P;
   constexpr uint32_t kRows = kTiles * 16, kPitch = kRanks * 16 + 4;
-  __shared__ float room[4][kRows][kPitch];
+  union Room {
+    Eight<T> stage[8][kRows][16];
+    float sums[8][kRows][kPitch];
+    __device__ Room() {}
+  };
+  __shared__ Room room;
   const Tile tile = tile_of<kRows>(a.by, blockIdx.x);
   if (tile.low >= tile.high) return;
-  const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 16, k = lane / 16;
+  const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
   f32x4 sum[kRanks][kTiles];
 #pragma unroll
   for (int r = 0; r < kRanks; ++r)
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) sum[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (tile.adapter != kNone) {
-    const T* x[kTiles];
-    const T* w[kRanks];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) x[t] = (const T*)a.x + min(tile.low + t * 16 + i, tile.high - 1) * a.x_stride + k * 8;
-#pragma unroll
-    for (int r = 0; r < kRanks; ++r)
-      w[r] = (const T*)a.w + ((uint64_t)tile.adapter * rank + min(r * 16 + i, rank - 1)) * a.features + k * 8;
+    const uint32_t stride = (uint32_t)a.x_stride, rows = tile.high - tile.low;
+    const Window<T, kOdd> x((const T*)a.x + tile.low * a.x_stride, (rows - 1) * stride + a.features);
+    const Window<T, kOdd> w((const T*)a.w + (uint64_t)tile.adapter * rank * a.features, rank * a.features);
     const uint32_t first = blockIdx.y * a.span, last = min(a.features, first + a.span);
-    auto step = [&](uint32_t at, auto whole) {
-      typename P::Fragment xs[2][kTiles], ws[2][kRanks];
+    for (uint32_t at = first + wave * 128; at < last; at += 1024) {
+      Eight<T> xs[kTiles * 4];
+      Eight<T> ws[4][kRanks];
+      const uint32_t n = at + i * 8 >= last ? 0 : min(8u, last - at - i * 8);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t from = at + u * 32, mine = from + k * 8;
-        const uint32_t n = whole ? 8 : mine >= last ? 0 : min(8u, last - mine);
+      for (uint32_t t = 0; t < kTiles * 4; ++t) xs[t] = x.read(t * 4 * stride + at, k * stride + i * 8, t * 4 + k < rows ? n : 0);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) xs[u][t] = P::load(x[t] + (n ? from : 0), n);
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t from = at + u * 32 + k * 8, m = from >= last ? 0 : min(8u, last - from);
 #pragma unroll
-        for (int r = 0; r < kRanks; ++r) ws[u][r] = P::load(w[r] + (n ? from : 0), n);
+        for (uint32_t r = 0; r < kRanks; ++r)
+          ws[u][r] = w.read(r * 16 * a.features + at + u * 32, i * a.features + k * 8, r * 16 + i < rank ? m : 0);
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int t = 0; t < kTiles * 4; ++t) room.stage[wave][t * 4 + k][i ^ (t * 4 + k) % 16] = xs[t];
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int r = 0; r < kRanks; ++r)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) P::multiply(sum[r][t], ws[u][r], xs[u][t]);
-    };
-    uint32_t at = first + wave * 64;
-    for (; at + 64 <= last; at += 256) step(at, std::true_type{});
-    if (at < last) step(at, std::false_type{});
+        for (int t = 0; t < kTiles; ++t) {
+          const typename P::Fragment f = P::of(room.stage[wave][t * 16 + i][(u * 4 + k) ^ i]);
+#pragma unroll
+          for (int r = 0; r < kRanks; ++r) P::multiply(sum[r][t], P::of(ws[u][r]), f);
+        }
+      __builtin_amdgcn_wave_barrier();
+    }
   }
+  __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRanks; ++r)
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) *(f32x4*)&room[wave][t * 16 + i][r * 16 + k * 4] = sum[r][t];
+    for (int t = 0; t < kTiles; ++t) *(f32x4*)&room.sums[wave][t * 16 + i][r * 16 + k * 4] = sum[r][t];
   __syncthreads();
   const float scale = a.scaled && tile.adapter != kNone ? scale_of(a.by, tile.adapter) : 1.0f;
   float* to = a.to + ((uint64_t)blockIdx.y * a.by.rows + tile.low) * rank;
-  const uint32_t rows = tile.high - tile.low;
-  for (uint32_t e = threadIdx.x; e < rows * (kRanks * 16); e += 256) {
+  for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * (kRanks * 16); e += 512) {
     const uint32_t row = e / (kRanks * 16), j = e % (kRanks * 16);
-    if (j < rank) to[(uint64_t)row * rank + j] = (room[0][row][j] + room[1][row][j] + room[2][row][j] + room[3][row][j]) * scale;
+    float total = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) total += room.sums[u][row][j];
+    if (j < rank) to[(uint64_t)row * rank + j] = total * scale;
   }
 }
 
 // ---- expand ------------------------------------------------------------------------------------------
 
-// A workgroup has kTiles * 16 rows, whose h stays in registers, and `cols` columns a wave, 32 at a time. The columns are
-// the instructions' rows, spread so that a lane ends with eight neighbouring columns of a row: 16 bytes to read
-// and to write. With ranks up to 16 the two parts of h lie beside each other in one fragment.
-template <class T, int kRank, int kTiles>
+// A value of a narrow matrix turned, for the instructions of an outer: [rows / 8][parts][rank][8 rows], fp32 in one part
+// or bfloat16 in two, so that a fragment is read from neighbouring places.
+template <class T>
+__device__ __forceinline__ void store_turned(void* to, uint32_t rank, uint32_t j, uint32_t row, float v) {
+  const float one[8] = {v};
+#pragma unroll
+  for (int p = 0; p < Path<T>::kParts; ++p) {
+    const uint64_t at = (((uint64_t)(row / 8) * Path<T>::kParts + p) * rank + j) * 8 + row % 8;
+    if (Path<T>::kParts == 2)
+      ((__bf16*)to)[at] = Path<__bf16>::part(one, p)[0];
+    else
+      ((float*)to)[at] = v;
+  }
+}
+
+// A workgroup has kTiles * 16 rows, whose h stays in registers, and `cols` columns, of which a wave takes 128 at a time. The
+// columns are the instructions' rows, so a lane ends with four neighbouring columns of a row; through the wave's own
+// part of LDS they come to lanes that read and write 256 bytes of a row side by side. With ranks up to 16 the two
+// parts of h lie beside each other in one fragment.
+template <class T, int kRank, int kTiles, bool kOdd>
 __device__ __forceinline__ void expand(const Expand& a) {
   typedef Path<T> P;
   constexpr uint32_t kRows = kTiles * 16;
   constexpr bool kBeside = kRank == 16 && P::kParts == 2;
   constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 1 : P::kParts;
+  __shared__ float room[4][16][132];
   const Tile tile = tile_of<kRows>(a.by, blockIdx.x);
   if (tile.low >= tile.high) return;
-  const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 16, k = lane / 16;
+  const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
   const bool has = tile.adapter != kNone;
+  const uint32_t first = blockIdx.y * a.cols, end = min(a.features, first + a.cols);
   typename P::Fragment h[kParts][kSteps][kTiles];
   float scale = 0.0f;
   if (has) {
     scale = a.scaled ? scale_of(a.by, tile.adapter) : 1.0f;
+    float sum[kTiles][kSteps][8];
+    for (uint32_t p = 0; p < a.splits; ++p) {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      const uint32_t row = min(tile.low + t * 16 + i, tile.high - 1);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
-        float v[8];
-        widen(v, load8(a.h + (uint64_t)row * rank + (n ? j : 0), n));
-        for (uint32_t p = 1; p < a.splits; ++p) {
-          float more[8];
-          widen(more, load8(a.h + ((uint64_t)p * a.by.rows + row) * rank + (n ? j : 0), n));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += more[e];
-        }
-        if (a.h_sum && blockIdx.y == 0 && wave == 0 && n && (!kBeside || k < 2) && tile.low + t * 16 + i < tile.high)
-          store8(a.h_sum + (uint64_t)row * rank + j, v, n);
-        if (kBeside) {
-          const typename P::Fragment low = P::part(v, 1);
-          h[0][s][t] = P::part(v, 0);
-          if (k >= 2) h[0][s][t] = low;
-        } else {
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) h[p][s][t] = P::part(v, p);
-        }
-      }
-    }
-  } else if (a.h_sum && blockIdx.y == 0) {
-    for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * rank; e += 256) a.h_sum[(uint64_t)tile.low * rank + e] = 0.0f;
-  }
-  const uint32_t first = (blockIdx.y * 4 + wave) * a.cols, last = min(a.features, first + a.cols);
-  for (uint32_t at = first; at < last; at += 32) {
-    const uint32_t col = at + k * 8, count = col >= a.features ? 0 : min(8u, a.features - col);
-    Eight<T> base[kTiles];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      const uint32_t row = min(tile.low + t * 16 + i, tile.high - 1);
-      const uint32_t n = a.base ? count : 0;
-      base[t] = load8((const T*)a.base + (n ? row * a.base_stride + col : 0), n);
-    }
-    f32x4 sum[2][kTiles];
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) sum[half][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (has) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t n = min(at + i / 4 * 8 + half * 4 + i % 4, a.features - 1);
-        const T* v = (const T*)a.v + ((uint64_t)tile.adapter * a.features + n) * rank;
+      for (int t = 0; t < kTiles; ++t) {
+        const uint32_t row = min(tile.low + t * 16 + i, tile.high - 1);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-          const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, m = j >= rank ? 0 : min(8u, rank - j);
-          const typename P::Fragment f = P::load(v + (m ? j : 0), m);
+          const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
+          float more[8];
+          widen(more, load8<kOdd>(a.h + ((uint64_t)p * a.by.rows + row) * rank + (n ? j : 0), n));
 #pragma unroll
-          for (int p = 0; p < kParts; ++p)
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) P::multiply(sum[half][t], f, h[p][s][t]);
+          for (int e = 0; e < 8; ++e) sum[t][s][e] = p ? sum[t][s][e] + more[e] : more[e];
         }
       }
     }
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       const uint32_t row = tile.low + t * 16 + i;
-      float v[8];
-      widen(v, base[t]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = has ? v[e] + scale * sum[e / 4][t][e % 4] : v[e];
-      if (row < tile.high && count) store8((T*)a.to + (uint64_t)row * a.features + col, v, count);
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
+        if (blockIdx.y == 0 && wave == 0 && n && (!kBeside || k < 2) && row < tile.high) {
+          if (a.h_sum) store8<kOdd>(a.h_sum + (uint64_t)row * rank + j, sum[t][s], n);
+          if (a.turned) {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e)
+              if (e < n) store_turned<T>(a.turned, rank, j + e, row, sum[t][s][e]);
+          }
+        }
+        if (kBeside) {
+          const typename P::Fragment low = P::part(sum[t][s], 1);
+          h[0][s][t] = P::part(sum[t][s], 0);
+          if (k >= 2) h[0][s][t] = low;
+        } else {
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) h[p][s][t] = P::part(sum[t][s], p);
+        }
+      }
+    }
+  } else if (blockIdx.y == 0 && a.h_sum) {
+    for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * rank; e += 256) a.h_sum[(uint64_t)tile.low * rank + e] = 0.0f;
+  }
+  const uint32_t stride = (uint32_t)a.base_stride, rows = tile.high - tile.low;
+  const Window<T, kOdd> base((const T*)a.base + tile.low * a.base_stride, a.base ? (rows - 1) * stride + a.features : 0);
+  const Window<T, kOdd> v((const T*)a.v + (uint64_t)(has ? tile.adapter : 0) * a.features * rank, a.features * rank);
+  const Window<T, kOdd> to((const T*)a.to + (uint64_t)tile.low * a.features, rows * a.features);
+  for (uint32_t at = first + wave * 128; at < end; at += 512) {
+    // a lane's rows (k, and every fourth after it) and columns where memory is read and written
+    const uint32_t count = at + i * 8 >= end ? 0 : min(8u, end - at - i * 8);
+    Eight<T> in[kTiles * 4];
+    Eight<T> vs[8][kSteps];
+#pragma unroll
+    for (uint32_t t = 0; t < kTiles * 4; ++t) {
+      if (kOdd && !a.base)
+        in[t] = Eight<T>{};
+      else
+        in[t] = base.read(t * 4 * stride + at, k * stride + i * 8, t * 4 + k < rows ? count : 0);
+    }
+    if (has) {
+#pragma unroll
+      for (uint32_t c = 0; c < 8; ++c)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
+          vs[c][s] = v.read((at + c * 16) * rank, i * rank + j, at + c * 16 + i < a.features ? n : 0);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      if (has) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) P::multiply(sum, P::of(vs[c][s]), h[p][s][t]);
+          *(f32x4*)&room[wave][i][c * 16 + k * 4] = sum;
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        float out[8];
+        widen(out, in[t * 4 + u]);
+        if (has) {
+          float more[8];
+          __builtin_memcpy(more, __builtin_assume_aligned(&room[wave][u * 4 + k][i * 8], 16), 32);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) out[e] += scale * more[e];
+        }
+        to.write(out, (t * 16 + u * 4) * a.features + at, k * a.features + i * 8, t * 16 + u * 4 + k < rows ? count : 0);
+      }
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
@@ -317,12 +418,12 @@ __device__ __forceinline__ void expand(const Expand& a) {
 
 // A workgroup has 128 columns, 64 ranks at most and an adapter's rows in one split; its waves take 32 rows in turn and
 // add up through LDS. A lane reads eight neighbouring columns of eight rows, and column q of all lanes makes the operand of
-// instruction q: the rows, which are reduced, lie beside each other in a lane without a way through LDS. Rows
-// past a request's end count as zeros on both sides (what lies there may be infinite).
-template <class T, int kRanks, bool kKept>
-__device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_t tile, float* room) {
+// instruction q: the rows, which are reduced, lie beside each other in a lane without a way through LDS. A step's rows
+// begin at a multiple of 32; those that are not the request's count as zeros on both sides (they may be infinite).
+template <class T, int kRanks, bool kOdd>
+__device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_t tile, f32x4* room) {
   typedef Path<T> P;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 16, k = lane / 16;
+  const uint32_t lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
   const uint32_t split = blockIdx.y, adapter = blockIdx.z % by.adapters, rank0 = blockIdx.z / by.adapters * (kRanks * 16);
   const uint32_t col = tile * kOuterCols + i * 8, count = col >= a.cols ? 0 : min(8u, a.cols - col);
   const uint32_t from = split * a.span, to = min(by.rows, from + a.span);
@@ -331,92 +432,120 @@ __device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_
   for (int r = 0; r < kRanks; ++r)
 #pragma unroll
     for (int q = 0; q < 8; ++q) sum[r][q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  bool any = false;
-  uint32_t turn = 0;
 
-  auto step = [&](uint32_t row0, uint32_t high, auto whole) {
-    Eight<T> wide[8];
-    float narrow[kRanks][8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t row = row0 + k * 8 + e;
-      const bool in = whole || row < high;
-      const uint32_t n = in ? count : 0;
-      if (kKept) {
-        uint2 q = {0, 0};
-        uint32_t exponent = 0;
-        if (n) {
-          q = *(const uint2*)((const int8_t*)a.wide + (uint64_t)row * a.groups * kGroup + col);
-          exponent = a.exponents[(uint64_t)row * a.groups + col / kGroup];
-        }
-        wide[e] = P::decoded(q, exponent);
-      } else {
-        wide[e] = load8((const T*)a.wide + (n ? row * a.stride + col : 0), n);
-      }
-#pragma unroll
-      for (int r = 0; r < kRanks; ++r) {
-        const uint32_t j = min(rank0 + r * 16 + i, by.rank - 1);
-        narrow[r][e] = in ? a.narrow[(uint64_t)row * by.rank + j] : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kRanks; ++r)
-#pragma unroll
-      for (int p = 0; p < P::kParts; ++p) {
-        const typename P::Fragment f = P::part(narrow[r], p);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) P::multiply(sum[r][q], f, P::column(wide, q));
-      }
-  };
-
-  // the adapter's requests, 64 looked at at once
-  for (uint32_t s0 = 0; s0 < by.requests; s0 += 64) {
+  // The wave's steps of 32 rows: the adapter's requests, 64 looked at at once, and in each every fourth step, from
+  // another wave on for the next request.
+  uint32_t s0 = 0, low = 0, high = 0, pieces = 0, row0 = 0, first = 0, last = 0;
+  uint64_t found = 0;
+  auto look = [&]() {
     const uint32_t s = s0 + lane;
-    uint32_t low = 0, high = 0;
+    low = high = 0;
     if (s < by.requests && adapter_of(by, s) == adapter) {
       low = max(begins(by, s), from);
       high = min(begins(by, s + 1), to);
     }
-    uint64_t found = __ballot(low < high);
-    any = any || found;
-    while (found) {
+    found = __ballot(low < high);
+    s0 += 64;
+  };
+  auto next = [&]() {
+    row0 += 128;
+    while (row0 >= last) {
+      while (!found && s0 < by.requests) look();
+      if (!found) break;
       const int at = __builtin_ctzll(found);
       found &= found - 1;
-      const uint32_t first = __builtin_amdgcn_readlane(low, at), last = __builtin_amdgcn_readlane(high, at);
-      for (uint32_t row0 = first; row0 < last; row0 += 32, ++turn) {
-        if (turn % 4 != wave) continue;
-        if (row0 + 32 <= last)
-          step(row0, last, std::true_type{});
-        else
-          step(row0, last, std::false_type{});
-      }
+      first = __builtin_amdgcn_readlane(low, at);
+      row0 = first / 32 * 32 + (wave - pieces) % 4 * 32;
+      last = __builtin_amdgcn_readlane(high, at);
+      ++pieces;
     }
+  };
+
+  next();
+  while (row0 < last) {
+    // of the step's rows, which are the request's
+    const uint32_t low_in = first > row0 ? first - row0 : 0, rows = min(32u, last - row0);
+    auto in_step = [&](uint32_t row) { return row >= low_in && row < rows; };
+    Eight<T> wide[8];
+    if (a.exponents) {
+      const uint32_t pitch = a.groups * kGroup, left = pitch - tile * kOuterCols;
+      const Window<int8_t, false> values((const int8_t*)a.wide + (uint64_t)row0 * pitch + tile * kOuterCols, (rows - 1) * pitch + left);
+      const Window<uint8_t, false> exponents(a.exponents + (uint64_t)row0 * a.groups + tile * (kOuterCols / kGroup),
+                                             (rows - 1) * a.groups + left / kGroup);
+      uint2 q[8];
+      uint32_t x[8];
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) {
+        const bool in = count && in_step(k * 8 + e);
+        typedef uint32_t Pair __attribute__((ext_vector_type(2)));
+        const Pair pair = __builtin_amdgcn_raw_buffer_load_b64(values.buffer, in ? k * 8 * pitch + i * 8 : kNowhere, e * pitch, 0);
+        q[e] = uint2{pair.x, pair.y};
+        x[e] = __builtin_amdgcn_raw_buffer_load_b8(exponents.buffer, in ? k * 8 * a.groups + i / 4 : kNowhere, e * a.groups, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wide[e] = P::decoded(q[e], x[e]);
+    } else {
+      const uint32_t stride = (uint32_t)a.stride;
+      const Window<T, kOdd> from((const T*)a.wide + row0 * a.stride + tile * kOuterCols, (rows - 1) * stride + a.cols - tile * kOuterCols);
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) wide[e] = from.read(e * stride, k * 8 * stride + i * 8, in_step(k * 8 + e) ? count : 0);
+    }
+    const uint32_t octet = P::kParts * by.rank * 8;
+    const Window<typename P::Narrow, false> narrow0((const typename P::Narrow*)a.narrow + (uint64_t)(row0 / 8) * octet, 4 * octet);
+    Eight<typename P::Narrow> narrow[kRanks][P::kParts];
+#pragma unroll
+    for (uint32_t r = 0; r < kRanks; ++r)
+#pragma unroll
+      for (uint32_t p = 0; p < P::kParts; ++p)
+        narrow[r][p] = narrow0.read((p * by.rank + rank0 + r * 16) * 8, k * octet + i * 8, rank0 + r * 16 + i < by.rank ? 8 : 0);
+    if (low_in || rows < 32) {
+#pragma unroll
+      for (uint32_t r = 0; r < kRanks; ++r)
+#pragma unroll
+        for (uint32_t p = 0; p < P::kParts; ++p)
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e)
+            narrow[r][p].v[e] = in_step(k * 8 + e) ? narrow[r][p].v[e] : (typename P::Narrow)0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const typename P::Fragment f = P::column(wide, q);
+#pragma unroll
+      for (int r = 0; r < kRanks; ++r)
+#pragma unroll
+        for (int p = 0; p < P::kParts; ++p) P::multiply(sum[r][q], Path<typename P::Narrow>::of(narrow[r][p]), f);
+    }
+    next();
   }
+  const bool any = pieces != 0;
   if (!any && a.splits > 1) return;  // nothing reads this plane
 
-  // waves 2 and 3 to 0 and 1, then 1 to 0
-  constexpr uint32_t kHeld = kRanks * 32;
+  // waves 2 and 3 to 0 and 1, then 1 to 0; whole vectors, since the loop above would hold the sums once more where they
+  // are taken apart
 #pragma unroll
   for (uint32_t apart = 2; apart; apart /= 2) {
-    float* spot = room + (wave % apart) * kHeld * 64 + lane;
+    f32x4* spot = room + (wave % apart) * kRanks * 8 * 64 + lane;
     __syncthreads();
     if (wave >= apart && wave < 2 * apart) {
 #pragma unroll
       for (int r = 0; r < kRanks; ++r)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) spot[(r * 32 + e) * 64] = sum[r][e / 4][e % 4];
+        for (int q = 0; q < 8; ++q) spot[(r * 8 + q) * 64] = sum[r][q];
     }
     __syncthreads();
     if (wave < apart) {
 #pragma unroll
       for (int r = 0; r < kRanks; ++r)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) sum[r][e / 4][e % 4] += spot[(r * 32 + e) * 64];
+        for (int q = 0; q < 8; ++q) {
+          sum[r][q] += spot[(r * 8 + q) * 64];
+          if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // not all of them in registers at once
+        }
     }
   }
   if (wave || !count) return;
-  const bool last = a.splits == 1;
-  const float scale = last && a.scaled ? scale_of(by, adapter) : 1.0f;
+  const bool alone = a.splits == 1;
+  const float scale = alone && a.scaled ? scale_of(by, adapter) : 1.0f;
   const uint64_t size = (uint64_t)a.cols * by.rank;
   float* plane = a.planes + ((uint64_t)split * by.adapters + adapter) * size;
   T* out = (T*)a.to + adapter * size;
@@ -425,6 +554,7 @@ __device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t j = rank0 + r * 16 + k * 4 + e;
+      __builtin_amdgcn_sched_barrier(0);
       if (j >= by.rank) continue;
       float v[8];
 #pragma unroll
@@ -434,32 +564,29 @@ __device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_
         for (uint32_t q = 0; q < 8; ++q) {
           if (q >= count) continue;
           const uint64_t at = (uint64_t)(col + q) * by.rank + j;
-          if (last)
+          if (alone)
             out[at] = (T)v[q];
           else
             plane[at] = v[q];
         }
       } else {
         const uint64_t at = (uint64_t)j * a.cols + col;
-        if (last)
-          store8(out + at, v, count);
+        if (alone)
+          store8<kOdd>(out + at, v, count);
         else
-          store8(plane + at, v, count);
+          store8<kOdd>(plane + at, v, count);
       }
     }
 }
 
-template <class T, int kRanks>
+template <class T, int kRanks, bool kOdd>
 __device__ __forceinline__ void outer_sides(const Outer& a) {
-  __shared__ float room[2 * kRanks * 32 * 64];
+  __shared__ f32x4 room[2 * kRanks * 8 * 64];
   const bool second = blockIdx.x >= a.side[0].tiles;
   const Side& side = a.side[second];
   if (blockIdx.y >= side.splits) return;
   const uint32_t tile = blockIdx.x - (second ? a.side[0].tiles : 0);
-  if (side.exponents)
-    outer<T, kRanks, true>(a.by, side, tile, room);
-  else
-    outer<T, kRanks, false>(a.by, side, tile, room);
+  outer<T, kRanks, kOdd>(a.by, side, tile, room);
 }
 
 // The planes of a gradient's splits that have rows of the adapter, added up in order.
@@ -501,58 +628,82 @@ __device__ __forceinline__ void join(const Outer& a) {
   for (uint32_t e = 0; e < n; ++e) to[e] = (T)(sum[e] * scale);
 }
 
-// The splits of a shrink added up in order, where no expand does it on the way.
-extern "C" __global__ __launch_bounds__(256) void mo_adapters_sum(const float* planes, float* to, uint64_t count, uint32_t splits) {
-  const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= count) return;
-  float sum = planes[at];
-  for (uint32_t p = 1; p < splits; ++p) sum += planes[p * count + at];
-  to[at] = sum;
-}
-
-// A weight turned, 32 x 32 through LDS.
+// A weight turned, 32 x 32 through LDS; behind the weights' tiles a narrow matrix, the sum of its splits.
 template <class T>
 __device__ __forceinline__ void turn(const Turn& a) {
-  __shared__ T room[32][33];
-  const bool second = blockIdx.x >= a.tiles[0];
-  const uint32_t tile = blockIdx.x - (second ? a.tiles[0] : 0), rows = a.rows[second], cols = a.cols[second];
-  const uint32_t across = (cols + 31) / 32, row0 = tile / across * 32, col0 = tile % across * 32;
   const uint32_t x = threadIdx.x % 32, y = threadIdx.x / 32;
-  const uint64_t size = (uint64_t)rows * cols * blockIdx.y;
-  const T* from = (const T*)a.from[second] + size;
-  T* to = (T*)a.to[second] + size;
-  for (uint32_t r = y; r < 32; r += 8)
-    if (row0 + r < rows && col0 + x < cols) room[r][x] = from[(uint64_t)(row0 + r) * cols + col0 + x];
+  uint32_t tile = blockIdx.x;
+  if (tile < a.tiles[0] + a.tiles[1]) {
+    __shared__ T room[32][33];
+    const bool second = tile >= a.tiles[0];
+    tile -= second ? a.tiles[0] : 0;
+    const uint32_t rows = a.rows[second], cols = a.cols[second];
+    const uint32_t across = (cols + 31) / 32, row0 = tile / across * 32, col0 = tile % across * 32;
+    for (uint32_t adapter = blockIdx.y; adapter < a.adapters; adapter += gridDim.y) {
+      const uint64_t size = (uint64_t)rows * cols * adapter;
+      const T* from = (const T*)a.from[second] + size;
+      T* to = (T*)a.to[second] + size;
+      __syncthreads();
+      for (uint32_t r = y; r < 32; r += 8)
+        if (row0 + r < rows && col0 + x < cols) room[r][x] = from[(uint64_t)(row0 + r) * cols + col0 + x];
+      __syncthreads();
+      for (uint32_t r = y; r < 32; r += 8)
+        if (col0 + r < cols && row0 + x < rows) to[(uint64_t)(col0 + r) * rows + row0 + x] = room[x][r];
+    }
+    return;
+  }
+  if (blockIdx.y) return;
+  __shared__ float room[32][33];
+  tile -= a.tiles[0] + a.tiles[1];
+  const uint32_t across = (a.rank + 31) / 32, row0 = tile / across * 32, col0 = tile % across * 32;
+  for (uint32_t r = y; r < 32; r += 8) {
+    if (row0 + r >= a.count || col0 + x >= a.rank) continue;
+    const uint64_t at = (uint64_t)(row0 + r) * a.rank + col0 + x;
+    float sum = a.narrow[at];
+    for (uint32_t p = 1; p < a.splits; ++p) sum += a.narrow[(uint64_t)p * a.count * a.rank + at];
+    room[r][x] = sum;
+  }
   __syncthreads();
   for (uint32_t r = y; r < 32; r += 8)
-    if (col0 + r < cols && row0 + x < rows) to[(uint64_t)(col0 + r) * rows + row0 + x] = room[x][r];
+    if (col0 + r < a.rank && row0 + x < a.count) store_turned<T>(a.turned, a.rank, col0 + r, row0 + x, room[x][r]);
 }
 
-#define MO_SHRINK(T, t, ranks, tiles)                                                                              \
-  extern "C" __global__ __launch_bounds__(256) void mo_adapters_shrink_##t##_##ranks##_##tiles(Shrink a) {         \
-    shrink<T, ranks, tiles>(a);                                                                                    \
+// Names: type, ranks, tiles of 16 rows; "odd": features or a rank that are no multiples of eight.
+#define MO_SHRINK(T, t, ranks, tiles, odd, name)                                                                   \
+  extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks##_##name(Shrink a) {          \
+    shrink<T, ranks, tiles, odd>(a);                                                                               \
   }
-#define MO_EXPAND(T, t, rank, tiles)                                                                               \
-  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_##tiles(Expand a) {          \
-    expand<T, rank, tiles>(a);                                                                                     \
+#define MO_EXPAND(T, t, rank, tiles, odd, name)                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_##name(Expand a) {           \
+    expand<T, rank, tiles, odd>(a);                                                                                \
   }
 #define MO_OUTER(T, t, ranks)                                                                                      \
-  extern "C" __global__ __launch_bounds__(256) void mo_adapters_outer_##t##_##ranks(Outer a) { outer_sides<T, ranks>(a); }
+  extern "C" __global__ __launch_bounds__(256, 2) void mo_adapters_outer_##t##_##ranks(Outer a) {                     \
+    outer_sides<T, ranks, false>(a);                                                                               \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(256, 2) void mo_adapters_outer_##t##_##ranks##_odd(Outer a) {               \
+    outer_sides<T, ranks, true>(a);                                                                                \
+  }
 #define MO_ADAPTERS(T, t)                                                                                          \
-  MO_SHRINK(T, t, 1, 1)                                                                                            \
-  MO_SHRINK(T, t, 1, 2)                                                                                            \
-  MO_SHRINK(T, t, 2, 1)                                                                                            \
-  MO_SHRINK(T, t, 2, 2)                                                                                            \
-  MO_SHRINK(T, t, 4, 1)                                                                                            \
-  MO_SHRINK(T, t, 4, 2)                                                                                            \
-  MO_SHRINK(T, t, 8, 1)                                                                                            \
-  MO_EXPAND(T, t, 16, 1)                                                                                           \
-  MO_EXPAND(T, t, 16, 4)                                                                                           \
-  MO_EXPAND(T, t, 32, 1)                                                                                           \
-  MO_EXPAND(T, t, 32, 4)                                                                                           \
-  MO_EXPAND(T, t, 64, 1)                                                                                           \
-  MO_EXPAND(T, t, 64, 4)                                                                                           \
-  MO_EXPAND(T, t, 128, 1)                                                                                          \
+  MO_SHRINK(T, t, 1, 1, false, 1)                                                                                  \
+  MO_SHRINK(T, t, 2, 1, false, 1)                                                                                  \
+  MO_SHRINK(T, t, 4, 1, false, 1)                                                                                  \
+  MO_SHRINK(T, t, 8, 1, false, 1)                                                                                  \
+  MO_SHRINK(T, t, 1, 1, true, odd)                                                                                 \
+  MO_SHRINK(T, t, 2, 1, true, odd)                                                                                 \
+  MO_SHRINK(T, t, 4, 1, true, odd)                                                                                 \
+  MO_SHRINK(T, t, 8, 1, true, odd)                                                                                 \
+  MO_EXPAND(T, t, 16, 1, false, 1)                                                                                 \
+  MO_EXPAND(T, t, 16, 2, false, 2)                                                                                 \
+  MO_EXPAND(T, t, 16, 1, true, odd)                                                                                \
+  MO_EXPAND(T, t, 32, 1, false, 1)                                                                                 \
+  MO_EXPAND(T, t, 32, 2, false, 2)                                                                                 \
+  MO_EXPAND(T, t, 32, 1, true, odd)                                                                                \
+  MO_EXPAND(T, t, 64, 1, false, 1)                                                                                 \
+  MO_EXPAND(T, t, 64, 2, false, 2)                                                                                 \
+  MO_EXPAND(T, t, 64, 1, true, odd)                                                                                \
+  MO_EXPAND(T, t, 128, 1, false, 1)                                                                                \
+  MO_EXPAND(T, t, 128, 1, true, odd)                                                                               \
   MO_OUTER(T, t, 1)                                                                                                \
   MO_OUTER(T, t, 2)                                                                                                \
   MO_OUTER(T, t, 4)                                                                                                \
@@ -561,5 +712,8 @@ __device__ __forceinline__ void turn(const Turn& a) {
 MO_ADAPTERS(_Float16, f16)
 MO_ADAPTERS(__bf16, bf16)
 MO_ADAPTERS(float, f32)
+MO_SHRINK(__bf16, bf16, 1, 2, false, 2)
+MO_SHRINK(__bf16, bf16, 2, 2, false, 2)
+MO_SHRINK(__bf16, bf16, 4, 2, false, 2)
 
 }  // namespace

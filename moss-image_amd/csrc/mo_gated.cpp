@@ -56,7 +56,7 @@ int gated(const mo_gated_call* c, bool backward, uint64_t stream) {
   a.rows = (uint32_t)c->rows, a.cols = c->cols, a.silu = c->silu;
   if (!shares(c->rows, c->cols, &a.lanes, &a.by_lanes)) return bad("too many values");
   const std::string name = std::string("mo_gated_") + (backward ? "backward_" : "forward_") + (kept ? "kept_" : keep ? "keep_" : "") +
-                           kTypeNames[c->dtype];
+                           kTypeNames[c->dtype] + (c->cols % 8 ? "_odd" : "");
   hipFunction_t kernel;
   if (int rc = kernels().get(name, &kernel)) return rc;
   void* params[] = {&a};
@@ -76,7 +76,7 @@ int keep(uint64_t x, uint64_t values, uint64_t exponents, uint32_t dtype, uint64
   a.stride = stride, a.rows = (uint32_t)rows, a.cols = cols, a.groups = (cols + 31) / 32;
   if (!shares(rows, cols, &a.lanes, &a.by_lanes)) return bad("too many values");
   hipFunction_t kernel;
-  if (int rc = kernels().get(std::string(restore ? "mo_keep_restore_" : "mo_keep_pack_") + kTypeNames[dtype], &kernel)) return rc;
+  if (int rc = kernels().get(std::string(restore ? "mo_keep_restore_" : "mo_keep_pack_") + kTypeNames[dtype] + (cols % 8 ? "_odd" : ""), &kernel)) return rc;
   void* params[] = {&a};
   const uint64_t items = rows * a.lanes;
   return mo::launch(kernel, (uint32_t)((items + 255) / 256), 1, 1, 256, stream, params, "8-bit activations launch");

@@ -40,9 +40,9 @@ struct Spot {
   }
 };
 
-template <class T>
+template <bool kOdd, class T>
 __device__ __forceinline__ void load_row(float (&to)[8], const void* base, uint64_t stride, const Spot& s) {
-  widen(to, load8((const T*)base + (s.n ? s.row * stride + s.at : 0), s.n));
+  widen(to, load8<kOdd>((const T*)base + (s.n ? s.row * stride + s.at : 0), s.n));
 }
 template <class T>
 __device__ __forceinline__ void write_kept(const float (&v)[8], int8_t* values, uint8_t* exponents, uint64_t stride,
@@ -64,12 +64,12 @@ __device__ __forceinline__ void read_kept(float (&to)[8], const void* values, co
   decode(to, q, exponent);
 }
 
-template <class T, bool kKeep>
+template <class T, bool kKeep, bool kOdd>
 __device__ __forceinline__ void forward(const GatedArgs& a) {
   const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
   float u[8], g[8];
-  load_row<T>(u, a.up, a.up_stride, s);
-  load_row<T>(g, a.gate, a.gate_stride, s);
+  load_row<kOdd, T>(u, a.up, a.up_stride, s);
+  load_row<kOdd, T>(g, a.gate, a.gate_stride, s);
   if (kKeep) {
     write_kept<T>(u, a.kept_up, a.kept_up_exponents, a.values_stride, a.exponents_stride, s);
     write_kept<T>(g, a.kept_gate, a.kept_gate_exponents, a.values_stride, a.exponents_stride, s);
@@ -79,10 +79,10 @@ __device__ __forceinline__ void forward(const GatedArgs& a) {
     const float gate = sigmoid_of(g[i]);
     u[i] = a.silu ? u[i] * (g[i] * gate) : 4.0f * tanh_of(g[i] * 0.25f) * gate * (25.0f * tanh_of(u[i] * 0.04f));
   }
-  if (s.n) store8((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
+  store8<kOdd>((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
 }
 
-template <class T, bool kKept>
+template <class T, bool kKept, bool kOdd>
 __device__ __forceinline__ void backward(const GatedArgs& a) {
   const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
   float u[8], g[8], d[8];
@@ -90,10 +90,10 @@ __device__ __forceinline__ void backward(const GatedArgs& a) {
     read_kept(u, a.up, a.up_exponents, a.values_stride, a.exponents_stride, s);
     read_kept(g, a.gate, a.gate_exponents, a.values_stride, a.exponents_stride, s);
   } else {
-    load_row<T>(u, a.up, a.up_stride, s);
-    load_row<T>(g, a.gate, a.gate_stride, s);
+    load_row<kOdd, T>(u, a.up, a.up_stride, s);
+    load_row<kOdd, T>(g, a.gate, a.gate_stride, s);
   }
-  load_row<T>(d, a.grad, a.grad_stride, s);
+  load_row<kOdd, T>(d, a.grad, a.grad_stride, s);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float gate = sigmoid_of(g[i]);
@@ -107,35 +107,38 @@ __device__ __forceinline__ void backward(const GatedArgs& a) {
     u[i] = d[i] * act * cap_slope;
     g[i] = d[i] * cap * slope;
   }
-  if (!s.n) return;
-  store8((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
-  store8((T*)a.out_gate + s.row * a.out_stride + s.at, g, s.n);
+  store8<kOdd>((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
+  store8<kOdd>((T*)a.out_gate + s.row * a.out_stride + s.at, g, s.n);
 }
 
-template <class T>
+template <class T, bool kOdd>
 __device__ __forceinline__ void pack(const KeepArgs& a) {
   const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
   float v[8];
-  load_row<T>(v, a.x, a.stride, s);
+  load_row<kOdd, T>(v, a.x, a.stride, s);
   write_kept<T>(v, a.values, a.exponents, (uint64_t)a.groups * kGroup, a.groups, s);
 }
-template <class T>
+template <class T, bool kOdd>
 __device__ __forceinline__ void restore(const KeepArgs& a) {
   const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
   float v[8];
   read_kept(v, a.values, a.exponents, (uint64_t)a.groups * kGroup, a.groups, s);
-  if (s.n) store8((T*)a.out + s.row * a.stride + s.at, v, s.n);
+  store8<kOdd>((T*)a.out + s.row * a.stride + s.at, v, s.n);
 }
 
-#define MO_GATED(T, t)                                                                                               \
-  extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_##t(GatedArgs a) { forward<T, false>(a); }      \
-  extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_keep_##t(GatedArgs a) { forward<T, true>(a); }  \
-  extern "C" __global__ __launch_bounds__(256) void mo_gated_backward_##t(GatedArgs a) { backward<T, false>(a); }    \
-  extern "C" __global__ __launch_bounds__(256) void mo_gated_backward_kept_##t(GatedArgs a) { backward<T, true>(a); } \
-  extern "C" __global__ __launch_bounds__(256) void mo_keep_pack_##t(KeepArgs a) { pack<T>(a); }                     \
-  extern "C" __global__ __launch_bounds__(256) void mo_keep_restore_##t(KeepArgs a) { restore<T>(a); }
-MO_GATED(_Float16, f16)
-MO_GATED(__bf16, bf16)
-MO_GATED(float, f32)
+// "odd": columns that are no multiple of eight.
+#define MO_GATED(T, t, odd)                                                                                   \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_##t(GatedArgs a) { forward<T, false, odd>(a); }      \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_keep_##t(GatedArgs a) { forward<T, true, odd>(a); }  \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_backward_##t(GatedArgs a) { backward<T, false, odd>(a); }    \
+  extern "C" __global__ __launch_bounds__(256) void mo_gated_backward_kept_##t(GatedArgs a) { backward<T, true, odd>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void mo_keep_pack_##t(KeepArgs a) { pack<T, odd>(a); }                     \
+  extern "C" __global__ __launch_bounds__(256) void mo_keep_restore_##t(KeepArgs a) { restore<T, odd>(a); }
+MO_GATED(_Float16, f16, false)
+MO_GATED(__bf16, bf16, false)
+MO_GATED(float, f32, false)
+MO_GATED(_Float16, f16_odd, true)
+MO_GATED(__bf16, bf16_odd, true)
+MO_GATED(float, f32_odd, true)
 
 }  // namespace

@@ -17,35 +17,53 @@ namespace mo_keep {
 
 constexpr uint32_t kGroup = 32;  // values an exponent; a lane holds 8, so four neighbouring lanes a group
 
-// Eight neighbouring values from anywhere that a T may lie: gfx950 takes 16-byte accesses at any address, so
-// rows of odd lengths need no kernel of their own. `n` < 8: that many, the rest zero and not read.
+// Eight neighbouring values from anywhere that a T may lie: gfx950 takes 16-byte accesses at any address.
 template <class T>
 struct alignas(T) Eight {
   T v[8];
 };
 template <class T>
-__device__ __forceinline__ Eight<T> load8(const T* p, uint32_t n = 8) {
+__device__ __forceinline__ Eight<T> load8(const T* p) {
   Eight<T> r;
-  if (n >= 8) {
-    __builtin_memcpy(&r, p, sizeof(r));
-  } else {
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+// The first n of them, the rest zero. Where sizes are multiples of eight, n is 8 or 0, and eight values are read all the
+// same (p has to be readable). Odd sizes have kernels of their own: single values need an address each, and the
+// registers for those would be taken from the others too.
+template <bool kOdd, class T>
+__device__ __forceinline__ Eight<T> load8(const T* p, uint32_t n) {
+  if (!kOdd || n >= 8) {
+    Eight<T> r = load8(p);
+    if (!kOdd) {
+      uint32_t word[sizeof(r) / 4];
+      __builtin_memcpy(word, &r, sizeof(r));
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : (T)0;
+      for (int i = 0; i < (int)(sizeof(r) / 4); ++i) word[i] = n ? word[i] : 0;
+      __builtin_memcpy(&r, word, sizeof(r));
+    }
+    return r;
   }
+  Eight<T> r;
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : (T)0;
   return r;
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&from)[8], uint32_t n = 8) {
+__device__ __forceinline__ void store8(T* p, const float (&from)[8]) {
   Eight<T> r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r.v[i] = (T)from[i];
-  if (n >= 8) {
-    __builtin_memcpy(p, &r, sizeof(r));
-  } else {
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+// The first n of them: 8 or 0 where sizes are multiples of eight.
+template <bool kOdd, class T>
+__device__ __forceinline__ void store8(T* p, const float (&from)[8], uint32_t n) {
+  if (n >= 8) return store8(p, from);
+  if (!kOdd) return;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-      if (i < n) p[i] = r.v[i];
-  }
+  for (uint32_t i = 0; i < 8; ++i)
+    if (i < n) p[i] = (T)from[i];
 }
 template <class T>
 __device__ __forceinline__ void widen(float (&to)[8], const Eight<T>& from) {
@@ -54,13 +72,14 @@ __device__ __forceinline__ void widen(float (&to)[8], const Eight<T>& from) {
 }
 
 // The same of a type known at run time (MO_DTYPE_*).
+template <bool kOdd>
 __device__ __forceinline__ void load8_kind(float (&to)[8], const void* base, uint64_t at, uint32_t kind, uint32_t n) {
   if (kind == 2)
-    widen(to, load8((const float*)base + at, n));
+    widen(to, load8<kOdd>((const float*)base + at, n));
   else if (kind == 1)
-    widen(to, load8((const __bf16*)base + at, n));
+    widen(to, load8<kOdd>((const __bf16*)base + at, n));
   else
-    widen(to, load8((const _Float16*)base + at, n));
+    widen(to, load8<kOdd>((const _Float16*)base + at, n));
 }
 __device__ __forceinline__ void store_kind(void* base, uint64_t at, uint32_t kind, float v) {
   if (kind == 2)

@@ -114,7 +114,7 @@ int run(const mo_norm_call* c, bool backward, uint64_t workspace, uint64_t bytes
   }
   const std::string name = std::string("mo_norm_") + (backward ? "backward_" : "forward_") +
                            (backward ? (a.x_exponents ? "kept_" : "") : (a.kept ? "keep_" : "")) + kTypeNames[c->dtype] +
-                           "_" + std::to_string(p.iter);
+                           "_" + std::to_string(p.iter) + (c->dim % 8 ? "_odd" : "");
   hipFunction_t kernel;
   if (int rc = kernels().get(name, &kernel)) return rc;
   void* params[] = {&a};

@@ -102,7 +102,7 @@ struct Place {
   }
 };
 
-template <int kIter>
+template <bool kOdd, int kIter>
 __device__ __forceinline__ void vectors(float (&to)[kIter][8], const NormArgs& a, uint32_t lane, const void* from,
                                         uint64_t offset, uint32_t kind, float otherwise) {
 #pragma unroll
@@ -110,11 +110,11 @@ __device__ __forceinline__ void vectors(float (&to)[kIter][8], const NormArgs& a
     const Place p(a, lane, k);
 #pragma unroll
     for (int i = 0; i < 8; ++i) to[k][i] = otherwise;
-    if (from) load8_kind(to[k], from, offset + (p.n ? p.at : 0), kind, p.n);
+    if (from) load8_kind<kOdd>(to[k], from, offset + (p.n ? p.at : 0), kind, p.n);
   }
 }
 
-template <class T, int kIter, bool kKeep>
+template <class T, int kIter, bool kKeep, bool kOdd>
 __device__ __forceinline__ void forward(const NormArgs& a) {
   __shared__ float room[64];
   uint32_t turn = 0;
@@ -123,16 +123,16 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
   const uint32_t end = min(a.rows, first + a.chunk);
   const float inv_dim = 1.0f / (float)a.dim;
   float weight[kIter][8], bias[kIter][8], factor[kIter][8], shift[kIter][8];
-  vectors<kIter>(weight, a, lane, a.weight, 0, a.weight_kind, 1.0f);
-  vectors<kIter>(bias, a, lane, a.bias, 0, a.weight_kind, 0.0f);
+  vectors<kOdd, kIter>(weight, a, lane, a.weight, 0, a.weight_kind, 1.0f);
+  vectors<kOdd, kIter>(bias, a, lane, a.bias, 0, a.weight_kind, 0.0f);
   int64_t until = 0;
   uint32_t sample = kNone;
   for (uint32_t row = first; row < end; ++row) {
     if ((int64_t)row >= until) {
       sample = sample_of(a, row, until);
       if (sample != kNone) {
-        vectors<kIter>(factor, a, lane, a.scale, sample * a.scale_stride, a.scale_kind, 0.0f);
-        vectors<kIter>(shift, a, lane, a.shift, sample * a.shift_stride, a.scale_kind, 0.0f);
+        vectors<kOdd, kIter>(factor, a, lane, a.scale, sample * a.scale_stride, a.scale_kind, 0.0f);
+        vectors<kOdd, kIter>(shift, a, lane, a.shift, sample * a.shift_stride, a.scale_kind, 0.0f);
       }
     }
     float x[kIter][8];
@@ -140,7 +140,7 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
 #pragma unroll
     for (int k = 0; k < kIter; ++k) {
       const Place p(a, lane, k);
-      widen(x[k], load8((const T*)a.x + (uint64_t)row * a.x_stride + (p.n ? p.at : 0), p.n));
+      widen(x[k], load8<kOdd>((const T*)a.x + row * a.x_stride + (p.n ? p.at : 0), p.n));
       if (kKeep) {
         uint32_t exponent;
         const uint2 q = encode<T>(x[k], exponent);
@@ -181,12 +181,12 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
         x[k][i] = x[k][i] * r * weight[k][i] + bias[k][i];
         x[k][i] = sample == kNone ? 0.0f : x[k][i] + x[k][i] * factor[k][i] + shift[k][i];
       }
-      if (p.n) store8((T*)a.out + (uint64_t)row * a.dim + p.at, x[k], p.n);
+      store8<kOdd>((T*)a.out + (uint64_t)row * a.dim + p.at, x[k], p.n);
     }
   }
 }
 
-template <class T, int kIter, bool kKept>
+template <class T, int kIter, bool kKept, bool kOdd>
 __device__ __forceinline__ void backward(const NormArgs& a) {
   __shared__ float room[64];
   uint32_t turn = 0;
@@ -217,8 +217,8 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
       flush();
       sample = sample_of(a, row, until);
       float weight[kIter][8];
-      vectors<kIter>(weight, a, lane, a.weight, 0, a.weight_kind, 1.0f);
-      vectors<kIter>(gain, a, lane, sample == kNone ? nullptr : a.scale, sample * a.scale_stride, a.scale_kind, 0.0f);
+      vectors<kOdd, kIter>(weight, a, lane, a.weight, 0, a.weight_kind, 1.0f);
+      vectors<kOdd, kIter>(gain, a, lane, sample == kNone ? nullptr : a.scale, sample * a.scale_stride, a.scale_kind, 0.0f);
 #pragma unroll
       for (int k = 0; k < kIter; ++k)
 #pragma unroll
@@ -243,9 +243,9 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
         }
         decode(n[k], q, exponent);
       } else {
-        widen(n[k], load8((const T*)a.x + (uint64_t)row * a.x_stride + (p.n ? p.at : 0), p.n));
+        widen(n[k], load8<kOdd>((const T*)a.x + row * a.x_stride + (p.n ? p.at : 0), p.n));
       }
-      widen(g, load8((const T*)a.grad + (uint64_t)row * a.grad_stride + (p.n ? p.at : 0), p.n));
+      widen(g, load8<kOdd>((const T*)a.grad + row * a.grad_stride + (p.n ? p.at : 0), p.n));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         n[k][i] = (uint32_t)i < p.n ? (n[k][i] - mean) * r : 0.0f;
@@ -263,31 +263,34 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
       const Place p(a, lane, k);
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[k][i] = sample == kNone ? 0.0f : r * (h[k][i] - mean_plain - n[k][i] * mean_along);
-      if (p.n) store8((T*)a.out + (uint64_t)row * a.dim + p.at, h[k], p.n);
+      store8<kOdd>((T*)a.out + (uint64_t)row * a.dim + p.at, h[k], p.n);
     }
   }
   flush();
 }
 
-#define MO_NORM(T, t, k)                                                                                     \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_forward_##t##_##k(NormArgs a) {                 \
-    forward<T, k, false>(a);                                                                                 \
+// Names: type, times a lane holds 8 values; "odd": a dim that is no multiple of eight.
+#define MO_NORM(T, t, k, odd, name)                                                                          \
+  extern "C" __global__ __launch_bounds__(1024) void mo_norm_forward_##t##_##name(NormArgs a) {              \
+    forward<T, k, false, odd>(a);                                                                            \
   }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_forward_keep_##t##_##k(NormArgs a) {            \
-    forward<T, k, true>(a);                                                                                  \
+  extern "C" __global__ __launch_bounds__(1024) void mo_norm_forward_keep_##t##_##name(NormArgs a) {         \
+    forward<T, k, true, odd>(a);                                                                             \
   }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_backward_##t##_##k(NormArgs a) {                \
-    backward<T, k, false>(a);                                                                                \
+  extern "C" __global__ __launch_bounds__(1024) void mo_norm_backward_##t##_##name(NormArgs a) {             \
+    backward<T, k, false, odd>(a);                                                                           \
   }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_backward_kept_##t##_##k(NormArgs a) {           \
-    backward<T, k, true>(a);                                                                                 \
+  extern "C" __global__ __launch_bounds__(1024) void mo_norm_backward_kept_##t##_##name(NormArgs a) {        \
+    backward<T, k, true, odd>(a);                                                                            \
   }
-MO_NORM(_Float16, f16, 1)
-MO_NORM(_Float16, f16, 2)
-MO_NORM(__bf16, bf16, 1)
-MO_NORM(__bf16, bf16, 2)
-MO_NORM(float, f32, 1)
-MO_NORM(float, f32, 2)
+#define MO_NORMS(T, t)           \
+  MO_NORM(T, t, 1, false, 1)     \
+  MO_NORM(T, t, 2, false, 2)     \
+  MO_NORM(T, t, 1, true, 1_odd)  \
+  MO_NORM(T, t, 2, true, 2_odd)
+MO_NORMS(_Float16, f16)
+MO_NORMS(__bf16, bf16)
+MO_NORMS(float, f32)
 
 __device__ __forceinline__ float value_kind(const void* base, uint64_t at, uint32_t kind) {
   return kind == 2 ? ((const float*)base)[at] : kind == 1 ? (float)((const __bf16*)base)[at]

@@ -19,11 +19,20 @@ import struct
 import torch
 
 from . import _native
-from ._operands import CODES, elsewhere, first_derivatives, pitch, plain, rows, stream, whole
+from ._operands import CODES, elsewhere, first_derivatives, pitch, plain, stream, whole
+from ._operands import rows as _dense_rows
 from .kept8 import Kept8, keep8
 
 MAX_RANK = 128
+MAX_STRIDE = 1 << 22
 _CALL = struct.Struct("=20Q6IfI")  # mo_adapters_call
+
+
+def rows(tensor: torch.Tensor, what: str) -> torch.Tensor:
+    """``_operands.rows``, near enough to each other for the kernels' 32-bit offsets."""
+
+    matrix = _dense_rows(tensor, what)
+    return matrix.contiguous() if matrix.shape[0] > 1 and matrix.stride(0) > MAX_STRIDE else matrix
 
 
 def _address(tensor: torch.Tensor | None) -> int:
