@@ -74,19 +74,24 @@ bool odd(const mo_adapters_call& c) {
   return off != 0;
 }
 
-// Rows a tile and splits of the features of a shrink: tiles of 16 rows where those are few or the requests short (the
-// other rows would be empty), and splits until there are four workgroups for every CU, 1024 features each at least.
+// Rows a tile and splits of the features of a shrink. Tiles of 16 rows where those are few or the requests short (the
+// other rows would be empty), or of 32; with more than 16 ranks and long requests tiles of 128, which share the weight.
+// Splits as long as all workgroups are on the GPU at once, 1024 features each at least: four of 16 rows a CU, or two of
+// 128 (past that, a few that come late cost as much as all others).
 struct ShrinkPlan {
-  uint32_t ranks, tiles, splits, span;
+  uint32_t ranks, rows, splits, span;
   uint64_t slots;
 };
 ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
   ShrinkPlan p = {};
   p.ranks = c.rank <= 16 ? 1 : c.rank <= 32 ? 2 : c.rank <= 64 ? 4 : 8;
-  p.tiles = !odd(c) && c.dtype == MO_DTYPE_BF16 && p.ranks < 8 && c.rows >= 32ull * c.requests && c.rows >= (p.ranks > 1 ? 4096 : 8192) ? 2 : 1;
-  const uint64_t tiles = div_up(c.rows, p.tiles * 16);
-  const uint64_t splits = between<uint64_t>(1, between<uint64_t>(1, div_up(1024, tiles), div_up(features, 1024)), 8);
-  p.span = (uint32_t)round_up(div_up(features, splits), 1024);
+  p.rows = 16;
+  const bool fits = c.dtype != MO_DTYPE_F32 || p.ranks < 8;  // in LDS, with two buffers of the weight
+  if (!odd(c) && p.ranks > 1 && fits && c.rows >= 128ull * c.requests && c.rows >= 1024) p.rows = 128;
+  if (!odd(c) && p.ranks == 1 && c.dtype == MO_DTYPE_BF16 && c.rows >= 32ull * c.requests && c.rows >= 8192) p.rows = 32;
+  const uint64_t tiles = div_up(c.rows, p.rows), most = p.rows == 128 ? 512 : 1024;
+  const uint64_t splits = between<uint64_t>(1, most / tiles, div_up(features, 1024));
+  p.span = (uint32_t)round_up(div_up(features, splits > 8 ? 8 : splits), 1024);
   p.splits = (uint32_t)div_up(features, p.span);
   p.slots = tiles + c.requests + 1;
   return p;
@@ -170,7 +175,7 @@ int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t s
   mo_adapters::Shrink a = {};
   a.by = by, a.x = (const void*)x, a.w = (const void*)w, a.to = (float*)to;
   a.x_stride = stride, a.features = features, a.span = p.span, a.scaled = scaled;
-  return start(std::string("shrink_") + kTypeNames[c.dtype] + "_" + std::to_string(p.ranks) + (odd(c) ? "_odd" : p.tiles == 2 ? "_2" : "_1"),
+  return start(std::string("shrink_") + kTypeNames[c.dtype] + "_" + std::to_string(p.ranks) + (odd(c) ? "_odd" : p.rows == 128 ? "_tall" : p.rows == 32 ? "_2" : "_1"),
                p.slots, p.splits, 1, &a, stream, 512);
 }
 

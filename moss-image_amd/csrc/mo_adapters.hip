@@ -279,6 +279,68 @@ __device__ __forceinline__ void shrink(const Shrink& a) {
   }
 }
 
+// The same for more than 16 ranks and long requests: a wave has 16 rows of its own and the weight, which is read for
+// each tile and would be more than the rows themselves, comes to LDS once for all eight waves, one step ahead.
+template <class T, int kRanks>
+__device__ __forceinline__ void shrink_tall(const Shrink& a) {
+  typedef Path<T> P;
+  constexpr uint32_t kRows = 128;
+  __shared__ Eight<T> stage[8][16][16], weight[2][kRanks * 16][16];
+  const Tile tile = tile_of<kRows>(a.by, blockIdx.x);
+  if (tile.low >= tile.high) return;
+  const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
+  f32x4 sum[kRanks];
+#pragma unroll
+  for (int r = 0; r < kRanks; ++r) sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint32_t low = tile.low + wave * 16, rows = low >= tile.high ? 0 : min(16u, tile.high - low);
+  if (tile.adapter != kNone) {
+    const uint32_t stride = (uint32_t)a.x_stride;
+    const Window<T, false> x((const T*)a.x + (rows ? low : tile.low) * a.x_stride, rows ? (rows - 1) * stride + a.features : 0);
+    const Window<T, false> w((const T*)a.w + (uint64_t)tile.adapter * rank * a.features, rank * a.features);
+    const uint32_t first = blockIdx.y * a.span, last = min(a.features, first + a.span);
+    Eight<T> xs[4], ws[(kRanks + 1) / 2];
+    // a thread's eight columns of four rows, and of every 32nd rank
+    const uint32_t wide = threadIdx.x % 16, tall = threadIdx.x / 16;
+    auto load = [&](uint32_t at) {
+#pragma unroll
+      for (uint32_t t = 0; t < 4; ++t)
+        xs[t] = x.read(t * 4 * stride + at, k * stride + i * 8, t * 4 + k < rows && at + i * 8 < last ? 8 : 0);
+#pragma unroll
+      for (uint32_t t = 0; t < (kRanks + 1) / 2; ++t)
+        ws[t] = w.read(t * 32 * a.features + at, tall * a.features + wide * 8, t * 32 + tall < rank && at + wide * 8 < last ? 8 : 0);
+    };
+    load(first);
+    uint32_t turn = 0;
+    for (uint32_t at = first; at < last; at += 128, turn ^= 1) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) stage[wave][t * 4 + k][i ^ (t * 4 + k)] = xs[t];
+#pragma unroll
+      for (uint32_t t = 0; t < (kRanks + 1) / 2; ++t)
+        if (t * 32 + tall < kRanks * 16) weight[turn][t * 32 + tall][wide ^ tall % 16] = ws[t];
+      __syncthreads();  // the other buffer has been read by all when they come here again
+      if (at + 128 < last) load(at + 128);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const typename P::Fragment f = P::of(stage[wave][i][(u * 4 + k) ^ i]);
+#pragma unroll
+        for (int r = 0; r < kRanks; ++r) P::multiply(sum[r], P::of(weight[turn][r * 16 + i][(u * 4 + k) ^ i]), f);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  if (i >= rows) return;
+  const float scale = a.scaled && tile.adapter != kNone ? scale_of(a.by, tile.adapter) : 1.0f;
+  float* to = a.to + ((uint64_t)blockIdx.y * a.by.rows + low + i) * rank;
+#pragma unroll
+  for (int r = 0; r < kRanks; ++r) {
+    const uint32_t j = r * 16 + k * 4;
+    if (j < rank) {  // a multiple of eight ranks
+      const f32x4 v = sum[r] * scale;
+      __builtin_memcpy(to + j, &v, 16);
+    }
+  }
+}
+
 // ---- expand ------------------------------------------------------------------------------------------
 
 // A value of a narrow matrix turned, for the instructions of an outer: [rows / 8][parts][rank][8 rows], fp32 in one part
@@ -420,7 +482,7 @@ __device__ __forceinline__ void expand(const Expand& a) {
 // add up through LDS. A lane reads eight neighbouring columns of eight rows, and column q of all lanes makes the operand of
 // instruction q: the rows, which are reduced, lie beside each other in a lane without a way through LDS. A step's rows
 // begin at a multiple of 32; those that are not the request's count as zeros on both sides (they may be infinite).
-template <class T, int kRanks, bool kOdd>
+template <class T, int kRanks, bool kKept, bool kOdd>
 __device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_t tile, f32x4* room) {
   typedef Path<T> P;
   const uint32_t lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
@@ -467,7 +529,7 @@ __device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_
     const uint32_t low_in = first > row0 ? first - row0 : 0, rows = min(32u, last - row0);
     auto in_step = [&](uint32_t row) { return row >= low_in && row < rows; };
     Eight<T> wide[8];
-    if (a.exponents) {
+    if (kKept) {
       const uint32_t pitch = a.groups * kGroup, left = pitch - tile * kOuterCols;
       const Window<int8_t, false> values((const int8_t*)a.wide + (uint64_t)row0 * pitch + tile * kOuterCols, (rows - 1) * pitch + left);
       const Window<uint8_t, false> exponents(a.exponents + (uint64_t)row0 * a.groups + tile * (kOuterCols / kGroup),
@@ -586,7 +648,10 @@ __device__ __forceinline__ void outer_sides(const Outer& a) {
   const Side& side = a.side[second];
   if (blockIdx.y >= side.splits) return;
   const uint32_t tile = blockIdx.x - (second ? a.side[0].tiles : 0);
-  outer<T, kRanks, kOdd>(a.by, side, tile, room);
+  if (side.exponents)
+    outer<T, kRanks, true, kOdd>(a.by, side, tile, room);
+  else
+    outer<T, kRanks, false, kOdd>(a.by, side, tile, room);
 }
 
 // The planes of a gradient's splits that have rows of the adapter, added up in order.
@@ -673,6 +738,10 @@ __device__ __forceinline__ void turn(const Turn& a) {
   extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks##_##name(Shrink a) {          \
     shrink<T, ranks, tiles, odd>(a);                                                                               \
   }
+#define MO_TALL(T, t, ranks)                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks##_tall(Shrink a) {            \
+    shrink_tall<T, ranks>(a);                                                                                      \
+  }
 #define MO_EXPAND(T, t, rank, tiles, odd, name)                                                                    \
   extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_##name(Expand a) {           \
     expand<T, rank, tiles, odd>(a);                                                                                \
@@ -693,6 +762,8 @@ __device__ __forceinline__ void turn(const Turn& a) {
   MO_SHRINK(T, t, 2, 1, true, odd)                                                                                 \
   MO_SHRINK(T, t, 4, 1, true, odd)                                                                                 \
   MO_SHRINK(T, t, 8, 1, true, odd)                                                                                 \
+  MO_TALL(T, t, 2)                                                                                                 \
+  MO_TALL(T, t, 4)                                                                                                 \
   MO_EXPAND(T, t, 16, 1, false, 1)                                                                                 \
   MO_EXPAND(T, t, 16, 2, false, 2)                                                                                 \
   MO_EXPAND(T, t, 16, 1, true, odd)                                                                                \
@@ -713,7 +784,7 @@ MO_ADAPTERS(_Float16, f16)
 MO_ADAPTERS(__bf16, bf16)
 MO_ADAPTERS(float, f32)
 MO_SHRINK(__bf16, bf16, 1, 2, false, 2)
-MO_SHRINK(__bf16, bf16, 2, 2, false, 2)
-MO_SHRINK(__bf16, bf16, 4, 2, false, 2)
+MO_TALL(_Float16, f16, 8)
+MO_TALL(__bf16, bf16, 8)
 
 }  // namespace
