@@ -13,8 +13,8 @@ using mo_adapters::Requests;
 const char* const kTypeNames[3] = {"f16", "bf16", "f32"};  // by MO_DTYPE_*
 constexpr uint32_t kTypeBytes[3] = {2, 2, 4};
 
-// Workgroups that a launch aims at: four and three for each of 256 CUs.
-constexpr uint64_t kExpandGroups = 1024, kOuterGroups = 768;
+// Workgroups that a launch aims at: an expand has two or three on a CU at a time, and many rounds leave no CU waiting long.
+constexpr uint64_t kExpandGroups = 4096, kOuterGroups = 768;
 
 mo::Kernels& kernels() {
   static mo::Kernels k(mo_adapters_code);
@@ -74,10 +74,10 @@ bool odd(const mo_adapters_call& c) {
   return off != 0;
 }
 
-// Rows a tile and splits of the features of a shrink. Tiles of 16 rows where those are few or the requests short (the
-// other rows would be empty), or of 32; with more than 16 ranks and long requests tiles of 128, which share the weight.
-// Splits as long as all workgroups are on the GPU at once, 1024 features each at least: four of 16 rows a CU, or two of
-// 128 (past that, a few that come late cost as much as all others).
+// Rows a tile and splits of the features of a shrink. Tiles of 128 rows, which share the weight, where they and the splits
+// make two workgroups for every CU; otherwise, and for short requests, whose other rows would be empty, tiles of 16.
+// Splits as long as all workgroups are on the GPU at once (past that, a few that come late cost as much as all
+// others), 512 features each at least for tiles of 128, 1024 for those of 16, and up to 16.
 struct ShrinkPlan {
   uint32_t ranks, rows, splits, span;
   uint64_t slots;
@@ -85,13 +85,12 @@ struct ShrinkPlan {
 ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
   ShrinkPlan p = {};
   p.ranks = c.rank <= 16 ? 1 : c.rank <= 32 ? 2 : c.rank <= 64 ? 4 : 8;
-  p.rows = 16;
   const bool fits = c.dtype != MO_DTYPE_F32 || p.ranks < 8;  // in LDS, with two buffers of the weight
-  if (!odd(c) && p.ranks > 1 && fits && c.rows >= 128ull * c.requests && c.rows >= 1024) p.rows = 128;
-  if (!odd(c) && p.ranks == 1 && c.dtype == MO_DTYPE_BF16 && c.rows >= 32ull * c.requests && c.rows >= 8192) p.rows = 32;
-  const uint64_t tiles = div_up(c.rows, p.rows), most = p.rows == 128 ? 512 : 1024;
-  const uint64_t splits = between<uint64_t>(1, most / tiles, div_up(features, 1024));
-  p.span = (uint32_t)round_up(div_up(features, splits > 8 ? 8 : splits), 1024);
+  const uint64_t tall = div_up(c.rows, 128), most = div_up(features, 512);
+  p.rows = !odd(c) && fits && c.rows >= 128ull * c.requests && tall * (most < 16 ? most : 16) >= 256 ? 128 : 16;
+  const uint64_t tiles = div_up(c.rows, p.rows), least = p.rows == 128 ? 512 : 1024;
+  const uint64_t splits = between<uint64_t>(1, (p.rows == 128 ? 512 : 1024) / tiles, div_up(features, least));
+  p.span = (uint32_t)round_up(div_up(features, splits > 16 ? 16 : splits), least);
   p.splits = (uint32_t)div_up(features, p.span);
   p.slots = tiles + c.requests + 1;
   return p;
@@ -175,7 +174,7 @@ int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t s
   mo_adapters::Shrink a = {};
   a.by = by, a.x = (const void*)x, a.w = (const void*)w, a.to = (float*)to;
   a.x_stride = stride, a.features = features, a.span = p.span, a.scaled = scaled;
-  return start(std::string("shrink_") + kTypeNames[c.dtype] + "_" + std::to_string(p.ranks) + (odd(c) ? "_odd" : p.rows == 128 ? "_tall" : p.rows == 32 ? "_2" : "_1"),
+  return start(std::string("shrink_") + kTypeNames[c.dtype] + "_" + std::to_string(p.ranks) + (odd(c) ? "_odd" : p.rows == 128 ? "_tall" : "_1"),
                p.slots, p.splits, 1, &a, stream, 512);
 }
 

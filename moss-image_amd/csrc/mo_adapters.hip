@@ -55,19 +55,16 @@ struct Window {
       words[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer, offset + i * 16, shared * (uint32_t)sizeof(T), 0);
     return __builtin_bit_cast(Eight<T>, words);
   }
-  __device__ __forceinline__ void write(const float (&v)[8], uint32_t shared, uint32_t own, uint32_t n) const {
+  __device__ __forceinline__ void write(const Eight<T>& v, uint32_t shared, uint32_t own, uint32_t n) const {
     if (kOdd) {
       store8<true>(at + shared + (n ? own : 0), v, n);
       return;
     }
     typedef uint32_t Words __attribute__((ext_vector_type(4)));
-    Eight<T> e;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = (T)v[i];
     struct All {
       Words words[sizeof(Eight<T>) / 16];
     };
-    const All all = __builtin_bit_cast(All, e);
+    const All all = __builtin_bit_cast(All, v);
     const uint32_t offset = n ? own * (uint32_t)sizeof(T) : kNowhere;
 #pragma unroll
     for (uint32_t i = 0; i < sizeof(Eight<T>) / 16; ++i)
@@ -175,16 +172,17 @@ __device__ __forceinline__ uint32_t adapter_of(const Requests& by, uint32_t s) {
   return i < 0 || i >= (int64_t)by.adapters ? kNone : (uint32_t)i;
 }
 
-// Rows `low` to `high` - 1 of one request with its adapter; none where the slot is between two pairs.
+// Rows `low` to `high` - 1 of one piece; none where the slot is between two pairs. The pieces are the requests, and before
+// and behind them the rows that are in none.
 struct Tile {
-  uint32_t low, high, adapter;
+  uint32_t low, high, piece;
 };
 
-// The requests, and before and behind them the rows that are in none: requests + 2 pieces, the rows of slot's.
+// The rows of a slot. What the lanes look at is read at once, so that this waits for memory once.
 template <uint32_t kRows>
 __device__ __forceinline__ Tile tile_of(const Requests& by, uint32_t slot) {
   const uint32_t pieces = by.requests + 2;
-  auto border = [&](uint32_t s) { return s == 0 ? 0u : s == pieces ? by.rows : begins(by, s - 1); };
+  auto border = [&](uint32_t s) { return s == 0 ? 0u : s >= pieces ? by.rows : begins(by, s - 1); };
   uint32_t low = 0, high = pieces - 1;  // the last piece whose first slot is not past this one
   while (high - low >= 64) {
     const uint32_t middle = (low + high + 1) / 2;
@@ -193,16 +191,20 @@ __device__ __forceinline__ Tile tile_of(const Requests& by, uint32_t slot) {
     else
       high = middle - 1;
   }
-  const uint32_t mine = low + threadIdx.x % 64;
-  const bool reached = mine <= high && border(mine) / kRows + mine <= slot;
-  low += __popcll(__ballot(reached)) - 1;
-  low = __builtin_amdgcn_readfirstlane(low);
-  const uint32_t first = (slot - low) * kRows;
+  const uint32_t mine = min(low + threadIdx.x % 64, high), from = border(mine), to = border(mine + 1);
+  const bool reached = low + threadIdx.x % 64 <= high && from / kRows + mine <= slot;
+  const int at = __popcll(__ballot(reached)) - 1;
   Tile t;
-  t.low = __builtin_amdgcn_readfirstlane(max(border(low), first));
-  t.high = __builtin_amdgcn_readfirstlane(min(border(low + 1), first + kRows));
-  t.adapter = __builtin_amdgcn_readfirstlane(low == 0 || low == pieces - 1 ? kNone : adapter_of(by, low - 1));
+  t.piece = __builtin_amdgcn_readfirstlane(low) + at;
+  const uint32_t first = (slot - t.piece) * kRows;
+  t.low = max((uint32_t)__builtin_amdgcn_readlane(from, at), first);
+  t.high = min((uint32_t)__builtin_amdgcn_readlane(to, at), first + kRows);
   return t;
+}
+// Its adapter: another wait, so asked for after what does not need it.
+__device__ __forceinline__ uint32_t adapter_of(const Requests& by, const Tile& t) {
+  if (t.piece == 0 || t.piece == by.requests + 1) return kNone;
+  return __builtin_amdgcn_readfirstlane(adapter_of(by, t.piece - 1));
 }
 
 // ---- shrink ------------------------------------------------------------------------------------------
@@ -230,10 +232,11 @@ __device__ __forceinline__ void shrink(const Shrink& a) {
   for (int r = 0; r < kRanks; ++r)
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) sum[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (tile.adapter != kNone) {
+  const uint32_t adapter = adapter_of(a.by, tile);
+  if (adapter != kNone) {
     const uint32_t stride = (uint32_t)a.x_stride, rows = tile.high - tile.low;
     const Window<T, kOdd> x((const T*)a.x + tile.low * a.x_stride, (rows - 1) * stride + a.features);
-    const Window<T, kOdd> w((const T*)a.w + (uint64_t)tile.adapter * rank * a.features, rank * a.features);
+    const Window<T, kOdd> w((const T*)a.w + (uint64_t)adapter * rank * a.features, rank * a.features);
     const uint32_t first = blockIdx.y * a.span, last = min(a.features, first + a.span);
     for (uint32_t at = first + wave * 128; at < last; at += 1024) {
       Eight<T> xs[kTiles * 4];
@@ -268,7 +271,7 @@ __device__ __forceinline__ void shrink(const Shrink& a) {
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) *(f32x4*)&room.sums[wave][t * 16 + i][r * 16 + k * 4] = sum[r][t];
   __syncthreads();
-  const float scale = a.scaled && tile.adapter != kNone ? scale_of(a.by, tile.adapter) : 1.0f;
+  const float scale = a.scaled && adapter != kNone ? scale_of(a.by, adapter) : 1.0f;
   float* to = a.to + ((uint64_t)blockIdx.y * a.by.rows + tile.low) * rank;
   for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * (kRanks * 16); e += 512) {
     const uint32_t row = e / (kRanks * 16), j = e % (kRanks * 16);
@@ -293,10 +296,11 @@ __device__ __forceinline__ void shrink_tall(const Shrink& a) {
 #pragma unroll
   for (int r = 0; r < kRanks; ++r) sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const uint32_t low = tile.low + wave * 16, rows = low >= tile.high ? 0 : min(16u, tile.high - low);
-  if (tile.adapter != kNone) {
+  const uint32_t adapter = adapter_of(a.by, tile);
+  if (adapter != kNone) {
     const uint32_t stride = (uint32_t)a.x_stride;
     const Window<T, false> x((const T*)a.x + (rows ? low : tile.low) * a.x_stride, rows ? (rows - 1) * stride + a.features : 0);
-    const Window<T, false> w((const T*)a.w + (uint64_t)tile.adapter * rank * a.features, rank * a.features);
+    const Window<T, false> w((const T*)a.w + (uint64_t)adapter * rank * a.features, rank * a.features);
     const uint32_t first = blockIdx.y * a.span, last = min(a.features, first + a.span);
     Eight<T> xs[4], ws[(kRanks + 1) / 2];
     // a thread's eight columns of four rows, and of every 32nd rank
@@ -329,7 +333,7 @@ __device__ __forceinline__ void shrink_tall(const Shrink& a) {
     }
   }
   if (i >= rows) return;
-  const float scale = a.scaled && tile.adapter != kNone ? scale_of(a.by, tile.adapter) : 1.0f;
+  const float scale = a.scaled && adapter != kNone ? scale_of(a.by, adapter) : 1.0f;
   float* to = a.to + ((uint64_t)blockIdx.y * a.by.rows + low + i) * rank;
 #pragma unroll
   for (int r = 0; r < kRanks; ++r) {
@@ -369,82 +373,100 @@ __device__ __forceinline__ void expand(const Expand& a) {
   constexpr bool kBeside = kRank == 16 && P::kParts == 2;
   constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 1 : P::kParts;
   __shared__ float room[4][16][132];
+  float(*shared)[132] = room[0];  // [kRows][132], before the waves use their parts
   const Tile tile = tile_of<kRows>(a.by, blockIdx.x);
   if (tile.low >= tile.high) return;
   const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
-  const bool has = tile.adapter != kNone;
   const uint32_t first = blockIdx.y * a.cols, end = min(a.features, first + a.cols);
-  typename P::Fragment h[kParts][kSteps][kTiles];
-  float scale = 0.0f;
-  if (has) {
-    scale = a.scaled ? scale_of(a.by, tile.adapter) : 1.0f;
-    float sum[kTiles][kSteps][8];
-    for (uint32_t p = 0; p < a.splits; ++p) {
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const uint32_t row = min(tile.low + t * 16 + i, tile.high - 1);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
-          float more[8];
-          widen(more, load8<kOdd>(a.h + ((uint64_t)p * a.by.rows + row) * rank + (n ? j : 0), n));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum[t][s][e] = p ? sum[t][s][e] + more[e] : more[e];
-        }
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      const uint32_t row = tile.low + t * 16 + i;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
-        if (blockIdx.y == 0 && wave == 0 && n && (!kBeside || k < 2) && row < tile.high) {
-          if (a.h_sum) store8<kOdd>(a.h_sum + (uint64_t)row * rank + j, sum[t][s], n);
-          if (a.turned) {
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-              if (e < n) store_turned<T>(a.turned, rank, j + e, row, sum[t][s][e]);
-          }
-        }
-        if (kBeside) {
-          const typename P::Fragment low = P::part(sum[t][s], 1);
-          h[0][s][t] = P::part(sum[t][s], 0);
-          if (k >= 2) h[0][s][t] = low;
-        } else {
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) h[p][s][t] = P::part(sum[t][s], p);
-        }
-      }
-    }
-  } else if (blockIdx.y == 0 && a.h_sum) {
-    for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * rank; e += 256) a.h_sum[(uint64_t)tile.low * rank + e] = 0.0f;
-  }
   const uint32_t stride = (uint32_t)a.base_stride, rows = tile.high - tile.low;
+  // a lane's rows (k, and every fourth after it) and columns where memory is read and written
   const Window<T, kOdd> base((const T*)a.base + tile.low * a.base_stride, a.base ? (rows - 1) * stride + a.features : 0);
-  const Window<T, kOdd> v((const T*)a.v + (uint64_t)(has ? tile.adapter : 0) * a.features * rank, a.features * rank);
   const Window<T, kOdd> to((const T*)a.to + (uint64_t)tile.low * a.features, rows * a.features);
-  for (uint32_t at = first + wave * 128; at < end; at += 512) {
-    // a lane's rows (k, and every fourth after it) and columns where memory is read and written
-    const uint32_t count = at + i * 8 >= end ? 0 : min(8u, end - at - i * 8);
-    Eight<T> in[kTiles * 4];
-    Eight<T> vs[8][kSteps];
+  Eight<T> in[kTiles * 4];
+  auto count = [&](uint32_t at) { return at + i * 8 >= end ? 0 : min(8u, end - at - i * 8); };
+  auto read_base = [&](uint32_t at, int tile) {
 #pragma unroll
-    for (uint32_t t = 0; t < kTiles * 4; ++t) {
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t t = tile * 4 + u;
       if (kOdd && !a.base)
         in[t] = Eight<T>{};
       else
-        in[t] = base.read(t * 4 * stride + at, k * stride + i * 8, t * 4 + k < rows ? count : 0);
+        in[t] = base.read(t * 4 * stride + at, k * stride + i * 8, t * 4 + k < rows ? count(at) : 0);
     }
-    if (has) {
+  };
+  // the first step's loads are on their way while h's are waited for
+  uint32_t at = first + wave * 128;
 #pragma unroll
-      for (uint32_t c = 0; c < 8; ++c)
+  for (int t = 0; t < kTiles; ++t) read_base(at, t);
+  const uint32_t adapter = adapter_of(a.by, tile);
+  const bool has = adapter != kNone;
+  const Window<T, kOdd> v((const T*)a.v + (uint64_t)(has ? adapter : 0) * a.features * rank, a.features * rank);
+  Eight<T> vs[8][kSteps];
+  auto read_v = [&](uint32_t at) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
-          vs[c][s] = v.read((at + c * 16) * rank, i * rank + j, at + c * 16 + i < a.features ? n : 0);
+    for (uint32_t c = 0; c < 8; ++c)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8, n = j >= rank ? 0 : min(8u, rank - j);
+        vs[c][s] = v.read((at + c * 16) * rank, i * rank + j, at + c * 16 + i < a.features ? n : 0);
+      }
+  };
+  if (has) read_v(at);
+  typename P::Fragment h[kParts][kSteps][kTiles];
+  float scale = 0.0f;
+  if (has) {
+    scale = a.scaled ? scale_of(a.by, adapter) : 1.0f;
+    // h's splits added up, a part of the tile a thread, and from LDS to the lanes that need it
+    for (uint32_t row = threadIdx.x / 16; row < kRows; row += 16)
+      for (uint32_t j0 = threadIdx.x % 16 * 4; j0 < kRank; j0 += 64) {
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < rows) {
+          const float* from = a.h + (uint64_t)(tile.low + row) * rank + j0;
+#pragma unroll 4
+          for (uint32_t p = 0; p < a.splits; ++p, from += (uint64_t)a.by.rows * rank) {
+            f32x4 more = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (!kOdd && j0 < rank) __builtin_memcpy(&more, from, 16);
+            if (kOdd) {
+#pragma unroll
+              for (uint32_t e = 0; e < 4; ++e)
+                if (j0 + e < rank) more[e] = from[e];
+            }
+            sum = p ? sum + more : more;
+          }
+          if (blockIdx.y == 0) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+              if (j0 + e >= rank) continue;
+              if (a.h_sum) a.h_sum[(uint64_t)(tile.low + row) * rank + j0 + e] = sum[e];
+              if (a.turned) store_turned<T>(a.turned, rank, j0 + e, tile.low + row, sum[e]);
+            }
+          }
         }
-    }
+        *(f32x4*)&shared[row][j0] = sum;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = j < kRank ? shared[t * 16 + i][j + e] : 0.0f;
+        if (kBeside) {
+          const typename P::Fragment low = P::part(v, 1);
+          h[0][s][t] = P::part(v, 0);
+          if (k >= 2) h[0][s][t] = low;
+        } else {
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) h[p][s][t] = P::part(v, p);
+        }
+      }
+    __syncthreads();
+  } else if (blockIdx.y == 0 && a.h_sum) {
+    for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * rank; e += 256) a.h_sum[(uint64_t)tile.low * rank + e] = 0.0f;
+  }
+  while (at < end) {
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       if (has) {
@@ -459,6 +481,9 @@ __device__ __forceinline__ void expand(const Expand& a) {
         }
         __builtin_amdgcn_wave_barrier();
       }
+      // the next step's loads go out before this one's writes, which a wait for later loads would wait for too
+      if (t == kTiles - 1 && has && at + 512 < end) read_v(at + 512);
+      Eight<T> results[4];
 #pragma unroll
       for (uint32_t u = 0; u < 4; ++u) {
         float out[8];
@@ -469,10 +494,16 @@ __device__ __forceinline__ void expand(const Expand& a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) out[e] += scale * more[e];
         }
-        to.write(out, (t * 16 + u * 4) * a.features + at, k * a.features + i * 8, t * 16 + u * 4 + k < rows ? count : 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) results[u].v[e] = (T)out[e];
       }
+      if (at + 512 < end) read_base(at + 512, t);
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u)
+        to.write(results[u], (t * 16 + u * 4) * a.features + at, k * a.features + i * 8, t * 16 + u * 4 + k < rows ? count(at) : 0);
       __builtin_amdgcn_wave_barrier();
     }
+    at += 512;
   }
 }
 
@@ -762,6 +793,7 @@ __device__ __forceinline__ void turn(const Turn& a) {
   MO_SHRINK(T, t, 2, 1, true, odd)                                                                                 \
   MO_SHRINK(T, t, 4, 1, true, odd)                                                                                 \
   MO_SHRINK(T, t, 8, 1, true, odd)                                                                                 \
+  MO_TALL(T, t, 1)                                                                                                 \
   MO_TALL(T, t, 2)                                                                                                 \
   MO_TALL(T, t, 4)                                                                                                 \
   MO_EXPAND(T, t, 16, 1, false, 1)                                                                                 \
@@ -783,7 +815,6 @@ __device__ __forceinline__ void turn(const Turn& a) {
 MO_ADAPTERS(_Float16, f16)
 MO_ADAPTERS(__bf16, bf16)
 MO_ADAPTERS(float, f32)
-MO_SHRINK(__bf16, bf16, 1, 2, false, 2)
 MO_TALL(_Float16, f16, 8)
 MO_TALL(__bf16, bf16, 8)
 

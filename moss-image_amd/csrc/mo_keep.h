@@ -58,12 +58,22 @@ __device__ __forceinline__ void store8(T* p, const float (&from)[8]) {
 }
 // The first n of them: 8 or 0 where sizes are multiples of eight.
 template <bool kOdd, class T>
-__device__ __forceinline__ void store8(T* p, const float (&from)[8], uint32_t n) {
-  if (n >= 8) return store8(p, from);
+__device__ __forceinline__ void store8(T* p, const Eight<T>& from, uint32_t n) {
+  if (n >= 8) {
+    __builtin_memcpy(p, &from, sizeof(from));
+    return;
+  }
   if (!kOdd) return;
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i)
-    if (i < n) p[i] = (T)from[i];
+    if (i < n) p[i] = from.v[i];
+}
+template <bool kOdd, class T>
+__device__ __forceinline__ void store8(T* p, const float (&from)[8], uint32_t n) {
+  Eight<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = (T)from[i];
+  store8<kOdd>(p, r, n);
 }
 template <class T>
 __device__ __forceinline__ void widen(float (&to)[8], const Eight<T>& from) {
