@@ -81,6 +81,46 @@ __device__ __forceinline__ void widen(float (&to)[8], const Eight<T>& from) {
   for (int i = 0; i < 8; ++i) to[i] = (float)from.v[i];
 }
 
+// A part of memory that all lanes share: its address stays in scalar registers, a lane has 32-bit offsets (the host keeps
+// rows near enough for that), and what a lane should not read or write it asks for past the end, where reads
+// give zeros and writes are dropped. Odd sizes, or addresses off the 4-byte grid, go value by value.
+constexpr uint32_t kNowhere = 0x80000000u;  // no window is as long
+
+template <class T, bool kOdd>
+struct Window {
+  T* at;
+  __amdgpu_buffer_rsrc_t buffer;
+  // `count` elements from `p`
+  __device__ __forceinline__ Window(const T* p, uint32_t count)
+      : at(const_cast<T*>(p)),
+        buffer(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, (int)(count * sizeof(T)), 0x00020000)) {}
+  // the first n (8 or 0, unless kOdd) of eight elements, `shared` + `own` from the beginning; the rest are zero
+  __device__ __forceinline__ Eight<T> read(uint32_t shared, uint32_t own, uint32_t n) const {
+    if (kOdd) return load8<true>(at + shared + (n ? own : 0), n);
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    Words words[sizeof(Eight<T>) / 16];
+    const uint32_t offset = n ? own * (uint32_t)sizeof(T) : kNowhere;
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(Eight<T>) / 16; ++i)
+      words[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer, offset + i * 16, shared * (uint32_t)sizeof(T), 0);
+    return __builtin_bit_cast(Eight<T>, words);
+  }
+  __device__ __forceinline__ void write(const Eight<T>& v, uint32_t shared, uint32_t own, uint32_t n) const {
+    if (kOdd) {
+      store8<true>(at + shared + (n ? own : 0), v, n);
+      return;
+    }
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    struct All {
+      Words words[sizeof(Eight<T>) / 16];
+    };
+    const All all = __builtin_bit_cast(All, v);
+    const uint32_t offset = n ? own * (uint32_t)sizeof(T) : kNowhere;
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(Eight<T>) / 16; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(all.words[i], buffer, offset + i * 16, shared * (uint32_t)sizeof(T), 0);
+  }
+};
 // The same of a type known at run time (MO_DTYPE_*).
 template <bool kOdd>
 __device__ __forceinline__ void load8_kind(float (&to)[8], const void* base, uint64_t at, uint32_t kind, uint32_t n) {

@@ -26,6 +26,16 @@ struct Plan {
   uint64_t slots;  // backward: pairs of a group of rows and a sample that have a place for sums
 };
 
+// Whether eight neighbouring values can be read at once: dim is a multiple of eight and every row lies on the 4-byte
+// grid. Other calls have kernels that read value by value.
+bool odd(const mo_norm_call& c) {
+  const uint64_t size = kTypeBytes[c.dtype];
+  uint64_t off = c.dim % 8;
+  for (uint64_t p : {c.x_exponents ? 0 : c.x, c.grad, c.out}) off |= p % 4;
+  if (c.rows > 1) off |= (c.x_exponents ? 0 : c.x_stride * size % 4) | c.grad_stride * size % 4;
+  return off != 0;
+}
+
 Plan plan_of(const mo_norm_call& c, bool backward) {
   Plan p = {};
   const uint64_t held = div_up(c.dim, 8);
@@ -33,8 +43,9 @@ Plan plan_of(const mo_norm_call& c, bool backward) {
   p.lanes = (uint32_t)div_up(div_up(held, p.iter), 64) * 64;
   p.per = p.lanes == 64 ? 4 : 1;
   // forward: enough workgroups for several on every CU; backward: each leaves sums of dim values, so fewer
-  const uint64_t most = backward ? 1024 : 2048;
+  const uint64_t most = backward ? 512 : 1024;
   p.chunk = (uint32_t)div_up(c.rows, most * p.per);
+  if (p.chunk > 1) p.chunk += p.chunk % 2;  // whole batches of two rows
   p.groups = (uint32_t)div_up(c.rows, p.chunk);
   p.slots = (uint64_t)p.groups + (c.samples ? c.samples - 1 : 0);
   return p;
@@ -114,7 +125,7 @@ int run(const mo_norm_call* c, bool backward, uint64_t workspace, uint64_t bytes
   }
   const std::string name = std::string("mo_norm_") + (backward ? "backward_" : "forward_") +
                            (backward ? (a.x_exponents ? "kept_" : "") : (a.kept ? "keep_" : "")) + kTypeNames[c->dtype] +
-                           "_" + std::to_string(p.iter) + (c->dim % 8 ? "_odd" : "");
+                           "_" + std::to_string(p.iter) + (odd(*c) ? "_odd" : "");
   hipFunction_t kernel;
   if (int rc = kernels().get(name, &kernel)) return rc;
   void* params[] = {&a};

@@ -77,7 +77,7 @@ __device__ __forceinline__ void sum_row(float (&v)[N], uint32_t waves, float* ro
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = sum_wave(v[i]);
   if (waves == 1) return;
-  float* to = room + (turn & 1) * 32;
+  float* to = room + (turn & 1) * N * 16;
   ++turn;
   const uint32_t wave = threadIdx.x / 64;
   if (threadIdx.x % 64 == 0) {
@@ -114,92 +114,181 @@ __device__ __forceinline__ void vectors(float (&to)[kIter][8], const NormArgs& a
   }
 }
 
+// Rows one after the other that a batch takes: their sums cross the waves together, and a batch's rows are read while
+// the one before is worked on.
+template <int kIter>
+constexpr int kBatch = kIter == 1 ? 2 : 1;
+
+// A workgroup's (or, side by side, a wave's) rows, batch by batch; a batch ends where a sample does.
+struct Walk {
+  uint32_t row, end, sample, count;  // the batch: first row, the sample, rows
+  int64_t until;
+  __device__ __forceinline__ Walk(const NormArgs& a, uint32_t first, uint32_t most) : row(first), end(min(a.rows, first + a.chunk)) {
+    find(a, most);
+  }
+  __device__ __forceinline__ void find(const NormArgs& a, uint32_t most) {
+    if (row >= end) return;
+    sample = __builtin_amdgcn_readfirstlane(sample_of(a, row, until));
+    take(most);
+  }
+  __device__ __forceinline__ void take(uint32_t most) {
+    count = min(most, end - row);
+    if (until < (int64_t)row + count) count = (uint32_t)(until - row);
+  }
+  __device__ __forceinline__ void next(const NormArgs& a, uint32_t most) {
+    row += count;
+    if (row >= end) return;
+    if ((int64_t)row >= until)
+      find(a, most);
+    else
+      take(most);
+  }
+};
+
 template <class T, int kIter, bool kKeep, bool kOdd>
 __device__ __forceinline__ void forward(const NormArgs& a) {
-  __shared__ float room[64];
+  constexpr int kRows = kBatch<kIter>;
+  __shared__ float room[2 * kRows * 16];
   uint32_t turn = 0;
-  const uint32_t side = threadIdx.x / a.lanes, lane = threadIdx.x - side * a.lanes, waves = a.lanes / 64;
-  const uint32_t first = (blockIdx.x * a.per + side) * a.chunk;
-  const uint32_t end = min(a.rows, first + a.chunk);
+  const uint32_t side = a.per > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0;
+  const uint32_t lane = threadIdx.x - side * a.lanes, waves = a.lanes / 64;
   const float inv_dim = 1.0f / (float)a.dim;
+  Walk now(a, (blockIdx.x * a.per + side) * a.chunk, kRows);
+  if (now.row >= now.end) return;
+  Eight<T> raw[kRows][kIter];
+  auto read = [&](const Walk& w) {
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i) {
+      const uint32_t row = w.row + min(i, w.count - 1);
+      const Window<T, kOdd> x((const T*)a.x + row * a.x_stride, a.dim);
+#pragma unroll
+      for (int k = 0; k < kIter; ++k) {
+        const Place p(a, lane, k);
+        raw[i][k] = x.read(0, p.at, p.n);
+      }
+    }
+  };
+  read(now);
   float weight[kIter][8], bias[kIter][8], factor[kIter][8], shift[kIter][8];
   vectors<kOdd, kIter>(weight, a, lane, a.weight, 0, a.weight_kind, 1.0f);
   vectors<kOdd, kIter>(bias, a, lane, a.bias, 0, a.weight_kind, 0.0f);
-  int64_t until = 0;
-  uint32_t sample = kNone;
-  for (uint32_t row = first; row < end; ++row) {
-    if ((int64_t)row >= until) {
-      sample = sample_of(a, row, until);
-      if (sample != kNone) {
-        vectors<kOdd, kIter>(factor, a, lane, a.scale, sample * a.scale_stride, a.scale_kind, 0.0f);
-        vectors<kOdd, kIter>(shift, a, lane, a.shift, sample * a.shift_stride, a.scale_kind, 0.0f);
+  bool fresh = true;
+  while (true) {
+    if (fresh && now.sample != kNone) {
+      vectors<kOdd, kIter>(factor, a, lane, a.scale, now.sample * a.scale_stride, a.scale_kind, 0.0f);
+      vectors<kOdd, kIter>(shift, a, lane, a.shift, now.sample * a.shift_stride, a.scale_kind, 0.0f);
+    }
+    float x[kRows][kIter][8], sum[kRows], mean[kRows];
+    uint2 kept[kRows][kIter];
+    uint32_t exponent[kRows][kIter];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      sum[i] = mean[i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kIter; ++k) {
+        widen(x[i][k], raw[i][k]);
+        if (kKeep) kept[i][k] = encode<T>(x[i][k], exponent[i][k]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[i] += x[i][k][e];
       }
     }
-    float x[kIter][8];
-    float sum[1] = {0.0f};
-#pragma unroll
-    for (int k = 0; k < kIter; ++k) {
-      const Place p(a, lane, k);
-      widen(x[k], load8<kOdd>((const T*)a.x + row * a.x_stride + (p.n ? p.at : 0), p.n));
-      if (kKeep) {
-        uint32_t exponent;
-        const uint2 q = encode<T>(x[k], exponent);
-        if (p.at < a.groups * kGroup) {
-          *(uint2*)(a.kept + (uint64_t)row * a.groups * kGroup + p.at) = q;
-          if (lane % 4 == 0) a.kept_exponents[(uint64_t)row * a.groups + p.at / kGroup] = (uint8_t)exponent;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum[0] += x[k][i];
-    }
-    float mean = 0.0f;
+    // before this batch's writes: a wait for later loads would wait for those too
+    Walk then = now;
+    then.next(a, kRows);
+    if (then.row < then.end) read(then);
     if (a.layer) {
       sum_row(sum, waves, room, turn);
-      mean = sum[0] * inv_dim;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) mean[i] = sum[i] * inv_dim;
     }
-    sum[0] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kIter; ++k) {
-      const Place p(a, lane, k);
+    for (int i = 0; i < kRows; ++i) {
+      sum[i] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[k][i] = (uint32_t)i < p.n ? x[k][i] - mean : 0.0f;
-        sum[0] += x[k][i] * x[k][i];
+      for (int k = 0; k < kIter; ++k) {
+        const Place p(a, lane, k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[i][k][e] = (kOdd ? (uint32_t)e < p.n : p.n != 0) ? x[i][k][e] - mean[i] : 0.0f;
+          sum[i] += x[i][k][e] * x[i][k][e];
+        }
       }
     }
     sum_row(sum, waves, room, turn);
-    const float r = rsqrtf(sum[0] * inv_dim + a.eps);
-    if (a.stats && lane == 0) {
-      a.stats[2 * (uint64_t)row] = mean;
-      a.stats[2 * (uint64_t)row + 1] = r;
-    }
 #pragma unroll
-    for (int k = 0; k < kIter; ++k) {
-      const Place p(a, lane, k);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[k][i] = x[k][i] * r * weight[k][i] + bias[k][i];
-        x[k][i] = sample == kNone ? 0.0f : x[k][i] + x[k][i] * factor[k][i] + shift[k][i];
+    for (uint32_t i = 0; i < kRows; ++i) {
+      if (i >= now.count) continue;
+      const uint32_t row = now.row + i;
+      const float r = rsqrtf(sum[i] * inv_dim + a.eps);
+      if (a.stats && lane == 0) {
+        a.stats[2 * (uint64_t)row] = mean[i];
+        a.stats[2 * (uint64_t)row + 1] = r;
       }
-      store8<kOdd>((T*)a.out + (uint64_t)row * a.dim + p.at, x[k], p.n);
+      const Window<T, kOdd> out((const T*)a.out + (uint64_t)row * a.dim, a.dim);
+#pragma unroll
+      for (int k = 0; k < kIter; ++k) {
+        const Place p(a, lane, k);
+        Eight<T> result;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = x[i][k][e] * r * weight[k][e] + bias[k][e];
+          v = now.sample == kNone ? 0.0f : v + v * factor[k][e] + shift[k][e];
+          result.v[e] = (T)v;
+        }
+        out.write(result, 0, p.at, p.n);
+        if (kKeep && p.at < a.groups * kGroup) {
+          *(uint2*)(a.kept + (uint64_t)row * a.groups * kGroup + p.at) = kept[i][k];
+          if (lane % 4 == 0) a.kept_exponents[(uint64_t)row * a.groups + p.at / kGroup] = (uint8_t)exponent[i][k];
+        }
+      }
     }
+    if (then.row >= then.end) return;
+    fresh = then.sample != now.sample;
+    now = then;
   }
 }
 
 template <class T, int kIter, bool kKept, bool kOdd>
 __device__ __forceinline__ void backward(const NormArgs& a) {
-  __shared__ float room[64];
+  constexpr int kRows = kBatch<kIter>;
+  __shared__ float room[2 * 2 * kRows * 16];
   uint32_t turn = 0;
-  const uint32_t side = threadIdx.x / a.lanes, lane = threadIdx.x - side * a.lanes, waves = a.lanes / 64;
-  const uint32_t group = blockIdx.x * a.per + side, first = group * a.chunk;
-  const uint32_t end = min(a.rows, first + a.chunk);
+  const uint32_t side = a.per > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0;
+  const uint32_t lane = threadIdx.x - side * a.lanes, waves = a.lanes / 64, group = blockIdx.x * a.per + side;
   const float inv_dim = 1.0f / (float)a.dim;
+  Walk now(a, group * a.chunk, kRows);
+  if (now.row >= now.end) return;
+  Eight<T> raw_x[kKept ? 1 : kRows][kIter], raw_g[kRows][kIter];
+  uint2 values[kKept ? kRows : 1][kIter];
+  uint32_t exponents[kKept ? kRows : 1][kIter];
+  float2 stats[kRows];
+  auto read = [&](const Walk& w) {
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i) {
+      const uint32_t row = w.row + min(i, w.count - 1), pitch = a.groups * kGroup;
+      const Window<T, kOdd> x((const T*)a.x + row * a.x_stride, a.dim), g((const T*)a.grad + row * a.grad_stride, a.dim);
+      const Window<int8_t, false> q((const int8_t*)a.x + (uint64_t)row * pitch, pitch);
+      const Window<uint8_t, false> exponent(a.x_exponents + (uint64_t)row * a.groups, a.groups);
+      stats[i] = ((const float2*)a.stats)[row];
+#pragma unroll
+      for (int k = 0; k < kIter; ++k) {
+        const Place p(a, lane, k);
+        if (kKept) {
+          typedef uint32_t Pair __attribute__((ext_vector_type(2)));
+          const Pair pair = __builtin_amdgcn_raw_buffer_load_b64(q.buffer, p.n ? p.at : kNowhere, 0, 0);
+          values[i][k] = uint2{pair.x, pair.y};
+          exponents[i][k] = __builtin_amdgcn_raw_buffer_load_b8(exponent.buffer, p.n ? p.at / kGroup : kNowhere, 0, 0);
+        } else {
+          raw_x[i][k] = x.read(0, p.at, p.n);
+        }
+        raw_g[i][k] = g.read(0, p.at, p.n);
+      }
+    }
+  };
+  read(now);
   float gain[kIter][8];  // (1 + scale) w
   float along[kIter][8], plain[kIter][8];  // P and Q
-  int64_t until = 0;
-  uint32_t sample = kNone;
-
-  auto flush = [&]() {
+  auto flush = [&](uint32_t sample) {
     if (sample == kNone || !a.partial) return;
     float* to = a.partial + (uint64_t)(group + sample) * 2 * a.pitch;
 #pragma unroll
@@ -211,62 +300,73 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
       }
     }
   };
-
-  for (uint32_t row = first; row < end; ++row) {
-    if ((int64_t)row >= until) {
-      flush();
-      sample = sample_of(a, row, until);
+  bool fresh = true;
+  while (true) {
+    if (fresh) {
       float weight[kIter][8];
       vectors<kOdd, kIter>(weight, a, lane, a.weight, 0, a.weight_kind, 1.0f);
-      vectors<kOdd, kIter>(gain, a, lane, sample == kNone ? nullptr : a.scale, sample * a.scale_stride, a.scale_kind, 0.0f);
+      vectors<kOdd, kIter>(gain, a, lane, now.sample == kNone ? nullptr : a.scale, now.sample * a.scale_stride, a.scale_kind, 0.0f);
 #pragma unroll
       for (int k = 0; k < kIter; ++k)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          gain[k][i] = sample == kNone ? 0.0f : weight[k][i] + weight[k][i] * gain[k][i];
-          along[k][i] = plain[k][i] = 0.0f;
+        for (int e = 0; e < 8; ++e) {
+          gain[k][e] = now.sample == kNone ? 0.0f : weight[k][e] + weight[k][e] * gain[k][e];
+          along[k][e] = plain[k][e] = 0.0f;
         }
     }
-    const float mean = a.stats[2 * (uint64_t)row], r = a.stats[2 * (uint64_t)row + 1];
-    float n[kIter][8], h[kIter][8];
-    float sums[2] = {0.0f, 0.0f};
+    float n[kRows][kIter][8], h[kRows][kIter][8], r[kRows], sums[2 * kRows];
 #pragma unroll
-    for (int k = 0; k < kIter; ++k) {
-      const Place p(a, lane, k);
-      float g[8];
-      if (kKept) {
-        uint2 q = {0, 0};
-        uint32_t exponent = 0;
-        if (p.n) {
-          q = *(const uint2*)((const int8_t*)a.x + (uint64_t)row * a.groups * kGroup + p.at);
-          exponent = a.x_exponents[(uint64_t)row * a.groups + p.at / kGroup];
+    for (uint32_t i = 0; i < kRows; ++i) {
+      const bool live = i < now.count;
+      const float mean = stats[i].x;
+      r[i] = stats[i].y;
+      sums[2 * i] = sums[2 * i + 1] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kIter; ++k) {
+        const Place p(a, lane, k);
+        float g[8];
+        if (kKept)
+          decode(n[i][k], values[i][k], exponents[i][k]);
+        else
+          widen(n[i][k], raw_x[i][k]);
+        widen(g, raw_g[i][k]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          n[i][k][e] = (kOdd ? (uint32_t)e < p.n : p.n != 0) ? (n[i][k][e] - mean) * r[i] : 0.0f;
+          h[i][k][e] = g[e] * gain[k][e];
+          along[k][e] += live ? g[e] * n[i][k][e] : 0.0f;
+          plain[k][e] += live ? g[e] : 0.0f;
+          sums[2 * i] += h[i][k][e] * n[i][k][e];
+          sums[2 * i + 1] += h[i][k][e];
         }
-        decode(n[k], q, exponent);
-      } else {
-        widen(n[k], load8<kOdd>((const T*)a.x + row * a.x_stride + (p.n ? p.at : 0), p.n));
-      }
-      widen(g, load8<kOdd>((const T*)a.grad + row * a.grad_stride + (p.n ? p.at : 0), p.n));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        n[k][i] = (uint32_t)i < p.n ? (n[k][i] - mean) * r : 0.0f;
-        h[k][i] = g[i] * gain[k][i];
-        along[k][i] += g[i] * n[k][i];
-        plain[k][i] += g[i];
-        sums[0] += h[k][i] * n[k][i];
-        sums[1] += h[k][i];
       }
     }
+    // before this batch's writes: a wait for later loads would wait for those too
+    Walk then = now;
+    then.next(a, kRows);
+    if (then.row < then.end) read(then);
     sum_row(sums, waves, room, turn);
-    const float mean_along = sums[0] * inv_dim, mean_plain = a.layer ? sums[1] * inv_dim : 0.0f;
 #pragma unroll
-    for (int k = 0; k < kIter; ++k) {
-      const Place p(a, lane, k);
+    for (uint32_t i = 0; i < kRows; ++i) {
+      if (i >= now.count) continue;
+      const float mean_along = sums[2 * i] * inv_dim, mean_plain = a.layer ? sums[2 * i + 1] * inv_dim : 0.0f;
+      const Window<T, kOdd> out((const T*)a.out + (uint64_t)(now.row + i) * a.dim, a.dim);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[k][i] = sample == kNone ? 0.0f : r * (h[k][i] - mean_plain - n[k][i] * mean_along);
-      store8<kOdd>((T*)a.out + (uint64_t)row * a.dim + p.at, h[k], p.n);
+      for (int k = 0; k < kIter; ++k) {
+        const Place p(a, lane, k);
+        Eight<T> result;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          result.v[e] = (T)(now.sample == kNone ? 0.0f : r[i] * (h[i][k][e] - mean_plain - n[i][k][e] * mean_along));
+        out.write(result, 0, p.at, p.n);
+      }
     }
+    if (then.row >= then.end) break;
+    fresh = then.sample != now.sample;
+    if (fresh) flush(now.sample);
+    now = then;
   }
-  flush();
+  flush(now.sample);
 }
 
 // Names: type, times a lane holds 8 values; "odd": a dim that is no multiple of eight.
@@ -312,6 +412,7 @@ extern "C" __global__ __launch_bounds__(1024) void mo_norm_sums(NormArgs a) {
   float along = 0.0f, plain = 0.0f;
   if (at < a.dim && low < high) {
     const uint32_t from = (uint32_t)low / a.chunk, to = (uint32_t)(high - 1) / a.chunk;
+#pragma unroll 8
     for (uint32_t i = from + run; i <= to; i += 32) {
       const float* p = a.partial + (uint64_t)(i + sample) * 2 * a.pitch + at;
       along += p[0];
