@@ -12,9 +12,11 @@ forwards with the offload context around the traversal (:439-544), and selective
 checkpointing (:672-710, :780-789). LoRA follows ``training/lora.py:21-86`` and the int8
 weight-only base follows ``training/quantization.py:23-131`` (eager dequantisation).
 
-Two ways of running the blocks that the reference does not have, both off until asked for: a base
-in 8-bit floating point (``quantize_joint_linears_fp8``) and fused head norms and rotary positions
-(``configure_rotary``).
+Ways of running the blocks that the reference does not have, all off until asked for: a base
+in 8-bit floating point (``quantize_joint_linears_fp8``), fused head norms and rotary positions
+(``configure_rotary``), fused norms, gated activations and LoRA updates that may keep what their backward
+needs in 8 bits (``configure_kernels``), and checkpointed blocks whose input is kept so
+(``checkpoint_keep8``).
 
 It is test and benchmark harness code: random-initialised weights, synthetic inputs.
 """
@@ -109,6 +111,23 @@ def attention_fused(query, key, value, rope, heads, q_norm, k_norm, cu_seqlens=N
     return mixed.transpose(1, 2).flatten(2)
 
 
+def norm_fused(norm, tokens, scale=None, shift=None, cu_seqlens=None, keep=False):
+    """An ``RMSNorm`` and the modulation after it in one launch. The norm's weight is read and its module not called, so
+    hooks on it do not run."""
+
+    from .norms import norm as fused
+
+    return fused(tokens, norm.weight, scale=scale, shift=shift, cu_seqlens=cu_seqlens, keep=keep)
+
+
+def situ_fused(up, gate=None, keep=False):
+    """``situ`` of a fused projection (``up`` first) or of two, in one launch."""
+
+    from .gated import gated
+
+    return gated(up, gate, keep=keep)
+
+
 def rope_coordinates(images, text_length: int, device) -> torch.Tensor:
     """``(r, t, h, w)`` per token: image grids (centred), then text (reference model.py:94-133)."""
 
@@ -161,6 +180,7 @@ class TextBlock(nn.Module):
     """Text adapter block with fused qkv (reference model.py:175-215)."""
 
     rotary = "composed"
+    kernels, keep8 = "composed", False
 
     def __init__(self, dim: int, ffn_dim: int, heads: int) -> None:
         super().__init__()
@@ -173,7 +193,9 @@ class TextBlock(nn.Module):
         self.ffn_down = nn.Linear(ffn_dim, dim)
 
     def forward(self, tokens, rope, cu_seqlens=None):
-        query, key, value = self.qkv(self.norm1(tokens)).chunk(3, -1)
+        fused = self.kernels == "hip"
+        hidden = norm_fused(self.norm1, tokens, keep=self.keep8) if fused else self.norm1(tokens)
+        query, key, value = self.qkv(hidden).chunk(3, -1)
         if self.rotary == "hip":
             mixed = attention_fused(query, key, value, rope, self.heads, self.q_norm, self.k_norm, cu_seqlens)
         else:
@@ -181,8 +203,9 @@ class TextBlock(nn.Module):
             key = self.k_norm(key.unflatten(-1, (self.heads, -1))).flatten(2)
             mixed = attention(query, key, value, rope, self.heads, cu_seqlens)
         tokens = tokens + self.proj(mixed)
-        hidden = self.norm2(tokens)
-        return tokens + self.ffn_down(situ(self.ffn_up(hidden), self.ffn_gate(hidden)))
+        hidden = norm_fused(self.norm2, tokens, keep=self.keep8) if fused else self.norm2(tokens)
+        up, gate = self.ffn_up(hidden), self.ffn_gate(hidden)
+        return tokens + self.ffn_down(situ_fused(up, gate, keep=self.keep8) if fused else situ(up, gate))
 
 
 class TextProjection(nn.Module):
@@ -229,6 +252,7 @@ class Block(nn.Module):
     """
 
     rotary = "composed"
+    kernels, keep8 = "composed", False
 
     def __init__(self, dim: int, ffn_dim: int, heads: int, mlp: str = "situ") -> None:
         super().__init__()
@@ -244,27 +268,50 @@ class Block(nn.Module):
             self.proj["ffn_up_gate"] = nn.Linear(dim, 2 * ffn_dim, bias=False)
         self.proj["ffn_down"] = nn.Linear(ffn_dim, dim, bias=False)
 
+    def _modulated(self, norm, tokens, scale, shift, cu_seqlens, index):
+        if self.kernels == "hip":
+            cu_seqlens = None if index is None else cu_seqlens
+            return norm_fused(norm, tokens, scale, shift, cu_seqlens, self.keep8)
+        hidden = norm(tokens)
+        hidden = hidden * (1 + _condition_for_tokens(scale, index))
+        return hidden + _condition_for_tokens(shift, index)
+
+    def _kept(self, names, hidden):
+        """``hidden`` in 8 bits, once for the LoRA updates of the projections that read it; False where none keeps it."""
+
+        if self.kernels != "hip" or not self.keep8 or not torch.is_grad_enabled():
+            return False
+        linears = [self.proj[name] for name in names]
+        if not any(isinstance(linear, LoRALinear) and linear.fuses(hidden) for linear in linears):
+            return False
+        from .kept8 import keep8
+
+        return keep8(hidden.detach())
+
+    def _project(self, name, hidden, kept=False):
+        linear = self.proj[name]
+        return linear(hidden, kept) if isinstance(linear, LoRALinear) and kept is not False else linear(hidden)
+
     def forward(self, tokens, rope, modulation, cu_seqlens=None, seq_lengths=None):
         shift_attn, scale_attn, gate_attn, shift_ffn, scale_ffn, gate_ffn = modulation.unbind(1)
         index = _modulation_sample_indices(modulation, tokens, cu_seqlens)
-        hidden = self.norm1(tokens)
-        hidden = hidden * (1 + _condition_for_tokens(scale_attn, index))
-        hidden = hidden + _condition_for_tokens(shift_attn, index)
+        hidden = self._modulated(self.norm1, tokens, scale_attn, shift_attn, cu_seqlens, index)
         weight_dtype = _linear_dtype(self.proj["q"])
         hidden = hidden.to(weight_dtype)
+        kept = self._kept(("q", "k", "v"), hidden)
         if self.rotary == "hip":
-            attended = attention_fused(self.proj["q"](hidden), self.proj["k"](hidden), self.proj["v"](hidden), rope,
-                                       self.heads, self.q_norm, self.k_norm, cu_seqlens, seq_lengths)
+            query, key, value = (self._project(name, hidden, kept) for name in ("q", "k", "v"))
+            attended = attention_fused(query, key, value, rope, self.heads, self.q_norm, self.k_norm, cu_seqlens, seq_lengths)
         else:
-            query = self.q_norm(self.proj["q"](hidden).unflatten(-1, (self.heads, -1))).flatten(2)
-            key = self.k_norm(self.proj["k"](hidden).unflatten(-1, (self.heads, -1))).flatten(2)
-            attended = attention(query, key, self.proj["v"](hidden), rope, self.heads, cu_seqlens, seq_lengths)
+            query = self.q_norm(self._project("q", hidden, kept).unflatten(-1, (self.heads, -1))).flatten(2)
+            key = self.k_norm(self._project("k", hidden, kept).unflatten(-1, (self.heads, -1))).flatten(2)
+            attended = attention(query, key, self._project("v", hidden, kept), rope, self.heads, cu_seqlens, seq_lengths)
         tokens = tokens + self.proj["o"](attended) * _condition_for_tokens(gate_attn, index)
-        hidden = self.norm2(tokens)
-        hidden = hidden * (1 + _condition_for_tokens(scale_ffn, index))
-        hidden = hidden + _condition_for_tokens(shift_ffn, index)
+        hidden = self._modulated(self.norm2, tokens, scale_ffn, shift_ffn, cu_seqlens, index)
         if self.mlp == "gelu":
             activated = F.gelu(self.proj["ffn_up"](hidden.to(weight_dtype)), approximate="tanh")
+        elif self.kernels == "hip":
+            activated = situ_fused(self.proj["ffn_up_gate"](hidden.to(weight_dtype)), keep=self.keep8)
         else:
             up, gate = self.proj["ffn_up_gate"](hidden.to(weight_dtype)).chunk(2, -1)
             activated = situ(up, gate)
@@ -284,6 +331,22 @@ def configure_rotary(model: nn.Module, backend: str) -> int:
     for block in blocks:
         block.rotary = backend
     return len(blocks)
+
+
+def configure_kernels(model: nn.Module, backend: str, *, keep8: bool = False) -> int:
+    """How every block norms and modulates its tokens, activates its feed-forward and adds its LoRA updates: ``composed``
+    (the reference's operations, the default) or ``hip`` (``moss_offload.norms``, ``gated``, ``adapters``: fp32 inside and
+    rounded once). ``keep8``: what their backward needs is kept in 8 bits (``moss_offload.kept8``), and gradients are
+    those at what 8 bits keep. Returns the blocks and LoRA linears set."""
+
+    if backend not in ROTARY_BACKENDS:
+        raise ValueError(f"kernels' backend must be one of {ROTARY_BACKENDS}")
+    if keep8 and backend != "hip":
+        raise ValueError("only the hip kernels keep activations in 8 bits")
+    modules = [module for module in model.modules() if isinstance(module, (Block, TextBlock, LoRALinear))]
+    for module in modules:
+        module.kernels, module.keep8 = backend, keep8
+    return len(modules)
 
 
 class RoPE(nn.Module):
@@ -342,6 +405,7 @@ class MOSSImageTransformer(nn.Module):
         checkpoint_fraction: float = 1.0,
         activation_offload: bool = False,
         mlp: str = "situ",
+        checkpoint_keep8: bool = False,
     ) -> None:
         super().__init__()
         if dim % num_heads or (dim // num_heads) % 8 or freq_dim % 2:
@@ -351,6 +415,7 @@ class MOSSImageTransformer(nn.Module):
         self.gradient_checkpointing = gradient_checkpointing
         checkpointed_layer_indices(num_layers, checkpoint_fraction)
         self.checkpoint_fraction = float(checkpoint_fraction)
+        self.checkpoint_keep8 = bool(checkpoint_keep8)
         self.activation_offload = bool(activation_offload)
         self.offload_context: Callable = activation_cpu_offload
         self.video_embedder = nn.Linear(latent_channels, dim)
@@ -487,7 +552,12 @@ class MOSSImageTransformer(nn.Module):
 
                 tokens = offloaded_block(layer, *inputs)
             elif self.gradient_checkpointing and self.training and index in checkpointed:
-                tokens = checkpoint(layer, *inputs, use_reentrant=False)
+                if self.checkpoint_keep8:
+                    from .kept8 import checkpoint_kept8
+
+                    tokens = checkpoint_kept8(layer, *inputs)
+                else:
+                    tokens = checkpoint(layer, *inputs, use_reentrant=False)
             else:
                 tokens = layer(*inputs)
         return tokens
@@ -499,6 +569,8 @@ class MOSSImageTransformer(nn.Module):
 
 class LoRALinear(nn.Module):
     """Frozen base linear plus ``(alpha / rank) * B @ A``; autocast casts A and B (lora.py:60-86)."""
+
+    kernels, keep8 = "composed", False
 
     def __init__(self, base: nn.Module, rank: int, alpha: float) -> None:
         super().__init__()
@@ -519,13 +591,30 @@ class LoRALinear(nn.Module):
     def in_features(self):
         return self.base.in_features
 
-    def forward(self, tokens):
+    def _dtype(self, tokens):
+        kind = tokens.device.type
+        return torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else None
+
+    def fuses(self, tokens) -> bool:
+        """Whether the update of these tokens runs as one (``moss_offload.adapters``): asked for, on a HIP device, and
+        the tokens come in the adapter's type."""
+
+        dtype = self._dtype(tokens) or self.lora_A.dtype
+        return self.kernels == "hip" and tokens.is_cuda and tokens.dtype == dtype and self.rank <= 128
+
+    def forward(self, tokens, kept=False):
+        """``kept``: the tokens in 8 bits, where the caller keeps them for several linears."""
+
         result = self.base(tokens)
-        dtype = torch.get_autocast_dtype(tokens.device.type) if torch.is_autocast_enabled(tokens.device.type) else None
+        dtype = self._dtype(tokens)
         if dtype is None:
             adapter_input, adapter_a, adapter_b = tokens.to(self.lora_A.dtype), self.lora_A, self.lora_B
         else:
             adapter_input, adapter_a, adapter_b = tokens.to(dtype), self.lora_A.to(dtype), self.lora_B.to(dtype)
+        if self.fuses(tokens) and result.dtype == tokens.dtype:
+            from .adapters import adapters
+
+            return adapters(tokens, result, adapter_a, adapter_b, self.scale, keep=kept or self.keep8)
         update = F.linear(F.linear(adapter_input, adapter_a), adapter_b)
         return result + update.to(result.dtype) * self.scale
 

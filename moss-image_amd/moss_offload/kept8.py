@@ -101,14 +101,13 @@ def keep8(x: torch.Tensor) -> Kept8:
 class _CheckpointFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, function, tokens, *others):
-        kind = tokens.device.type
+        kept, kind = keep8(tokens), tokens.device.type
         ctx.function, ctx.dtype, ctx.cols, ctx.kind = function, tokens.dtype, tokens.shape[-1], kind
         ctx.autocast = (torch.is_autocast_enabled(kind), torch.get_autocast_dtype(kind), torch.is_autocast_cache_enabled())
         ctx.random = torch.get_rng_state(), torch.cuda.get_rng_state(tokens.device)
         ctx.others = [None if isinstance(t, torch.Tensor) else t for t in others]
         ctx.places = [i for i, t in enumerate(others) if isinstance(t, torch.Tensor)]
         ctx.wanted = [t.requires_grad for t in others if isinstance(t, torch.Tensor)]
-        kept = keep8(tokens)
         ctx.save_for_backward(kept.values, kept.exponents, *(others[i] for i in ctx.places))
         return function(tokens, *others)
 
