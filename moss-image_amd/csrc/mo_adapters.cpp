@@ -160,10 +160,25 @@ Room room_of(const mo_adapters_call& c, bool backward) {
   return r;
 }
 
-int start(const std::string& name, uint64_t gx, uint64_t gy, uint64_t gz, void* args, uint64_t stream, uint32_t threads = 256) {
+// The kernels of one type: each with a size and a form, which make its name and its number.
+enum Kind { kShrink, kExpand, kOuter, kJoin, kTurn };
+int start(const mo_adapters_call& c, Kind kind, uint32_t size, const char* form, uint64_t gx, uint64_t gy, uint64_t gz, void* args,
+          uint64_t stream, uint32_t threads = 256) {
   if (gx >= (1ull << 31) || gy >= (1u << 16) || gz > (1u << 16)) return mo::set_error(MO_E_INVALID, "too many values");
-  hipFunction_t kernel;
-  if (int rc = kernels().get("mo_adapters_" + name, &kernel)) return rc;
+  static const char* const names[] = {"shrink_", "expand_", "outer_", "join_", "turn_"};
+  auto name = [&]() {
+    std::string n = std::string("mo_adapters_") + names[kind] + kTypeNames[c.dtype];
+    if (size) n += "_" + std::to_string(size);
+    if (*form) n += std::string("_") + form;
+    return n;
+  };
+  const int step = size >= 128 ? 7 : size >= 64 ? 6 : size >= 32 ? 5 : size >= 16 ? 4 : size >= 8 ? 3 : size >= 4 ? 2 : size >= 2 ? 1 : 0;
+  // sizes: up to 8 of a shrink and an outer, 16 to 128 of an expand; forms: "", "1", "2", "odd", "tall"
+  const int place = *form == 0 ? 0 : *form == '2' || *form == 't' ? 1 : *form == 'o' ? 2 : 0;
+  const int id = kind == kShrink ? step * 3 + place : kind == kExpand ? 12 + (step - 4) * 3 + place
+                 : kind == kOuter ? 24 + step * 3 + place : kind == kJoin ? 36 : 37;
+  hipFunction_t kernel = nullptr;
+  if (int rc = kernels().get((int)c.dtype * 40 + id, name, &kernel)) return rc;
   void* params[] = {args};
   return mo::launch(kernel, (uint32_t)gx, (uint32_t)gy, (uint32_t)gz, threads, stream, params, "adapters launch");
 }
@@ -174,14 +189,14 @@ int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t s
   mo_adapters::Shrink a = {};
   a.by = by, a.x = (const void*)x, a.w = (const void*)w, a.to = (float*)to;
   a.x_stride = stride, a.features = features, a.span = p.span, a.scaled = scaled;
-  return start(std::string("shrink_") + kTypeNames[c.dtype] + "_" + std::to_string(p.ranks) + (odd(c) ? "_odd" : p.rows == 128 ? "_tall" : "_1"),
+  return start(c, kShrink, p.ranks, odd(c) ? "odd" : p.rows == 128 ? "tall" : "1",
                p.slots, p.splits, 1, &a, stream, 512);
 }
 
 int expand(const mo_adapters_call& c, mo_adapters::Expand& a, uint64_t stream) {
   const ExpandPlan p = expand_plan(c, a.features);
   a.cols = p.cols;
-  return start(std::string("expand_") + kTypeNames[c.dtype] + "_" + std::to_string(p.rank) + (odd(c) ? "_odd" : p.tiles == 2 ? "_2" : "_1"),
+  return start(c, kExpand, p.rank, odd(c) ? "odd" : p.tiles == 2 ? "2" : "1",
                p.slots, div_up(a.features, p.cols), 1, &a, stream);
 }
 
@@ -196,7 +211,6 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
   by.rows = (uint32_t)c.rows, by.requests = c.requests, by.adapters = c.adapters, by.rank = c.rank;
   by.share = c.cu ? 0 : (uint32_t)(c.rows / c.requests);
   const uint64_t planes = workspace + room.planes;
-  const char* type = kTypeNames[c.dtype];
   mo_adapters::Expand e = {};
   e.by = by;
   if (!backward) {
@@ -219,7 +233,7 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
   const uint64_t narrow = div_up(c.rows, 32) * div_up(c.rank, 32);
   if (c.db) t.narrow = (const float*)c.hidden, t.turned = (void*)(workspace + room.turned_hidden), t.splits = 1;
   const uint64_t weights = (uint64_t)t.tiles[0] + t.tiles[1];
-  if (int rc = start(std::string("turn_") + type, weights + (c.db ? narrow : 0), weights ? c.adapters : 1, 1, &t, stream)) return rc;
+  if (int rc = start(c, kTurn, 0, "", weights + (c.db ? narrow : 0), weights ? c.adapters : 1, 1, &t, stream)) return rc;
   if (c.dx || c.da) {
     if (int rc = shrink(c, by, c.grad, stride_of(c, c.grad_stride, c.out_features), workspace + room.turned_b, c.out_features, planes, true, stream)) return rc;
     const uint32_t splits = shrink_plan(c, c.out_features).splits;
@@ -231,7 +245,7 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
     } else {
       t.tiles[0] = t.tiles[1] = 0;
       t.narrow = (const float*)planes, t.turned = (void*)(workspace + room.turned_back), t.splits = splits;
-      if (int rc = start(std::string("turn_") + type, narrow, 1, 1, &t, stream)) return rc;
+      if (int rc = start(c, kTurn, 0, "", narrow, 1, 1, &t, stream)) return rc;
     }
   }
   if (!c.da && !c.db) return 0;
@@ -245,12 +259,12 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
   b.planes = (float*)(workspace + room.db), b.to = (void*)c.db, b.stride = stride_of(c, c.grad_stride, c.out_features);
   b.turned = 1, b.scaled = 1;
   const uint32_t ranks = c.rank <= 16 ? 1 : c.rank <= 32 ? 2 : 4;
-  if (int rc = start(std::string("outer_") + type + "_" + std::to_string(ranks) + (odd(c) ? "_odd" : ""), (uint64_t)a.tiles + b.tiles, a.splits,
+  if (int rc = start(c, kOuter, ranks, odd(c) ? "odd" : "", (uint64_t)a.tiles + b.tiles, a.splits,
                      (uint64_t)c.adapters * div_up(c.rank, ranks * 16), &o, stream))
     return rc;
   if (a.splits == 1) return 0;
   const uint64_t size = (uint64_t)c.rank * (a.cols > b.cols ? a.cols : b.cols);
-  return start(std::string("join_") + type, div_up(size, 1024), c.adapters, 2, &o, stream);
+  return start(c, kJoin, 0, "", div_up(size, 1024), c.adapters, 2, &o, stream);
 }
 
 }  // namespace

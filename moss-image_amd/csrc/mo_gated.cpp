@@ -55,10 +55,13 @@ int gated(const mo_gated_call* c, bool backward, uint64_t stream) {
   a.values_stride = c->values_stride, a.exponents_stride = c->exponents_stride;
   a.rows = (uint32_t)c->rows, a.cols = c->cols, a.silu = c->silu;
   if (!shares(c->rows, c->cols, &a.lanes, &a.by_lanes)) return bad("too many values");
-  const std::string name = std::string("mo_gated_") + (backward ? "backward_" : "forward_") + (kept ? "kept_" : keep ? "keep_" : "") +
-                           kTypeNames[c->dtype] + (c->cols % 8 ? "_odd" : "");
-  hipFunction_t kernel;
-  if (int rc = kernels().get(name, &kernel)) return rc;
+  const bool eights = kept || keep, singly = c->cols % 8 != 0;
+  auto name = [&]() {
+    return std::string("mo_gated_") + (backward ? "backward_" : "forward_") + (kept ? "kept_" : keep ? "keep_" : "") +
+           kTypeNames[c->dtype] + (singly ? "_odd" : "");
+  };
+  hipFunction_t kernel = nullptr;
+  if (int rc = kernels().get(((backward * 2 + eights) * 3 + (int)c->dtype) * 2 + singly, name, &kernel)) return rc;
   void* params[] = {&a};
   const uint64_t items = c->rows * a.lanes;
   return mo::launch(kernel, (uint32_t)((items + 255) / 256), 1, 1, 256, stream, params, "gated activation launch");
@@ -75,8 +78,12 @@ int keep(uint64_t x, uint64_t values, uint64_t exponents, uint32_t dtype, uint64
   a.x = (const void*)x, a.out = (void*)x, a.values = (int8_t*)values, a.exponents = (uint8_t*)exponents;
   a.stride = stride, a.rows = (uint32_t)rows, a.cols = cols, a.groups = (cols + 31) / 32;
   if (!shares(rows, cols, &a.lanes, &a.by_lanes)) return bad("too many values");
-  hipFunction_t kernel;
-  if (int rc = kernels().get(std::string(restore ? "mo_keep_restore_" : "mo_keep_pack_") + kTypeNames[dtype] + (cols % 8 ? "_odd" : ""), &kernel)) return rc;
+  const bool singly = cols % 8 != 0;
+  auto name = [&]() {
+    return std::string(restore ? "mo_keep_restore_" : "mo_keep_pack_") + kTypeNames[dtype] + (singly ? "_odd" : "");
+  };
+  hipFunction_t kernel = nullptr;
+  if (int rc = kernels().get(24 + (restore * 3 + (int)dtype) * 2 + singly, name, &kernel)) return rc;
   void* params[] = {&a};
   const uint64_t items = rows * a.lanes;
   return mo::launch(kernel, (uint32_t)((items + 255) / 256), 1, 1, 256, stream, params, "8-bit activations launch");

@@ -2,10 +2,10 @@
 #pragma once
 #include <hip/hip_runtime_api.h>
 
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <string>
-#include <utility>
 
 #include "../../include/moss_offload.h"
 
@@ -16,29 +16,30 @@ int set_hip_error(int e, const char* what);
 
 class Kernels {
  public:
+  static constexpr int kIds = 128, kDevices = 16;
+
   explicit Kernels(const unsigned char* code) : code_(code) {}
 
-  // The kernel `name` on the current device.
-  int get(const std::string& name, hipFunction_t* out) {
+  // The kernel `name()` on the current device; `id` below kIds is the same name every time. Found once, without a lock.
+  template <class Name>
+  int get(int id, Name&& name, hipFunction_t* out) {
     int device = 0;
     hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return set_hip_error((int)e, "hipGetDevice");
+    std::atomic<hipFunction_t>* known = device < kDevices ? &known_[device][id] : nullptr;
+    if (known && (*out = known->load(std::memory_order_acquire))) return 0;
     std::lock_guard<std::mutex> lock(mu_);
-    const auto key = std::make_pair(device, name);
-    auto it = functions_.find(key);
-    if (it == functions_.end()) {
-      auto module = modules_.find(device);
-      if (module == modules_.end()) {
-        hipModule_t m = nullptr;
-        if ((e = hipModuleLoadData(&m, code_)) != hipSuccess) return set_hip_error((int)e, "hipModuleLoadData");
-        module = modules_.emplace(device, m).first;
-      }
-      hipFunction_t f = nullptr;
-      if ((e = hipModuleGetFunction(&f, module->second, name.c_str())) != hipSuccess)
-        return set_hip_error((int)e, "hipModuleGetFunction");
-      it = functions_.emplace(key, f).first;
+    auto module = modules_.find(device);
+    if (module == modules_.end()) {
+      hipModule_t m = nullptr;
+      if ((e = hipModuleLoadData(&m, code_)) != hipSuccess) return set_hip_error((int)e, "hipModuleLoadData");
+      module = modules_.emplace(device, m).first;
     }
-    *out = it->second;
+    hipFunction_t f = nullptr;
+    if ((e = hipModuleGetFunction(&f, module->second, std::string(name()).c_str())) != hipSuccess)
+      return set_hip_error((int)e, "hipModuleGetFunction");
+    if (known) known->store(f, std::memory_order_release);
+    *out = f;
     return 0;
   }
 
@@ -46,7 +47,7 @@ class Kernels {
   const unsigned char* code_;
   std::mutex mu_;
   std::map<int, hipModule_t> modules_;
-  std::map<std::pair<int, std::string>, hipFunction_t> functions_;
+  std::atomic<hipFunction_t> known_[kDevices][kIds] = {};
 };
 
 inline int launch(hipFunction_t f, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t threads, uint64_t stream, void** params,

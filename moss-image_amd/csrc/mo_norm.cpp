@@ -123,20 +123,23 @@ int run(const mo_norm_call* c, bool backward, uint64_t workspace, uint64_t bytes
     if (wants_sums(*c)) a.partial = (float*)workspace;
     if (wants_sample_sums(*c)) a.sample_sums = (float*)workspace + p.slots * 2 * a.pitch;
   }
-  const std::string name = std::string("mo_norm_") + (backward ? "backward_" : "forward_") +
-                           (backward ? (a.x_exponents ? "kept_" : "") : (a.kept ? "keep_" : "")) + kTypeNames[c->dtype] +
-                           "_" + std::to_string(p.iter) + (odd(*c) ? "_odd" : "");
-  hipFunction_t kernel;
-  if (int rc = kernels().get(name, &kernel)) return rc;
+  const bool eights = backward ? a.x_exponents != nullptr : a.kept != nullptr, singly = odd(*c);
+  auto name = [&]() {
+    return std::string("mo_norm_") + (backward ? "backward_" : "forward_") + (!eights ? "" : backward ? "kept_" : "keep_") +
+           kTypeNames[c->dtype] + "_" + std::to_string(p.iter) + (singly ? "_odd" : "");
+  };
+  const int id = ((backward * 2 + eights) * 3 + (int)c->dtype) * 4 + (p.iter - 1) * 2 + singly;
+  hipFunction_t kernel = nullptr;
+  if (int rc = kernels().get(id, name, &kernel)) return rc;
   void* params[] = {&a};
   if (int rc = mo::launch(kernel, (uint32_t)div_up(p.groups, p.per), 1, 1, p.lanes * p.per, stream, params, "norm launch"))
     return rc;
   if (!a.partial) return 0;
-  if (int rc = kernels().get("mo_norm_sums", &kernel)) return rc;
+  if (int rc = kernels().get(48, [] { return "mo_norm_sums"; }, &kernel)) return rc;
   if (int rc = mo::launch(kernel, (c->dim + 31) / 32, c->samples ? c->samples : 1, 1, 1024, stream, params, "norm sums launch"))
     return rc;
   if (!a.sample_sums) return 0;
-  if (int rc = kernels().get("mo_norm_sample_sums", &kernel)) return rc;
+  if (int rc = kernels().get(49, [] { return "mo_norm_sample_sums"; }, &kernel)) return rc;
   return mo::launch(kernel, (c->dim + 255) / 256, 1, 1, 256, stream, params, "norm sums launch");
 }
 

@@ -43,6 +43,12 @@ def rows(tensor: torch.Tensor, what: str) -> torch.Tensor:
     return matrix
 
 
+def like(tensor: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """A contiguous tensor of ``tensor``'s shape, not filled: half the host time of ``torch.empty``."""
+
+    return torch.empty_like(tensor, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def pitch(matrix: torch.Tensor) -> int:
     return matrix.stride(0) if matrix.shape[0] > 1 else matrix.shape[1]
 

@@ -19,7 +19,7 @@ import struct
 import torch
 
 from . import _native
-from ._operands import CODES, elsewhere, first_derivatives, pitch, plain, stream, whole
+from ._operands import CODES, elsewhere, first_derivatives, like as _like, pitch, plain, stream, whole
 from ._operands import rows as _dense_rows
 from .kept8 import Kept8, keep8
 
@@ -73,7 +73,7 @@ def _check(like, shape, a, b, scale, cu_seqlens, index):
 def _space(lib, call, backward: bool, like: torch.Tensor):
     # freed to the caching allocator after the call; stream order keeps it alive for the kernels
     nbytes = lib.mo_adapters_workspace_bytes(ctypes.byref(call), backward)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=like.device), nbytes) if nbytes else (None, 0)
+    return (like.new_empty(nbytes, dtype=torch.uint8), nbytes) if nbytes else (None, 0)
 
 
 def adapters_forward(x: torch.Tensor, result: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale=1.0, *,
@@ -95,8 +95,8 @@ def adapters_forward(x: torch.Tensor, result: torch.Tensor, a: torch.Tensor, b: 
         with torch.cuda.device(x.device):
             return adapters_forward(x, result, a, b, scale, cu_seqlens=cu_seqlens, index=index, hidden=hidden)
     rank = a.shape[1]
-    y = torch.empty(result.shape, dtype=x.dtype, device=x.device)
-    between = torch.empty((count, rank), dtype=torch.float32, device=x.device)
+    y = _like(result)
+    between = x.new_empty((count, rank), dtype=torch.float32)
     if count:
         call = _native.MoAdaptersCall.from_buffer_copy(_CALL.pack(
             tokens.data_ptr(), 0, base.data_ptr(), y.data_ptr(), a.data_ptr(), b.data_ptr(), _address(scales), _address(cu),
@@ -131,8 +131,8 @@ def _backward(grad, x, hidden, a, b, scale, cu_seqlens, index, add, wanted):
     source = None if x is None else x.values if kept else rows(x, "adapters' tokens")
     hidden = hidden.contiguous()
     added = None if add is None else rows(add, "adapters' add")
-    dx = torch.empty((*grad.shape[:-1], in_features), dtype=grad.dtype, device=grad.device) if wanted[0] else None
-    da, db = (torch.empty_like(t) if w else None for t, w in zip((a, b), wanted[1:]))
+    dx = grad.new_empty((*grad.shape[:-1], in_features)) if wanted[0] else None
+    da, db = (_like(t) if w else None for t, w in zip((a, b), wanted[1:]))
     if count and any(wanted):
         call = _native.MoAdaptersCall.from_buffer_copy(_CALL.pack(
             _address(source), x.exponents.data_ptr() if kept else 0, 0, 0, a.data_ptr(), b.data_ptr(), _address(scales),

@@ -17,7 +17,7 @@ import struct
 import torch
 
 from . import _native
-from ._operands import CODES, elsewhere, first_derivatives, pitch, plain, rows, stream
+from ._operands import CODES, elsewhere, first_derivatives, like, pitch, plain, rows, stream
 from .kept8 import Kept8, empty
 
 KINDS = ("situ", "silu")
@@ -57,15 +57,15 @@ def gated_forward(up: torch.Tensor, gate: torch.Tensor | None = None, *, kind: s
         with torch.cuda.device(up.device):
             return gated_forward(up, gate, kind=kind, keep=keep)
     count = first.shape[0]
-    out = torch.empty(shape, dtype=up.dtype, device=up.device)
+    out = up.new_empty(shape) if gate is None else like(up)
     kept, kept_gate, places, strides = None, None, (0, 0, 0, 0), (0, 0)
     if keep and gate is None:
-        kept = empty((*shape[:-1], 2, cols), up.dtype, up.device)
+        kept = empty((*shape[:-1], 2, cols), up)
         values, groups = kept.values.shape[-1], kept.exponents.shape[-1]
         at, exponents = kept.values.data_ptr(), kept.exponents.data_ptr()
         places, strides = (at, at + values, exponents, exponents + groups), (2 * values, 2 * groups)
     elif keep:
-        kept, kept_gate = empty(shape, up.dtype, up.device), empty(shape, up.dtype, up.device)
+        kept, kept_gate = empty(shape, up), empty(shape, up)
         places = tuple(t.data_ptr() for t in (kept.values, kept_gate.values, kept.exponents, kept_gate.exponents))
         strides = kept.values.shape[-1], kept.exponents.shape[-1]
     if count:
@@ -109,10 +109,10 @@ def gated_backward(grad: torch.Tensor, up, gate=None, *, kind: str = "situ"):
         with torch.cuda.device(grad.device):
             return gated_backward(grad, up, gate, kind=kind)
     if fused:
-        out = torch.empty((*grad.shape[:-1], 2 * cols), dtype=grad.dtype, device=grad.device)
+        out = grad.new_empty((*grad.shape[:-1], 2 * cols))
         outs = out.data_ptr(), out.data_ptr() + cols * out.element_size()
     else:
-        out = tuple(torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) for _ in range(2))
+        out = like(grad), like(grad)
         outs = out[0].data_ptr(), out[1].data_ptr()
     if count:
         call = _native.MoGatedCall.from_buffer_copy(_CALL.pack(

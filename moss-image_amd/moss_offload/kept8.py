@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from ._operands import CODES, elsewhere, first_derivatives, pitch, plain, rows, stream
+from ._operands import CODES, elsewhere, first_derivatives, like, pitch, plain, rows, stream
 
 GROUP = 32
 
@@ -59,7 +59,8 @@ class Kept8:
         if elsewhere(self.values, "Kept8"):
             with torch.cuda.device(self.values.device):
                 return self.restore(dtype)
-        out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
+        exact = self.cols == self.values.shape[-1]
+        out = like(self.values, dtype) if exact else self.values.new_empty(self.shape, dtype=dtype)
         if out.numel():
             _native.check("mo_keep_restore", lib.mo_keep_restore(
                 self.values.data_ptr(), self.exponents.data_ptr(), out.data_ptr(), CODES[dtype],
@@ -67,14 +68,17 @@ class Kept8:
         return out
 
 
-def empty(shape, dtype: torch.dtype, device: torch.device) -> Kept8:
-    """Room for a kernel to write a tensor of ``shape`` in 8 bits."""
+def empty(shape, tensor: torch.Tensor) -> Kept8:
+    """Room for a kernel to write a tensor of ``shape``, and ``tensor``'s type, in 8 bits."""
 
     kept = Kept8.__new__(Kept8)
     groups = -(-shape[-1] // GROUP)
-    kept.values = torch.empty((*shape[:-1], groups * GROUP), dtype=torch.int8, device=device)
-    kept.exponents = torch.empty((*shape[:-1], groups), dtype=torch.uint8, device=device)
-    kept.cols, kept.dtype = shape[-1], dtype
+    if shape == tensor.shape and shape[-1] % GROUP == 0:
+        kept.values = like(tensor, torch.int8)
+    else:
+        kept.values = tensor.new_empty((*shape[:-1], groups * GROUP), dtype=torch.int8)
+    kept.exponents = tensor.new_empty((*shape[:-1], groups), dtype=torch.uint8)
+    kept.cols, kept.dtype = shape[-1], tensor.dtype
     return kept
 
 
@@ -87,7 +91,7 @@ def keep8(x: torch.Tensor) -> Kept8:
     if elsewhere(x, "keep8"):
         with torch.cuda.device(x.device):
             return keep8(x)
-    kept = empty(x.shape, x.dtype, x.device)
+    kept = empty(x.shape, x)
     if matrix.shape[0]:
         _native.check("mo_keep_pack", lib.mo_keep_pack(
             matrix.data_ptr(), CODES[x.dtype], matrix.shape[0], matrix.shape[1], pitch(matrix), kept.values.data_ptr(),

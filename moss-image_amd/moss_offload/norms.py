@@ -19,7 +19,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native
-from ._operands import CODES, elsewhere, first_derivatives, pitch, plain, rows, stream, whole
+from ._operands import CODES, elsewhere, first_derivatives, like as _like, pitch, plain, rows, stream, whole
 from .kept8 import Kept8, empty
 
 KINDS = ("layer", "rms")
@@ -86,7 +86,8 @@ def _run(name, lib, fields, like):
     if name == "mo_norm_forward":
         return _native.check(name, lib.mo_norm_forward(ctypes.byref(call), stream(like)))
     nbytes = lib.mo_norm_workspace_bytes(ctypes.byref(call))
-    space = torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+    # freed to the caching allocator after the call; stream order keeps it alive for the kernels
+    space = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _native.check(name, lib.mo_norm_backward(ctypes.byref(call), _address(space), nbytes, stream(like)))
 
 
@@ -107,9 +108,9 @@ def norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torc
             return norm_forward(x, weight, bias, kind=kind, scale=scale, shift=shift, cu_seqlens=cu, eps=eps, stats=stats,
                                 keep=keep)
     count, dim = matrix.shape
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    statistics = torch.empty((count, 2), dtype=torch.float32, device=x.device) if stats else None
-    kept = empty(x.shape, x.dtype, x.device) if keep else None
+    out = _like(x)
+    statistics = x.new_empty((count, 2), dtype=torch.float32) if stats else None
+    kept = empty(x.shape, x) if keep else None
     if count:
         _run("mo_norm_forward", lib, _CALL.pack(
             matrix.data_ptr(), 0, 0, out.data_ptr(), _address(statistics), _address(weight), _address(bias), _address(scale),
@@ -137,9 +138,9 @@ def _backward(grad, x, stats, weight, bias, kind, scale, shift, cu_seqlens, want
             return _backward(grad, x, stats, weight, bias, kind, scale, shift, cu, wanted)
     source = x.values if kept else rows(x, "norm rows")
     stats = stats.contiguous()
-    out = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device)
+    out = _like(grad)
     # the sums are as wide as their tensors; with no rows they are zero
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and w else None
+    grads = [_like(t) if t is not None and w else None
              for t, w in zip((weight, bias, scale, shift), wanted)]
     if count:
         _run("mo_norm_backward", lib, _CALL.pack(

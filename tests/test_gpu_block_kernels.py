@@ -269,16 +269,13 @@ class Guarded:
 
     def __init__(self, monkeypatch):
         self.rooms, self.empty = [], torch.empty
-        monkeypatch.setattr(torch, "empty", self.make)
-        monkeypatch.setattr(torch, "empty_like", lambda t: self.make(t.shape, dtype=t.dtype, device=t.device))
+        monkeypatch.setattr(torch, "empty_like", lambda t, dtype=None, memory_format=None: self.make(t.shape, dtype or t.dtype))
+        monkeypatch.setattr(torch.Tensor, "new_empty", lambda t, shape, dtype=None: self.make(shape, dtype or t.dtype))
 
-    def make(self, *shape, dtype=torch.float32, device=None):
-        shape = tuple(shape[0]) if len(shape) == 1 and not isinstance(shape[0], int) else shape
-        count = 1
-        for s in shape:
-            count *= s
-        nbytes = count * torch.zeros((), dtype=dtype).element_size()
-        room = self.empty(2 * self.GUARD + nbytes, dtype=torch.uint8, device=device)
+    def make(self, shape, dtype):
+        shape = (shape,) if isinstance(shape, int) else tuple(shape)
+        nbytes = torch.Size(shape).numel() * torch.zeros((), dtype=dtype).element_size()
+        room = self.empty(2 * self.GUARD + nbytes, dtype=torch.uint8, device=DEV)
         room.fill_(0xA5)
         self.rooms.append((room, nbytes))
         return room[self.GUARD : self.GUARD + nbytes].view(dtype).view(shape)
