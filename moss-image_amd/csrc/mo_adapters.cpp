@@ -96,17 +96,20 @@ ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
   return p;
 }
 
-// Rows a tile and columns a workgroup of an expand: as many as leave some workgroups for every CU.
+// Rows a tile and columns a workgroup of an expand. Tiles of 32 rows, with more than 16 ranks of 128, which share v, or
+// for short requests, whose other rows would be empty, of 16; columns so that there are some rounds of workgroups.
 struct ExpandPlan {
-  uint32_t rank, tiles, cols;
+  uint32_t rank, rows, cols;
   uint64_t slots;
 };
 ExpandPlan expand_plan(const mo_adapters_call& c, uint32_t features) {
   ExpandPlan p = {};
   p.rank = c.rank <= 16 ? 16 : c.rank <= 32 ? 32 : c.rank <= 64 ? 64 : 128;
-  p.tiles = !odd(c) && p.rank < 128 && c.rows >= 32ull * c.requests ? 2 : 1;
-  const uint64_t tiles = div_up(c.rows, p.tiles * 16);
-  p.cols = (uint32_t)round_up(between<uint64_t>(1, tiles * features / kExpandGroups, 4096), 512);
+  p.rows = 16;
+  if (!odd(c) && p.rank == 16 && c.rows >= 32ull * c.requests) p.rows = 32;
+  if (!odd(c) && p.rank > 16 && c.rows >= 128ull * c.requests && c.rows >= 1024) p.rows = 128;
+  const uint64_t tiles = div_up(c.rows, p.rows), least = p.rows == 128 ? 128 : 512;
+  p.cols = (uint32_t)round_up(between<uint64_t>(1, tiles * features / (p.rows == 128 ? 1024 : kExpandGroups), 4096), least);
   p.slots = tiles + c.requests + 1;
   return p;
 }
@@ -196,7 +199,7 @@ int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t s
 int expand(const mo_adapters_call& c, mo_adapters::Expand& a, uint64_t stream) {
   const ExpandPlan p = expand_plan(c, a.features);
   a.cols = p.cols;
-  return start(c, kExpand, p.rank, odd(c) ? "odd" : p.tiles == 2 ? "2" : "1",
+  return start(c, kExpand, p.rank, odd(c) ? "odd" : p.rows == 128 ? "tall" : p.rows == 32 ? "2" : "1",
                p.slots, div_up(a.features, p.cols), 1, &a, stream);
 }
 

@@ -467,6 +467,135 @@ __device__ __forceinline__ void expand(const Expand& a) {
   }
 }
 
+// The same for more than 16 ranks and long requests: a wave has 32 rows of its own, all four waves take the same columns,
+// and v's part of them, as large as the rows' own at 64 ranks, comes to LDS once, a step ahead in registers.
+template <class T, int kRank>
+__device__ __forceinline__ void expand_tall(const Expand& a) {
+  typedef Path<T> P;
+  constexpr uint32_t kRows = 128, kChunks = kRank / 8, kMine = 128 * kChunks / 256;
+  constexpr int kSteps = kRank / 32;
+  __shared__ float room[4][16][132];
+  __shared__ Eight<T> weight[128][kChunks];
+  const Tile tile = tile_of<kRows>(a.by, blockIdx.x);
+  if (tile.low >= tile.high) return;
+  const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
+  const uint32_t first = blockIdx.y * a.cols, end = min(a.features, first + a.cols);
+  const uint32_t low = tile.low + wave * 32, rows = low >= tile.high ? 0 : min(32u, tile.high - low);
+  const uint32_t stride = (uint32_t)a.base_stride;
+  const uint64_t from = rows ? low : tile.low;  // a wave without rows reads and writes none
+  const Window<T, false> base((const T*)a.base + from * a.base_stride, a.base && rows ? (rows - 1) * stride + a.features : 0);
+  const Window<T, false> to((const T*)a.to + from * a.features, rows * a.features);
+  Eight<T> in[8];
+  auto count = [&](uint32_t at) { return at + i * 8 < end ? 8u : 0u; };
+  auto read_base = [&](uint32_t at, int t) {
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t row = t * 16 + u * 4;
+      in[t * 4 + u] = base.read(row * stride + at, k * stride + i * 8, row + k < rows ? count(at) : 0);
+    }
+  };
+  read_base(first, 0);
+  read_base(first, 1);
+  const uint32_t adapter = adapter_of(a.by, tile);
+  const bool has = adapter != kNone;
+  const Window<T, false> v((const T*)a.v + (uint64_t)(has ? adapter : 0) * a.features * rank, a.features * rank);
+  Eight<T> mine[kMine];
+  auto read_v = [&](uint32_t at) {
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e) {
+      const uint32_t place = e * 256 + threadIdx.x, n = place / kChunks, j = place % kChunks * 8;
+      mine[e] = v.read(at * rank, n * rank + j, j < rank && at + n < a.features ? 8 : 0);
+    }
+  };
+  typename P::Fragment h[P::kParts][kSteps][2];
+  float scale = 0.0f;
+  if (has) {
+    read_v(first);
+    scale = a.scaled ? scale_of(a.by, adapter) : 1.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t j = s * 32 + k * 8, row = t * 16 + i;
+        float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < rows && j < rank) {
+          const float* p = a.h + (uint64_t)(low + row) * rank + j;
+          widen(sum, load8(p));
+#pragma unroll 2
+          for (uint32_t split = 1; split < a.splits; ++split) {
+            float more[8];
+            widen(more, load8(p + (uint64_t)split * a.by.rows * rank));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += more[e];
+          }
+          if (blockIdx.y == 0) {
+            if (a.h_sum) store8(a.h_sum + (uint64_t)(low + row) * rank + j, sum);
+            if (a.turned) {
+#pragma unroll
+              for (uint32_t e = 0; e < 8; ++e) store_turned<T>(a.turned, rank, j + e, low + row, sum[e]);
+            }
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < P::kParts; ++p) h[p][s][t] = P::part(sum, p);
+      }
+  } else if (blockIdx.y == 0 && a.h_sum) {
+    for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * rank; e += 256) a.h_sum[(uint64_t)tile.low * rank + e] = 0.0f;
+  }
+  for (uint32_t at = first; at < end; at += 128) {
+    const bool more_cols = at + 128 < end;
+    if (has) {
+      __syncthreads();  // the last step's part has been read
+#pragma unroll
+      for (uint32_t e = 0; e < kMine; ++e) {
+        const uint32_t place = e * 256 + threadIdx.x, n = place / kChunks, chunk = place % kChunks;
+        weight[n][chunk ^ n % kChunks] = mine[e];
+      }
+      __syncthreads();
+      if (more_cols) read_v(at + 128);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (has) {
+#pragma unroll
+        for (uint32_t c = 0; c < 8; ++c) {
+          const uint32_t n = c * 16 + i;
+          f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (uint32_t s = 0; s < kSteps; ++s) {
+            const typename P::Fragment f = P::of(weight[n][(s * 4 + k) ^ n % kChunks]);
+#pragma unroll
+            for (int p = 0; p < P::kParts; ++p) P::multiply(sum, f, h[p][s][t]);
+          }
+          *(f32x4*)&room[wave][i][c * 16 + k * 4] = sum;
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+      Eight<T> results[4];
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        float out[8];
+        widen(out, in[t * 4 + u]);
+        if (has) {
+          float more[8];
+          __builtin_memcpy(more, __builtin_assume_aligned(&room[wave][u * 4 + k][i * 8], 16), 32);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) out[e] += scale * more[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) results[u].v[e] = (T)out[e];
+      }
+      if (more_cols) read_base(at + 128, t);  // before the writes, which a wait for later loads would wait for too
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t row = t * 16 + u * 4;
+        to.write(results[u], row * a.features + at, k * a.features + i * 8, row + k < rows ? count(at) : 0);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
 // ---- outer -------------------------------------------------------------------------------------------
 
 // A workgroup has 128 columns, 64 ranks at most and an adapter's rows in one split; its waves take 32 rows in turn and
@@ -737,6 +866,10 @@ __device__ __forceinline__ void turn(const Turn& a) {
   extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_##name(Expand a) {           \
     expand<T, rank, tiles, odd>(a);                                                                                \
   }
+#define MO_EXPAND_TALL(T, t, rank)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_tall(Expand a) {             \
+    expand_tall<T, rank>(a);                                                                                       \
+  }
 #define MO_OUTER(T, t, ranks)                                                                                      \
   extern "C" __global__ __launch_bounds__(256, 2) void mo_adapters_outer_##t##_##ranks(Outer a) {                     \
     outer_sides<T, ranks, false>(a);                                                                               \
@@ -760,12 +893,13 @@ __device__ __forceinline__ void turn(const Turn& a) {
   MO_EXPAND(T, t, 16, 2, false, 2)                                                                                 \
   MO_EXPAND(T, t, 16, 1, true, odd)                                                                                \
   MO_EXPAND(T, t, 32, 1, false, 1)                                                                                 \
-  MO_EXPAND(T, t, 32, 2, false, 2)                                                                                 \
+  MO_EXPAND_TALL(T, t, 32)                                                                                         \
   MO_EXPAND(T, t, 32, 1, true, odd)                                                                                \
   MO_EXPAND(T, t, 64, 1, false, 1)                                                                                 \
-  MO_EXPAND(T, t, 64, 2, false, 2)                                                                                 \
+  MO_EXPAND_TALL(T, t, 64)                                                                                         \
   MO_EXPAND(T, t, 64, 1, true, odd)                                                                                \
   MO_EXPAND(T, t, 128, 1, false, 1)                                                                                \
+  MO_EXPAND_TALL(T, t, 128)                                                                                        \
   MO_EXPAND(T, t, 128, 1, true, odd)                                                                               \
   MO_OUTER(T, t, 1)                                                                                                \
   MO_OUTER(T, t, 2)                                                                                                \
