@@ -5,7 +5,7 @@
 
 namespace mo_block {
 
-constexpr uint32_t kMaxDim = 16384;  // values a row of a norm: 1024 lanes of 16
+constexpr uint32_t kMaxDim = 16384;  // values a row of a norm: 512 lanes of 32
 
 // Division of a number under 2^31 by a fixed one: (n + n m / 2^32) >> s (mo_layout.h makes m and s).
 struct Divisor {

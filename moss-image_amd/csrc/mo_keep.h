@@ -115,10 +115,12 @@ struct Window {
       Words words[sizeof(Eight<T>) / 16];
     };
     const All all = __builtin_bit_cast(All, v);
-    const uint32_t offset = n ? own * (uint32_t)sizeof(T) : kNowhere;
+    // No scalar offset: with one, the compiler lets the next instruction overwrite the registers that a 16-byte store has
+    // yet to read (it counts that case as safe), and single values came out as addresses here.
+    const uint32_t offset = (n ? own * (uint32_t)sizeof(T) : kNowhere) + shared * (uint32_t)sizeof(T);
 #pragma unroll
     for (uint32_t i = 0; i < sizeof(Eight<T>) / 16; ++i)
-      __builtin_amdgcn_raw_buffer_store_b128(all.words[i], buffer, offset + i * 16, shared * (uint32_t)sizeof(T), 0);
+      __builtin_amdgcn_raw_buffer_store_b128(all.words[i], buffer, offset + i * 16, 0, 0);
   }
 };
 // The same of a type known at run time (MO_DTYPE_*).

@@ -39,7 +39,7 @@ bool odd(const mo_norm_call& c) {
 Plan plan_of(const mo_norm_call& c, bool backward) {
   Plan p = {};
   const uint64_t held = div_up(c.dim, 8);
-  p.iter = held > 1024 ? 2 : 1;
+  p.iter = held > 1024 ? 4 : held > 512 ? 2 : 1;
   p.lanes = (uint32_t)div_up(div_up(held, p.iter), 64) * 64;
   p.per = p.lanes == 64 ? 4 : 1;
   // forward: enough workgroups for several on every CU; backward: each leaves sums of dim values, so fewer
@@ -128,18 +128,18 @@ int run(const mo_norm_call* c, bool backward, uint64_t workspace, uint64_t bytes
     return std::string("mo_norm_") + (backward ? "backward_" : "forward_") + (!eights ? "" : backward ? "kept_" : "keep_") +
            kTypeNames[c->dtype] + "_" + std::to_string(p.iter) + (singly ? "_odd" : "");
   };
-  const int id = ((backward * 2 + eights) * 3 + (int)c->dtype) * 4 + (p.iter - 1) * 2 + singly;
+  const int id = ((backward * 2 + eights) * 3 + (int)c->dtype) * 6 + p.iter / 2 * 2 + singly;
   hipFunction_t kernel = nullptr;
   if (int rc = kernels().get(id, name, &kernel)) return rc;
   void* params[] = {&a};
   if (int rc = mo::launch(kernel, (uint32_t)div_up(p.groups, p.per), 1, 1, p.lanes * p.per, stream, params, "norm launch"))
     return rc;
   if (!a.partial) return 0;
-  if (int rc = kernels().get(48, [] { return "mo_norm_sums"; }, &kernel)) return rc;
+  if (int rc = kernels().get(72, [] { return "mo_norm_sums"; }, &kernel)) return rc;
   if (int rc = mo::launch(kernel, (c->dim + 31) / 32, c->samples ? c->samples : 1, 1, 1024, stream, params, "norm sums launch"))
     return rc;
   if (!a.sample_sums) return 0;
-  if (int rc = kernels().get(49, [] { return "mo_norm_sample_sums"; }, &kernel)) return rc;
+  if (int rc = kernels().get(73, [] { return "mo_norm_sample_sums"; }, &kernel)) return rc;
   return mo::launch(kernel, (c->dim + 255) / 256, 1, 1, 256, stream, params, "norm sums launch");
 }
 

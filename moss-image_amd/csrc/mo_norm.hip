@@ -8,8 +8,8 @@
 // (the reference's block: RMSNorm model.py:154-172, modulated :291-314.)
 //
 // All arithmetic is fp32 and each result is rounded once. The mean is taken first and the squares around it, so that
-// a row far from zero loses nothing. Bound by memory: a row is read once, held in registers by up to 1024 lanes of 8
-// or 16 values, and the forward pass can write it in 8 bits on the way, which the backward pass reads in place
+// a row far from zero loses nothing. Bound by memory: a row is read once, held in registers by up to 512 lanes of 8
+// to 32 values, and the forward pass can write it in 8 bits on the way, which the backward pass reads in place
 // of it. P and Q stay in registers over a workgroup's rows; what a workgroup has of a sample is stored when its rows of
 // the sample end, at slot (workgroup + sample), which no other pair has, and added up in that order.
 #include <hip/hip_runtime.h>
@@ -115,7 +115,8 @@ __device__ __forceinline__ void vectors(float (&to)[kIter][8], const NormArgs& a
 }
 
 // Rows one after the other that a batch takes: their sums cross the waves together, and a batch's rows are read while
-// the one before is worked on.
+// the one before is worked on. (Two batches ahead take registers for which a workgroup less fits on a CU: a backward pass
+// through 8 bits took 107 us where this takes 71.)
 template <int kIter>
 constexpr int kBatch = kIter == 1 ? 2 : 1;
 
@@ -127,7 +128,10 @@ struct Walk {
     find(a, most);
   }
   __device__ __forceinline__ void find(const NormArgs& a, uint32_t most) {
-    if (row >= end) return;
+    if (row >= end) {
+      sample = kNone, count = 0;
+      return;
+    }
     sample = __builtin_amdgcn_readfirstlane(sample_of(a, row, until));
     take(most);
   }
@@ -137,8 +141,7 @@ struct Walk {
   }
   __device__ __forceinline__ void next(const NormArgs& a, uint32_t most) {
     row += count;
-    if (row >= end) return;
-    if ((int64_t)row >= until)
+    if ((int64_t)row >= until || row >= end)
       find(a, most);
     else
       take(most);
@@ -155,28 +158,43 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
   const float inv_dim = 1.0f / (float)a.dim;
   Walk now(a, (blockIdx.x * a.per + side) * a.chunk, kRows);
   if (now.row >= now.end) return;
-  Eight<T> raw[kRows][kIter];
-  auto read = [&](const Walk& w) {
+  struct Raw {
+    Eight<T> x[kRows][kIter];
+  };
+  // rows that are none are read from and written to windows of no length: branches around memory instructions would
+  // have every wait be for all of them
+  auto read = [&](Raw& raw, const Walk& w) {
 #pragma unroll
     for (uint32_t i = 0; i < kRows; ++i) {
-      const uint32_t row = w.row + min(i, w.count - 1);
-      const Window<T, kOdd> x((const T*)a.x + row * a.x_stride, a.dim);
+      const bool live = i < w.count;
+      const uint32_t row = live ? w.row + i : 0;
+      const Window<T, kOdd> x((const T*)a.x + row * a.x_stride, live ? a.dim : 0);
 #pragma unroll
       for (int k = 0; k < kIter; ++k) {
         const Place p(a, lane, k);
-        raw[i][k] = x.read(0, p.at, p.n);
+        raw.x[i][k] = x.read(0, p.at, live ? p.n : 0);
       }
     }
   };
-  read(now);
-  float weight[kIter][8], bias[kIter][8], factor[kIter][8], shift[kIter][8];
-  vectors<kOdd, kIter>(weight, a, lane, a.weight, 0, a.weight_kind, 1.0f);
-  vectors<kOdd, kIter>(bias, a, lane, a.bias, 0, a.weight_kind, 0.0f);
+  Raw raw;
+  read(raw, now);
+  float gain[kIter][8], level[kIter][8];  // w (1 + scale), b (1 + scale) + shift
   bool fresh = true;
   while (true) {
-    if (fresh && now.sample != kNone) {
-      vectors<kOdd, kIter>(factor, a, lane, a.scale, now.sample * a.scale_stride, a.scale_kind, 0.0f);
-      vectors<kOdd, kIter>(shift, a, lane, a.shift, now.sample * a.shift_stride, a.scale_kind, 0.0f);
+    if (fresh) {
+      const bool none = now.sample == kNone;
+      float factor[kIter][8], shift[kIter][8];
+      vectors<kOdd, kIter>(gain, a, lane, a.weight, 0, a.weight_kind, 1.0f);
+      vectors<kOdd, kIter>(level, a, lane, a.bias, 0, a.weight_kind, 0.0f);
+      vectors<kOdd, kIter>(factor, a, lane, none ? nullptr : a.scale, now.sample * a.scale_stride, a.scale_kind, 0.0f);
+      vectors<kOdd, kIter>(shift, a, lane, none ? nullptr : a.shift, now.sample * a.shift_stride, a.scale_kind, 0.0f);
+#pragma unroll
+      for (int k = 0; k < kIter; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          gain[k][e] += gain[k][e] * factor[k][e];
+          level[k][e] += level[k][e] * factor[k][e] + shift[k][e];
+        }
     }
     float x[kRows][kIter][8], sum[kRows], mean[kRows];
     uint2 kept[kRows][kIter];
@@ -186,7 +204,7 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
       sum[i] = mean[i] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kIter; ++k) {
-        widen(x[i][k], raw[i][k]);
+        widen(x[i][k], raw.x[i][k]);
         if (kKeep) kept[i][k] = encode<T>(x[i][k], exponent[i][k]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[i] += x[i][k][e];
@@ -195,7 +213,7 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
     // before this batch's writes: a wait for later loads would wait for those too
     Walk then = now;
     then.next(a, kRows);
-    if (then.row < then.end) read(then);
+    read(raw, then);
     if (a.layer) {
       sum_row(sum, waves, room, turn);
 #pragma unroll
@@ -207,9 +225,11 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
 #pragma unroll
       for (int k = 0; k < kIter; ++k) {
         const Place p(a, lane, k);
+        const float here = p.n ? mean[i] : 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[i][k][e] = (kOdd ? (uint32_t)e < p.n : p.n != 0) ? x[i][k][e] - mean[i] : 0.0f;
+          // what is not in the row is zero already, and stays it
+          x[i][k][e] -= kOdd ? ((uint32_t)e < p.n ? mean[i] : 0.0f) : here;
           sum[i] += x[i][k][e] * x[i][k][e];
         }
       }
@@ -217,34 +237,35 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
     sum_row(sum, waves, room, turn);
 #pragma unroll
     for (uint32_t i = 0; i < kRows; ++i) {
-      if (i >= now.count) continue;
-      const uint32_t row = now.row + i;
+      const bool live = i < now.count;
+      const uint32_t row = live ? now.row + i : 0, pitch = a.groups * kGroup;
       const float r = rsqrtf(sum[i] * inv_dim + a.eps);
-      if (a.stats && lane == 0) {
-        a.stats[2 * (uint64_t)row] = mean[i];
-        a.stats[2 * (uint64_t)row + 1] = r;
-      }
-      const Window<T, kOdd> out((const T*)a.out + (uint64_t)row * a.dim, a.dim);
+      const Window<float, false> stats(a.stats + 2 * (uint64_t)row, live && a.stats ? 2 : 0);
+      typedef uint32_t Pair __attribute__((ext_vector_type(2)));
+      __builtin_amdgcn_raw_buffer_store_b64(Pair{__builtin_bit_cast(uint32_t, mean[i]), __builtin_bit_cast(uint32_t, r)}, stats.buffer,
+                                            lane == 0 ? 0 : kNowhere, 0, 0);
+      const Window<T, kOdd> out((const T*)a.out + (uint64_t)row * a.dim, live ? a.dim : 0);
+      const Window<int8_t, false> values(a.kept + (uint64_t)row * pitch, kKeep && live ? pitch : 0);
+      const Window<uint8_t, false> exponents(a.kept_exponents + (uint64_t)row * a.groups, kKeep && live ? a.groups : 0);
 #pragma unroll
       for (int k = 0; k < kIter; ++k) {
         const Place p(a, lane, k);
         Eight<T> result;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float v = x[i][k][e] * r * weight[k][e] + bias[k][e];
-          v = now.sample == kNone ? 0.0f : v + v * factor[k][e] + shift[k][e];
-          result.v[e] = (T)v;
+          const float v = x[i][k][e] * r * gain[k][e] + level[k][e];
+          result.v[e] = (T)(now.sample == kNone ? 0.0f : v);
         }
-        out.write(result, 0, p.at, p.n);
-        if (kKeep && p.at < a.groups * kGroup) {
-          *(uint2*)(a.kept + (uint64_t)row * a.groups * kGroup + p.at) = kept[i][k];
-          if (lane % 4 == 0) a.kept_exponents[(uint64_t)row * a.groups + p.at / kGroup] = (uint8_t)exponent[i][k];
+        out.write(result, 0, p.at, live ? p.n : 0);
+        if (kKeep) {
+          __builtin_amdgcn_raw_buffer_store_b64(Pair{kept[i][k].x, kept[i][k].y}, values.buffer, p.at, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b8((uint8_t)exponent[i][k], exponents.buffer, lane % 4 == 0 ? p.at / kGroup : kNowhere, 0, 0);
         }
       }
     }
-    if (then.row >= then.end) return;
     fresh = then.sample != now.sample;
     now = then;
+    if (now.row >= now.end) return;
   }
 }
 
@@ -258,34 +279,40 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
   const float inv_dim = 1.0f / (float)a.dim;
   Walk now(a, group * a.chunk, kRows);
   if (now.row >= now.end) return;
-  Eight<T> raw_x[kKept ? 1 : kRows][kIter], raw_g[kRows][kIter];
-  uint2 values[kKept ? kRows : 1][kIter];
-  uint32_t exponents[kKept ? kRows : 1][kIter];
-  float2 stats[kRows];
-  auto read = [&](const Walk& w) {
+  struct Raw {
+    Eight<T> x[kKept ? 1 : kRows][kIter], g[kRows][kIter];
+    uint2 values[kKept ? kRows : 1][kIter];
+    uint32_t exponents[kKept ? kRows : 1][kIter];
+    float2 stats[kRows];
+  };
+  auto read = [&](Raw& raw, const Walk& w) {  // without branches, as in the forward pass
 #pragma unroll
     for (uint32_t i = 0; i < kRows; ++i) {
-      const uint32_t row = w.row + min(i, w.count - 1), pitch = a.groups * kGroup;
-      const Window<T, kOdd> x((const T*)a.x + row * a.x_stride, a.dim), g((const T*)a.grad + row * a.grad_stride, a.dim);
-      const Window<int8_t, false> q((const int8_t*)a.x + (uint64_t)row * pitch, pitch);
-      const Window<uint8_t, false> exponent(a.x_exponents + (uint64_t)row * a.groups, a.groups);
-      stats[i] = ((const float2*)a.stats)[row];
+      const bool live = i < w.count;
+      const uint32_t row = live ? w.row + i : 0, pitch = a.groups * kGroup;
+      const Window<T, kOdd> x((const T*)a.x + row * a.x_stride, live ? a.dim : 0);
+      const Window<T, kOdd> g((const T*)a.grad + row * a.grad_stride, live ? a.dim : 0);
+      const Window<int8_t, false> q((const int8_t*)a.x + (uint64_t)row * pitch, live ? pitch : 0);
+      const Window<uint8_t, false> exponent(a.x_exponents + (uint64_t)row * a.groups, live ? a.groups : 0);
+      raw.stats[i] = ((const float2*)a.stats)[row];
+      if (!live) raw.stats[i] = float2{0.0f, 0.0f};  // and zeros for what is read: nothing for any sum
 #pragma unroll
       for (int k = 0; k < kIter; ++k) {
         const Place p(a, lane, k);
         if (kKept) {
           typedef uint32_t Pair __attribute__((ext_vector_type(2)));
           const Pair pair = __builtin_amdgcn_raw_buffer_load_b64(q.buffer, p.n ? p.at : kNowhere, 0, 0);
-          values[i][k] = uint2{pair.x, pair.y};
-          exponents[i][k] = __builtin_amdgcn_raw_buffer_load_b8(exponent.buffer, p.n ? p.at / kGroup : kNowhere, 0, 0);
+          raw.values[i][k] = uint2{pair.x, pair.y};
+          raw.exponents[i][k] = __builtin_amdgcn_raw_buffer_load_b8(exponent.buffer, p.n ? p.at / kGroup : kNowhere, 0, 0);
         } else {
-          raw_x[i][k] = x.read(0, p.at, p.n);
+          raw.x[i][k] = x.read(0, p.at, live ? p.n : 0);
         }
-        raw_g[i][k] = g.read(0, p.at, p.n);
+        raw.g[i][k] = g.read(0, p.at, live ? p.n : 0);
       }
     }
   };
-  read(now);
+  Raw raw;
+  read(raw, now);
   float gain[kIter][8];  // (1 + scale) w
   float along[kIter][8], plain[kIter][8];  // P and Q
   auto flush = [&](uint32_t sample) {
@@ -317,25 +344,24 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
     float n[kRows][kIter][8], h[kRows][kIter][8], r[kRows], sums[2 * kRows];
 #pragma unroll
     for (uint32_t i = 0; i < kRows; ++i) {
-      const bool live = i < now.count;
-      const float mean = stats[i].x;
-      r[i] = stats[i].y;
+      const float mean = raw.stats[i].x;
+      r[i] = raw.stats[i].y;
       sums[2 * i] = sums[2 * i + 1] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kIter; ++k) {
         const Place p(a, lane, k);
         float g[8];
         if (kKept)
-          decode(n[i][k], values[i][k], exponents[i][k]);
+          decode(n[i][k], raw.values[i][k], raw.exponents[i][k]);
         else
-          widen(n[i][k], raw_x[i][k]);
-        widen(g, raw_g[i][k]);
+          widen(n[i][k], raw.x[i][k]);
+        widen(g, raw.g[i][k]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          n[i][k][e] = (kOdd ? (uint32_t)e < p.n : p.n != 0) ? (n[i][k][e] - mean) * r[i] : 0.0f;
+          n[i][k][e] = (n[i][k][e] - mean) * r[i];  // past the row's end g is zero
           h[i][k][e] = g[e] * gain[k][e];
-          along[k][e] += live ? g[e] * n[i][k][e] : 0.0f;
-          plain[k][e] += live ? g[e] : 0.0f;
+          along[k][e] += g[e] * n[i][k][e];
+          plain[k][e] += g[e];
           sums[2 * i] += h[i][k][e] * n[i][k][e];
           sums[2 * i + 1] += h[i][k][e];
         }
@@ -344,13 +370,13 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
     // before this batch's writes: a wait for later loads would wait for those too
     Walk then = now;
     then.next(a, kRows);
-    if (then.row < then.end) read(then);
+    read(raw, then);
     sum_row(sums, waves, room, turn);
 #pragma unroll
     for (uint32_t i = 0; i < kRows; ++i) {
-      if (i >= now.count) continue;
+      const bool live = i < now.count;
       const float mean_along = sums[2 * i] * inv_dim, mean_plain = a.layer ? sums[2 * i + 1] * inv_dim : 0.0f;
-      const Window<T, kOdd> out((const T*)a.out + (uint64_t)(now.row + i) * a.dim, a.dim);
+      const Window<T, kOdd> out((const T*)a.out + (uint64_t)(live ? now.row + i : 0) * a.dim, live ? a.dim : 0);
 #pragma unroll
       for (int k = 0; k < kIter; ++k) {
         const Place p(a, lane, k);
@@ -358,36 +384,38 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           result.v[e] = (T)(now.sample == kNone ? 0.0f : r[i] * (h[i][k][e] - mean_plain - n[i][k][e] * mean_along));
-        out.write(result, 0, p.at, p.n);
+        out.write(result, 0, p.at, live ? p.n : 0);
       }
     }
-    if (then.row >= then.end) break;
-    fresh = then.sample != now.sample;
-    if (fresh) flush(now.sample);
+    const bool done = then.row >= then.end;
+    fresh = !done && then.sample != now.sample;
+    if (done || fresh) flush(now.sample);
     now = then;
+    if (now.row >= now.end) return;
   }
-  flush(now.sample);
 }
 
 // Names: type, times a lane holds 8 values; "odd": a dim that is no multiple of eight.
 #define MO_NORM(T, t, k, odd, name)                                                                          \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_forward_##t##_##name(NormArgs a) {              \
+  extern "C" __global__ __launch_bounds__(512) void mo_norm_forward_##t##_##name(NormArgs a) {              \
     forward<T, k, false, odd>(a);                                                                            \
   }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_forward_keep_##t##_##name(NormArgs a) {         \
+  extern "C" __global__ __launch_bounds__(512) void mo_norm_forward_keep_##t##_##name(NormArgs a) {         \
     forward<T, k, true, odd>(a);                                                                             \
   }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_backward_##t##_##name(NormArgs a) {             \
+  extern "C" __global__ __launch_bounds__(512) void mo_norm_backward_##t##_##name(NormArgs a) {             \
     backward<T, k, false, odd>(a);                                                                           \
   }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(1024) void mo_norm_backward_kept_##t##_##name(NormArgs a) {        \
+  extern "C" __global__ __launch_bounds__(512) void mo_norm_backward_kept_##t##_##name(NormArgs a) {        \
     backward<T, k, true, odd>(a);                                                                            \
   }
 #define MO_NORMS(T, t)           \
   MO_NORM(T, t, 1, false, 1)     \
   MO_NORM(T, t, 2, false, 2)     \
+  MO_NORM(T, t, 4, false, 4)     \
   MO_NORM(T, t, 1, true, 1_odd)  \
-  MO_NORM(T, t, 2, true, 2_odd)
+  MO_NORM(T, t, 2, true, 2_odd)  \
+  MO_NORM(T, t, 4, true, 4_odd)
 MO_NORMS(_Float16, f16)
 MO_NORMS(__bf16, bf16)
 MO_NORMS(float, f32)

@@ -111,6 +111,24 @@ def test_requests(cu, index, rank, dtype) -> None:
         Case(50, 136, 104, rank, dtype, count=3, cu=cu, index=index).run(keep)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 64, 72, 128])
+def test_long_requests(rank, dtype) -> None:
+    """Tiles of 128 rows that share the weight, splits of the features, borders inside tiles."""
+
+    for keep in (False, True):
+        Case(4100, 4104, 4104, rank, dtype, count=2, cu=[3, 1500, 1500, 4000, 4090], index=[1, 0, 0, 1], add=keep).run(keep)
+    Case(1100, 72, 2056, rank, dtype).run()
+
+
+def test_the_same_in_one_launch_a_kernel_of_each_form() -> None:
+    """Rows that are no multiple of anything, around the sizes where the form of a kernel changes."""
+
+    for rows in (1023, 1024, 1025):
+        for rank in (16, 40):
+            Case(rows, 264, 1032, rank, torch.bfloat16, count=3, cu=[0, 300, 900, rows - 1], index=[2, 0, 1]).run()
+
+
 def test_requests_by_batch() -> None:
     for dtype in DTYPES:
         Case(60, 72, 88, 8, dtype, count=4, batch=4).run()
