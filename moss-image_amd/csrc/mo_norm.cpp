@@ -136,7 +136,7 @@ int run(const mo_norm_call* c, bool backward, uint64_t workspace, uint64_t bytes
     return rc;
   if (!a.partial) return 0;
   if (int rc = kernels().get(72, [] { return "mo_norm_sums"; }, &kernel)) return rc;
-  if (int rc = mo::launch(kernel, (c->dim + 31) / 32, c->samples ? c->samples : 1, 1, 1024, stream, params, "norm sums launch"))
+  if (int rc = mo::launch(kernel, (c->dim + 15) / 16, c->samples ? c->samples : 1, 1, 1024, stream, params, "norm sums launch"))
     return rc;
   if (!a.sample_sums) return 0;
   if (int rc = kernels().get(73, [] { return "mo_norm_sample_sums"; }, &kernel)) return rc;

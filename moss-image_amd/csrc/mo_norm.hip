@@ -425,11 +425,12 @@ __device__ __forceinline__ float value_kind(const void* base, uint64_t at, uint3
                                                           : (float)((const _Float16*)base)[at];
 }
 
-// A sample's sums over its workgroups for 32 columns: 32 runs of them side by side, then the runs, both in order.
+// A sample's sums over its workgroups for 16 columns: 64 runs of them side by side, then eight runs at a time, then the
+// eight, all in order.
 extern "C" __global__ __launch_bounds__(1024) void mo_norm_sums(NormArgs a) {
-  __shared__ float room[2][32][33];
-  const uint32_t column = threadIdx.x % 32, run = threadIdx.x / 32, sample = blockIdx.y;
-  const uint32_t at = blockIdx.x * 32 + column;
+  __shared__ float room[2][64][17];
+  const uint32_t column = threadIdx.x % 16, run = threadIdx.x / 16, sample = blockIdx.y;
+  const uint32_t at = blockIdx.x * 16 + column;
   int64_t low = 0, high = a.rows;
   if (a.scale || a.shift) {
     low = a.cu ? a.cu[sample] : (int64_t)sample * a.by_share.d;
@@ -441,7 +442,7 @@ extern "C" __global__ __launch_bounds__(1024) void mo_norm_sums(NormArgs a) {
   if (at < a.dim && low < high) {
     const uint32_t from = (uint32_t)low / a.chunk, to = (uint32_t)(high - 1) / a.chunk;
 #pragma unroll 8
-    for (uint32_t i = from + run; i <= to; i += 32) {
+    for (uint32_t i = from + run; i <= to; i += 64) {
       const float* p = a.partial + (uint64_t)(i + sample) * 2 * a.pitch + at;
       along += p[0];
       plain += p[a.pitch];
@@ -450,10 +451,20 @@ extern "C" __global__ __launch_bounds__(1024) void mo_norm_sums(NormArgs a) {
   room[0][run][column] = along;
   room[1][run][column] = plain;
   __syncthreads();
+  if (run < 16) {  // the first eight add up the one, the others the other
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += room[run / 8][run % 8 * 8 + i][column];
+    __builtin_amdgcn_wave_barrier();
+    room[run / 8][run % 8 * 8][column] = sum;
+  }
+  __syncthreads();
   if (run || at >= a.dim) return;
-  for (int i = 1; i < 32; ++i) {
-    along += room[0][i][column];
-    plain += room[1][i][column];
+  along = plain = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    along += room[0][i * 8][column];
+    plain += room[1][i * 8][column];
   }
   const uint64_t here = (uint64_t)sample * a.dim + at;
   if (a.scale_grad) {
