@@ -128,6 +128,17 @@ void share_rows(const mo_adapters_call& c, mo_adapters::Side* a, mo_adapters::Si
   a->splits = b->splits = (uint32_t)div_up(c.rows, a->span);
 }
 
+// Whether a forward pass runs in one launch, where every workgroup reads the adapter's whole a: up to 128 KB of it and
+// with no more workgroups than CUs. bfloat16, one launch and two in us: 16 rows with an adapter each, 16 ranks, 1024 x 1024
+// 9.7 and 11.7, 3072 x 3072 (98 KB) 11.9 and 12.4; 32 ranks of 3072 (196 KB) 15.1 and 13.3; 64 of 1024 (128 KB) 16.0 and 16.4;
+// 1333 rows, 16 ranks, 3072 x 3072 (252 workgroups) 14.9 and 16.2, 3072 x 8192 (672) 30.8 and 20.8. float32 of more than
+// 32 ranks has not the registers: 64 of 512 25.8 and 20.9. The host's time for a launch, some 5 us, is saved besides.
+bool is_few(const mo_adapters_call& c) {
+  const uint64_t tiles = div_up(c.rows, 16) + c.requests - 1, weight = (uint64_t)c.rank * c.in_features * kTypeBytes[c.dtype];
+  return !odd(c) && c.rank <= (c.dtype == MO_DTYPE_F32 ? 32 : 64) && weight <= (128u << 10) &&
+         tiles * div_up(c.out_features, 1024) <= 256;
+}
+
 // Where what a call needs for itself lies in its workspace.
 struct Room {
   uint64_t back, planes, turned_a, turned_b, turned_hidden, turned_back, da, db, bytes;  // offsets
@@ -142,6 +153,7 @@ Room room_of(const mo_adapters_call& c, bool backward) {
   const uint64_t between_bytes = c.rows * c.rank * 4, size = kTypeBytes[c.dtype];
   const uint64_t turned = round_up(c.rows, 32) * c.rank * 4;  // one fp32 or two bfloat16, in whole steps of 32 rows
   if (!backward) {
+    if (is_few(c)) return r;
     const ShrinkPlan p = shrink_plan(c, c.in_features);
     if (p.splits > 1) r.planes = take(p.splits * between_bytes);
     return r;
@@ -164,11 +176,11 @@ Room room_of(const mo_adapters_call& c, bool backward) {
 }
 
 // The kernels of one type: each with a size and a form, which make its name and its number.
-enum Kind { kShrink, kExpand, kOuter, kJoin, kTurn };
+enum Kind { kShrink, kExpand, kOuter, kJoin, kTurn, kFew };
 int start(const mo_adapters_call& c, Kind kind, uint32_t size, const char* form, uint64_t gx, uint64_t gy, uint64_t gz, void* args,
           uint64_t stream, uint32_t threads = 256) {
-  if (gx >= (1ull << 31) || gy >= (1u << 16) || gz > (1u << 16)) return mo::set_error(MO_E_INVALID, "too many values");
-  static const char* const names[] = {"shrink_", "expand_", "outer_", "join_", "turn_"};
+  if (gx >= (1ull << 31) || gy >= (1u << 16) || gz >= (1u << 16)) return mo::set_error(MO_E_INVALID, "too many values");
+  static const char* const names[] = {"shrink_", "expand_", "outer_", "join_", "turn_", "few_"};
   auto name = [&]() {
     std::string n = std::string("mo_adapters_") + names[kind] + kTypeNames[c.dtype];
     if (size) n += "_" + std::to_string(size);
@@ -176,10 +188,13 @@ int start(const mo_adapters_call& c, Kind kind, uint32_t size, const char* form,
     return n;
   };
   const int step = size >= 128 ? 7 : size >= 64 ? 6 : size >= 32 ? 5 : size >= 16 ? 4 : size >= 8 ? 3 : size >= 4 ? 2 : size >= 2 ? 1 : 0;
-  // sizes: up to 8 of a shrink and an outer, 16 to 128 of an expand; forms: "", "1", "2", "odd", "tall"
-  const int place = *form == 0 ? 0 : *form == '2' || *form == 't' ? 1 : *form == 'o' ? 2 : 0;
+  // sizes: up to 8 of a shrink and an outer, 16 to 128 of an expand; forms: "", "2", "odd", "tall"
+  const int place = *form == '2' || *form == 't' ? 1 : *form == 'o' ? 2 : 0;
   const int id = kind == kShrink ? step * 3 + place : kind == kExpand ? 12 + (step - 4) * 3 + place
-                 : kind == kOuter ? 24 + step * 3 + place : kind == kJoin ? 36 : 37;
+                 : kind == kOuter ? 24 + step * 3 + place
+                 : kind == kFew   ? 33 + step
+                 : kind == kJoin  ? 36
+                                  : 37;
   hipFunction_t kernel = nullptr;
   if (int rc = kernels().get((int)c.dtype * 40 + id, name, &kernel)) return rc;
   void* params[] = {args};
@@ -192,15 +207,14 @@ int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t s
   mo_adapters::Shrink a = {};
   a.by = by, a.x = (const void*)x, a.w = (const void*)w, a.to = (float*)to;
   a.x_stride = stride, a.features = features, a.span = p.span, a.scaled = scaled;
-  return start(c, kShrink, p.ranks, odd(c) ? "odd" : p.rows == 128 ? "tall" : "1",
-               p.slots, p.splits, 1, &a, stream, 512);
+  return start(c, kShrink, p.ranks, odd(c) ? "odd" : p.rows == 128 ? "tall" : "", p.slots, p.splits, 1, &a, stream, 512);
 }
 
 int expand(const mo_adapters_call& c, mo_adapters::Expand& a, uint64_t stream) {
   const ExpandPlan p = expand_plan(c, a.features);
   a.cols = p.cols;
-  return start(c, kExpand, p.rank, odd(c) ? "odd" : p.rows == 128 ? "tall" : p.rows == 32 ? "2" : "1",
-               p.slots, div_up(a.features, p.cols), 1, &a, stream);
+  return start(c, kExpand, p.rank, odd(c) ? "odd" : p.rows == 128 ? "tall" : p.rows == 32 ? "2" : "", p.slots,
+               div_up(a.features, p.cols), 1, &a, stream);
 }
 
 int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_t bytes, uint64_t stream) {
@@ -216,6 +230,15 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
   const uint64_t planes = workspace + room.planes;
   mo_adapters::Expand e = {};
   e.by = by;
+  if (!backward && is_few(c)) {
+    mo_adapters::Few f = {};
+    f.in.by = by, f.in.x = (const void*)c.x, f.in.w = (const void*)c.a, f.in.to = (float*)c.hidden;
+    f.in.x_stride = stride_of(c, c.x_stride, c.in_features), f.in.features = c.in_features;
+    f.out.v = (const void*)c.b, f.out.base = (const void*)c.result, f.out.to = (void*)c.y;
+    f.out.base_stride = stride_of(c, c.result_stride, c.out_features), f.out.features = c.out_features;
+    return start(c, kFew, c.rank <= 16 ? 1 : c.rank <= 32 ? 2 : 4, "", div_up(c.rows, 16) + c.requests + 1,
+                 div_up(c.out_features, 1024), 1, &f, stream, 512);
+  }
   if (!backward) {
     e.splits = shrink_plan(c, c.in_features).splits;
     const uint64_t to = e.splits > 1 ? planes : c.hidden;

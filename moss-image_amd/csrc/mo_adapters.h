@@ -46,6 +46,12 @@ struct Expand {
   uint32_t scaled;
 };
 
+// Both for a forward pass of few rows.
+struct Few {
+  Shrink in;
+  Expand out;
+};
+
 // One gradient of a weight: sum over an adapter's rows of narrow[row][j] wide[row][c].
 struct Side {
   const void* wide;          // [rows][cols], or 8-bit values [rows][groups * 32]

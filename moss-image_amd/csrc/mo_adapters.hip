@@ -169,29 +169,27 @@ __device__ __forceinline__ uint32_t adapter_of(const Requests& by, const Tile& t
 
 // ---- shrink ------------------------------------------------------------------------------------------
 
-// A workgroup has kTiles * 16 rows, all ranks and one split of the features; its eight waves take 128 features in turn and
+// A workgroup has 16 rows, all ranks and one split of the features; its eight waves take 128 features in turn and
 // add up through LDS. A wave reads 256 bytes of each row side by side (64 bytes a row, as the instructions want them, came
 // at 4.2 TB/s where this comes at 5.4) and turns them through its own part of LDS, eight values at a time; those of
 // row r lie at (place ^ r), so that neither writing nor reading meets a bank twice. The rows are the instruction's
 // columns, so a lane ends with four neighbouring ranks of a row. Nothing is loaded ahead: sixteen waves a CU are enough.
-template <class T, int kRanks, int kTiles, bool kOdd>
+template <class T, int kRanks, bool kOdd>
 __device__ __forceinline__ void shrink(const Shrink& a) {
   typedef Path<T> P;
-  constexpr uint32_t kRows = kTiles * 16, kPitch = kRanks * 16 + 4;
+  constexpr uint32_t kPitch = kRanks * 16 + 4;
   union Room {
-    Eight<T> stage[8][kRows][16];
-    float sums[8][kRows][kPitch];
+    Eight<T> stage[8][16][16];
+    float sums[8][16][kPitch];
     __device__ Room() {}
   };
   __shared__ Room room;
-  const Tile tile = tile_of<kRows>(a.by, blockIdx.x);
+  const Tile tile = tile_of<16>(a.by, blockIdx.x);
   if (tile.low >= tile.high) return;
   const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
-  f32x4 sum[kRanks][kTiles];
+  f32x4 sum[kRanks];
 #pragma unroll
-  for (int r = 0; r < kRanks; ++r)
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) sum[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int r = 0; r < kRanks; ++r) sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const uint32_t adapter = adapter_of(a.by, tile);
   if (adapter != kNone) {
     const uint32_t stride = (uint32_t)a.x_stride, rows = tile.high - tile.low;
@@ -199,11 +197,10 @@ __device__ __forceinline__ void shrink(const Shrink& a) {
     const Window<T, kOdd> w((const T*)a.w + (uint64_t)adapter * rank * a.features, rank * a.features);
     const uint32_t first = blockIdx.y * a.span, last = min(a.features, first + a.span);
     for (uint32_t at = first + wave * 128; at < last; at += 1024) {
-      Eight<T> xs[kTiles * 4];
-      Eight<T> ws[4][kRanks];
+      Eight<T> xs[4], ws[4][kRanks];
       const uint32_t n = at + i * 8 >= last ? 0 : min(8u, last - at - i * 8);
 #pragma unroll
-      for (uint32_t t = 0; t < kTiles * 4; ++t) xs[t] = x.read(t * 4 * stride + at, k * stride + i * 8, t * 4 + k < rows ? n : 0);
+      for (uint32_t t = 0; t < 4; ++t) xs[t] = x.read(t * 4 * stride + at, k * stride + i * 8, t * 4 + k < rows ? n : 0);
 #pragma unroll
       for (uint32_t u = 0; u < 4; ++u) {
         const uint32_t from = at + u * 32 + k * 8, m = from >= last ? 0 : min(8u, last - from);
@@ -212,24 +209,20 @@ __device__ __forceinline__ void shrink(const Shrink& a) {
           ws[u][r] = w.read(r * 16 * a.features + at + u * 32, i * a.features + k * 8, r * 16 + i < rank ? m : 0);
       }
 #pragma unroll
-      for (int t = 0; t < kTiles * 4; ++t) room.stage[wave][t * 4 + k][i ^ (t * 4 + k) % 16] = xs[t];
+      for (int t = 0; t < 4; ++t) room.stage[wave][t * 4 + k][i ^ (t * 4 + k)] = xs[t];
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 4; ++u) {
+        const typename P::Fragment f = P::of(room.stage[wave][i][(u * 4 + k) ^ i]);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const typename P::Fragment f = P::of(room.stage[wave][t * 16 + i][(u * 4 + k) ^ i]);
-#pragma unroll
-          for (int r = 0; r < kRanks; ++r) P::multiply(sum[r][t], P::of(ws[u][r]), f);
-        }
+        for (int r = 0; r < kRanks; ++r) P::multiply(sum[r], P::of(ws[u][r]), f);
+      }
       __builtin_amdgcn_wave_barrier();
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kRanks; ++r)
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) *(f32x4*)&room.sums[wave][t * 16 + i][r * 16 + k * 4] = sum[r][t];
+  for (int r = 0; r < kRanks; ++r) *(f32x4*)&room.sums[wave][i][r * 16 + k * 4] = sum[r];
   __syncthreads();
   const float scale = a.scaled && adapter != kNone ? scale_of(a.by, adapter) : 1.0f;
   float* to = a.to + ((uint64_t)blockIdx.y * a.by.rows + tile.low) * rank;
@@ -596,6 +589,135 @@ __device__ __forceinline__ void expand_tall(const Expand& a) {
   }
 }
 
+// A forward pass of few rows in one launch: a workgroup has 16 rows and 1024 columns, 128 a wave, and makes its own h over
+// all features, its waves by turns of 128, added up in one order. What it reads of b and the base arrives meanwhile, and a
+// comes from the caches after its first reading. Bound by the way to memory and back: 16 rows of 3072 with 16 adapters of
+// 16 ranks in bfloat16 8.4 us (3.4 MB), in two launches 9.4.
+template <class T, int kRanks>
+__device__ __forceinline__ void few(const Few& f) {
+  typedef Path<T> P;
+  const Shrink& a = f.in;
+  const Expand& b = f.out;
+  constexpr uint32_t kRank = kRanks * 16, kPitch = kRank + 4;
+  constexpr bool kBeside = kRanks == 1 && P::kParts == 2;
+  constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 1 : P::kParts;
+  union Room {
+    Eight<T> stage[8][16][16];
+    float sums[8][16][kPitch];
+    float out[8][16][132];
+    __device__ Room() {}
+  };
+  __shared__ Room room;
+  __shared__ float h[16][kPitch];
+  const Tile tile = tile_of<16>(a.by, blockIdx.x);
+  if (tile.low >= tile.high) return;
+  const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
+  const uint32_t rows = tile.high - tile.low, x_stride = (uint32_t)a.x_stride, stride = (uint32_t)b.base_stride;
+  const uint32_t at = blockIdx.y * 1024 + wave * 128, count = at + i * 8 < b.features ? 8 : 0;
+  const Window<T, false> base((const T*)b.base + tile.low * b.base_stride, (rows - 1) * stride + b.features);
+  const Window<T, false> to((const T*)b.to + (uint64_t)tile.low * b.features, rows * b.features);
+  Eight<T> in[4];
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) in[u] = base.read(u * 4 * stride + at, k * stride + i * 8, u * 4 + k < rows ? count : 0);
+  const uint32_t adapter = adapter_of(a.by, tile);
+  const bool has = adapter != kNone;
+  Eight<T> vs[8][kSteps];
+  f32x4 sum[kRanks];
+#pragma unroll
+  for (int r = 0; r < kRanks; ++r) sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (has) {
+    const Window<T, false> v((const T*)b.v + (uint64_t)adapter * b.features * rank, b.features * rank);
+#pragma unroll
+    for (uint32_t c = 0; c < 8; ++c)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8;
+        vs[c][s] = v.read((at + c * 16) * rank, i * rank + j, j < rank && at + c * 16 + i < b.features ? 8 : 0);
+      }
+    const Window<T, false> x((const T*)a.x + tile.low * a.x_stride, (rows - 1) * x_stride + a.features);
+    const Window<T, false> w((const T*)a.w + (uint64_t)adapter * rank * a.features, rank * a.features);
+    for (uint32_t from = wave * 128; from < a.features; from += 1024) {
+      Eight<T> xs[4], ws[4][kRanks];
+#pragma unroll
+      for (uint32_t t = 0; t < 4; ++t)
+        xs[t] = x.read(t * 4 * x_stride + from, k * x_stride + i * 8, t * 4 + k < rows && from + i * 8 < a.features ? 8 : 0);
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+        for (uint32_t r = 0; r < kRanks; ++r)
+          ws[u][r] = w.read(r * 16 * a.features + from + u * 32, i * a.features + k * 8,
+                            r * 16 + i < rank && from + u * 32 + k * 8 < a.features ? 8 : 0);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) room.stage[wave][t * 4 + k][i ^ (t * 4 + k)] = xs[t];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const typename P::Fragment of = P::of(room.stage[wave][i][(u * 4 + k) ^ i]);
+#pragma unroll
+        for (int r = 0; r < kRanks; ++r) P::multiply(sum[r], P::of(ws[u][r]), of);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRanks; ++r) *(f32x4*)&room.sums[wave][i][r * 16 + k * 4] = sum[r];
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < 16 * kRank; e += 512) {
+    const uint32_t row = e / kRank, j = e % kRank;
+    float total = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) total += room.sums[u][row][j];
+    h[row][j] = total;
+    if (blockIdx.y == 0 && row < rows && j < rank) a.to[(uint64_t)(tile.low + row) * rank + j] = total;
+  }
+  __syncthreads();
+  if (has) {
+    typename P::Fragment hs[kParts][kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = j < kRank ? h[i][j + e] : 0.0f;
+      if (kBeside) {
+        const typename P::Fragment low = P::part(v, 1);
+        hs[0][s] = P::part(v, 0);
+        if (k >= 2) hs[0][s] = low;
+      } else {
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) hs[p][s] = P::part(v, p);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      f32x4 part = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) P::multiply(part, P::of(vs[c][s]), hs[p][s]);
+      *(f32x4*)&room.out[wave][i][c * 16 + k * 4] = part;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  const float scale = has ? scale_of(a.by, adapter) : 0.0f;
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) {
+    float out[8];
+    widen(out, in[u]);
+    if (has) {
+      float more[8];
+      __builtin_memcpy(more, __builtin_assume_aligned(&room.out[wave][u * 4 + k][i * 8], 16), 32);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] += scale * more[e];
+    }
+    Eight<T> result;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) result.v[e] = (T)out[e];
+    to.write(result, u * 4 * b.features + at, k * b.features + i * 8, u * 4 + k < rows ? count : 0);
+  }
+}
+
 // ---- outer -------------------------------------------------------------------------------------------
 
 // A workgroup has 128 columns, 64 ranks at most and an adapter's rows in one split; its waves take 32 rows in turn and
@@ -854,22 +976,30 @@ __device__ __forceinline__ void turn(const Turn& a) {
 }
 
 // Names: type, ranks, tiles of 16 rows; "odd": features or a rank that are no multiples of eight.
-#define MO_SHRINK(T, t, ranks, tiles, odd, name)                                                                   \
-  extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks##_##name(Shrink a) {          \
-    shrink<T, ranks, tiles, odd>(a);                                                                               \
+#define MO_SHRINK(T, t, ranks)                                                                                     \
+  extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks(Shrink a) {                   \
+    shrink<T, ranks, false>(a);                                                                                    \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks##_odd(Shrink a) {             \
+    shrink<T, ranks, true>(a);                                                                                     \
   }
 #define MO_TALL(T, t, ranks)                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks##_tall(Shrink a) {            \
     shrink_tall<T, ranks>(a);                                                                                      \
   }
-#define MO_EXPAND(T, t, rank, tiles, odd, name)                                                                    \
-  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_##name(Expand a) {           \
-    expand<T, rank, tiles, odd>(a);                                                                                \
+#define MO_EXPAND(T, t, rank)                                                                                      \
+  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank(Expand a) {                    \
+    expand<T, rank, 1, false>(a);                                                                                  \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_odd(Expand a) {              \
+    expand<T, rank, 1, true>(a);                                                                                   \
   }
 #define MO_EXPAND_TALL(T, t, rank)                                                                                 \
   extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_tall(Expand a) {             \
     expand_tall<T, rank>(a);                                                                                       \
   }
+#define MO_FEW(T, t, ranks)                                                                                        \
+  extern "C" __global__ __launch_bounds__(512) void mo_adapters_few_##t##_##ranks(Few f) { few<T, ranks>(f); }
 #define MO_OUTER(T, t, ranks)                                                                                      \
   extern "C" __global__ __launch_bounds__(256, 2) void mo_adapters_outer_##t##_##ranks(Outer a) {                     \
     outer_sides<T, ranks, false>(a);                                                                               \
@@ -878,29 +1008,25 @@ __device__ __forceinline__ void turn(const Turn& a) {
     outer_sides<T, ranks, true>(a);                                                                                \
   }
 #define MO_ADAPTERS(T, t)                                                                                          \
-  MO_SHRINK(T, t, 1, 1, false, 1)                                                                                  \
-  MO_SHRINK(T, t, 2, 1, false, 1)                                                                                  \
-  MO_SHRINK(T, t, 4, 1, false, 1)                                                                                  \
-  MO_SHRINK(T, t, 8, 1, false, 1)                                                                                  \
-  MO_SHRINK(T, t, 1, 1, true, odd)                                                                                 \
-  MO_SHRINK(T, t, 2, 1, true, odd)                                                                                 \
-  MO_SHRINK(T, t, 4, 1, true, odd)                                                                                 \
-  MO_SHRINK(T, t, 8, 1, true, odd)                                                                                 \
+  MO_SHRINK(T, t, 1)                                                                                               \
+  MO_SHRINK(T, t, 2)                                                                                               \
+  MO_SHRINK(T, t, 4)                                                                                               \
+  MO_SHRINK(T, t, 8)                                                                                               \
   MO_TALL(T, t, 1)                                                                                                 \
   MO_TALL(T, t, 2)                                                                                                 \
   MO_TALL(T, t, 4)                                                                                                 \
-  MO_EXPAND(T, t, 16, 1, false, 1)                                                                                 \
-  MO_EXPAND(T, t, 16, 2, false, 2)                                                                                 \
-  MO_EXPAND(T, t, 16, 1, true, odd)                                                                                \
-  MO_EXPAND(T, t, 32, 1, false, 1)                                                                                 \
+  MO_EXPAND(T, t, 16)                                                                                              \
+  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_16_2(Expand a) {                      \
+    expand<T, 16, 2, false>(a);                                                                                    \
+  }                                                                                                                \
+  MO_EXPAND(T, t, 32)                                                                                              \
   MO_EXPAND_TALL(T, t, 32)                                                                                         \
-  MO_EXPAND(T, t, 32, 1, true, odd)                                                                                \
-  MO_EXPAND(T, t, 64, 1, false, 1)                                                                                 \
+  MO_EXPAND(T, t, 64)                                                                                              \
   MO_EXPAND_TALL(T, t, 64)                                                                                         \
-  MO_EXPAND(T, t, 64, 1, true, odd)                                                                                \
-  MO_EXPAND(T, t, 128, 1, false, 1)                                                                                \
+  MO_EXPAND(T, t, 128)                                                                                             \
   MO_EXPAND_TALL(T, t, 128)                                                                                        \
-  MO_EXPAND(T, t, 128, 1, true, odd)                                                                               \
+  MO_FEW(T, t, 1)                                                                                                  \
+  MO_FEW(T, t, 2)                                                                                                  \
   MO_OUTER(T, t, 1)                                                                                                \
   MO_OUTER(T, t, 2)                                                                                                \
   MO_OUTER(T, t, 4)                                                                                                \
@@ -909,6 +1035,8 @@ __device__ __forceinline__ void turn(const Turn& a) {
 MO_ADAPTERS(_Float16, f16)
 MO_ADAPTERS(__bf16, bf16)
 MO_ADAPTERS(float, f32)
+MO_FEW(_Float16, f16, 4)
+MO_FEW(__bf16, bf16, 4)
 MO_TALL(_Float16, f16, 8)
 MO_TALL(__bf16, bf16, 8)
 
