@@ -659,7 +659,7 @@ typedef struct mo_norm_call {
   uint64_t x_exponents;  /* backward: their exponents, or 0 */
   uint64_t grad;         /* backward: the output's gradient [rows][dim] */
   uint64_t out;          /* forward: the output; backward: the input's gradient */
-  uint64_t stats;        /* fp32 [rows][2]: mean and 1 / sqrt(..): written forward (or 0), read backward */
+  uint64_t stats;        /* fp32 [rows][2], 8-byte aligned: mean and 1 / sqrt(..): written forward (or 0), read backward */
   uint64_t weight, bias; /* [dim] of weight_dtype */
   uint64_t scale, shift; /* [samples][dim] of scale_dtype */
   uint64_t kept, kept_exponents; /* forward: x in 8 bits, as mo_keep_pack writes it */

@@ -82,7 +82,7 @@ int check(const mo_norm_call* c, bool backward) {
     if (p % kTypeBytes[c->weight_dtype]) return bad("misaligned weight");
   for (uint64_t p : {c->scale, c->shift, c->scale_grad, c->shift_grad})
     if (p % kTypeBytes[c->scale_dtype]) return bad("misaligned modulation");
-  if (c->stats % 4) return bad("misaligned statistics");
+  if (c->stats % 8) return bad("misaligned statistics");  // read in pairs
   if (!backward) {
     if ((c->kept != 0) != (c->kept_exponents != 0) || c->kept % 8) return bad("both the 8-bit values and their exponents");
     return 0;

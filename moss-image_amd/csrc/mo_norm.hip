@@ -395,7 +395,7 @@ __device__ __forceinline__ void backward(const NormArgs& a) {
   }
 }
 
-// Names: type, times a lane holds 8 values; "odd": a dim that is no multiple of eight.
+// Names: type, times a lane holds 8 values; "odd": a dim that is no multiple of eight, or rows off the 4-byte grid.
 #define MO_NORM(T, t, k, odd, name)                                                                          \
   extern "C" __global__ __launch_bounds__(512) void mo_norm_forward_##t##_##name(NormArgs a) {              \
     forward<T, k, false, odd>(a);                                                                            \

@@ -113,7 +113,10 @@ class _CheckpointFunction(torch.autograd.Function):
         ctx.places = [i for i, t in enumerate(others) if isinstance(t, torch.Tensor)]
         ctx.wanted = [t.requires_grad for t in others if isinstance(t, torch.Tensor)]
         ctx.save_for_backward(kept.values, kept.exponents, *(others[i] for i in ctx.places))
-        return function(tokens, *others)
+        out = function(tokens, *others)
+        if not isinstance(out, torch.Tensor):
+            raise TypeError("checkpoint_kept8 takes a function that returns one tensor.")
+        return out
 
     @staticmethod
     def backward(ctx, gradient):
@@ -144,10 +147,13 @@ def checkpoint_kept8(function, tokens: torch.Tensor, *others) -> torch.Tensor:
     the rest again from that: the result is the exact input's, the gradients are taken at what 8 bits keep of it.
 
     As with a reentrant checkpoint, the parameters inside get their gradients by accumulation (``backward()``, not
-    ``torch.autograd.grad``), and an input must want a gradient: the function's parameters alone are not seen."""
+    ``torch.autograd.grad``), and an input must want a gradient: the function's parameters alone are not seen. Not while a
+    graph is captured: the random numbers' state, which the second run starts from, cannot be read then."""
 
     if not torch.is_grad_enabled():
         return function(tokens, *others)
     if not any(isinstance(t, torch.Tensor) and t.requires_grad for t in (tokens, *others)):
         raise RuntimeError("checkpoint_kept8 needs an input that requires grad.")
+    if tokens.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("checkpoint_kept8 cannot be captured into a graph.")
     return _CheckpointFunction.apply(function, tokens, *others)

@@ -138,6 +138,7 @@ def _backward(grad, x, stats, weight, bias, kind, scale, shift, cu_seqlens, want
             return _backward(grad, x, stats, weight, bias, kind, scale, shift, cu, wanted)
     source = x.values if kept else rows(x, "norm rows")
     stats = stats.contiguous()
+    stats = stats.clone() if stats.data_ptr() % 8 else stats
     out = _like(grad)
     # the sums are as wide as their tensors; with no rows they are zero
     grads = [_like(t) if t is not None and w else None
