@@ -919,16 +919,28 @@ __device__ __forceinline__ void join(const Outer& a) {
   if (at >= size) return;
   const uint32_t n = (uint32_t)min((uint64_t)4, size - at);
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint64_t left = active; left; left &= left - 1) {
-    const float* from = side.planes + ((uint64_t)__builtin_ctzll(left) * a.by.adapters + adapter) * size + at;
-    if (n == 4) {
-      float more[4];
-      __builtin_memcpy(more, from, 16);
+  const uint64_t all = active;
+  uint64_t left = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(all >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)all);
+  while (left) {  // eight planes asked for at a time
+    float more[8][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += more[e];
-    } else {
-      for (uint32_t e = 0; e < n; ++e) sum[e] += from[e];
+    for (int u = 0; u < 8; ++u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) more[u][e] = 0.0f;
+      if (!left) continue;
+      const float* from = side.planes + ((uint64_t)__builtin_ctzll(left) * a.by.adapters + adapter) * size + at;
+      left &= left - 1;
+      if (n == 4)
+        __builtin_memcpy(more[u], from, 16);
+      else
+#pragma unroll
+        for (uint32_t e = 0; e < 3; ++e)
+          if (e < n) more[u][e] = from[e];
     }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += more[u][e];
   }
   const float scale = side.scaled ? scale_of(a.by, adapter) : 1.0f;
   T* to = (T*)side.to + adapter * size + at;
