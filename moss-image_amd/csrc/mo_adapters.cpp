@@ -13,8 +13,9 @@ using mo_adapters::Requests;
 const char* const kTypeNames[3] = {"f16", "bf16", "f32"};  // by MO_DTYPE_*
 constexpr uint32_t kTypeBytes[3] = {2, 2, 4};
 
-// Workgroups that a launch aims at: an expand has two or three on a CU at a time, and many rounds leave no CU waiting long.
-constexpr uint64_t kExpandGroups = 4096, kOuterGroups = 768;
+// Workgroups that a launch aims at: an expand has three on a CU at a time, and many rounds leave no CU waiting long (half or twice
+// as many: the same within 2 %).
+constexpr uint64_t kExpandGroups = 4096, kOuterGroups = 384;
 
 mo::Kernels& kernels() {
   static mo::Kernels k(mo_adapters_code);
@@ -75,9 +76,10 @@ bool odd(const mo_adapters_call& c) {
 }
 
 // Rows a tile and splits of the features of a shrink. Tiles of 128 rows, which share the weight, where they and the splits
-// make two workgroups for every CU; otherwise, and for short requests, whose other rows would be empty, tiles of 16.
-// Splits as long as all workgroups are on the GPU at once (past that, a few that come late cost as much as all
-// others), 512 features each at least for tiles of 128, 1024 for those of 16, and up to 16.
+// make a workgroup for every CU (tiles of 16 and of 128 in a call, us: 4608 rows of 16384, 16 ranks 60.4 and 47.6; 17792 rows of 8192,
+// 64 ranks 222 and 146; 1333 rows of 3072, 16 ranks 14.8 and 16.6; 1333 of 8192, 64 ranks 36.3 and 46.1); not for short requests,
+// whose other rows would be empty. Splits as long as all workgroups are on the GPU at once (past that, a few that
+// come late cost as much as all others), 512 features each at least for tiles of 128, 1024 for those of 16, and up to 16.
 struct ShrinkPlan {
   uint32_t ranks, rows, splits, span;
   uint64_t slots;
@@ -96,8 +98,10 @@ ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
   return p;
 }
 
-// Rows a tile and columns a workgroup of an expand. Tiles of 32 rows, with more than 16 ranks of 128, which share v, or
-// for short requests, whose other rows would be empty, of 16; columns so that there are some rounds of workgroups.
+// Rows a tile and columns a workgroup of an expand. Tiles of 128 rows, which share v, with more than 16 ranks and 8192 rows or
+// more, where whole workgroups of them fill the GPU (tiles of 16 and of 128, a call of 64 ranks in us: 17792 rows, 3072 columns 162
+// and 146, 8192 columns 228 and 174; 4608 rows 44.0 and 46.0; 1333 rows of 8192 29.3 and 41.3), but not for short requests, whose other
+// rows would be empty. Columns so that there are some rounds of workgroups.
 struct ExpandPlan {
   uint32_t rank, rows, cols;
   uint64_t slots;
@@ -106,16 +110,16 @@ ExpandPlan expand_plan(const mo_adapters_call& c, uint32_t features) {
   ExpandPlan p = {};
   p.rank = c.rank <= 16 ? 16 : c.rank <= 32 ? 32 : c.rank <= 64 ? 64 : 128;
   p.rows = 16;
-  if (!odd(c) && p.rank == 16 && c.rows >= 32ull * c.requests) p.rows = 32;
-  if (!odd(c) && p.rank > 16 && c.rows >= 128ull * c.requests && c.rows >= 1024) p.rows = 128;
+  if (!odd(c) && p.rank > 16 && c.rows >= 128ull * c.requests && c.rows >= 8192) p.rows = 128;
   const uint64_t tiles = div_up(c.rows, p.rows), least = p.rows == 128 ? 128 : 512;
   p.cols = (uint32_t)round_up(between<uint64_t>(1, tiles * features / (p.rows == 128 ? 1024 : kExpandGroups), 4096), least);
   p.slots = tiles + c.requests + 1;
   return p;
 }
 
-// Splits of the rows of the weights' gradients, the same for both: some workgroups for every CU again, 128 rows each at
-// least, and no more planes than 256 MB hold.
+// Splits of the rows of the weights' gradients, the same for both: a workgroup or two for every CU (twice as many, which leave
+// twice the planes: 4608 rows of 3072, 64 ranks, a backward pass 93.9 us for 80.1; fewer: 17792 of 8192 320 for 288), 128 rows
+// each at least, and no more planes than 256 MB hold.
 void share_rows(const mo_adapters_call& c, mo_adapters::Side* a, mo_adapters::Side* b) {
   a->cols = c.da ? c.in_features : 0, b->cols = c.db ? c.out_features : 0;
   a->tiles = (uint32_t)div_up(a->cols, mo_adapters::kOuterCols), b->tiles = (uint32_t)div_up(b->cols, mo_adapters::kOuterCols);
@@ -188,8 +192,8 @@ int start(const mo_adapters_call& c, Kind kind, uint32_t size, const char* form,
     return n;
   };
   const int step = size >= 128 ? 7 : size >= 64 ? 6 : size >= 32 ? 5 : size >= 16 ? 4 : size >= 8 ? 3 : size >= 4 ? 2 : size >= 2 ? 1 : 0;
-  // sizes: up to 8 of a shrink and an outer, 16 to 128 of an expand; forms: "", "2", "odd", "tall"
-  const int place = *form == '2' || *form == 't' ? 1 : *form == 'o' ? 2 : 0;
+  // sizes: up to 8 of a shrink and an outer, 16 to 128 of an expand; forms: "", "odd", "tall"
+  const int place = *form == 't' ? 1 : *form == 'o' ? 2 : 0;
   const int id = kind == kShrink ? step * 3 + place : kind == kExpand ? 12 + (step - 4) * 3 + place
                  : kind == kOuter ? 24 + step * 3 + place
                  : kind == kFew   ? 33 + step
@@ -213,8 +217,7 @@ int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t s
 int expand(const mo_adapters_call& c, mo_adapters::Expand& a, uint64_t stream) {
   const ExpandPlan p = expand_plan(c, a.features);
   a.cols = p.cols;
-  return start(c, kExpand, p.rank, odd(c) ? "odd" : p.rows == 128 ? "tall" : p.rows == 32 ? "2" : "", p.slots,
-               div_up(a.features, p.cols), 1, &a, stream);
+  return start(c, kExpand, p.rank, odd(c) ? "odd" : p.rows == 128 ? "tall" : "", p.slots, div_up(a.features, p.cols), 1, &a, stream);
 }
 
 int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_t bytes, uint64_t stream) {

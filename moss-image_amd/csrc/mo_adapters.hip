@@ -315,19 +315,19 @@ __device__ __forceinline__ void store_turned(void* to, uint32_t rank, uint32_t j
   }
 }
 
-// A workgroup has kTiles * 16 rows, whose h stays in registers, and `cols` columns, of which a wave takes 128 at a time. The
+// A workgroup has 16 rows, whose h stays in registers, and `cols` columns, of which a wave takes 128 at a time. The
 // columns are the instructions' rows, so a lane ends with four neighbouring columns of a row; through the wave's own
 // part of LDS they come to lanes that read and write 256 bytes of a row side by side. With ranks up to 16 the two
-// parts of h lie beside each other in one fragment.
-template <class T, int kRank, int kTiles, bool kOdd>
+// parts of h lie beside each other in one fragment. (32 rows, which read v half as often, were slower: 4608 rows, 16 ranks,
+// 3072 columns 25.5 us.)
+template <class T, int kRank, bool kOdd>
 __device__ __forceinline__ void expand(const Expand& a) {
   typedef Path<T> P;
-  constexpr uint32_t kRows = kTiles * 16;
   constexpr bool kBeside = kRank == 16 && P::kParts == 2;
   constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 1 : P::kParts;
   __shared__ float room[4][16][132];
-  float(*shared)[132] = room[0];  // [kRows][132], before the waves use their parts
-  const Tile tile = tile_of<kRows>(a.by, blockIdx.x);
+  float(*shared)[132] = room[0];  // before the waves use their parts
+  const Tile tile = tile_of<16>(a.by, blockIdx.x);
   if (tile.low >= tile.high) return;
   const uint32_t rank = a.by.rank, lane = threadIdx.x % 64, wave = wave_of(), i = lane % 16, k = lane / 16;
   const uint32_t first = blockIdx.y * a.cols, end = min(a.features, first + a.cols);
@@ -335,12 +335,11 @@ __device__ __forceinline__ void expand(const Expand& a) {
   // a lane's rows (k, and every fourth after it) and columns where memory is read and written
   const Window<T, kOdd> base((const T*)a.base + tile.low * a.base_stride, a.base ? (rows - 1) * stride + a.features : 0);
   const Window<T, kOdd> to((const T*)a.to + (uint64_t)tile.low * a.features, rows * a.features);
-  Eight<T> in[kTiles * 4];
+  Eight<T> in[4];
   auto count = [&](uint32_t at) { return at + i * 8 >= end ? 0 : min(8u, end - at - i * 8); };
-  auto read_base = [&](uint32_t at, int tile) {
+  auto read_base = [&](uint32_t at) {
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-      const uint32_t t = tile * 4 + u;
+    for (uint32_t t = 0; t < 4; ++t) {
       if (kOdd && !a.base)
         in[t] = Eight<T>{};
       else
@@ -349,8 +348,7 @@ __device__ __forceinline__ void expand(const Expand& a) {
   };
   // the first step's loads are on their way while h's are waited for
   uint32_t at = first + wave * 128;
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) read_base(at, t);
+  read_base(at);
   const uint32_t adapter = adapter_of(a.by, tile);
   const bool has = adapter != kNone;
   const Window<T, kOdd> v((const T*)a.v + (uint64_t)(has ? adapter : 0) * a.features * rank, a.features * rank);
@@ -365,97 +363,92 @@ __device__ __forceinline__ void expand(const Expand& a) {
       }
   };
   if (has) read_v(at);
-  typename P::Fragment h[kParts][kSteps][kTiles];
+  typename P::Fragment h[kParts][kSteps];
   float scale = 0.0f;
   if (has) {
     scale = a.scaled ? scale_of(a.by, adapter) : 1.0f;
     // h's splits added up, a part of the tile a thread, and from LDS to the lanes that need it
-    for (uint32_t row = threadIdx.x / 16; row < kRows; row += 16)
-      for (uint32_t j0 = threadIdx.x % 16 * 4; j0 < kRank; j0 += 64) {
-        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (row < rows) {
-          const float* from = a.h + (uint64_t)(tile.low + row) * rank + j0;
+    const uint32_t row = threadIdx.x / 16;
+    for (uint32_t j0 = threadIdx.x % 16 * 4; j0 < kRank; j0 += 64) {
+      f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (row < rows) {
+        const float* from = a.h + (uint64_t)(tile.low + row) * rank + j0;
 #pragma unroll 4
-          for (uint32_t p = 0; p < a.splits; ++p, from += (uint64_t)a.by.rows * rank) {
-            f32x4 more = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (!kOdd && j0 < rank) __builtin_memcpy(&more, from, 16);
-            if (kOdd) {
+        for (uint32_t p = 0; p < a.splits; ++p, from += (uint64_t)a.by.rows * rank) {
+          f32x4 more = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          if (!kOdd && j0 < rank) __builtin_memcpy(&more, from, 16);
+          if (kOdd) {
 #pragma unroll
-              for (uint32_t e = 0; e < 4; ++e)
-                if (j0 + e < rank) more[e] = from[e];
-            }
-            sum = p ? sum + more : more;
+            for (uint32_t e = 0; e < 4; ++e)
+              if (j0 + e < rank) more[e] = from[e];
           }
-          if (blockIdx.y == 0) {
+          sum = p ? sum + more : more;
+        }
+        if (blockIdx.y == 0) {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
-              if (j0 + e >= rank) continue;
-              if (a.h_sum) a.h_sum[(uint64_t)(tile.low + row) * rank + j0 + e] = sum[e];
-              if (a.turned) store_turned<T>(a.turned, rank, j0 + e, tile.low + row, sum[e]);
-            }
+          for (uint32_t e = 0; e < 4; ++e) {
+            if (j0 + e >= rank) continue;
+            if (a.h_sum) a.h_sum[(uint64_t)(tile.low + row) * rank + j0 + e] = sum[e];
+            if (a.turned) store_turned<T>(a.turned, rank, j0 + e, tile.low + row, sum[e]);
           }
         }
-        *(f32x4*)&shared[row][j0] = sum;
       }
+      *(f32x4*)&shared[row][j0] = sum;
+    }
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+    for (int s = 0; s < kSteps; ++s) {
+      const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8;
+      float v[8];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const uint32_t j = kBeside ? k % 2 * 8 : s * 32 + k * 8;
-        float v[8];
+      for (int e = 0; e < 8; ++e) v[e] = j < kRank ? shared[i][j + e] : 0.0f;
+      if (kBeside) {
+        const typename P::Fragment low = P::part(v, 1);
+        h[0][s] = P::part(v, 0);
+        if (k >= 2) h[0][s] = low;
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = j < kRank ? shared[t * 16 + i][j + e] : 0.0f;
-        if (kBeside) {
-          const typename P::Fragment low = P::part(v, 1);
-          h[0][s][t] = P::part(v, 0);
-          if (k >= 2) h[0][s][t] = low;
-        } else {
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) h[p][s][t] = P::part(v, p);
-        }
+        for (int p = 0; p < kParts; ++p) h[p][s] = P::part(v, p);
       }
+    }
     __syncthreads();
   } else if (blockIdx.y == 0 && a.h_sum) {
     for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * rank; e += 256) a.h_sum[(uint64_t)tile.low * rank + e] = 0.0f;
   }
   while (at < end) {
+    if (has) {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      if (has) {
+      for (int c = 0; c < 8; ++c) {
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) P::multiply(sum, P::of(vs[c][s]), h[p][s][t]);
-          *(f32x4*)&room[wave][i][c * 16 + k * 4] = sum;
-        }
-        __builtin_amdgcn_wave_barrier();
+          for (int p = 0; p < kParts; ++p) P::multiply(sum, P::of(vs[c][s]), h[p][s]);
+        *(f32x4*)&room[wave][i][c * 16 + k * 4] = sum;
       }
-      // the next step's loads go out before this one's writes, which a wait for later loads would wait for too
-      if (t == kTiles - 1 && has && at + 512 < end) read_v(at + 512);
-      Eight<T> results[4];
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) {
-        float out[8];
-        widen(out, in[t * 4 + u]);
-        if (has) {
-          float more[8];
-          __builtin_memcpy(more, __builtin_assume_aligned(&room[wave][u * 4 + k][i * 8], 16), 32);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) out[e] += scale * more[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) results[u].v[e] = (T)out[e];
-      }
-      if (at + 512 < end) read_base(at + 512, t);
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u)
-        to.write(results[u], (t * 16 + u * 4) * a.features + at, k * a.features + i * 8, t * 16 + u * 4 + k < rows ? count(at) : 0);
       __builtin_amdgcn_wave_barrier();
     }
+    // the next step's loads go out before this one's writes, which a wait for later loads would wait for too
+    if (has && at + 512 < end) read_v(at + 512);
+    Eight<T> results[4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      float out[8];
+      widen(out, in[u]);
+      if (has) {
+        float more[8];
+        __builtin_memcpy(more, __builtin_assume_aligned(&room[wave][u * 4 + k][i * 8], 16), 32);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] += scale * more[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) results[u].v[e] = (T)out[e];
+    }
+    if (at + 512 < end) read_base(at + 512);
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u)
+      to.write(results[u], u * 4 * a.features + at, k * a.features + i * 8, u * 4 + k < rows ? count(at) : 0);
+    __builtin_amdgcn_wave_barrier();
     at += 512;
   }
 }
@@ -987,7 +980,7 @@ __device__ __forceinline__ void turn(const Turn& a) {
     if (col0 + r < a.rank && row0 + x < a.count) store_turned<T>(a.turned, a.rank, col0 + r, row0 + x, room[x][r]);
 }
 
-// Names: type, ranks, tiles of 16 rows; "odd": features or a rank that are no multiples of eight.
+// Names: type, ranks; "tall": tiles of 128 rows; "odd": features or a rank that are no multiples of eight.
 #define MO_SHRINK(T, t, ranks)                                                                                     \
   extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks(Shrink a) {                   \
     shrink<T, ranks, false>(a);                                                                                    \
@@ -1001,10 +994,10 @@ __device__ __forceinline__ void turn(const Turn& a) {
   }
 #define MO_EXPAND(T, t, rank)                                                                                      \
   extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank(Expand a) {                    \
-    expand<T, rank, 1, false>(a);                                                                                  \
+    expand<T, rank, false>(a);                                                                                     \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_odd(Expand a) {              \
-    expand<T, rank, 1, true>(a);                                                                                   \
+    expand<T, rank, true>(a);                                                                                      \
   }
 #define MO_EXPAND_TALL(T, t, rank)                                                                                 \
   extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_tall(Expand a) {             \
@@ -1028,9 +1021,6 @@ __device__ __forceinline__ void turn(const Turn& a) {
   MO_TALL(T, t, 2)                                                                                                 \
   MO_TALL(T, t, 4)                                                                                                 \
   MO_EXPAND(T, t, 16)                                                                                              \
-  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_16_2(Expand a) {                      \
-    expand<T, 16, 2, false>(a);                                                                                    \
-  }                                                                                                                \
   MO_EXPAND(T, t, 32)                                                                                              \
   MO_EXPAND_TALL(T, t, 32)                                                                                         \
   MO_EXPAND(T, t, 64)                                                                                              \

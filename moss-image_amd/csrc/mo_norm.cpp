@@ -39,13 +39,20 @@ bool odd(const mo_norm_call& c) {
 Plan plan_of(const mo_norm_call& c, bool backward) {
   Plan p = {};
   const uint64_t held = div_up(c.dim, 8);
-  p.iter = held > 1024 ? 4 : held > 512 ? 2 : 1;
+  // 8 values a lane up to 512 lanes, more past that; 5 to 7 waves of 8 values were slower than 3 or 4 of 16 (17792 rows of
+  // 3072 bfloat16, forward and backward: 41.8 and 78.1 us against 37.1 and 74.6), 8 waves faster (4608 of 4096: 13.8 and 28.5
+  // against 15.1 and 30.8)
+  p.iter = held > 1024 ? 4 : held > 512 || (held > 256 && held <= 448) ? 2 : 1;
   p.lanes = (uint32_t)div_up(div_up(held, p.iter), 64) * 64;
+  // rows of a wave four to a workgroup: 17792 of 256 7.4 and 23.3 us, one to a workgroup 10.2 and 26.1
   p.per = p.lanes == 64 ? 4 : 1;
-  // forward: enough workgroups for several on every CU; backward: each leaves sums of dim values, so fewer
-  const uint64_t most = backward ? 512 : 1024;
+  // Forward: enough workgroups for several on every CU (half as many: 4608 rows of 3072 14.8 us for 12.9; twice: 3584 17.9
+  // for 14.5). Backward each leaves sums of dim values, so fewer: two a CU, or one where a workgroup is large (twice as many
+  // of those: 4608 rows of 8192 58.9 us for 47.7, of 12288 102 for 92; half as many of the others: 17792 of 3072 92 for 74.6),
+  // and of two rows at least (333 rows of 3072: 16.0 us for 12.0).
+  const uint64_t most = !backward ? 1024 : p.lanes == 512 || p.iter == 4 || p.per > 1 ? 256 : 512;
   p.chunk = (uint32_t)div_up(c.rows, most * p.per);
-  if (p.chunk > 1) p.chunk += p.chunk % 2;  // whole batches of two rows
+  if (p.chunk > 1 || backward) p.chunk += p.chunk % 2;  // whole batches of two rows
   p.groups = (uint32_t)div_up(c.rows, p.chunk);
   p.slots = (uint64_t)p.groups + (c.samples ? c.samples - 1 : 0);
   return p;
