@@ -236,6 +236,7 @@ class EngineError(RuntimeError):
 
 
 _P = ctypes.POINTER
+_call = ctypes.c_void_p  # a descriptor: a structure by reference, or its bytes as struct packs them
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint32
 
@@ -339,16 +340,16 @@ SIGNATURES: dict[str, tuple] = {
     "mo_rotary_backward": (ctypes.c_int, [_P(MoRotaryCall), _u64, _u64, _u64]),
     "mo_rotary_workspace_bytes": (_u64, [_P(MoRotaryCall)]),
     "mo_rotary_table": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u32, _u32, ctypes.c_float, _u64]),
-    "mo_norm_forward": (ctypes.c_int, [_P(MoNormCall), _u64]),
-    "mo_norm_backward": (ctypes.c_int, [_P(MoNormCall), _u64, _u64, _u64]),
-    "mo_norm_workspace_bytes": (_u64, [_P(MoNormCall)]),
+    "mo_norm_forward": (ctypes.c_int, [_call, _u64]),
+    "mo_norm_backward": (ctypes.c_int, [_call, _u64, _u64, _u64]),
+    "mo_norm_workspace_bytes": (_u64, [_call]),
     "mo_keep_pack": (ctypes.c_int, [_u64, _u32, _u64, _u32, _u64, _u64, _u64, _u64]),
     "mo_keep_restore": (ctypes.c_int, [_u64, _u64, _u64, _u32, _u64, _u32, _u64, _u64]),
-    "mo_gated_forward": (ctypes.c_int, [_P(MoGatedCall), _u64]),
-    "mo_gated_backward": (ctypes.c_int, [_P(MoGatedCall), _u64]),
-    "mo_adapters_forward": (ctypes.c_int, [_P(MoAdaptersCall), _u64, _u64, _u64]),
-    "mo_adapters_backward": (ctypes.c_int, [_P(MoAdaptersCall), _u64, _u64, _u64]),
-    "mo_adapters_workspace_bytes": (_u64, [_P(MoAdaptersCall), _u32]),
+    "mo_gated_forward": (ctypes.c_int, [_call, _u64]),
+    "mo_gated_backward": (ctypes.c_int, [_call, _u64]),
+    "mo_adapters_forward": (ctypes.c_int, [_call, _u64, _u64, _u64]),
+    "mo_adapters_backward": (ctypes.c_int, [_call, _u64, _u64, _u64]),
+    "mo_adapters_workspace_bytes": (_u64, [_call, _u32]),
 }
 
 _lock = threading.Lock()

@@ -61,7 +61,7 @@ def whole(tensor: torch.Tensor | None, count: int, like: torch.Tensor, what: str
     if tensor.dtype not in (torch.int64, torch.int32) or tensor.shape != (count,) \
             or tensor.get_device() != like.get_device():
         raise ValueError(f"{what} must be {count} int64 (or int32) numbers on the tokens' device.")
-    return tensor.to(torch.int64).contiguous()
+    return tensor if tensor.dtype == torch.int64 and tensor.is_contiguous() else tensor.to(torch.int64).contiguous()
 
 
 def first_derivatives(what: str) -> None:

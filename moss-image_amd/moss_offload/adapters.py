@@ -13,7 +13,6 @@ adapter ``i``, or the only one.
 
 from __future__ import annotations
 
-import ctypes
 import struct
 
 import torch
@@ -72,7 +71,7 @@ def _check(like, shape, a, b, scale, cu_seqlens, index):
 
 def _space(lib, call, backward: bool, like: torch.Tensor):
     # freed to the caching allocator after the call; stream order keeps it alive for the kernels
-    nbytes = lib.mo_adapters_workspace_bytes(ctypes.byref(call), backward)
+    nbytes = lib.mo_adapters_workspace_bytes(call, backward)
     return (like.new_empty(nbytes, dtype=torch.uint8), nbytes) if nbytes else (None, 0)
 
 
@@ -98,13 +97,13 @@ def adapters_forward(x: torch.Tensor, result: torch.Tensor, a: torch.Tensor, b: 
     y = _like(result)
     between = x.new_empty((count, rank), dtype=torch.float32)
     if count:
-        call = _native.MoAdaptersCall.from_buffer_copy(_CALL.pack(
+        call = _CALL.pack(
             tokens.data_ptr(), 0, base.data_ptr(), y.data_ptr(), a.data_ptr(), b.data_ptr(), _address(scales), _address(cu),
             _address(which), between.data_ptr(), 0, 0, 0, 0, 0, count, pitch(tokens), pitch(base), 0, 0, requests, a.shape[0],
-            rank, features, base.shape[1], CODES[x.dtype], factor, 0))
+            rank, features, base.shape[1], CODES[x.dtype], factor, 0)
         space, nbytes = _space(lib, call, False, x)
         _native.check("mo_adapters_forward",
-                      lib.mo_adapters_forward(ctypes.byref(call), _address(space), nbytes, stream(x)))
+                      lib.mo_adapters_forward(call, _address(space), nbytes, stream(x)))
     return (y, between) if hidden else y
 
 
@@ -134,15 +133,15 @@ def _backward(grad, x, hidden, a, b, scale, cu_seqlens, index, add, wanted):
     dx = grad.new_empty((*grad.shape[:-1], in_features)) if wanted[0] else None
     da, db = (_like(t) if w else None for t, w in zip((a, b), wanted[1:]))
     if count and any(wanted):
-        call = _native.MoAdaptersCall.from_buffer_copy(_CALL.pack(
+        call = _CALL.pack(
             _address(source), x.exponents.data_ptr() if kept else 0, 0, 0, a.data_ptr(), b.data_ptr(), _address(scales),
             _address(cu), _address(which), hidden.data_ptr(), matrix.data_ptr(), _address(added), _address(dx), _address(da),
             _address(db), count, 0 if kept or source is None else pitch(source), 0, pitch(matrix),
             0 if added is None else pitch(added), requests, a.shape[0], rank, in_features, out_features, CODES[grad.dtype],
-            factor, 0))
+            factor, 0)
         space, nbytes = _space(lib, call, True, grad)
         _native.check("mo_adapters_backward",
-                      lib.mo_adapters_backward(ctypes.byref(call), _address(space), nbytes, stream(grad)))
+                      lib.mo_adapters_backward(call, _address(space), nbytes, stream(grad)))
     else:
         for t in (da, db):
             if t is not None:

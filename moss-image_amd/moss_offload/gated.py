@@ -11,7 +11,6 @@ first, as a fused projection leaves them (``gate=None``).
 
 from __future__ import annotations
 
-import ctypes
 import struct
 
 import torch
@@ -69,10 +68,10 @@ def gated_forward(up: torch.Tensor, gate: torch.Tensor | None = None, *, kind: s
         places = tuple(t.data_ptr() for t in (kept.values, kept_gate.values, kept.exponents, kept_gate.exponents))
         strides = kept.values.shape[-1], kept.exponents.shape[-1]
     if count:
-        call = _native.MoGatedCall.from_buffer_copy(_CALL.pack(
+        call = _CALL.pack(
             *addresses, 0, 0, 0, out.data_ptr(), 0, *places, count, pitch(first), pitch(second), 0, cols, *strides, cols,
-            CODES[up.dtype], silu, 0))
-        _native.check("mo_gated_forward", lib.mo_gated_forward(ctypes.byref(call), stream(up)))
+            CODES[up.dtype], silu, 0)
+        _native.check("mo_gated_forward", lib.mo_gated_forward(call, stream(up)))
     return (out, kept, kept_gate) if keep else out
 
 
@@ -115,10 +114,10 @@ def gated_backward(grad: torch.Tensor, up, gate=None, *, kind: str = "situ"):
         out = like(grad), like(grad)
         outs = out[0].data_ptr(), out[1].data_ptr()
     if count:
-        call = _native.MoGatedCall.from_buffer_copy(_CALL.pack(
+        call = _CALL.pack(
             *addresses, matrix.data_ptr(), *outs, 0, 0, 0, 0, count, *strides, pitch(matrix), cols * (1 + fused), *steps, cols,
-            CODES[grad.dtype], silu, 0))
-        _native.check("mo_gated_backward", lib.mo_gated_backward(ctypes.byref(call), stream(grad)))
+            CODES[grad.dtype], silu, 0)
+        _native.check("mo_gated_backward", lib.mo_gated_backward(call, stream(grad)))
     return out
 
 

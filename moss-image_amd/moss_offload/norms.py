@@ -12,7 +12,6 @@ sample give zeros, get a gradient of zero and take part in no sum.
 
 from __future__ import annotations
 
-import ctypes
 import struct
 from typing import NamedTuple
 
@@ -81,14 +80,13 @@ def _check(like, shape, kind, weight, bias, scale, shift, cu_seqlens):
     return samples, weight, bias, weight_code, scale, shift, scale_code, cu_seqlens
 
 
-def _run(name, lib, fields, like):
-    call = _native.MoNormCall.from_buffer_copy(fields)
+def _run(name, lib, call, like):
     if name == "mo_norm_forward":
-        return _native.check(name, lib.mo_norm_forward(ctypes.byref(call), stream(like)))
-    nbytes = lib.mo_norm_workspace_bytes(ctypes.byref(call))
+        return _native.check(name, lib.mo_norm_forward(call, stream(like)))
+    nbytes = lib.mo_norm_workspace_bytes(call)
     # freed to the caching allocator after the call; stream order keeps it alive for the kernels
     space = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _native.check(name, lib.mo_norm_backward(ctypes.byref(call), _address(space), nbytes, stream(like)))
+    _native.check(name, lib.mo_norm_backward(call, _address(space), nbytes, stream(like)))
 
 
 def norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
