@@ -92,7 +92,7 @@ ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
   p.rows = !odd(c) && fits && c.rows >= 128ull * c.requests && tall * (most < 16 ? most : 16) >= 256 ? 128 : 16;
   const uint64_t tiles = div_up(c.rows, p.rows), least = p.rows == 128 ? 512 : 1024;
   const uint64_t splits = between<uint64_t>(1, (p.rows == 128 ? 512 : 1024) / tiles, div_up(features, least));
-  p.span = (uint32_t)round_up(div_up(features, splits > 16 ? 16 : splits), least);
+  p.span = (uint32_t)round_up(div_up(features, splits > 16 ? 16 : splits), p.rows == 128 ? 128 : 1024);  // whole steps
   p.splits = (uint32_t)div_up(features, p.span);
   p.slots = tiles + c.requests + 1;
   return p;
