@@ -238,7 +238,7 @@ __device__ __forceinline__ void shrink(const Shrink& a) {
 
 // The same for many rows in long requests: a wave has 16 rows of its own and the weight, which is read for each tile and
 // with many ranks would be more than the rows themselves, comes to LDS once for all eight waves, one step ahead. Bound by
-// memory: bfloat16, 16 ranks, 4608 rows of 16384 (151 MB) in 43 us, 3.5 TB/s; 64 ranks, 17792 rows of 8192 (292 MB) in 71, 4.1 TB/s.
+// memory: bfloat16, 16 ranks, 4608 rows of 16384 (151 MB) in 42.5 us, 3.6 TB/s; 64 ranks, 17792 rows of 8192 (292 MB) in 65, 4.5 TB/s.
 template <class T, int kRanks>
 __device__ __forceinline__ void shrink_tall(const Shrink& a) {
   typedef Path<T> P;
