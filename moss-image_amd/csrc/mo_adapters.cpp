@@ -156,7 +156,7 @@ Room room_of(const mo_adapters_call& c, bool backward) {
     return at;
   };
   const uint64_t between_bytes = c.rows * c.rank * 4, size = kTypeBytes[c.dtype];
-  const uint64_t turned = round_up(c.rows, 32) * c.rank * 4;  // one fp32 or two bfloat16, in whole steps of 32 rows
+  const uint64_t turned = round_up(c.rows, 32) * c.rank * 4;  // in whole steps of 32 rows
   if (!backward) {
     if (is_few(c)) return r;
     const ShrinkPlan p = shrink_plan(c, c.in_features);
@@ -261,20 +261,20 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
   if (c.dx || c.da) turned(0, c.b, workspace + room.turned_b, c.out_features, c.rank);
   if (c.dx) turned(1, c.a, workspace + room.turned_a, c.rank, c.in_features);
   const uint64_t narrow = div_up(c.rows, 32) * div_up(c.rank, 32);
-  if (c.db) t.narrow = (const float*)c.hidden, t.turned = (void*)(workspace + room.turned_hidden), t.splits = 1;
+  if (c.db) t.narrow = (const float*)c.hidden, t.turned = (float*)(workspace + room.turned_hidden), t.splits = 1;
   const uint64_t weights = (uint64_t)t.tiles[0] + t.tiles[1];
   if (int rc = start(c, kTurn, 0, "", weights + (c.db ? narrow : 0), weights ? c.adapters : 1, 1, &t, stream)) return rc;
   if (c.dx || c.da) {
     if (int rc = shrink(c, by, c.grad, stride_of(c, c.grad_stride, c.out_features), workspace + room.turned_b, c.out_features, planes, true, stream)) return rc;
     const uint32_t splits = shrink_plan(c, c.out_features).splits;
     if (c.dx) {
-      e.splits = splits, e.h = (const float*)planes, e.turned = c.da ? (void*)(workspace + room.turned_back) : nullptr;
+      e.splits = splits, e.h = (const float*)planes, e.turned = c.da ? (float*)(workspace + room.turned_back) : nullptr;
       e.v = (const void*)(workspace + room.turned_a), e.base = (const void*)c.add, e.base_stride = stride_of(c, c.add_stride, c.in_features);
       e.to = (void*)c.dx, e.features = c.in_features;
       if (int rc = expand(c, e, stream)) return rc;
     } else {
       t.tiles[0] = t.tiles[1] = 0;
-      t.narrow = (const float*)planes, t.turned = (void*)(workspace + room.turned_back), t.splits = splits;
+      t.narrow = (const float*)planes, t.turned = (float*)(workspace + room.turned_back), t.splits = splits;
       if (int rc = start(c, kTurn, 0, "", narrow, 1, 1, &t, stream)) return rc;
     }
   }
@@ -283,9 +283,9 @@ int run(const mo_adapters_call* call, bool backward, uint64_t workspace, uint64_
   o.by = by;
   mo_adapters::Side &a = o.side[0], &b = o.side[1];
   share_rows(c, &a, &b);
-  a.wide = (const void*)c.x, a.exponents = (const uint8_t*)c.x_exponents, a.narrow = (const void*)(workspace + room.turned_back);
+  a.wide = (const void*)c.x, a.exponents = (const uint8_t*)c.x_exponents, a.narrow = (const float*)(workspace + room.turned_back);
   a.planes = (float*)(workspace + room.da), a.to = (void*)c.da, a.stride = stride_of(c, c.x_stride, c.in_features), a.groups = (c.in_features + 31) / 32;
-  b.wide = (const void*)c.grad, b.narrow = (const void*)(workspace + room.turned_hidden);
+  b.wide = (const void*)c.grad, b.narrow = (const float*)(workspace + room.turned_hidden);
   b.planes = (float*)(workspace + room.db), b.to = (void*)c.db, b.stride = stride_of(c, c.grad_stride, c.out_features);
   b.turned = 1, b.scaled = 1;
   // up to 64 ranks a workgroup (by 32, which read the rows again: 17792 rows of 8192 and 3072, 64 ranks, 200 us for 138)

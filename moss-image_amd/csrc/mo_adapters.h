@@ -37,7 +37,7 @@ struct Expand {
   Requests by;
   const float* h;         // [splits][rows][rank]
   float* h_sum;           // [rows][rank] or null
-  void* turned;           // h turned, for an outer, or null
+  float* turned;          // h turned, for an outer, or null
   const void* v;          // [adapters][features][rank]
   const void* base;       // [rows][features], or null: 0
   void* to;
@@ -56,7 +56,7 @@ struct Few {
 struct Side {
   const void* wide;          // [rows][cols], or 8-bit values [rows][groups * 32]
   const uint8_t* exponents;  // [rows][groups], or null
-  const void* narrow;        // turned: [rows / 8][parts][rank][8]
+  const float* narrow;       // turned: [rows / 8][rank][8]
   float* planes;             // [splits][adapters][cols * rank] sums over a split's rows, where there are several
   void* to;                  // [adapters][rank][cols], or turned: [adapters][cols][rank]; null: not wanted
   uint64_t stride;
@@ -69,13 +69,13 @@ struct Outer {
 };
 
 // Copies of both weights, each [adapters] matrices turned, and of a narrow matrix for an outer: the sum of its splits,
-// turned, [rows / 8][parts][rank][8].
+// turned, [rows / 8][rank][8].
 struct Turn {
   const void* from[2];
   void* to[2];
   uint32_t rows[2], cols[2], tiles[2];  // of `from`; tiles of 32 x 32, 0: not wanted
   const float* narrow;                  // [splits][count][rank]
-  void* turned;
+  float* turned;
   uint32_t adapters, count, rank, splits;
 };
 

@@ -8,7 +8,7 @@
 // Three kernels: shrink (h and d h: rows against a weight's ranks, reduced over the features), expand (y and d x:
 // reduced over the rank), outer (both weights' gradients: reduced over the rows). All are bound by the tokens that they
 // read and write, so the matrix instructions have room: bfloat16 operands go into 16 x 16 x 32 ones, and the fp32
-// numbers between the products in two bfloat16 parts, which leaves out 2^-16 of them at most; float16 and float32 go
+// numbers between the products in three bfloat16 parts, which are all of their 24 bits; float16 and float32 go
 // into the fp32 ones, 16 x 16 x 4, where float16 parts would under- and overflow.
 //
 // Rows are taken in tiles that lie in one request. Tile and request are found from the workgroup's number alone: what
@@ -48,12 +48,9 @@ struct Path {  // fp32 instructions: lane (i, k) has values k * 8 to k * 8 + 7, 
     widen(f.v, v);
     return f;
   }
-  typedef float Narrow;
-  static __device__ __forceinline__ Fragment part(const float (&v)[8], int) {
-    Fragment f;
+  static __device__ __forceinline__ void split(Fragment (&to)[1], const float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f.v[i] = v[i];
-    return f;
+    for (int i = 0; i < 8; ++i) to[0].v[i] = v[i];
   }
   static __device__ __forceinline__ void multiply(f32x4& to, const Fragment& a, const Fragment& b) {
 #pragma unroll
@@ -79,20 +76,29 @@ struct Path {  // fp32 instructions: lane (i, k) has values k * 8 to k * 8 + 7, 
 template <>
 struct Path<__bf16> {
   typedef bf16x8 Fragment;
-  static constexpr int kParts = 2;
+  static constexpr int kParts = 3;
   static __device__ __forceinline__ Fragment of(const Eight<__bf16>& v) { return __builtin_bit_cast(Fragment, v); }
-  typedef __bf16 Narrow;
-  // The upper half of an fp32 number (cut, so that nothing overflows), and the rest of it rounded to the nearest. What
-  // is not finite has no rest.
-  static __device__ __forceinline__ Fragment part(const float (&v)[8], int which) {
-    Fragment f;
+  // fp32 numbers as sums of three bfloat16 ones: the upper half of the number (cut, so that nothing overflows), that of
+  // the rest, and what is left, eight bits each: none is lost. What is not finite has no rest.
+  static __device__ __forceinline__ void split(Fragment (&to)[3], const float (&v)[8]) {
+    uint32_t words[3][4];
+    float rest[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t bits = __builtin_bit_cast(uint32_t, v[i]);
-      const float high = __builtin_bit_cast(float, bits & 0xffff0000u);
-      f[i] = which == 0 ? (__bf16)high : (bits & 0x7f800000u) == 0x7f800000u ? (__bf16)0.0f : (__bf16)(v[i] - high);
+    for (int i = 0; i < 8; ++i) rest[i] = v[i];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      uint32_t bits[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bits[i] = __builtin_bit_cast(uint32_t, rest[i]);
+        rest[i] -= __builtin_bit_cast(float, bits[i] & 0xffff0000u);
+        if (p == 0) rest[i] = (bits[i] & 0x7f800000u) == 0x7f800000u ? 0.0f : rest[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) words[p][i] = __builtin_amdgcn_perm(bits[2 * i + 1], bits[2 * i], 0x07060302u);
     }
-    return f;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) to[p] = __builtin_bit_cast(Fragment, words[p]);
   }
   static __device__ __forceinline__ void multiply(f32x4& to, const Fragment& a, const Fragment& b) {
     to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, to, 0, 0, 0);
@@ -302,31 +308,22 @@ __device__ __forceinline__ void shrink_tall(const Shrink& a) {
 
 // ---- expand ------------------------------------------------------------------------------------------
 
-// A value of a narrow matrix turned, for the instructions of an outer: [rows / 8][parts][rank][8 rows], fp32 in one part
-// or bfloat16 in two, so that a fragment is read from neighbouring places.
-template <class T>
-__device__ __forceinline__ void store_turned(void* to, uint32_t rank, uint32_t j, uint32_t row, float v) {
-  const float one[8] = {v};
-#pragma unroll
-  for (int p = 0; p < Path<T>::kParts; ++p) {
-    const uint64_t at = (((uint64_t)(row / 8) * Path<T>::kParts + p) * rank + j) * 8 + row % 8;
-    if (Path<T>::kParts == 2)
-      ((__bf16*)to)[at] = Path<__bf16>::part(one, p)[0];
-    else
-      ((float*)to)[at] = v;
-  }
+// Where a value of a narrow matrix lies turned, for the instructions of an outer: fp32 [rows / 8][rank][8 rows], so that a
+// fragment is read from neighbouring places.
+__device__ __forceinline__ uint64_t turned_at(uint32_t rank, uint32_t j, uint32_t row) {
+  return ((uint64_t)(row / 8) * rank + j) * 8 + row % 8;
 }
 
 // A workgroup has 16 rows, whose h stays in registers, and `cols` columns, of which a wave takes 128 at a time. The
 // columns are the instructions' rows, so a lane ends with four neighbouring columns of a row; through the wave's own
-// part of LDS they come to lanes that read and write 256 bytes of a row side by side. With ranks up to 16 the two
-// parts of h lie beside each other in one fragment. (32 rows, which read v half as often, were slower: 4608 rows, 16 ranks,
+// part of LDS they come to lanes that read and write 256 bytes of a row side by side. With ranks up to 16 the first two
+// parts of h lie beside each other in one fragment, the third beside nothing in another. (32 rows, which read v half as often, were slower: 4608 rows, 16 ranks,
 // 3072 columns 25.5 us for 21.2.) Bound by memory: 16 ranks, 4608 rows of 16384 (302 MB, read and written) in 61 us, 4.9 TB/s.
 template <class T, int kRank, bool kOdd>
 __device__ __forceinline__ void expand(const Expand& a) {
   typedef Path<T> P;
-  constexpr bool kBeside = kRank == 16 && P::kParts == 2;
-  constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 1 : P::kParts;
+  constexpr bool kBeside = kRank == 16 && P::kParts == 3;
+  constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 2 : P::kParts;
   __shared__ float room[4][16][132];
   float(*shared)[132] = room[0];  // before the waves use their parts
   const Tile tile = tile_of<16>(a.by, blockIdx.x);
@@ -391,7 +388,7 @@ __device__ __forceinline__ void expand(const Expand& a) {
           for (uint32_t e = 0; e < 4; ++e) {
             if (j0 + e >= rank) continue;
             if (a.h_sum) a.h_sum[(uint64_t)(tile.low + row) * rank + j0 + e] = sum[e];
-            if (a.turned) store_turned<T>(a.turned, rank, j0 + e, tile.low + row, sum[e]);
+            if (a.turned) a.turned[turned_at(rank, j0 + e, tile.low + row)] = sum[e];
           }
         }
       }
@@ -404,13 +401,14 @@ __device__ __forceinline__ void expand(const Expand& a) {
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = j < kRank ? shared[i][j + e] : 0.0f;
+      typename P::Fragment parts[P::kParts];
+      P::split(parts, v);
       if (kBeside) {
-        const typename P::Fragment low = P::part(v, 1);
-        h[0][s] = P::part(v, 0);
-        if (k >= 2) h[0][s] = low;
+        h[0][s] = k < 2 ? parts[0] : parts[P::kParts / 2];
+        h[kParts - 1][s] = k < 2 ? parts[P::kParts - 1] : typename P::Fragment{};
       } else {
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) h[p][s] = P::part(v, p);
+        for (int p = 0; p < kParts; ++p) h[p][s] = parts[p];
       }
     }
     __syncthreads();
@@ -521,12 +519,14 @@ __device__ __forceinline__ void expand_tall(const Expand& a) {
             if (a.h_sum) store8(a.h_sum + (uint64_t)(low + row) * rank + j, sum);
             if (a.turned) {
 #pragma unroll
-              for (uint32_t e = 0; e < 8; ++e) store_turned<T>(a.turned, rank, j + e, low + row, sum[e]);
+              for (uint32_t e = 0; e < 8; ++e) a.turned[turned_at(rank, j + e, low + row)] = sum[e];
             }
           }
         }
+        typename P::Fragment parts[P::kParts];
+        P::split(parts, sum);
 #pragma unroll
-        for (int p = 0; p < P::kParts; ++p) h[p][s][t] = P::part(sum, p);
+        for (int p = 0; p < P::kParts; ++p) h[p][s][t] = parts[p];
       }
   } else if (blockIdx.y == 0 && a.h_sum) {
     for (uint32_t e = threadIdx.x; e < (tile.high - tile.low) * rank; e += 256) a.h_sum[(uint64_t)tile.low * rank + e] = 0.0f;
@@ -595,8 +595,8 @@ __device__ __forceinline__ void few(const Few& f) {
   const Shrink& a = f.in;
   const Expand& b = f.out;
   constexpr uint32_t kRank = kRanks * 16, kPitch = kRank + 4;
-  constexpr bool kBeside = kRanks == 1 && P::kParts == 2;
-  constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 1 : P::kParts;
+  constexpr bool kBeside = kRanks == 1 && P::kParts == 3;
+  constexpr int kSteps = kRank < 32 ? 1 : kRank / 32, kParts = kBeside ? 2 : P::kParts;
   union Room {
     Eight<T> stage[8][16][16];
     float sums[8][16][kPitch];
@@ -676,13 +676,14 @@ __device__ __forceinline__ void few(const Few& f) {
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = j < kRank ? h[i][j + e] : 0.0f;
+      typename P::Fragment parts[P::kParts];
+      P::split(parts, v);
       if (kBeside) {
-        const typename P::Fragment low = P::part(v, 1);
-        hs[0][s] = P::part(v, 0);
-        if (k >= 2) hs[0][s] = low;
+        hs[0][s] = k < 2 ? parts[0] : parts[P::kParts / 2];
+        hs[kParts - 1][s] = k < 2 ? parts[P::kParts - 1] : typename P::Fragment{};
       } else {
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) hs[p][s] = P::part(v, p);
+        for (int p = 0; p < kParts; ++p) hs[p][s] = parts[p];
       }
     }
 #pragma unroll
@@ -792,30 +793,44 @@ __device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_
 #pragma unroll
       for (uint32_t e = 0; e < 8; ++e) wide[e] = from.read(e * stride, k * 8 * stride + i * 8, in_step(k * 8 + e) ? count : 0);
     }
-    const uint32_t octet = P::kParts * by.rank * 8;
-    const Window<typename P::Narrow, false> narrow0((const typename P::Narrow*)a.narrow + (uint64_t)(row0 / 8) * octet, 4 * octet);
-    Eight<typename P::Narrow> narrow[kRanks][P::kParts];
+    const uint32_t octet = by.rank * 8;
+    const Window<float, false> narrow0(a.narrow + (uint64_t)(row0 / 8) * octet, 4 * octet);
+    Eight<float> narrow[kRanks];
 #pragma unroll
     for (uint32_t r = 0; r < kRanks; ++r)
-#pragma unroll
-      for (uint32_t p = 0; p < P::kParts; ++p)
-        narrow[r][p] = narrow0.read((p * by.rank + rank0 + r * 16) * 8, k * octet + i * 8, rank0 + r * 16 + i < by.rank ? 8 : 0);
+      narrow[r] = narrow0.read((rank0 + r * 16) * 8, k * octet + i * 8, rank0 + r * 16 + i < by.rank ? 8 : 0);
     if (low_in || rows < 32) {
 #pragma unroll
       for (uint32_t r = 0; r < kRanks; ++r)
 #pragma unroll
-        for (uint32_t p = 0; p < P::kParts; ++p)
-#pragma unroll
-          for (uint32_t e = 0; e < 8; ++e)
-            narrow[r][p].v[e] = in_step(k * 8 + e) ? narrow[r][p].v[e] : (typename P::Narrow)0.0f;
+        for (uint32_t e = 0; e < 8; ++e) narrow[r].v[e] = in_step(k * 8 + e) ? narrow[r].v[e] : 0.0f;
     }
+    if constexpr (kRanks <= 2 || P::kParts == 1) {  // one column's operand at a time
+      typename P::Fragment parts[kRanks][P::kParts];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const typename P::Fragment f = P::column(wide, q);
+      for (int r = 0; r < kRanks; ++r) P::split(parts[r], narrow[r].v);
 #pragma unroll
-      for (int r = 0; r < kRanks; ++r)
+      for (int q = 0; q < 8; ++q) {
+        const typename P::Fragment f = P::column(wide, q);
 #pragma unroll
-        for (int p = 0; p < P::kParts; ++p) P::multiply(sum[r][q], Path<typename P::Narrow>::of(narrow[r][p]), f);
+        for (int r = 0; r < kRanks; ++r)
+#pragma unroll
+          for (int p = 0; p < P::kParts; ++p) P::multiply(sum[r][q], parts[r][p], f);
+      }
+    } else {  // one narrow operand's parts at a time: those of all would not fit in registers
+      typename P::Fragment columns[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) columns[q] = P::column(wide, q);
+#pragma unroll
+      for (int r = 0; r < kRanks; ++r) {
+        typename P::Fragment parts[P::kParts];
+        P::split(parts, narrow[r].v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+          for (int p = 0; p < P::kParts; ++p) P::multiply(sum[r][q], parts[p], columns[q]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     next();
   }
@@ -984,10 +999,12 @@ __device__ __forceinline__ void turn(const Turn& a) {
   }
   __syncthreads();
   for (uint32_t r = y; r < 32; r += 8)
-    if (col0 + r < a.rank && row0 + x < a.count) store_turned<T>(a.turned, a.rank, col0 + r, row0 + x, room[x][r]);
+    if (col0 + r < a.rank && row0 + x < a.count) a.turned[turned_at(a.rank, col0 + r, row0 + x)] = room[x][r];
 }
 
 // Names: type, ranks; "tall": tiles of 128 rows; "odd": features or a rank that are no multiples of eight.
+// Waves a SIMD asked for where the compiler would take registers for one less: an expand of 16 ranks (4608 rows of 3072 bfloat16
+// 21.0 us, 23.4 with three), an outer of 32 (three of its values go to scratch; 4608 rows of 8192 and 3072 27.1 us).
 #define MO_SHRINK(T, t, ranks)                                                                                     \
   extern "C" __global__ __launch_bounds__(512) void mo_adapters_shrink_##t##_##ranks(Shrink a) {                   \
     shrink<T, ranks, false>(a);                                                                                    \
@@ -1000,7 +1017,8 @@ __device__ __forceinline__ void turn(const Turn& a) {
     shrink_tall<T, ranks>(a);                                                                                      \
   }
 #define MO_EXPAND(T, t, rank)                                                                                      \
-  extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank(Expand a) {                    \
+  extern "C" __global__ __launch_bounds__(256, rank == 16 && sizeof(T) == 2 ? 4 : 1)                     \
+  void mo_adapters_expand_##t##_##rank(Expand a) {                                                                 \
     expand<T, rank, false>(a);                                                                                     \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256) void mo_adapters_expand_##t##_##rank##_odd(Expand a) {              \
@@ -1013,7 +1031,7 @@ __device__ __forceinline__ void turn(const Turn& a) {
 #define MO_FEW(T, t, ranks)                                                                                        \
   extern "C" __global__ __launch_bounds__(512) void mo_adapters_few_##t##_##ranks(Few f) { few<T, ranks>(f); }
 #define MO_OUTER(T, t, ranks)                                                                                      \
-  extern "C" __global__ __launch_bounds__(256, 2) void mo_adapters_outer_##t##_##ranks(Outer a) {                     \
+  extern "C" __global__ __launch_bounds__(256, ranks == 2 && sizeof(T) == 2 ? 3 : 2) void mo_adapters_outer_##t##_##ranks(Outer a) {                     \
     outer_sides<T, ranks, false>(a);                                                                               \
   }                                                                                                                \
   extern "C" __global__ __launch_bounds__(256, 2) void mo_adapters_outer_##t##_##ranks##_odd(Outer a) {               \
