@@ -664,7 +664,7 @@ __device__ __forceinline__ void few(const Few& f) {
     float total = 0.0f;
 #pragma unroll
     for (int u = 0; u < 8; ++u) total += room.sums[u][row][j];
-    h[row][j] = total;
+    h[row][j] = j < rank ? total : 0.0f;  // past the rank the sum is of zeros times the tokens, NaN for infinite ones
     if (blockIdx.y == 0 && row < rows && j < rank) a.to[(uint64_t)(tile.low + row) * rank + j] = total;
   }
   __syncthreads();
