@@ -107,13 +107,16 @@ class _CheckpointFunction(torch.autograd.Function):
     def forward(ctx, function, tokens, *others):
         kept, kind = keep8(tokens), tokens.device.type
         ctx.function, ctx.dtype, ctx.cols, ctx.kind = function, tokens.dtype, tokens.shape[-1], kind
-        ctx.autocast = (torch.is_autocast_enabled(kind), torch.get_autocast_dtype(kind), torch.is_autocast_cache_enabled())
+        ctx.autocast = {"enabled": torch.is_autocast_enabled(kind), "dtype": torch.get_autocast_dtype(kind), "cache_enabled": False}
         ctx.random = torch.get_rng_state(), torch.cuda.get_rng_state(tokens.device)
         ctx.others = [None if isinstance(t, torch.Tensor) else t for t in others]
         ctx.places = [i for i, t in enumerate(others) if isinstance(t, torch.Tensor)]
         ctx.wanted = [t.requires_grad for t in others if isinstance(t, torch.Tensor)]
         ctx.save_for_backward(kept.values, kept.exponents, *(others[i] for i in ctx.places))
-        out = function(tokens, *others)
+        # without autocast's cache, in both runs: what is cast here has no graph, and whoever found it there, the second run
+        # or a layer's next use in the same region, would lose the weights' gradients
+        with torch.autocast(kind, **ctx.autocast):
+            out = function(tokens, *others)
         if not isinstance(out, torch.Tensor):
             raise TypeError("checkpoint_kept8 takes a function that returns one tensor.")
         return out
@@ -128,11 +131,10 @@ class _CheckpointFunction(torch.autograd.Function):
         for place, tensor, wanted in zip(ctx.places, given, ctx.wanted):
             others[place] = tensor.detach().requires_grad_(wanted)
             leaves.append(others[place])
-        enabled, dtype, cache = ctx.autocast
         with torch.random.fork_rng([tokens.device]):
             torch.set_rng_state(ctx.random[0])
             torch.cuda.set_rng_state(ctx.random[1], tokens.device)
-            with torch.enable_grad(), torch.autocast(ctx.kind, enabled=enabled, dtype=dtype, cache_enabled=cache):
+            with torch.enable_grad(), torch.autocast(ctx.kind, **ctx.autocast):
                 out = ctx.function(tokens, *others)
         if out.requires_grad:
             torch.autograd.backward(out, gradient)
