@@ -8,7 +8,8 @@
 // (the reference's SiTU-GLU: model.py:27-38.)
 //
 // fp32 inside, each result rounded once. A gate takes one exponential, e = exp(-|g| / 2): s is 1 / (1 + e^2) or
-// e^2 / (1 + e^2), tanh |g / 4| is (1 - e) / (1 + e). Near zero that difference cancels, and the odd series takes over:
+// e^2 / (1 + e^2), 1 - s the other, tanh |g / 4| is (1 - e) / (1 + e) and 1 - t^2 is 4 e / (1 + e)^2: as differences from 1
+// the last two would be nothing but rounding for a gate that is far from zero. Near zero that difference cancels, and the odd series takes over:
 // x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835, below 1/4, where the rest is under 2^-26 of x. tanh(u / 25) is
 // nearly always there, so its exponential is behind a branch. With the library's tanhf and expf the forward pass was
 // bound by arithmetic.
@@ -29,9 +30,9 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, const mo_block::Divisor& 
 }
 
 // exp(-x c) for 0 <= x: 2^(-x c log2 e), the product's rounding put right, which would be x c units of the result.
-// `high` and `low` are c log2 e in two parts. Past 1024 x is as good as infinite.
+// `high` and `low` are c log2 e in two parts. Past 4096 x is as good as infinite.
 __device__ __forceinline__ float decay(float x, float high, float low) {
-  x = x > 1024.0f ? 1024.0f : x;  // keeps a NaN
+  x = x > 4096.0f ? 4096.0f : x;  // keeps a NaN
   const float power = -x * high;
   const float rest = fmaf(-x, high, -power) - x * low;
   const float e = __builtin_amdgcn_exp2f(power);
@@ -42,28 +43,43 @@ __device__ __forceinline__ float tanh_series(float x) {
   const float y = x * x;
   return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
 }
-// s = sigmoid g and t = tanh(g / 4). log2 e / 2 = 0.72134752 + 1.4e-8 - ...
-__device__ __forceinline__ void gate_of(float g, float& s, float& t) {
+// s = sigmoid g, t = tanh(g / 4), rest = 1 - s and bend = 1 - t^2. log2 e / 2 = 0.72134752 + 1.4e-8 - ...
+struct Gate {
+  float s, t, rest, bend;
+};
+__device__ __forceinline__ Gate gate_of(float g) {
   const float e = decay(fabsf(g), 0x1.715476p-1f, 0x1.4ae0cp-27f), e2 = e * e;
   const float one = 1.0f + e, two = 1.0f + e2, r = __builtin_amdgcn_rcpf(one * two);
-  s = (g >= 0.0f ? 1.0f : e2) * (one * r);
-  s = g != g ? g : s;
+  const float near = one * r, far = e2 * near, q = two * r;
+  Gate to;
+  to.s = g >= 0.0f ? near : far;
+  to.s = g != g ? g : to.s;
+  to.rest = g >= 0.0f ? far : near;
+  to.bend = 4.0f * e * (q * q);
   const float x = 0.25f * g;
-  t = fabsf(x) < kSeries ? tanh_series(x) : copysignf((1.0f - e) * (two * r), g);
+  to.t = fabsf(x) < kSeries ? tanh_series(x) : copysignf((1.0f - e) * q, g);
+  return to;
 }
 __device__ __forceinline__ float sigmoid_of(float g) {
   const float e = decay(fabsf(g), 0x1.715476p+0f, 0x1.4ae0cp-26f);
   const float s = (g >= 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(1.0f + e);
   return g != g ? g : s;
 }
-__device__ __forceinline__ float cap_of(float u) {  // tanh(u / 25)
+struct Cap {
+  float c, bend;  // tanh(u / 25), 1 - its square
+};
+__device__ __forceinline__ Cap cap_of(float u) {
   const float x = u * 0.04f;
-  float c = tanh_series(x);
+  Cap to;
+  to.c = tanh_series(x);
+  to.bend = 1.0f - to.c * to.c;
   if (!(fabsf(x) < kSeries)) {
-    const float e = decay(fabsf(x), 0x1.715476p+1f, 0x1.4ae0cp-25f);
-    c = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+    const float e = decay(fabsf(u), 0x1.d8be08p-4f, 0x1.7f5ffep-32f);  // exp(-2 |u| / 25)
+    const float q = __builtin_amdgcn_rcpf(1.0f + e);
+    to.c = copysignf((1.0f - e) * q, u);
+    to.bend = 4.0f * e * (q * q);
   }
-  return c;
+  return to;
 }
 
 // A lane's place: row, first column, how many of its 8 are in the row, its group and whether it has a row at all.
@@ -120,9 +136,8 @@ __device__ __forceinline__ void forward(const GatedArgs& a) {
     if (a.silu) {
       u[i] = u[i] * (g[i] * sigmoid_of(g[i]));
     } else {
-      float gate, t;
-      gate_of(g[i], gate, t);
-      u[i] = 100.0f * (t * gate) * cap_of(u[i]);
+      const Gate gate = gate_of(g[i]);
+      u[i] = 100.0f * (gate.t * gate.s) * cap_of(u[i]).c;
     }
   }
   store8<kOdd>((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
@@ -148,10 +163,9 @@ __device__ __forceinline__ void backward(const GatedArgs& a) {
       const float gate = sigmoid_of(g[i]);
       act = g[i] * gate, slope = gate * (1.0f + g[i] * (1.0f - gate)), cap = u[i], cap_slope = 1.0f;
     } else {
-      float gate, t;
-      gate_of(g[i], gate, t);
-      const float c = cap_of(u[i]);
-      act = 4.0f * t * gate, slope = (1.0f - t * t) * gate + act * (1.0f - gate), cap = 25.0f * c, cap_slope = 1.0f - c * c;
+      const Gate gate = gate_of(g[i]);
+      const Cap to = cap_of(u[i]);
+      act = 4.0f * gate.t * gate.s, slope = gate.bend * gate.s + act * gate.rest, cap = 25.0f * to.c, cap_slope = to.bend;
     }
     u[i] = d[i] * act * cap_slope;
     g[i] = d[i] * cap * slope;
