@@ -30,6 +30,7 @@ struct Shrink {
   uint64_t x_stride;
   uint32_t features, span;  // features a split, a multiple of 128
   uint32_t scaled;        // times the adapter's scale
+  uint32_t by_request;    // w is [requests] of them: the request's place holds its adapter's
 };
 
 // to[row][n] = base[row][n] + s sum over the rank of h[row][j] v_i[n][j], h the sum of its splits.
@@ -44,6 +45,7 @@ struct Expand {
   uint64_t base_stride;
   uint32_t features, splits, cols;  // columns a workgroup, a multiple of 512
   uint32_t scaled;
+  uint32_t by_request;    // v is, as above
 };
 
 // Both for a forward pass of few rows.
@@ -68,15 +70,16 @@ struct Outer {
   Side side[2];
 };
 
-// Copies of both weights, each [adapters] matrices turned, and of a narrow matrix for an outer: the sum of its splits,
+// Copies of both weights, each [places] matrices turned, and of a narrow matrix for an outer: the sum of its splits,
 // turned, [rows / 8][rank][8].
 struct Turn {
+  Requests by;
   const void* from[2];
   void* to[2];
   uint32_t rows[2], cols[2], tiles[2];  // of `from`; tiles of 32 x 32, 0: not wanted
   const float* narrow;                  // [splits][count][rank]
   float* turned;
-  uint32_t adapters, count, rank, splits;
+  uint32_t places, by_request, count, rank, splits;  // places: the adapters, or the requests
 };
 
 }  // namespace mo_adapters

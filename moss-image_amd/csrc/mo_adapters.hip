@@ -201,7 +201,7 @@ __device__ __forceinline__ void shrink(const Shrink& a) {
   if (adapter != kNone) {
     const uint32_t stride = (uint32_t)a.x_stride, rows = tile.high - tile.low;
     const Window<T, kOdd> x((const T*)a.x + tile.low * a.x_stride, (rows - 1) * stride + a.features);
-    const Window<T, kOdd> w((const T*)a.w + (uint64_t)adapter * rank * a.features, rank * a.features);
+    const Window<T, kOdd> w((const T*)a.w + (uint64_t)(a.by_request ? tile.piece - 1 : adapter) * rank * a.features, rank * a.features);
     const uint32_t first = blockIdx.y * a.span, last = min(a.features, first + a.span);
     for (uint32_t at = first + wave * 128; at < last; at += 1024) {
       Eight<T> xs[4], ws[4][kRanks];
@@ -261,7 +261,7 @@ __device__ __forceinline__ void shrink_tall(const Shrink& a) {
   if (adapter != kNone) {
     const uint32_t stride = (uint32_t)a.x_stride;
     const Window<T, false> x((const T*)a.x + (rows ? low : tile.low) * a.x_stride, rows ? (rows - 1) * stride + a.features : 0);
-    const Window<T, false> w((const T*)a.w + (uint64_t)adapter * rank * a.features, rank * a.features);
+    const Window<T, false> w((const T*)a.w + (uint64_t)(a.by_request ? tile.piece - 1 : adapter) * rank * a.features, rank * a.features);
     const uint32_t first = blockIdx.y * a.span, last = min(a.features, first + a.span);
     Eight<T> xs[4], ws[(kRanks + 1) / 2];
     // a thread's eight columns of four rows, and of every 32nd rank
@@ -350,7 +350,7 @@ __device__ __forceinline__ void expand(const Expand& a) {
   read_base(at);
   const uint32_t adapter = adapter_of(a.by, tile);
   const bool has = adapter != kNone;
-  const Window<T, kOdd> v((const T*)a.v + (uint64_t)(has ? adapter : 0) * a.features * rank, a.features * rank);
+  const Window<T, kOdd> v((const T*)a.v + (uint64_t)(!has ? 0 : a.by_request ? tile.piece - 1 : adapter) * a.features * rank, a.features * rank);
   Eight<T> vs[8][kSteps];
   auto read_v = [&](uint32_t at) {
 #pragma unroll
@@ -485,7 +485,7 @@ __device__ __forceinline__ void expand_tall(const Expand& a) {
   read_base(first, 1);
   const uint32_t adapter = adapter_of(a.by, tile);
   const bool has = adapter != kNone;
-  const Window<T, false> v((const T*)a.v + (uint64_t)(has ? adapter : 0) * a.features * rank, a.features * rank);
+  const Window<T, false> v((const T*)a.v + (uint64_t)(!has ? 0 : a.by_request ? tile.piece - 1 : adapter) * a.features * rank, a.features * rank);
   Eight<T> mine[kMine];
   auto read_v = [&](uint32_t at) {
 #pragma unroll
@@ -973,10 +973,15 @@ __device__ __forceinline__ void turn(const Turn& a) {
     tile -= second ? a.tiles[0] : 0;
     const uint32_t rows = a.rows[second], cols = a.cols[second];
     const uint32_t across = (cols + 31) / 32, row0 = tile / across * 32, col0 = tile % across * 32;
-    for (uint32_t adapter = blockIdx.y; adapter < a.adapters; adapter += gridDim.y) {
-      const uint64_t size = (uint64_t)rows * cols * adapter;
-      const T* from = (const T*)a.from[second] + size;
-      T* to = (T*)a.to[second] + size;
+    for (uint32_t place = blockIdx.y; place < a.places; place += gridDim.y) {
+      uint32_t adapter = place;
+      if (a.by_request) {
+        adapter = begins(a.by, place) < begins(a.by, place + 1) ? adapter_of(a.by, place) : kNone;
+        if (adapter == kNone) continue;  // nothing reads its place
+      }
+      const uint64_t size = (uint64_t)rows * cols;
+      const T* from = (const T*)a.from[second] + size * adapter;
+      T* to = (T*)a.to[second] + size * place;
       __syncthreads();
       for (uint32_t r = y; r < 32; r += 8)
         if (row0 + r < rows && col0 + x < cols) room[r][x] = from[(uint64_t)(row0 + r) * cols + col0 + x];
