@@ -69,7 +69,7 @@ def _check(like, shape, kind, weight, bias, scale, shift, cu_seqlens):
         if cu_seqlens is not None:
             raise ValueError("norm cu_seqlens go with a scale or a shift.")
         return 0, weight, bias, weight_code, None, None, 2, None
-    if given.ndim != 2 or not given.shape[0]:
+    if given.ndim != 2 or not given.shape[0] and shape[:-1].numel():
         raise ValueError("norm scale and shift must be [samples, dim].")
     samples = given.shape[0]
     scale, shift, scale_code = _pair(scale, shift, (samples, dim), like, ("scale", "shift"))
