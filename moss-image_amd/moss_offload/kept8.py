@@ -1,7 +1,8 @@
 """Activations in 8 bits between the forward and the backward pass (``csrc/mo_keep.h``, ``csrc/mo_gated.hip``).
 
 A matrix is kept as int8 and a power of two for each 32 values of a row: the smallest, from 2**-126 on, with which
-127 reaches the largest of them. Each value is off by at most half a step, 2**-7 of its group's largest at worst.
+127 reaches the largest of them. Each value is off by at most half a step, 1/127 of its group's largest (2**-127 where
+that is less, in groups of the smallest numbers); where a step's 64 is past the type's largest value, by less than a whole one, 1/64.
 1 + 1/32 bytes a value, where bfloat16 has two; the offload moves as many fewer bytes. The reference keeps and moves
 what autograd saved (``training/activation_offload.py:80-149``).
 
