@@ -99,22 +99,33 @@ ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
   return p;
 }
 
-// Rows a tile and columns a workgroup of an expand. Tiles of 128 rows, which share v, with more than 16 ranks and 8192 rows or
-// more, where whole workgroups of them fill the GPU (tiles of 16 and of 128, a call of 64 ranks in us: 17792 rows, 3072 columns 162
-// and 146, 8192 columns 228 and 174; 4608 rows 44.0 and 46.0; 1333 rows of 8192 29.3 and 41.3), but not for short requests, whose other
-// rows would be empty. Columns so that there are some rounds of workgroups.
+// Rows a tile and columns a workgroup of an expand. Tiles of 128 rows share v, but each of their workgroups adds up h's planes, one for
+// each split of the shrink, for the columns that it has. They are taken with more than 16 ranks and 2048 rows or more: in float32
+// always, in bfloat16 where a workgroup's columns times its ranks are 4096 for every plane or more, in float16 so with more than
+// 64 ranks; not for short requests, whose other rows would be empty. The expand alone in tiles of 16 and of 128, us:
+//   bfloat16  32 ranks, one plane: 1333 rows of 8192 12.1 and 11.7, 4608 of 8192 29.5 and 26.3; two: 17792 of 8192 126 and 134; 64 ranks, one
+//     plane: 4608 of 3072 21.1 and 18.2; two: 17792 of 8192 186 and 134; three: 4608 of 3072 (2730 a plane) 24.3 and 26.2, of 8192
+//     (8192) 49.5 and 42.2; eight: 8192 of 3072 (2048) 43.3 and 53.7, of 8192 (4096) 95.3 and 84.1; 128 ranks, one plane: 1333 of 3072 16.2 and
+//     16.7, 4608 of 8192 114 and 63
+//   float32   32 ranks: 4608 of 3072 33.3 and 27.3; 64: 17792 of 8192 390 and 274; eight planes: 8192 of 1024 36.1 and 35.7
+//   float16   32 ranks: 17792 of 8192 147 and 175; 64: 4608 of 3072 30.2 and 31.9; 128: 4608 of 3072 85.1 and 54.0
+// Columns so that there are some rounds of workgroups.
 struct ExpandPlan {
   uint32_t rank, rows, cols;
   uint64_t slots;
 };
-ExpandPlan expand_plan(const mo_adapters_call& c, uint32_t features) {
+ExpandPlan expand_plan(const mo_adapters_call& c, uint32_t features, uint32_t planes) {
   ExpandPlan p = {};
   p.rank = c.rank <= 16 ? 16 : c.rank <= 32 ? 32 : c.rank <= 64 ? 64 : 128;
-  p.rows = 16;
-  if (!odd(c) && p.rank > 16 && c.rows >= 128ull * c.requests && c.rows >= 8192) p.rows = 128;
-  const uint64_t tiles = div_up(c.rows, p.rows), least = p.rows == 128 ? 128 : 512;
-  p.cols = (uint32_t)round_up(between<uint64_t>(1, tiles * features / (p.rows == 128 ? 1024 : kExpandGroups), 4096), least);
-  p.slots = tiles + c.requests + 1;
+  auto cols = [&](uint64_t rows) {
+    return (uint32_t)round_up(between<uint64_t>(1, div_up(c.rows, rows) * features / (rows == 128 ? 1024 : kExpandGroups), 4096),
+                              rows == 128 ? 128 : 512);
+  };
+  const bool worth = c.dtype == MO_DTYPE_F32 ||
+                     (cols(128) * p.rank >= 4096 * planes && (c.dtype == MO_DTYPE_BF16 || p.rank > 64));
+  p.rows = !odd(c) && p.rank > 16 && c.rows >= 2048 && c.rows >= 128ull * c.requests && worth ? 128 : 16;
+  p.cols = cols(p.rows);
+  p.slots = div_up(c.rows, p.rows) + c.requests + 1;
   return p;
 }
 
@@ -222,7 +233,7 @@ int shrink(const mo_adapters_call& c, const Requests& by, uint64_t x, uint64_t s
 }
 
 int expand(const mo_adapters_call& c, mo_adapters::Expand& a, uint64_t stream) {
-  const ExpandPlan p = expand_plan(c, a.features);
+  const ExpandPlan p = expand_plan(c, a.features, a.splits);
   a.cols = p.cols;
   return start(c, kExpand, p.rank, odd(c) ? "odd" : p.rows == 128 ? "tall" : "", p.slots, div_up(a.features, p.cols), 1, &a, stream);
 }

@@ -453,9 +453,10 @@ __device__ __forceinline__ void expand(const Expand& a) {
   }
 }
 
-// The same for more than 16 ranks and long requests: a wave has 32 rows of its own, all four waves take the same columns,
-// and v's part of them, as large as the rows' own at 64 ranks, comes to LDS once, a step ahead in registers. Bound by memory:
-// bfloat16, 64 ranks, 17792 rows of 8192 (583 MB, read and written) in 121 us, 4.8 TB/s; of 3072 (219 MB) in 59, 3.7 TB/s.
+// The same for more than 16 ranks and many rows: a wave has 32 rows of its own, all four waves take the same columns,
+// and v's part of them, as large as the rows' own at 64 ranks, comes to LDS once, a step ahead in registers. Bound by memory,
+// of which h's planes are a part, since every workgroup beside another reads them: bfloat16, 64 ranks, 17792 rows of 8192 (583 MB, and 109 of
+// planes for eight workgroups) in 121 us, 5.7 TB/s; of 3072 (219 MB, and 82 of planes for six) in 59, 5.1 TB/s.
 template <class T, int kRank>
 __device__ __forceinline__ void expand_tall(const Expand& a) {
   typedef Path<T> P;
@@ -1052,9 +1053,7 @@ __device__ __forceinline__ void turn(const Turn& a) {
   MO_TALL(T, t, 4)                                                                                                 \
   MO_EXPAND(T, t, 16)                                                                                              \
   MO_EXPAND(T, t, 32)                                                                                              \
-  MO_EXPAND_TALL(T, t, 32)                                                                                         \
   MO_EXPAND(T, t, 64)                                                                                              \
-  MO_EXPAND_TALL(T, t, 64)                                                                                         \
   MO_EXPAND(T, t, 128)                                                                                             \
   MO_EXPAND_TALL(T, t, 128)                                                                                        \
   MO_FEW(T, t, 1)                                                                                                  \
@@ -1067,6 +1066,10 @@ __device__ __forceinline__ void turn(const Turn& a) {
 MO_ADAPTERS(_Float16, f16)
 MO_ADAPTERS(__bf16, bf16)
 MO_ADAPTERS(float, f32)
+MO_EXPAND_TALL(__bf16, bf16, 32)
+MO_EXPAND_TALL(float, f32, 32)
+MO_EXPAND_TALL(__bf16, bf16, 64)
+MO_EXPAND_TALL(float, f32, 64)
 MO_FEW(_Float16, f16, 4)
 MO_FEW(__bf16, bf16, 4)
 MO_TALL(_Float16, f16, 8)
