@@ -64,8 +64,9 @@ uint64_t round_up(uint64_t a, uint64_t b) { return div_up(a, b) * b; }
 template <class N>
 N between(N low, N value, N high) { return value < low ? low : value > high ? high : value; }
 
-// Whether eight neighbouring values can be read at once: features and rank are multiples of eight and every row lies on
-// the 4-byte grid. Other calls have kernels that read value by value.
+// Whether every eight neighbouring values lie in a row and on the 4-byte grid: features and rank are multiples of eight, and so on.
+// Other calls have kernels in which each lane reads its eight at an address of its own, and the last of a row value by value (bfloat16, 4608
+// rows of 3072 to 8192 both ways: ranks 4 and 12 196 and 205 us, 8 and 16 114 and 118; 16 ranks of 3071 features 200).
 bool odd(const mo_adapters_call& c) {
   const uint64_t size = kTypeBytes[c.dtype];
   uint64_t off = (c.in_features | c.out_features | c.rank) % 8;
@@ -101,13 +102,14 @@ ShrinkPlan shrink_plan(const mo_adapters_call& c, uint32_t features) {
 
 // Rows a tile and columns a workgroup of an expand. Tiles of 128 rows share v, but each of their workgroups adds up h's planes, one for
 // each split of the shrink, for the columns that it has. They are taken with more than 16 ranks and 2048 rows or more: in float32
-// always, in bfloat16 where a workgroup's columns times its ranks are 4096 for every plane or more, in float16 so with more than
-// 64 ranks; not for short requests, whose other rows would be empty. The expand alone in tiles of 16 and of 128, us:
+// where a workgroup has 20 columns for every plane, in bfloat16 where its columns times its ranks are 4096 for every plane, in float16
+// so with more than 64 ranks; not for short requests, whose other rows would be empty. The expand alone in tiles of 16 and of 128, us:
 //   bfloat16  32 ranks, one plane: 1333 rows of 8192 12.1 and 11.7, 4608 of 8192 29.5 and 26.3; two: 17792 of 8192 126 and 134; 64 ranks, one
 //     plane: 4608 of 3072 21.1 and 18.2; two: 17792 of 8192 186 and 134; three: 4608 of 3072 (2730 a plane) 24.3 and 26.2, of 8192
 //     (8192) 49.5 and 42.2; eight: 8192 of 3072 (2048) 43.3 and 53.7, of 8192 (4096) 95.3 and 84.1; 128 ranks, one plane: 1333 of 3072 16.2 and
 //     16.7, 4608 of 8192 114 and 63
-//   float32   32 ranks: 4608 of 3072 33.3 and 27.3; 64: 17792 of 8192 390 and 274; eight planes: 8192 of 1024 36.1 and 35.7
+//   float32   32 ranks, one plane: 4608 of 3072 33.3 and 27.3; 13: 4608 of 3072 (10 columns a plane) 45.9 and 50.3, of 8192 (30) 91.5 and 85.8; 64
+//     ranks, two: 17792 of 8192 390 and 274; eight: 8192 of 1024 (16) 36.1 and 35.7, of 3072 (32) 87.3 and 76.5; 16: 2048 of 8192 (8) 67 and 109
 //   float16   32 ranks: 17792 of 8192 147 and 175; 64: 4608 of 3072 30.2 and 31.9; 128: 4608 of 3072 85.1 and 54.0
 // Columns so that there are some rounds of workgroups.
 struct ExpandPlan {
@@ -121,8 +123,8 @@ ExpandPlan expand_plan(const mo_adapters_call& c, uint32_t features, uint32_t pl
     return (uint32_t)round_up(between<uint64_t>(1, div_up(c.rows, rows) * features / (rows == 128 ? 1024 : kExpandGroups), 4096),
                               rows == 128 ? 128 : 512);
   };
-  const bool worth = c.dtype == MO_DTYPE_F32 ||
-                     (cols(128) * p.rank >= 4096 * planes && (c.dtype == MO_DTYPE_BF16 || p.rank > 64));
+  const bool worth = c.dtype == MO_DTYPE_F32 ? cols(128) >= 20 * planes
+                                             : cols(128) * p.rank >= 4096 * planes && (c.dtype == MO_DTYPE_BF16 || p.rank > 64);
   p.rows = !odd(c) && p.rank > 16 && c.rows >= 2048 && c.rows >= 128ull * c.requests && worth ? 128 : 16;
   p.cols = cols(p.rows);
   p.slots = div_up(c.rows, p.rows) + c.requests + 1;
