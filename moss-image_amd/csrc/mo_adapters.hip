@@ -6,10 +6,12 @@
 // (one request with one adapter: the reference's LoRA linear, lora.py:60-86.)
 //
 // Three kernels: shrink (h and d h: rows against a weight's ranks, reduced over the features), expand (y and d x:
-// reduced over the rank), outer (both weights' gradients: reduced over the rows). All are bound by the tokens that they
-// read and write, so the matrix instructions have room: bfloat16 operands go into 16 x 16 x 32 ones, and the fp32
-// numbers between the products in three bfloat16 parts, which are all of their 24 bits; float16 and float32 go
-// into the fp32 ones, 16 x 16 x 4, where float16 parts would under- and overflow.
+// reduced over the rank), outer (both weights' gradients: reduced over the rows). bfloat16 operands go into 16 x 16 x 32
+// matrix instructions, and the fp32 numbers between the products in three bfloat16 parts, which are all of their 24 bits: what
+// bounds these kernels is the tokens that they read and write. float16 and float32 go into the fp32 instructions, 16 x 16 x 4,
+// where float16 parts would under- and overflow; at a sixteenth of the rate those are the bound from some 64 ranks on (17792 rows
+// of 8192 and 3072 both ways, 64 ranks: 490 us by operations, 300 by bytes in float16; measured for 4608 rows 320 us, bfloat16 with 32
+// ranks 137).
 //
 // Rows are taken in tiles that lie in one request. Tile and request are found from the workgroup's number alone: what
 // lies between a tile's border and a request's is at slot (tile + request), which no other pair has.
@@ -180,7 +182,8 @@ __device__ __forceinline__ uint32_t adapter_of(const Requests& by, const Tile& t
 // at 4.2 TB/s where this comes at 5.4) and turns them through its own part of LDS, eight values at a time; those of
 // row r lie at (place ^ r), so that neither writing nor reading meets a bank twice. The rows are the instruction's
 // columns, so a lane ends with four neighbouring ranks of a row. Nothing is loaded ahead: sixteen waves a CU are enough.
-// Bound by memory: bfloat16, 16 ranks, 4608 rows of 3072 (28 MB) in 11.5 us, 2.5 TB/s, most of it the way there and back.
+// Bound by the way to memory and back: bfloat16, 16 ranks, 4608 rows of 3072 (28 MB) in 11.5 us, 2.5 TB/s. More than 64 ranks of float32,
+// or of float16 in odd sizes, leave no registers for all (268 to 432 bytes a lane in scratch): 4608 rows of 8192, 128 ranks, float32 265 us.
 template <class T, int kRanks, bool kOdd>
 __device__ __forceinline__ void shrink(const Shrink& a) {
   typedef Path<T> P;
@@ -318,7 +321,8 @@ __device__ __forceinline__ uint64_t turned_at(uint32_t rank, uint32_t j, uint32_
 // columns are the instructions' rows, so a lane ends with four neighbouring columns of a row; through the wave's own
 // part of LDS they come to lanes that read and write 256 bytes of a row side by side. With ranks up to 16 the first two
 // parts of h lie beside each other in one fragment, the third beside nothing in another. (32 rows, which read v half as often, were slower: 4608 rows, 16 ranks,
-// 3072 columns 25.5 us for 21.2.) Bound by memory: 16 ranks, 4608 rows of 16384 (302 MB, read and written) in 61 us, 4.9 TB/s.
+// 3072 columns 25.5 us for 21.2.) Bound by memory: 16 ranks, 4608 rows of 16384 (302 MB, read and written) in 61 us, 4.9 TB/s; of 3072
+// (57 MB, and 23 of h's 13 planes, which each of six workgroups beside another adds up) in 20.7, 3.8 TB/s.
 template <class T, int kRank, bool kOdd>
 __device__ __forceinline__ void expand(const Expand& a) {
   typedef Path<T> P;
@@ -722,8 +726,9 @@ __device__ __forceinline__ void few(const Few& f) {
 // add up through LDS. A lane reads eight neighbouring columns of eight rows, and column q of all lanes makes the operand of
 // instruction q: the rows, which are reduced, lie beside each other in a lane without a way through LDS. A step's rows
 // begin at a multiple of 32; those that are not the request's count as zeros on both sides (they may be infinite). bfloat16:
-// 16 ranks, 4608 rows of 16384 and, in 8 bits, 3072 (166 MB) in 30.5 us, 5.4 TB/s, bound by memory; 64 ranks, 17792 rows of 8192 and
-// 3072 (401 MB) in 138, 2.9 TB/s, where the sums leave registers for two waves a SIMD, too few to cover the loads.
+// 16 ranks, 4608 rows of 16384 and, in 8 bits, 3072 (166 MB) in 31 us, 5.3 TB/s, bound by memory; 64 ranks, 17792 rows of 8192 and
+// 3072 (401 MB) in 142, 2.8 TB/s, where the sums leave registers for two waves a SIMD (seven more values go to scratch), too few to
+// cover the loads, of which none is asked for a step ahead.
 template <class T, int kRanks, bool kKept, bool kOdd>
 __device__ __forceinline__ void outer(const Requests& by, const Side& a, uint32_t tile, f32x4* room) {
   typedef Path<T> P;
@@ -1008,7 +1013,8 @@ __device__ __forceinline__ void turn(const Turn& a) {
     if (col0 + r < a.rank && row0 + x < a.count) a.turned[turned_at(a.rank, col0 + r, row0 + x)] = room[x][r];
 }
 
-// Names: type, ranks; "tall": tiles of 128 rows; "odd": features or a rank that are no multiples of eight.
+// Names: type, ranks; "tall": tiles of 128 rows; "odd": features or a rank that are no multiples of eight, or addresses off the
+// 4-byte grid.
 // Waves a SIMD asked for where the compiler would take registers for one less: an expand of 16 ranks (4608 rows of 3072 bfloat16
 // 21.0 us, 23.4 with three), an outer of 32 (three of its values go to scratch; 4608 rows of 8192 and 3072 27.1 us).
 #define MO_SHRINK(T, t, ranks)                                                                                     \

@@ -119,8 +119,10 @@ __device__ __forceinline__ void read_kept(float (&to)[8], const void* values, co
   decode(to, q, exponent);
 }
 
-// A lane has eight neighbouring columns, so that a wave reads 1 KB of a row side by side; one pass, nothing held. Bound by
-// memory: bfloat16, 17792 x 12288 (1.31 GB) in 299 us, 4.4 TB/s; 4608 x 8192, both inputs written in 8 bits (304 MB) in 66, 4.6 TB/s.
+// A lane has eight neighbouring columns, so that a wave reads 1 KB of a row side by side; one pass, nothing held. SiLU is bound by
+// memory, SiTU by its arithmetic too: bfloat16, 4608 x 8192 (226 MB) 41 us, 5.5 TB/s, and 46 to 49. SiTU of 17792 x 12288 (1.31 GB) takes 294
+// to 325 us, 4.0 to 4.5 TB/s, in which a SIMD issues 189 000 vector instructions; 4608 x 8192, both inputs written in 8 bits (304 MB)
+// 65, 4.7 TB/s.
 template <class T, bool kKeep, bool kOdd>
 __device__ __forceinline__ void forward(const GatedArgs& a) {
   const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
@@ -143,7 +145,8 @@ __device__ __forceinline__ void forward(const GatedArgs& a) {
   store8<kOdd>((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
 }
 
-// The same: 17792 x 12288 (2.19 GB) in 369 us, 5.9 TB/s; 4608 x 8192 from 8 bits (304 MB) in 62, 4.9 TB/s.
+// Bound by memory: 17792 x 12288 (2.19 GB) in 376 to 414 us, 5.3 to 5.8 TB/s; 4608 x 8192 (377 MB) 63 us, SiLU 61, 6 TB/s; from 8 bits
+// (304 MB) 63, 4.8 TB/s.
 template <class T, bool kKept, bool kOdd>
 __device__ __forceinline__ void backward(const GatedArgs& a) {
   const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
@@ -190,7 +193,7 @@ __device__ __forceinline__ void restore(const KeepArgs& a) {
   store8<kOdd>((T*)a.out + s.row * a.stride + s.at, v, s.n);
 }
 
-// "odd": columns that are no multiple of eight.
+// "odd": columns that are no multiple of eight (4608 x 8191 55 and 90 us both ways, 8192 47 and 63).
 #define MO_GATED(T, t, odd)                                                                                   \
   extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_##t(GatedArgs a) { forward<T, false, odd>(a); }      \
   extern "C" __global__ __launch_bounds__(256) void mo_gated_forward_keep_##t(GatedArgs a) { forward<T, true, odd>(a); }  \

@@ -83,7 +83,8 @@ __device__ __forceinline__ void widen(float (&to)[8], const Eight<T>& from) {
 
 // A part of memory that all lanes share: its address stays in scalar registers, a lane has 32-bit offsets (the host keeps
 // rows near enough for that), and what a lane should not read or write it asks for past the end, where reads
-// give zeros and writes are dropped. Odd sizes, or addresses off the 4-byte grid, go value by value.
+// give zeros and writes are dropped. Odd sizes, or addresses off the 4-byte grid, go by each lane's own address, the last of a row
+// value by value.
 constexpr uint32_t kNowhere = 0x80000000u;  // no window is as long
 
 template <class T, bool kOdd>

@@ -5,8 +5,8 @@ that a row belongs to. With one request and one adapter it is the reference's Lo
 a packed batch may bring an adapter for each sample, a batch of sampling requests one for each row. The products in
 between stay in fp32 and ``y`` is rounded once. The gradients read ``x`` or what 8 bits keep of it.
 
-Rows are ``[..., features]``, dense, any distance apart; ranks go up to 128. The requests are ``x``'s first dimension, or
-``cu_seqlens`` (``[requests + 1]``) says which rows each has; ``index`` (``[requests]``) says which adapter, any number
+Rows are ``[..., features]``, dense, any distance apart; ranks go up to 128. The requests are the first dimension of an ``x`` of
+three or more (one of two is one request), or ``cu_seqlens`` (``[requests + 1]``) says which rows each has; ``index`` (``[requests]``) says which adapter, any number
 outside ``[0, adapters)`` none. Rows without an adapter pass ``result`` on. Without an index request ``i`` has
 adapter ``i``, or the only one.
 """
