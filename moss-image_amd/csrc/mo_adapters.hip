@@ -50,7 +50,7 @@ struct Path {  // fp32 instructions: lane (i, k) has values k * 8 to k * 8 + 7, 
     widen(f.v, v);
     return f;
   }
-  static __device__ __forceinline__ void split(Fragment (&to)[1], const float (&v)[8]) {
+  static __device__ __forceinline__ void split(Fragment (&to)[1], const float (&v)[8], float = 1.0f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) to[0].v[i] = v[i];
   }
@@ -81,8 +81,9 @@ struct Path<__bf16> {
   static constexpr int kParts = 3;
   static __device__ __forceinline__ Fragment of(const Eight<__bf16>& v) { return __builtin_bit_cast(Fragment, v); }
   // fp32 numbers as sums of three bfloat16 ones: the upper half of the number (cut, so that nothing overflows), that of
-  // the rest, and what is left, eight bits each: none is lost. What is not finite has no rest.
-  static __device__ __forceinline__ void split(Fragment (&to)[3], const float (&v)[8]) {
+  // the rest, and `last` times what is left, eight bits each: none is lost. What is not finite has no rest. (A number of few bits
+  // has parts of zero, which make NaN of an infinity on the other side.)
+  static __device__ __forceinline__ void split(Fragment (&to)[3], const float (&v)[8], float last = 1.0f) {
     uint32_t words[3][4];
     float rest[8];
 #pragma unroll
@@ -92,7 +93,7 @@ struct Path<__bf16> {
       uint32_t bits[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        bits[i] = __builtin_bit_cast(uint32_t, rest[i]);
+        bits[i] = __builtin_bit_cast(uint32_t, p == 2 ? rest[i] * last : rest[i]);
         rest[i] -= __builtin_bit_cast(float, bits[i] & 0xffff0000u);
         if (p == 0) rest[i] = (bits[i] & 0x7f800000u) == 0x7f800000u ? 0.0f : rest[i];
       }
@@ -320,8 +321,8 @@ __device__ __forceinline__ uint64_t turned_at(uint32_t rank, uint32_t j, uint32_
 // A workgroup has 16 rows, whose h stays in registers, and `cols` columns, of which a wave takes 128 at a time. The
 // columns are the instructions' rows, so a lane ends with four neighbouring columns of a row; through the wave's own
 // part of LDS they come to lanes that read and write 256 bytes of a row side by side. With ranks up to 16 the first two
-// parts of h lie beside each other in one fragment, the third beside nothing in another. (32 rows, which read v half as often, were slower: 4608 rows, 16 ranks,
-// 3072 columns 25.5 us for 21.2.) Bound by memory: 16 ranks, 4608 rows of 16384 (302 MB, read and written) in 61 us, 4.9 TB/s; of 3072
+// parts of h lie beside each other in one fragment, the third's halves in another (beside zeros an infinite v would
+// give NaN). (32 rows, which read v half as often, were slower: 4608 rows, 16 ranks, 3072 columns 25.5 us for 21.2.) Bound by memory: 16 ranks, 4608 rows of 16384 (302 MB, read and written) in 61 us, 4.9 TB/s; of 3072
 // (57 MB, and 23 of h's 13 planes, which each of six workgroups beside another adds up) in 20.7, 3.8 TB/s.
 template <class T, int kRank, bool kOdd>
 __device__ __forceinline__ void expand(const Expand& a) {
@@ -406,10 +407,10 @@ __device__ __forceinline__ void expand(const Expand& a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = j < kRank ? shared[i][j + e] : 0.0f;
       typename P::Fragment parts[P::kParts];
-      P::split(parts, v);
+      P::split(parts, v, kBeside ? 0.5f : 1.0f);
       if (kBeside) {
         h[0][s] = k < 2 ? parts[0] : parts[P::kParts / 2];
-        h[kParts - 1][s] = k < 2 ? parts[P::kParts - 1] : typename P::Fragment{};
+        h[kParts - 1][s] = parts[P::kParts - 1];
       } else {
 #pragma unroll
         for (int p = 0; p < kParts; ++p) h[p][s] = parts[p];
@@ -682,10 +683,10 @@ __device__ __forceinline__ void few(const Few& f) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = j < kRank ? h[i][j + e] : 0.0f;
       typename P::Fragment parts[P::kParts];
-      P::split(parts, v);
+      P::split(parts, v, kBeside ? 0.5f : 1.0f);
       if (kBeside) {
         hs[0][s] = k < 2 ? parts[0] : parts[P::kParts / 2];
-        hs[kParts - 1][s] = k < 2 ? parts[P::kParts - 1] : typename P::Fragment{};
+        hs[kParts - 1][s] = parts[P::kParts - 1];
       } else {
 #pragma unroll
         for (int p = 0; p < kParts; ++p) hs[p][s] = parts[p];

@@ -43,3 +43,21 @@ def test_infinities_stay_infinities(rows, features, out, rank, dtype) -> None:
     dx, _, _ = adapters.adapters_backward(grad, x, hidden, a, b.abs(), 0.5)
     assert dx[0].eq(float("inf")).all() and dx[rows // 3].eq(float("-inf")).all()
     assert torch.isfinite(dx[[i for i in range(rows) if i not in (0, rows // 3)]]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,out,rank", [(16, 80, 8), (16, 80, 16), (40, 1032, 16), (1400, 3080, 16), (33, 72, 24), (2100, 264, 32), (31, 51, 13)])
+def test_an_infinite_weight_gives_an_infinity(rows, out, rank, dtype) -> None:
+    """h has all of its 24 bits, so that no part of it is zero."""
+
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    n = torch.randint(1 << 23, 1 << 24, (rows, rank), device=DEV, generator=g) | 0x8001
+    x, a = torch.zeros(rows, 3 * rank, device=DEV, dtype=dtype), torch.zeros(1, rank, 3 * rank, device=DEV, dtype=dtype)
+    for i, mask in enumerate((0xFF0000, 0xFF00, 0xFF)):
+        x[:, i::3] = ((n & mask).double() * 2.0**-24).to(dtype)
+        a[0, range(rank), range(i, 3 * rank, 3)] = 1.0
+    b = _randn(1, out, rank, dtype=dtype, seed=1)
+    b[0, 3, rank - 1], b[0, out - 1, 0] = float("inf"), float("-inf")
+    y = adapters.adapters_forward(x, torch.zeros(rows, out, device=DEV, dtype=dtype), a, b)
+    assert y[:, 3].eq(float("inf")).all() and y[:, out - 1].eq(float("-inf")).all()
+    assert torch.isfinite(y[:, [i for i in range(out) if i not in (3, out - 1)]]).all()
