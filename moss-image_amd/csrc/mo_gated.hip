@@ -120,9 +120,9 @@ __device__ __forceinline__ void read_kept(float (&to)[8], const void* values, co
 }
 
 // A lane has eight neighbouring columns, so that a wave reads 1 KB of a row side by side; one pass, nothing held. SiLU is bound by
-// memory, SiTU by its arithmetic too: bfloat16, 4608 x 8192 (226 MB) 41 us, 5.5 TB/s, and 46 to 49. SiTU of 17792 x 12288 (1.31 GB) takes 294
-// to 325 us, 4.0 to 4.5 TB/s, in which a SIMD issues 189 000 vector instructions; 4608 x 8192, both inputs written in 8 bits (304 MB)
-// 65, 4.7 TB/s.
+// memory, SiTU by its arithmetic too: bfloat16, 4608 x 8192 (226 MB) 41 us, 5.5 TB/s, and 46 to 49. SiTU of 17792 x 12288 (1.31 GB), in
+// which a SIMD issues 189 000 vector instructions, takes 245 us at the full clock, 5.4 TB/s, and 285 where power holds it at 2 GHz;
+// 4608 x 8192, both inputs written in 8 bits (304 MB) 65, 4.7 TB/s.
 template <class T, bool kKeep, bool kOdd>
 __device__ __forceinline__ void forward(const GatedArgs& a) {
   const Spot s(a.rows, a.cols, a.lanes, a.by_lanes);
@@ -145,7 +145,7 @@ __device__ __forceinline__ void forward(const GatedArgs& a) {
   store8<kOdd>((T*)a.out + s.row * a.out_stride + s.at, u, s.n);
 }
 
-// Bound by memory: 17792 x 12288 (2.19 GB) in 376 to 414 us, 5.3 to 5.8 TB/s; 4608 x 8192 (377 MB) 63 us, SiLU 61, 6 TB/s; from 8 bits
+// Bound by memory: 17792 x 12288 (2.19 GB) in 370 us at either clock, 5.9 TB/s; 4608 x 8192 (377 MB) 63 us, SiLU 61, 6 TB/s; from 8 bits
 // (304 MB) 63, 4.8 TB/s.
 template <class T, bool kKept, bool kOdd>
 __device__ __forceinline__ void backward(const GatedArgs& a) {
