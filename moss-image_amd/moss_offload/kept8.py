@@ -103,6 +103,11 @@ def keep8(x: torch.Tensor) -> Kept8:
 # ---- a checkpointed block whose input is kept in 8 bits -------------------------------------------------
 
 
+def _not_captured(tensor: torch.Tensor) -> None:
+    if tensor.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("checkpoint_kept8 cannot be captured into a graph.")
+
+
 class _CheckpointFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, function, tokens, *others):
@@ -125,6 +130,7 @@ class _CheckpointFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gradient):
         first_derivatives("checkpoint_kept8")
+        _not_captured(gradient)
         values, exponents, *given = ctx.saved_tensors
         tokens = Kept8(values, exponents, ctx.cols, ctx.dtype).restore().requires_grad_(ctx.needs_input_grad[1])
         others = list(ctx.others)
@@ -150,13 +156,12 @@ def checkpoint_kept8(function, tokens: torch.Tensor, *others) -> torch.Tensor:
     the rest again from that: the result is the exact input's, the gradients are taken at what 8 bits keep of it.
 
     As with a reentrant checkpoint, the parameters inside get their gradients by accumulation (``backward()``, not
-    ``torch.autograd.grad``), and an input must want a gradient: the function's parameters alone are not seen. Not while a
-    graph is captured: the random numbers' state, which the second run starts from, cannot be read then."""
+    ``torch.autograd.grad``), and an input must want a gradient: the function's parameters alone are not seen. Neither
+    pass while a graph is captured: the random numbers' state, which the second run starts from, cannot be had then."""
 
     if not torch.is_grad_enabled():
         return function(tokens, *others)
     if not any(isinstance(t, torch.Tensor) and t.requires_grad for t in (tokens, *others)):
         raise RuntimeError("checkpoint_kept8 needs an input that requires grad.")
-    if tokens.is_cuda and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("checkpoint_kept8 cannot be captured into a graph.")
+    _not_captured(tokens)
     return _CheckpointFunction.apply(function, tokens, *others)
